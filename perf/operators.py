@@ -13,9 +13,10 @@ score    log probability of a given token a row, the row's entropy, its most
 
 The 4-bit entry of a token: per KV head, each group of 32 adjacent channels has
 a minimum m and a step s = fp16((max - m) / 15) (difference and quotient in
-fp32), both fp16; a channel's code is the whole number nearest to (x - m) / s
-(ties to even), kept in 0..15 (0 where s is 0), and it stands for
-fp16(m + s * code).  The pools (nb pages of 16 tokens, H heads, 128 channels):
+fp32; the values here are far from fp16's largest, where the next smaller s is
+taken if m + 15 s would pass it), both fp16; a channel's code is the whole number
+nearest to (x - m) / s (ties to even), kept in 0..15 (0 where s is 0), and it
+stands for fp16(m + s * code).  The pools (nb pages of 16 tokens, H heads, 128 channels):
 
 k_codes   uint8 [nb, H, 16, 64]     a token's row: 16 words of 8 codes, word
                                     4 g + j the channels 32 j + 8 g + (0..7)

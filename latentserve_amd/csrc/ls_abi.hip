@@ -227,6 +227,11 @@ int set_norm(ls::GemmParams& a, const void* res, int64_t res_stride, const void*
 
 }  // namespace
 
+namespace ls {
+// For the entry points of the other ABI files: one message a thread.
+int abi_fail(int code, const char* message) { return fail(code, "%s", message); }
+}  // namespace ls
+
 extern "C" {
 
 const char* ls_last_error(void) { return g_err.c_str(); }

@@ -1,0 +1,147 @@
+// The 4-bit cache's write and read kernels: K and V of new tokens quantized into
+// their slots, and pool rows read back as fp16 values.
+//
+//   m = min, s = fp16((max - m) / 15) over a (token, head)'s 32 adjacent channels
+//   (the next smaller s where m + 15 s would round past fp16's largest value),
+//   code = nearest whole number to (x - m) / s (ties to even) in 0..15, 0 where
+//   s is 0; an entry stands for fp16(m + s * code).
+//
+// Sixteen lanes take a (token, head)'s 16 octets of channels, so a group of 32 is
+// a quad of lanes and its minimum and maximum two lane exchanges; a lane reads 16
+// bytes and writes one word of codes.  Both kernels are bound by their loads
+// and stores.
+
+#include "ls_common.h"
+#include "ls_serving.h"
+
+namespace ls {
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+
+constexpr int I4_THREADS = 256;
+constexpr int I4_LANES = HEAD_DIM / 8;      // lanes a (token, head)
+
+// Minimum / maximum over the lane's quad.
+__device__ __forceinline__ float quad_min(float v) {
+    v = fminf(v, dpp_move<0xB1>(v));
+    return fminf(v, dpp_move<0x4E>(v));
+}
+__device__ __forceinline__ float quad_max(float v) {
+    v = fmaxf(v, dpp_move<0xB1>(v));
+    return fmaxf(v, dpp_move<0x4E>(v));
+}
+
+// (blockIdx.y: K, V)
+__global__ __launch_bounds__(I4_THREADS) void int4_write_kernel(const Int4WriteParams a) {
+    const int z = blockIdx.y;
+    const int64_t i = (int64_t)blockIdx.x * I4_THREADS + threadIdx.x;
+    const int o = threadIdx.x % I4_LANES;
+    const int item = (int)(i / I4_LANES);               // (sequence, head, token)
+    if (item >= a.B * a.H * a.N) return;                // (whole groups of 16 lanes)
+    const int bh = item / a.N, t_new = item - bh * a.N;
+    const int b = bh / a.H, h = bh - b * a.H;
+    const int64_t slot = a.slots[(int64_t)b * a.N + t_new];
+    if (slot < 0 || slot >= (int64_t)a.p.num_blocks * PAGE) return;
+    const h8 x = *(const h8*)(a.src[z] + b * a.ss_b[z] + h * a.ss_h[z] + t_new * a.ss_t[z] + 16 * o);
+    float lo = (float)x[0], hi = lo;
+#pragma unroll
+    for (int e = 1; e < 8; ++e) {
+        lo = fminf(lo, (float)x[e]);
+        hi = fmaxf(hi, (float)x[e]);
+    }
+    lo = quad_min(lo);
+    hi = quad_max(hi);
+    half_t s = (half_t)((hi - lo) / 15.f);
+    // (65520 is where fp16 rounds to infinity; s is then over 4000, and a step of it
+    // less takes 15 s below max)
+    if (lo + 15.f * (float)s >= 65520.f && hi <= 65504.f)
+        s = __builtin_bit_cast(half_t, (uint16_t)(__builtin_bit_cast(uint16_t, s) - 1));
+    // The quotient in 64 bits: the difference and the border between two codes
+    // are exact there (fp16 operands span 40 bits), so the code is the one the
+    // definition names.
+    uint32_t word = 0;
+    const double sd = (double)(float)s;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        double c = sd > 0. ? rint(((double)(float)x[e] - (double)lo) / sd) : 0.;
+        c = c < 15. ? c : 15.;
+        word |= (uint32_t)c << (4 * e);
+    }
+    const int64_t blk = slot / PAGE;
+    const int t = (int)(slot % PAGE);
+    char* codes = a.p.codes[z] + blk * a.p.sc[z] + (int64_t)h * I4_CODES;
+    char* aff = a.p.affine[z] + blk * a.p.sa[z] + (int64_t)h * I4_AFFINE;
+    const int grp = o / 4;
+    if (z == 0) {
+        *(uint32_t*)(codes + 64 * t + 16 * (o % 4) + 4 * grp) = word;
+        if (o % 4 == 0) {
+            const h2 sm = {s, (half_t)lo};
+            *(h2*)(aff + 16 * t + 4 * grp) = sm;
+        }
+    } else {
+        *(uint32_t*)(codes + 64 * o + 4 * t) = word;
+        if (o % 4 == 0) {
+            half_t* q = (half_t*)(aff + 64 * grp + 16 * (t / 4)) + t % 4;
+            q[0] = s;
+            q[4] = (half_t)lo;
+        }
+    }
+}
+
+// The eight entries of a word: fp16(m + s * code), each pair one fused multiply-add.
+__device__ __forceinline__ h8 word_values(uint32_t w, half_t s, half_t m) {
+    h8 r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const half_t c = (half_t)(float)((w >> (4 * e)) & 15);
+        r[e] = __builtin_fmaf16(c, s, m);
+    }
+    return r;
+}
+
+// (blockIdx.y: K, V)  Items (sequence, token, head), 16 lanes each.
+__global__ __launch_bounds__(I4_THREADS) void int4_read_kernel(const Int4ReadParams a) {
+    const int z = blockIdx.y;
+    const int64_t i = (int64_t)blockIdx.x * I4_THREADS + threadIdx.x;
+    const int o = threadIdx.x % I4_LANES;
+    const int64_t item = i / I4_LANES;
+    if (item >= (int64_t)a.B * a.L * a.H) return;
+    const int64_t bt = item / a.H;
+    const int h = (int)(item - bt * a.H);
+    const int b = (int)(bt / a.L), pos = (int)(bt - (int64_t)b * a.L);
+    h8 y = {};
+    const int page = pos / PAGE, t = pos % PAGE;
+    if (pos < a.lens[b] && page < a.max_pages) {
+        const int blk = a.tables[(int64_t)b * a.st_b + page];
+        if ((unsigned)blk < (unsigned)a.p.num_blocks) {
+            const char* codes = a.p.codes[z] + blk * a.p.sc[z] + (int64_t)h * I4_CODES;
+            const char* aff = a.p.affine[z] + blk * a.p.sa[z] + (int64_t)h * I4_AFFINE;
+            const int grp = o / 4;
+            if (z == 0) {
+                const h2 sm = *(const h2*)(aff + 16 * t + 4 * grp);
+                y = word_values(*(const uint32_t*)(codes + 64 * t + 16 * (o % 4) + 4 * grp), sm[0],
+                                sm[1]);
+            } else {
+                const half_t* q = (const half_t*)(aff + 64 * grp + 16 * (t / 4)) + t % 4;
+                y = word_values(*(const uint32_t*)(codes + 64 * o + 4 * t), q[0], q[4]);
+            }
+        }
+    }
+    *(h8*)(a.out[z] + item * HEAD_DIM + 8 * o) = y;
+}
+
+hipError_t launch_int4_write(const Int4WriteParams& a, hipStream_t stream) {
+    const int64_t lanes = (int64_t)a.B * a.H * a.N * I4_LANES;
+    hipLaunchKernelGGL(int4_write_kernel, dim3((unsigned)((lanes + I4_THREADS - 1) / I4_THREADS), 2),
+                       dim3(I4_THREADS), 0, stream, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_int4_read(const Int4ReadParams& a, hipStream_t stream) {
+    const int64_t lanes = (int64_t)a.B * a.L * a.H * I4_LANES;
+    hipLaunchKernelGGL(int4_read_kernel, dim3((unsigned)((lanes + I4_THREADS - 1) / I4_THREADS), 2),
+                       dim3(I4_THREADS), 0, stream, a);
+    return hipGetLastError();
+}
+
+}  // namespace ls

@@ -1,0 +1,38 @@
+// Pages copied to other pages of the same pools: t[dst[i]] = t[src[i]] for every
+// tensor t (all layers' K and V pools, scales, bounds) in one launch.
+//
+// Bound by HBM, and for a few pages by the launch itself: the pointers, strides
+// and page numbers travel in the kernel's arguments, so a branch of a sequence
+// costs one launch and no transfer.
+
+#include "ls_common.h"
+#include "ls_serving.h"
+
+namespace ls {
+
+constexpr int COPY_THREADS = 256;
+
+// (blockIdx.x: pair, blockIdx.y: tensor)
+template <class T>
+__global__ __launch_bounds__(COPY_THREADS) void page_copy_kernel(const PageCopyParams a) {
+    const int i = blockIdx.x, k = blockIdx.y;
+    const int64_t stride = a.stride[k];
+    const T* src = (const T*)(a.base[k] + a.src[i] * stride);
+    T* dst = (T*)(a.base[k] + a.dst[i] * stride);
+    const int n = a.bytes[k] / (int)sizeof(T);
+    for (int e = threadIdx.x; e < n; e += COPY_THREADS) dst[e] = src[e];
+}
+
+hipError_t launch_page_copy(const PageCopyParams& a, int tensors, int pairs, int max_bytes,
+                            int vec, hipStream_t stream) {
+    (void)max_bytes;
+    const dim3 grid(pairs, tensors), block(COPY_THREADS);
+    if (vec == 16) hipLaunchKernelGGL(page_copy_kernel<u4>, grid, block, 0, stream, a);
+    else if (vec == 8) hipLaunchKernelGGL(page_copy_kernel<u2>, grid, block, 0, stream, a);
+    else if (vec == 4) hipLaunchKernelGGL(page_copy_kernel<uint32_t>, grid, block, 0, stream, a);
+    else if (vec == 2) hipLaunchKernelGGL(page_copy_kernel<uint16_t>, grid, block, 0, stream, a);
+    else hipLaunchKernelGGL(page_copy_kernel<uint8_t>, grid, block, 0, stream, a);
+    return hipGetLastError();
+}
+
+}  // namespace ls

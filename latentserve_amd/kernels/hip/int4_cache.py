@@ -1,0 +1,207 @@
+"""4-bit paged K/V pools on HIP kernels: write, read back, decode attention.
+
+The KV cache in a quarter of the fp16 pools' bytes (160 a token and KV head
+instead of 512).  Unlike the INT8 pools a token's entry depends on that token
+alone, so there is no last-page residual: pages can be shared, copied and
+rewound at any token.
+
+Per (token, head), each group of 32 adjacent channels has a minimum m and a step
+s = fp16((max - m) / 15) (the next smaller one where m + 15 s would pass fp16's
+largest value), both fp16; a channel's code is the whole number nearest
+to (x - m) / s (ties to even) in 0..15 and stands for fp16(m + s * code).
+
+``Int4Pools`` holds the four tensors of a layer:
+
+    k_codes   uint8 [nb, H, 16, 64]      k_affine  fp16 [nb, H, 16, 4, 2]
+    v_codes   uint8 [nb, H, 16, 16, 4]   v_affine  fp16 [nb, H, 4, 4, 2, 4]
+
+(include/latentserve_amd_serving.h says where each channel lies).  A page's heads
+are contiguous; from page to page any stride of whole 16 bytes will do, so the
+pools of several layers may share one allocation.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import NamedTuple, Optional, Tuple
+
+import torch
+
+from latentserve_amd import _lib, _serving
+
+HEAD_DIM = 128
+PAGE = 16
+GROUP = 32
+MAX_NREP = 16
+
+_SHAPES = ((PAGE, 64), (PAGE, 4, 2), (16, PAGE, 4), (4, 4, 2, 4))
+_INNER = ((64, 1), (8, 2, 1), (64, 4, 1), (32, 8, 4, 1))
+_HEAD = (1024, 128, 1024, 128)          # elements of one head's part of a page
+_DTYPES = (torch.uint8, torch.float16, torch.uint8, torch.float16)
+
+
+class Int4Pools(NamedTuple):
+    k_codes: torch.Tensor
+    k_affine: torch.Tensor
+    v_codes: torch.Tensor
+    v_affine: torch.Tensor
+
+
+def empty_pools(num_blocks: int, kv_heads: int, device) -> Int4Pools:
+    """Zeroed pools of num_blocks pages (every entry stands for 0)."""
+    return Int4Pools(*(torch.zeros((num_blocks, kv_heads) + s, dtype=d, device=device)
+                       for s, d in zip(_SHAPES, _DTYPES)))
+
+
+def _pools(pools, written: bool = False):
+    """(num_blocks, heads, C arguments) of checked pools."""
+    if len(pools) != 4:
+        raise ValueError("4-bit pools are (k_codes, k_affine, v_codes, v_affine)")
+    nb, h = pools[0].shape[:2]
+    dev = pools[0].device
+    steps = []
+    for name, t, shape, inner, head, dtype in zip(Int4Pools._fields, pools, _SHAPES, _INNER, _HEAD,
+                                                  _DTYPES):
+        st = t.stride()
+        if t.dtype != dtype or t.shape != (nb, h) + shape:
+            raise ValueError(f"{name} must be {dtype} {(nb, h) + shape}, got {t.dtype} "
+                             f"{tuple(t.shape)}")
+        if t.device != dev:
+            raise ValueError("the pools must be on one device")
+        if st[2:] != inner or (h > 1 and st[1] != head):
+            raise ValueError(f"{name}: a page's heads must be contiguous")
+        if written and nb > 1 and st[0] < h * head:
+            raise ValueError(f"{name}: pages that overlap cannot be written")
+        steps.append(st[0] * t.element_size())
+    return nb, h, (pools[0].data_ptr(), pools[1].data_ptr(), pools[2].data_ptr(),
+                   pools[3].data_ptr(), _lib._I64N[4](*steps), nb)
+
+
+def _rows(name: str, t: torch.Tensor) -> None:
+    if t.dtype != torch.float16:
+        raise ValueError(f"{name} must be float16, got {t.dtype}")
+    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(
+            s % 8 for s, n in zip(t.stride()[:-1], t.shape) if n > 1):
+        raise ValueError(f"{name} rows must be 16-byte aligned and unit-stride")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, which a 4-bit cache does not carry")
+
+
+def _strides(t: torch.Tensor):
+    """The first three strides; a dimension of one row has none that matters."""
+    return _lib._I64N[3](*(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape)))
+
+
+def _tables(block_tables: torch.Tensor, seq_lens: torch.Tensor, b: int, device) -> None:
+    if block_tables.dtype != torch.int32 or seq_lens.dtype != torch.int32 \
+            or block_tables.dim() != 2 or block_tables.stride(-1) != 1 \
+            or (b > 1 and seq_lens.stride(-1) != 1):
+        raise ValueError("block tables [B, pages] and sequence lengths [B] must be unit-stride "
+                         "int32")
+    if block_tables.shape[0] != b or seq_lens.shape != (b,):
+        raise ValueError(f"block tables and sequence lengths must have {b} rows")
+    if block_tables.device != device or seq_lens.device != device:
+        raise ValueError("block tables and sequence lengths must be on the pools' device")
+
+
+def write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, pools) -> None:
+    """k, v [B, H, n, 128] fp16 (any strides of whole 16 bytes) quantized into flat
+    token slots [B * n] int64 (block * 16 + offset; outside the pool: not
+    written).  Slots are distinct.  Other tokens keep their entries."""
+    nb, h, args = _pools(pools, written=True)
+    dev = pools[0].device
+    if k.dim() != 4 or k.shape != v.shape or k.shape[1] != h or k.shape[3] != HEAD_DIM:
+        raise ValueError(f"k and v must be [B, {h}, n, {HEAD_DIM}], got {tuple(k.shape)} and "
+                         f"{tuple(v.shape)}")
+    b, _, n, _ = k.shape
+    if slots.dtype != torch.int64 or slots.shape != (b * n,) \
+            or (b * n > 1 and slots.stride(0) != 1):
+        raise ValueError(f"slots must be {b * n} unit-stride int64 values")
+    if k.device != dev or v.device != dev or slots.device != dev:
+        raise ValueError("k, v and slots must be on the pools' device")
+    stream = _lib.stream_of(dev)
+    if b * n == 0:
+        return
+    _rows("k", k)
+    _rows("v", v)
+    with _serving.on(dev):
+        rc = _serving.lib().ls_int4_write(k.data_ptr(), _strides(k), v.data_ptr(), _strides(v),
+                                          slots.data_ptr(), *args, b, h, n, HEAD_DIM, PAGE, stream)
+    _lib.check(rc, "ls_int4_write")
+
+
+def read(pools, block_tables: torch.Tensor, seq_lens: torch.Tensor,
+         length: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(k, v) [B, H, length, 128] fp16: the values that each sequence's first
+    `length` entries stand for (default: the table's width), zeros past its
+    end.  Views of [B, length, H, 128] buffers, as paged_gather.read's."""
+    nb, h, args = _pools(pools)
+    dev = pools[0].device
+    b = block_tables.shape[0]
+    _tables(block_tables, seq_lens, b, dev)
+    length = block_tables.shape[1] * PAGE if length is None else int(length)
+    if length < 0:
+        raise ValueError(f"length must be >= 0, got {length}")
+    stream = _lib.stream_of(dev)
+    k, v = (torch.empty(b, length, h, HEAD_DIM, dtype=torch.float16, device=dev)
+            for _ in range(2))
+    if b * length:
+        if block_tables.shape[1] == 0:
+            k.zero_(), v.zero_()
+        else:
+            with _serving.on(dev):
+                rc = _serving.lib().ls_int4_read(
+                    *args, block_tables.data_ptr(), block_tables.stride(0),
+                    block_tables.shape[1], seq_lens.data_ptr(), k.data_ptr(), v.data_ptr(), b, h,
+                    HEAD_DIM, PAGE, length, stream)
+            _lib.check(rc, "ls_int4_read")
+    return k.permute(0, 2, 1, 3), v.permute(0, 2, 1, 3)
+
+
+def paged_decode_int4(q: torch.Tensor, pools, block_tables: torch.Tensor, seq_lens: torch.Tensor,
+                      max_seq_len: Optional[int] = None, softmax_scale: Optional[float] = None,
+                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Decode attention over 4-bit pools: q [B, H, n_rep, 128] fp16, n_rep 1..16 ->
+    a new tensor of its shape, or `out`.
+
+    max_seq_len: the longest sequence expected (a graph's bucket); it only sizes
+    the launch, a longer one is attended whole.  Sequences of no tokens give
+    zeros.  Each call has its own scratch, so calls may run at once on several
+    streams and from several graphs."""
+    nb, h, args = _pools(pools)
+    dev = pools[0].device
+    if q.dim() != 4 or q.shape[1] != h or q.shape[3] != HEAD_DIM \
+            or not 1 <= q.shape[2] <= MAX_NREP:
+        raise ValueError(f"q must be [B, {h}, n_rep 1..{MAX_NREP}, {HEAD_DIM}], got "
+                         f"{tuple(q.shape)}")
+    if q.device != dev:
+        raise ValueError("q must be on the pools' device")
+    b, _, n_rep, _ = q.shape
+    _tables(block_tables, seq_lens, b, dev)
+    stream = _lib.stream_of(dev)
+    _rows("q", q)
+    if out is None:
+        out = torch.empty((b, h, n_rep, HEAD_DIM), dtype=torch.float16, device=dev)
+    else:
+        if out.shape != q.shape or out.device != dev:
+            raise ValueError(f"out must be {tuple(q.shape)} on {dev}")
+        _rows("out", out)
+    if b == 0:
+        return out
+    width = block_tables.shape[1]
+    if width == 0:
+        return out.zero_()
+    lib = _serving.lib()
+    bound = 0 if max_seq_len is None else max(1, int(max_seq_len))
+    groups = lib.ls_int4_decode_groups(b, h, width, bound)
+    nbytes = lib.ls_int4_decode_workspace_bytes(groups, h, n_rep)
+    scale = 1.0 / math.sqrt(HEAD_DIM) if softmax_scale is None else float(softmax_scale)
+    with _serving.on(dev):
+        work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        cnt = _serving.counters(dev, stream, lib.ls_int4_decode_counter_ints(groups, h))
+        rc = lib.ls_paged_decode_int4(
+            q.data_ptr(), _strides(q), *args, block_tables.data_ptr(), block_tables.stride(0),
+            width, seq_lens.data_ptr(), out.data_ptr(), _strides(out), work.data_ptr(), nbytes,
+            cnt.data_ptr(), b, h, n_rep, HEAD_DIM, PAGE, groups, scale, stream)
+    _lib.check(rc, "ls_paged_decode_int4")
+    return out

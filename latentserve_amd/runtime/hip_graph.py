@@ -36,6 +36,7 @@ from typing import Dict, Optional, Sequence, Tuple
 import torch
 
 from latentserve_amd.kernels import fused_elementwise as fe
+from latentserve_amd.kernels.logprobs import TokenLogprobs, token_logprobs
 
 DEFAULT_BUCKETS = (1024, 2048, 4096, 8192, 16384, 32768)
 
@@ -47,12 +48,14 @@ class GraphUnsupported(RuntimeError):
 
 def check_capturable(model) -> None:
     """Raise GraphUnsupported unless the model's decode step is capturable."""
+    from latentserve_amd.runtime.int4_cache import Int4PagedKVCache
     from latentserve_amd.runtime.int8_cache import Int8PagedKVCache
     from latentserve_amd.runtime.kv_cache import PagedKVCache
 
     if model.cache is None:
         raise GraphUnsupported("no cache: allocate it before capturing")
-    if not isinstance(model.cache, (PagedKVCache, Int8PagedKVCache)):
+    if not isinstance(model.cache, (PagedKVCache, Int8PagedKVCache,
+                                    Int4PagedKVCache)):
         raise GraphUnsupported(f"{type(model.cache).__name__} has no fixed-address step "
                                "inputs; only the paged caches can be captured")
     if model.rope is None:
@@ -74,14 +77,22 @@ def _pinned_splits(model, splits: Optional[int]):
             layer.attn.num_splits = s
 
 
+def _greedy(logits: torch.Tensor, top: Optional[int]):
+    """(next tokens [B, 1], their TokenLogprobs with `top` alternatives or None)."""
+    last = logits[:, -1, :]
+    nxt = fe.argmax_rows(last)
+    return nxt, None if top is None else token_logprobs(last, nxt[:, 0], top)
+
+
 class CapturedDecode:
     """One recorded decode step for a fixed (batch, bucket, ratio)."""
 
     WARMUP_RUNS = 2
 
     def __init__(self, model, batch_size: int, bucket_tokens: int, num_splits: int,
-                 greedy: bool = False):
+                 greedy: bool = False, logprobs: Optional[int] = None):
         self.model = model
+        self.logprobs = logprobs
         self.batch_size = batch_size
         self.bucket_tokens = bucket_tokens
         self.num_splits = num_splits
@@ -92,13 +103,14 @@ class CapturedDecode:
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.logits_buf: Optional[torch.Tensor] = None
         self.next_buf: Optional[torch.Tensor] = None
+        self.logprobs_buf: Optional[TokenLogprobs] = None
         self.replays = 0
 
     def _forward(self):
         logits = self.model.decode_forward_static(self.ids, self.positions,
                                                   max_position=self.bucket_tokens - 1)
-        nxt = fe.argmax_rows(logits[:, -1, :]) if self.greedy else None
-        return logits, nxt
+        nxt, scores = _greedy(logits, self.logprobs) if self.greedy else (None, None)
+        return logits, nxt, scores
 
     def set_inputs(self, token_ids: torch.Tensor, positions: torch.Tensor) -> None:
         self.ids.copy_(token_ids)
@@ -117,7 +129,7 @@ class CapturedDecode:
             torch.cuda.current_stream().wait_stream(side)
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g, pool=pool):
-                self.logits_buf, self.next_buf = self._forward()
+                self.logits_buf, self.next_buf, self.logprobs_buf = self._forward()
         self.graph = g
 
     def replay(self) -> torch.Tensor:
@@ -134,13 +146,23 @@ class GraphedDecoder:
     `slots` names the cache rows (sequences) of this step; the cache is
     advanced by one token for each.  The returned logits of a graphed step
     are the graph's static buffer, valid until that graph's next replay.
+
+    `logprobs` (with greedy; 0..32): step_greedy() also leaves the chosen tokens'
+    log probabilities, the entropies and that many alternatives in
+    ``last_logprobs`` (a graph's static buffers too).
     """
 
     def __init__(self, model, buckets: Sequence[int] = DEFAULT_BUCKETS,
                  num_splits: Optional[Dict[Tuple[int, int], int]] = None,
-                 enabled: bool = True, greedy: bool = False, policy=None):
+                 enabled: bool = True, greedy: bool = False, policy=None,
+                 logprobs: Optional[int] = None):
+        if logprobs is not None and not greedy:
+            raise ValueError("logprobs are of the greedy steps' tokens: GraphedDecoder(..., "
+                             "greedy=True)")
         self.model = model
         self.greedy = greedy
+        self.logprobs = logprobs
+        self.last_logprobs: Optional[TokenLogprobs] = None
         self.policy = policy
         self.split_overrides = dict(num_splits or {})
         self.enabled = bool(enabled) and torch.cuda.is_available() \
@@ -170,6 +192,8 @@ class GraphedDecoder:
         from latentserve_amd.kernels.gqa.paged_decode import choose_num_splits
 
         c = self.model.cache
+        if not hasattr(c, "k_pool"):
+            return 1                      # (4 bits: the launch is partitioned on the device)
         return choose_num_splits(batch, c.spec.num_kv_heads, bucket, c.block_size,
                                  self.model.device, int8=c.k_pool[0].dtype == torch.int8)
 
@@ -206,7 +230,7 @@ class GraphedDecoder:
         g = self.graphs.get(key)
         if g is None:
             g = CapturedDecode(self.model, batch, bucket, self._splits(batch, bucket),
-                               greedy=self.greedy)
+                               greedy=self.greedy, logprobs=self.logprobs)
             g.set_inputs(token_ids, positions)
             t_cap = time.perf_counter()
             cache.sparse_context_hint = bucket      # selection sized for the bucket's top
@@ -235,8 +259,10 @@ class GraphedDecoder:
             raise RuntimeError("greedy steps need GraphedDecoder(..., greedy=True)")
         logits = self.step(token_ids, positions, slots)
         if self._last_graph is not None:
+            self.last_logprobs = self._last_graph.logprobs_buf
             return self._last_graph.next_buf
-        return fe.argmax_rows(logits[:, -1, :])
+        nxt, self.last_logprobs = _greedy(logits, self.logprobs)
+        return nxt
 
     def stats(self) -> dict:
         def order(k):

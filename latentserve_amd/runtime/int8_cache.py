@@ -127,6 +127,20 @@ class Int8PagedKVCache(_PagedBase):
         for layer in self._pooled:
             layer[index] = len(blocks)
 
+    def _page_tensors(self) -> List[torch.Tensor]:
+        return (self.k_pool + self.v_pool + self.k_scale_pool + self.v_scale_pool
+                + self.k_zero_pool + self.v_zero_pool)
+
+    def fork(self, index: int, children: Sequence[int]) -> None:
+        """As the fp16 cache; the last page's K, which only the residual holds, is
+        copied to the children's rows at once."""
+        children = list(children)
+        super().fork(index, children)
+        self._copy_rows(self._residual, [index] * len(children), children)
+        for layer in self._pooled:
+            for c in children:
+                layer[c] = layer[index]
+
     def reset(self) -> None:
         super().reset()
         for layer in self._pooled:

@@ -24,7 +24,7 @@ few list operations and one small copy.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Callable, Iterable, List, Optional, Sequence
+from typing import Callable, Dict, Iterable, List, Optional, Sequence
 
 import numpy as np
 import torch
@@ -63,6 +63,8 @@ class BlockAllocator:
         self.reclaimer: Optional[Callable[[int], object]] = None
         self.reclaimable: Optional[Callable[[], int]] = None
         self.on_ref_change: Optional[Callable[[int, int, int], None]] = None
+        # told of compact()'s moves, {old block: new block}, once they are made
+        self.on_move: Optional[Callable[[Dict[int, int]], None]] = None
         self.reset()
 
     def reset(self) -> None:
@@ -135,6 +137,22 @@ class BlockAllocator:
                 self._stack.append(b)
             if self.on_ref_change is not None:
                 self.on_ref_change(b, self._refs[b] + 1, self._refs[b])
+
+    def compacting_moves(self) -> Dict[int, int]:
+        """{old: new}, ascending: the held blocks past the pool's first num_used go to
+        its free ones below, after which the held blocks are 0 .. num_used - 1."""
+        n = self.num_used
+        low = [b for b in range(n) if self._refs[b] == 0]
+        return dict(zip((b for b in range(n, self.num_blocks) if self._refs[b]), low))
+
+    def move(self, moves: Dict[int, int]) -> None:
+        """Renumber held blocks (their contents have been copied): counts move along,
+        the free blocks are handed out lowest first again."""
+        for old, new in moves.items():
+            self._refs[new], self._refs[old] = self._refs[old], 0
+        self._stack = [b for b in range(self.num_blocks - 1, -1, -1) if self._refs[b] == 0]
+        if self.on_move is not None:
+            self.on_move(moves)
 
     def ref_count(self, block: int) -> int:
         return self._refs[block]
@@ -367,6 +385,98 @@ class _PagedBase:
         prefix cache may hand them to another sequence."""
         return self.tables[index].length // self.block_size
 
+    # ---- branching and compaction -------------------------------------------
+    def _page_tensors(self) -> List[torch.Tensor]:
+        """Every tensor indexed by block, all layers'."""
+        raise NotImplementedError
+
+    def _copy_rows(self, tensors: Sequence[torch.Tensor], src: Sequence[int],
+                   dst: Sequence[int]) -> None:
+        if not src:
+            return
+        if self.device.type == "cuda":
+            from latentserve_amd.kernels.hip import page_copy as pc
+            pc.copy_pages(tensors, src, dst)
+        else:
+            for t in tensors:
+                t[list(dst)] = t[list(src)]
+
+    def fork(self, index: int, children: Sequence[int]) -> None:
+        """Branch the sequence in slot `index` into the empty slots `children`: each
+        holds the same tokens, on the same pages, and grows its own way from
+        there.  Nothing is copied now: a page that several sequences hold is
+        copied when one of them is about to write it (advance()).  Between
+        steps only: the tokens of the last advance() must have been written."""
+        children = list(children)
+        t = self.tables[index]
+        if len(set(children)) != len(children):
+            raise ValueError(f"slots {children}: a child is named twice")
+        for c in children:
+            if self.tables[c].length or self.tables[c].blocks:
+                raise ValueError(f"slot {c} already holds a sequence")
+        pages = t.blocks[:self.allocator.blocks_for_tokens(t.length)]
+        for c in children:
+            child = self.tables[c]
+            self.allocator.incref(pages)
+            child.blocks = list(pages)
+            child.length = t.length
+            child.version += 1
+            child.lineage += 1
+
+    def _own_pages(self, seqs: Sequence[int], n: int) -> None:
+        """Before n tokens are written: the pages they go to that other sequences
+        (or a prefix cache) hold too are replaced by pages of their own, with
+        the tokens they keep."""
+        bs, refs = self.block_size, self.allocator.ref_count
+        todo, left = [], {}
+        for s in seqs:
+            t = self.tables[s]
+            first = t.length // bs
+            for page in range(first, min(len(t.blocks), -(-(t.length + n) // bs))):
+                blk = t.blocks[page]
+                count = left.get(blk, refs(blk))
+                if count > 1:
+                    left[blk] = count - 1              # the last to write keeps the page
+                    todo.append((t, page, blk, page == first and t.length % bs > 0))
+        if not todo:
+            return
+        fresh = self.allocator.allocate(len(todo))     # (OutOfBlocks: nothing has changed)
+        kept = [(blk, new) for (_, _, blk, keeps), new in zip(todo, fresh) if keeps]
+        self._copy_rows(self._page_tensors(), [a for a, _ in kept], [b for _, b in kept])
+        for (t, page, blk, _), new in zip(todo, fresh):
+            t.blocks[page] = new
+            t.version += 1
+            t.lineage += 1
+        self.allocator.free([blk for _, _, blk, _ in todo])
+
+    def compact(self) -> Dict[int, int]:
+        """Move the held pages to the pool's lowest blocks, so that they are blocks
+        0 .. num_used - 1 (one slice a tensor to save, send or trim), and
+        renumber them in the tables and the prefix cache.  Returns the moves, {old
+        block: new block}, for holders the cache does not know.  Between
+        steps only, as fork(); captured graphs stay valid."""
+        moves = self.allocator.compacting_moves()
+        if moves:
+            self._copy_rows(self._page_tensors(), list(moves), list(moves.values()))
+            for t in self.tables:
+                if any(b in moves for b in t.blocks):
+                    t.blocks = [moves.get(b, b) for b in t.blocks]
+                    t.version += 1
+                    t.lineage += 1
+            self.allocator.move(moves)
+            if self._batch:
+                self._publish(0, [self.tables[s].length for s in self._active])
+        return moves
+
+    def _shorten(self, length: int, seqs: Sequence[int]) -> None:
+        for s in seqs:
+            t = self.tables[s]
+            if not 0 <= length <= t.length:
+                raise ValueError(f"slot {s} holds {t.length} tokens; cannot rewind it to "
+                                 f"{length}")
+        for s in seqs:
+            self.tables[s].length = length
+
     def reset(self) -> None:
         """Forget every sequence; storage (and every address a graph holds)
         is kept."""
@@ -387,6 +497,7 @@ class _PagedBase:
         elif batch_size is not None:
             self.set_active(range(batch_size))
         starts = [self.tables[s].length for s in self._active]
+        self._own_pages(self._active, n)
         for s in self._active:
             self.tables[s].append(n)
         return starts
@@ -465,6 +576,9 @@ class PagedKVCache(_PagedBase):
         self.kmin: Optional[List[torch.Tensor]] = None
         self.kmax: Optional[List[torch.Tensor]] = None
 
+    def _page_tensors(self) -> List[torch.Tensor]:
+        return self.k_pool + self.v_pool + (self.kmin or []) + (self.kmax or [])
+
     def advance(self, n: int, batch_size: Optional[int] = None,
                 slots: Optional[Sequence[int]] = None) -> None:
         """Reserve n more tokens for each active sequence (paged_cache.py:
@@ -476,14 +590,16 @@ class PagedKVCache(_PagedBase):
         """Shorten sequences to `length` tokens, keeping their pages
         (paged_cache.py:273-303): growing again lands on the same slots."""
         seqs = self._active if slots is None else list(slots)
-        for s in seqs:
-            t = self.tables[s]
-            if not 0 <= length <= t.length:
-                raise ValueError(f"slot {s} holds {t.length} tokens; cannot rewind it to "
-                                 f"{length}")
-        for s in seqs:
-            self.tables[s].length = length
-            if self.kmin is not None and length % self.block_size:
+        before = [self.tables[s].length for s in seqs]
+        self._shorten(length, seqs)
+        if self.kmin is not None and length % self.block_size:
+            try:
+                self._own_pages(seqs, 0)      # (its bounds change: no one else's may)
+            except OutOfBlocks:
+                for s, n in zip(seqs, before):
+                    self.tables[s].length = n
+                raise
+            for s in seqs:
                 self._bound_partial_page(s, length)
         self._publish(0, [self.tables[s].length for s in self._active])
 

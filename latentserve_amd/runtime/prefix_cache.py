@@ -76,6 +76,7 @@ class PrefixCache:
         allocator.reclaimer = self.reclaim
         allocator.reclaimable = self.num_reclaimable
         allocator.on_ref_change = self._count_change
+        allocator.on_move = self._renumber
 
     # ---- the allocator's hooks -------------------------------------------
     def _count_change(self, block: int, old: int, new: int) -> None:
@@ -86,6 +87,12 @@ class PrefixCache:
                 self._alone += 1
             elif (old, new) == (1, 2):
                 self._alone -= 1
+
+    def _renumber(self, moves: Dict[int, int]) -> None:
+        """The pool was compacted: recorded pages under their new numbers."""
+        self.entry = {moves.get(b, b): e for b, e in self.entry.items()}
+        self.by_key = {k: moves.get(b, b) for k, b in self.by_key.items()}
+        self.lru = OrderedDict((moves.get(b, b), None) for b in self.lru)
 
     def num_reclaimable(self) -> int:
         return self._alone

@@ -29,8 +29,10 @@ import torch.nn.functional as F
 
 from latentserve_amd.kernels import decode_gemm as dg
 from latentserve_amd.kernels import fused_elementwise as fe
+from latentserve_amd.kernels.hip import int4_cache as i4
 from latentserve_amd.kernels.hip import paged_decode_hip as pdh
 from latentserve_amd.kernels.hip import paged_sparse as ps
+from latentserve_amd.runtime.int4_cache import Int4PagedKVCache
 from latentserve_amd.runtime.int8_cache import Int8PagedKVCache
 from latentserve_amd.runtime.kv_cache import KVCacheSpec, PagedKVCache
 
@@ -168,17 +170,18 @@ class QwenDecoder:
     def allocate_cache(self, max_batch_size: int, max_seq_len: int,
                        num_blocks: Optional[int] = None, kv_dtype: str = "fp16",
                        asymmetric: bool = False):
-        """A paged cache for this model: fp16 (PagedKVCache) or INT8
+        """A paged cache for this model: fp16 (PagedKVCache), INT8
         (Int8PagedKVCache: int8 pools, fp32 scales, the fp16 last-page K
-        residual)."""
+        residual) or 4 bits (Int4PagedKVCache)."""
         spec = KVCacheSpec(num_layers=self.cfg.num_layers, num_kv_heads=self.cfg.num_kv_heads,
                            head_dim=self.cfg.head_dim, max_batch_size=max_batch_size,
                            max_seq_len=max_seq_len, device=str(self.device))
         if kv_dtype == "fp16":
             self.cache = PagedKVCache(spec, num_blocks=num_blocks)
             self._stage = None
-        elif kv_dtype == "int8":
-            self.cache = Int8PagedKVCache(spec, num_blocks=num_blocks, asymmetric=asymmetric)
+        elif kv_dtype in ("int8", "int4"):
+            self.cache = Int4PagedKVCache(spec, num_blocks=num_blocks) if kv_dtype == "int4" \
+                else Int8PagedKVCache(spec, num_blocks=num_blocks, asymmetric=asymmetric)
             # the decode token's rotated K and its V are stored here by the
             # q/k/v launch (one 16-row block per sequence, row 0), then
             # quantized into the cache by its write
@@ -188,7 +191,7 @@ class QwenDecoder:
                 torch.zeros(max_batch_size, 16, hk, hd, dtype=torch.float16, device=self.device),
                 torch.arange(max_batch_size, dtype=torch.long, device=self.device) * 16)
         else:
-            raise ValueError(f"kv_dtype must be 'fp16' or 'int8', got {kv_dtype!r}")
+            raise ValueError(f"kv_dtype must be 'fp16', 'int8' or 'int4', got {kv_dtype!r}")
         self.rope = Rope(self.cfg.head_dim, self.cfg.rope_theta, max_seq_len, self.device)
         return self.cache
 
@@ -200,6 +203,8 @@ class QwenDecoder:
         if ratio is not None:
             if isinstance(self.cache, Int8PagedKVCache):
                 raise ValueError("sparse decode reads fp16 pools; this cache is INT8")
+            if isinstance(self.cache, Int4PagedKVCache):
+                raise ValueError("sparse decode reads fp16 pools; this cache is in 4 bits")
             self.cache.enable_page_bounds()
         self.sparse_ratio = ratio
         for layer in self.layers:
@@ -219,11 +224,12 @@ class QwenDecoder:
         eps = cfg.rms_norm_eps
         tables = cache.block_tables_tensor(b)
         lens = cache.seq_lens_tensor(b)
-        int8 = self._stage is not None
-        if int8:
+        staged = self._stage is not None               # quantized by the cache's write
+        int4 = isinstance(cache, Int4PagedKVCache)
+        if staged:
             stage_k, stage_v, stage_slots = self._stage
             slots = stage_slots[:b]
-            res_rows = cache.residual_rows_tensor(b)
+            res_rows = None if int4 else cache.residual_rows_tensor(b)
         else:
             slots = cache.write_slots(b)
         pos = positions.reshape(b)
@@ -251,7 +257,7 @@ class QwenDecoder:
             # (and the page bounds) and q folded to [B, hk, n_rep, hd]: one
             # launch at decode batch sizes (the projection's epilogue)
             wq = layer.p_qkv if layer.p_qkv is not None else layer.w_qkv
-            kdst, vdst = (stage_k, stage_v) if int8 else (cache.k_pool[li], cache.v_pool[li])
+            kdst, vdst = (stage_k, stage_v) if staged else (cache.k_pool[li], cache.v_pool[li])
             if fold1:
                 _, residual = dg.qkv_rope_write(
                     x, wq, layer.b_qkv, pos, self.rope.cos, self.rope.sin, slots,
@@ -266,9 +272,15 @@ class QwenDecoder:
                 qkv = F.linear(h, layer.w_qkv, layer.b_qkv)       # [B, (hq + 2 hk) hd]
                 fe.rope_write_decode(qkv, pos, self.rope.cos, self.rope.sin, slots,
                                      kdst, vdst, hq, hk, q_out=q, kmin=kmin, kmax=kmax)
-            if int8:
-                # V quantized into the pool, K into the sequence's residual row
+            if staged:
+                # INT8: V quantized into the pool, K into the sequence's residual row;
+                # 4 bits: both into the pools
                 cache.write(li, stage_k[:b, :1].transpose(1, 2), stage_v[:b, :1].transpose(1, 2))
+            if int4:
+                i4.paged_decode_int4(q, cache.pools[li], tables, lens,
+                                     max_seq_len=max_position + 1, softmax_scale=self.scale,
+                                     out=o)
+            elif staged:
                 pdh.paged_decode_hip(
                     q, cache.k_pool[li], cache.v_pool[li], tables, lens,
                     max_seq_len=max_position + 1, num_splits=layer.attn.num_splits,

@@ -7,20 +7,21 @@
 //    runs, one a workgroup, from the lengths on the device (one fixed grid serves
 //    growing sequences under graph replay, and ragged batches balance without a
 //    deal).  A run that crosses sequences takes them one after the other; a
-//    sequence that crosses runs leaves one record a run (acc, m, l), and the last
-//    of its groups to arrive merges them: one launch.
-//  * A wave takes a page at a time.  QK: S^T[16 tok x 16 rows] = K . Q^T, four
-//    16x16x32 MFMAs (one a channel group); PV: O^T[128 ch x 16 rows] += V^T . P^T,
-//    eight 16x16x16 MFMAs.  The QK result is already the PV operand's layout, as
+//    sequence that crosses runs leaves one record a run (acc, m, l), merged by the
+//    last of its groups to arrive (over 16 runs: by the last of each 16, then the
+//    last of those): one launch.
+//  * The waves of a group claim pairs of pages.  QK: S^T[32 tok x 16 rows] = K . Q^T,
+//    eight 16x16x32 MFMAs (one a channel group and page); PV: O^T[128 ch x 16 rows]
+//    += V^T . P^T, eight more.  The QK result is already the PV operand's layout, as
 //    in the fp16 walk (ls_decode.hip).
-//  * Codes to fp16: two of a word's codes at once are masked under the exponent
+//  * Codes to fp16: two of a word's codes at once are spliced under the exponent
 //    of 1024.0h (bits 0..3 of a half) or 64.0h (bits 4..7), the bias subtracted
 //    exactly, then one packed fused multiply-add gives fp16(m + s * code).  V's
 //    words of two tokens are first spliced by halves, so that a pair is two tokens
 //    of one channel, the operand V^T needs.
-//  * Online softmax in the log2 domain; rows whose maximum did not move skip the
-//    rescale.  Sums and maxima are fp32; the weights are rounded to fp16 for the
-//    MFMA as the fp16 walk rounds them.
+//  * Online softmax in the log2 domain; a step in which no row's maximum moved skips
+//    the rescale.  Maxima and sums are fp32; the weights are rounded to fp16 for the
+//    MFMA as the fp16 walk rounds them, and summed as rounded, by an MFMA with ones.
 
 #include "ls_common.h"
 #include "ls_serving.h"
@@ -32,15 +33,20 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 constexpr float I4_LOG2E = 1.4426950408889634f;
 constexpr int I4_NW = 4;                 // waves a group
 constexpr int I4_ROW = HEAD_DIM + 4;     // LDS row: 16 rows written at once fall in different banks
-// Fewest pages a group takes: one a wave.
-constexpr int I4_MIN_PAGES = I4_NW;
-// Groups resident at once on the 256 CUs.
-constexpr int I4_RESIDENT = 256 * 2;
+constexpr int I4_RESIDENT = 512;         // groups resident at once: two a CU
+// Fewest pages a run has: a pair a wave.
+constexpr int I4_MIN_PAGES = 2 * I4_NW;
+// Pages whose blocks a group holds in LDS at once.
+constexpr int I4_TABLE = 2048;
+// Records that one group merges.
+constexpr int I4_CLUSTER = 16;
 
 struct Int4Smem {
     float m[I4_NW][MAX_NREP];
     float l[I4_NW][MAX_NREP];
     alignas(16) float acc[I4_NW][MAX_NREP][I4_ROW];
+    alignas(8) int blk[I4_TABLE];
+    int claim;
     int is_last;
 };
 
@@ -50,20 +56,33 @@ struct Int4Page {
 
 struct Int4State {
     f4 acc[8];    // O^T tile e: row c, channels 8 (4 g + i) + e
-    float m, l;   // running maximum of row c (log2 units), lane-partial sum
+    f4 l;         // the sum of row c's weights, in every element and lane group
+    float m;      // running maximum of row c (log2 units)
 };
 
 __device__ __forceinline__ h2 as_h2(uint32_t x) { return __builtin_bit_cast(h2, x); }
+__device__ __forceinline__ uint32_t bits(h2 v) { return __builtin_bit_cast(uint32_t, v); }
+
+// The splice's constants in registers (masks scalar, exponents vector), where one
+// v_and_or_b32 takes both; as literals each would be an instruction of its own.
+struct Splice {
+    uint32_t lo, hi, e1024, e64;
+};
+__device__ __forceinline__ Splice make_splice() {
+    Splice s = {0x000F000Fu, 0x00F000F0u, 0x64006400u, 0x54005400u};
+    asm("" : "+s"(s.lo), "+s"(s.hi), "+v"(s.e1024), "+v"(s.e64));
+    return s;
+}
 
 // Four pairs of codes: pair i is codes i and i + 4 of the word (of each half of
 // the dword), as fp16, exactly.
-__device__ __forceinline__ void code_pairs(uint32_t x, h2 (&p)[4]) {
+__device__ __forceinline__ void code_pairs(const Splice& k, uint32_t x, h2 (&p)[4]) {
     const h2 b1024 = {(half_t)1024.f, (half_t)1024.f}, b64 = {(half_t)64.f, (half_t)64.f};
     const uint32_t y = x >> 8;
-    p[0] = as_h2((x & 0x000F000Fu) | 0x64006400u) - b1024;
-    p[1] = as_h2((x & 0x00F000F0u) | 0x54005400u) - b64;
-    p[2] = as_h2((y & 0x000F000Fu) | 0x64006400u) - b1024;
-    p[3] = as_h2((y & 0x00F000F0u) | 0x54005400u) - b64;
+    p[0] = as_h2((x & k.lo) | k.e1024) - b1024;
+    p[1] = as_h2((x & k.hi) | k.e64) - b64;
+    p[2] = as_h2((y & k.lo) | k.e1024) - b1024;
+    p[3] = as_h2((y & k.hi) | k.e64) - b64;
 }
 
 __device__ __forceinline__ h2 splat_lo(uint32_t x) {
@@ -74,7 +93,10 @@ __device__ __forceinline__ h2 splat_hi(uint32_t x) {
     const h2 v = as_h2(x);
     return (h2){v[1], v[1]};
 }
-__device__ __forceinline__ uint32_t bits(h2 v) { return __builtin_bit_cast(uint32_t, v); }
+
+__device__ __forceinline__ f4 mfma32(u4 a, h8 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), b, c, 0, 0, 0);
+}
 
 // blk < 0: zeros, without a memory request.
 __device__ __forceinline__ void int4_load(const Int4DecodeParams& a, Int4Page& d, int blk, int h,
@@ -88,83 +110,104 @@ __device__ __forceinline__ void int4_load(const Int4DecodeParams& a, Int4Page& d
     d.va = page_load16(page_rsrc(a.p.affine[1] + bk * a.p.sa[1] + ha, fetch), 64 * (c / 4) + 16 * g);
 }
 
-// The page's first token is tok0; tokens at or past len do not count.
-__device__ __forceinline__ void int4_compute(const Int4Page& d, Int4State& st, const h8 (&q)[4],
-                                             int tok0, int len, float scale_log2, int g) {
-    f4 s = {0.f, 0.f, 0.f, 0.f};
+// Two adjacent pages, the first one's first token tok0; token tok0 + i counts if it is
+// below len[i / 16].  scale >= 0.
+__device__ __forceinline__ void int4_compute(const Splice& sp, const Int4Page (&d)[2],
+                                             Int4State& st, const h8 (&q)[4], int tok0,
+                                             const int (&len)[2], float scale, int g) {
+    f4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        h2 p[4];
-        code_pairs(d.kc[j], p);
-        const h2 ks = splat_lo(d.ka[j]), km = splat_hi(d.ka[j]);
-        u4 w;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = bits(__builtin_elementwise_fma(p[i], ks, km));
-        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, w), q[j], s, 0, 0, 0);
+        for (int z = 0; z < 2; ++z) {
+            h2 p[4];
+            code_pairs(sp, d[z].kc[j], p);
+            const h2 ks = splat_lo(d[z].ka[j]), km = splat_hi(d[z].ka[j]);
+            u4 w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = bits(__builtin_elementwise_fma(p[i], ks, km));
+            s[z] = mfma32(w, q[j], s[z]);
+        }
     }
 
-    const int t0 = tok0 + 4 * g;
-    float x[4];
-    float mloc = neg_inf();
+    u4 va[2] = {d[0].va, d[1].va};
+    // (the same in every lane)
+    if (tok0 + PAGE > len[0] || tok0 + 2 * PAGE > len[1]) {
+        const int t0 = tok0 + 4 * g;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        x[i] = t0 + i < len ? s[i] * scale_log2 : neg_inf();
-        mloc = fmaxf(mloc, x[i]);
-    }
-    const float m_new = fmaxf(st.m, group4_max(mloc));
-    const bool dead = m_new == neg_inf();      // nothing valid yet in this row
-    const float alpha = dead ? 0.f : fast_exp2(st.m - m_new);
-    float psum = 0.f;
-    h4 pb;
+        for (int z = 0; z < 2; ++z) {
+            const int t = t0 + 16 * z, n = len[z];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float p = dead ? 0.f : fast_exp2(x[i] - m_new);
-        psum += p;
-        pb[i] = (half_t)p;
+            for (int i = 0; i < 4; ++i) s[z][i] = t + i < n ? s[z][i] : neg_inf();
+            // tokens past the end may hold anything, NaN steps included: entry 0
+            // (a weight of 0 does not remove a NaN)
+            const uint32_t m01 = (t < n ? 0xFFFFu : 0u) | (t + 1 < n ? 0xFFFF0000u : 0u);
+            const uint32_t m23 = (t + 2 < n ? 0xFFFFu : 0u) | (t + 3 < n ? 0xFFFF0000u : 0u);
+            va[z].x &= m01;
+            va[z].y &= m23;
+            va[z].z &= m01;
+            va[z].w &= m23;
+        }
     }
-    st.l = st.l * alpha + psum;
-    st.m = m_new;
+    float top = fmaxf(fmaxf(s[0][0], s[0][1]), s[0][2]);
+    top = fmaxf(fmaxf(top, s[0][3]), s[1][0]);
+    top = fmaxf(fmaxf(top, s[1][1]), fmaxf(s[1][2], s[1][3]));
+    top = group4_max(top);
+    // (a row of -inf only, nothing valid yet: -inf also where scale is 0)
+    const float m_new = fmaxf(st.m, top == neg_inf() ? top : top * scale);
+    const float m_use = m_new == neg_inf() ? 0.f : m_new;
+    const float alpha = fast_exp2(st.m - m_use);
+    h8 pb;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float x = s[i / 4][i % 4];
+        pb[i] = (half_t)fast_exp2(x == neg_inf() ? x : __builtin_fmaf(x, scale, -m_use));
+    }
     if (__any(alpha != 1.f)) {
+        st.l *= alpha;
 #pragma unroll
         for (int t = 0; t < 8; ++t) st.acc[t] *= alpha;
     }
+    st.m = m_new;
+    constexpr uint32_t ONES = 0x3C003C00u;
+    st.l = mfma32((u4){ONES, ONES, ONES, ONES}, pb, st.l);
 
-    u4 va = d.va;
-    if (tok0 + PAGE > len) {
-        // tokens past the end may hold anything, NaN steps included: entry 0
-        // (a weight of 0 does not remove a NaN)
-        const uint32_t m01 = (t0 < len ? 0xFFFFu : 0u) | (t0 + 1 < len ? 0xFFFF0000u : 0u);
-        const uint32_t m23 = (t0 + 2 < len ? 0xFFFFu : 0u) | (t0 + 3 < len ? 0xFFFF0000u : 0u);
-        va.x &= m01;
-        va.y &= m23;
-        va.z &= m01;
-        va.w &= m23;
-    }
-    const h2 s01 = as_h2(va.x), s23 = as_h2(va.y), m01 = as_h2(va.z), m23 = as_h2(va.w);
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
         // this half's four codes of tokens 4g, 4g + 1 (and 4g + 2, 4g + 3)
         const uint32_t sel = half ? 0x07060302u : 0x05040100u;
-        h2 p01[4], p23[4];
-        code_pairs(__builtin_amdgcn_perm(d.vc.y, d.vc.x, sel), p01);
-        code_pairs(__builtin_amdgcn_perm(d.vc.w, d.vc.z, sel), p23);
+        u4 w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const h2 v01 = __builtin_elementwise_fma(p01[i], s01, m01);
-            const h2 v23 = __builtin_elementwise_fma(p23[i], s23, m23);
-            const int e = 4 * half + i;
-            st.acc[e] = mfma16(as_h4(bits(v01), bits(v23)), pb, st.acc[e]);
+        for (int z = 0; z < 2; ++z) {
+            h2 p01[4], p23[4];
+            code_pairs(sp, __builtin_amdgcn_perm(d[z].vc.y, d[z].vc.x, sel), p01);
+            code_pairs(sp, __builtin_amdgcn_perm(d[z].vc.w, d[z].vc.z, sel), p23);
+            const h2 s01 = as_h2(va[z].x), s23 = as_h2(va[z].y), m01 = as_h2(va[z].z),
+                     m23 = as_h2(va[z].w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i][2 * z] = bits(__builtin_elementwise_fma(p01[i], s01, m01));
+                w[i][2 * z + 1] = bits(__builtin_elementwise_fma(p23[i], s23, m23));
+            }
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st.acc[4 * half + i] = mfma32(w[i], pb, st.acc[4 * half + i]);
     }
 }
 
-__device__ __forceinline__ int wave_incl_scan(int x, int lane) {
-#pragma unroll
-    for (int o = 1; o < WAVE; o <<= 1) {
-        const int y = __shfl_up(x, o);
-        if (lane >= o) x += y;
-    }
-    return x;
+// Inclusive prefix sum over the wave's lanes, and its total: rows of 16 lanes by DPP
+// row shifts (a lane whose source is outside its row adds 0), then the rows' totals.
+template <int CTRL>
+__device__ __forceinline__ int dpp_add(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, false);
+}
+__device__ __forceinline__ int wave_incl_scan(int x, int lane, int& total) {
+    x = dpp_add<0x118>(dpp_add<0x114>(dpp_add<0x112>(dpp_add<0x111>(x))));
+    const int r0 = __builtin_amdgcn_readlane(x, 15), r1 = __builtin_amdgcn_readlane(x, 31),
+              r2 = __builtin_amdgcn_readlane(x, 47), r3 = __builtin_amdgcn_readlane(x, 63);
+    total = r0 + r1 + r2 + r3;
+    const int row = lane >> 4;
+    return x + (row > 0 ? r0 : 0) + (row > 1 ? r1 : 0) + (row > 2 ? r2 : 0);
 }
 
 __device__ __forceinline__ void store_coherent(float* p, f4 v) {
@@ -177,6 +220,68 @@ __device__ __forceinline__ void store_coherent(float* p, float x, float y) {
     asm volatile("global_store_dwordx2 %0, %1, off sc1" : : "v"(p), "v"(v) : "memory");
 }
 
+// The records of a sequence of a KV head: its first group's among those of sequences
+// that start in their group, the others' among those that go on.
+struct Int4Records {
+    float* work;              // this head's
+    int row_bytes;            // of a group's heads (the workspace is below 2^31 bytes)
+    int groups, first;
+    __device__ __forceinline__ int at(int k) const {
+        return (k == 0 ? first : groups + first + k) * row_bytes;
+    }
+};
+
+// Rows of the records k0, k0 + step, ... (S of them) merged by half-waves (lane j:
+// channels 4 j .. 4 j + 3).  A round takes up to 16: lane j reads m and l of record j
+// and its weight goes to the others by readlane, so every load of a round is requested
+// at once.  The result goes to out, or (out null) to record k0.
+__device__ __forceinline__ void merge_records(const Int4Records& R, int k0, int step, int S, int NR,
+                                              half_t* out, int64_t so_r) {
+    const int j = threadIdx.x % 32, d0 = 4 * j;
+    const bool upper = (threadIdx.x & 32) != 0;
+    const __amdgpu_buffer_rsrc_t rs = coherent_rsrc(wave_uniform(R.work));
+    for (int r = threadIdx.x / 32; r < NR; r += I4_NW * 2) {
+        float mg = neg_inf(), lt = 0.f;
+        f4 acc = {0.f, 0.f, 0.f, 0.f};
+        const int vo_a = (r * HEAD_DIM + d0) * (int)sizeof(float);
+        const int vo_m = (NR * HEAD_DIM + 2 * r) * (int)sizeof(float);
+        for (int i0 = 0; i0 < S; i0 += I4_CLUSTER) {
+            const int n = S - i0 < I4_CLUSTER ? S - i0 : I4_CLUSTER;      // the same in every lane
+            const uint64_t ml = load_coherent8(rs, vo_m + R.at(k0 + step * (i0 + (j < n ? j : n - 1))), 0);
+            f4 av[I4_CLUSTER];
+#pragma unroll
+            for (int i = 0; i < I4_CLUSTER; ++i)
+                av[i] = load_coherent4(rs, vo_a, R.at(k0 + step * (i0 + (i < n ? i : n - 1))));
+            const float mj = j < n ? __builtin_bit_cast(float, (uint32_t)ml) : neg_inf();
+            const float cm = fmaxf(half_max(mj), mg);
+            const bool none = cm == neg_inf();
+            const float sc = none ? 1.f : fast_exp2(mg - cm);
+            const float wj = none || j >= n ? 0.f : fast_exp2(mj - cm);
+            lt = lt * sc + half_sum(wj * __builtin_bit_cast(float, (uint32_t)(ml >> 32)));
+            acc *= sc;
+#pragma unroll
+            for (int i = 0; i < I4_CLUSTER; ++i) {
+                const float w0 = __builtin_bit_cast(
+                    float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wj), i));
+                const float w1 = __builtin_bit_cast(
+                    float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wj), 32 + i));
+                acc += av[i] * (upper ? w1 : w0);
+            }
+            mg = cm;
+        }
+        if (out) {
+            const float inv = 1.f / fmaxf(lt, 1e-20f);
+            half_t* o = out + (int64_t)r * so_r + d0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = (half_t)(acc[e] * inv);
+        } else {
+            float* rk = (float*)((char*)R.work + R.at(k0));
+            store_coherent(rk + r * HEAD_DIM + d0, acc);
+            if (j == 0) store_coherent(rk + NR * HEAD_DIM + 2 * r, mg, lt);
+        }
+    }
+}
+
 __global__ __launch_bounds__(WAVE* I4_NW) __attribute__((amdgpu_waves_per_eu(2)))
 void int4_decode_kernel(const Int4DecodeParams a) {
     __shared__ Int4Smem sm;
@@ -187,31 +292,49 @@ void int4_decode_kernel(const Int4DecodeParams a) {
     const int w = u / H, h = u - w * H;          // this group's run and head
 
     // ---- its run of the head's page list, and the sequence that run starts in ----
-    // (a sequence of no tokens counts one page, which nobody reads: its group
-    // stores the zeros)
-    auto units_of = [&](int len) {
+    // A sequence weighs its pages and `extra` (what starting on it costs a group, in
+    // pages), which lie before them.  (One of no tokens counts a page, which nobody
+    // reads: its group stores the zeros.)
+    const int extra = a.extra;
+    auto pages_of = [&](int len) {
         int p = len > 0 ? (len + PAGE - 1) / PAGE : 1;
         return p < a.max_pages ? p : a.max_pages;
     };
-    const int per_lane = (a.B + WAVE - 1) / WAVE;
-    const int b0 = lane * per_lane < a.B ? lane * per_lane : a.B;
-    const int b1 = b0 + per_lane < a.B ? b0 + per_lane : a.B;
-    int mine = 0;
-    for (int i = b0; i < b1; ++i) mine += units_of(a.lens[i]);
-    const int incl = wave_incl_scan(mine, lane);
-    const int T = __builtin_amdgcn_readlane(incl, WAVE - 1);
-    int per = (T + a.groups - 1) / a.groups;
-    per = per > I4_MIN_PAGES ? per : I4_MIN_PAGES;
-    if ((int64_t)w * per >= T) return;           // (every wave alike, before any barrier)
-    const int u0 = w * per, u1 = T - u0 < per ? T : u0 + per;
-    int b = 0, P = 0, len = 0;
-    {
-        int pos = incl - mine;
+    auto run_of = [&](int T, int& u0, int& u1) {
+        int per = (T + a.groups - 1) / a.groups;
+        per = per > I4_MIN_PAGES ? per : I4_MIN_PAGES;
+        u0 = (int64_t)w * per < T ? w * per : T;
+        u1 = T - u0 < per ? T : u0 + per;
+        return per;
+    };
+    int per, b, P, len, u0, u1;          // weight of a run; the sequence, its start, length
+    if (a.B <= WAVE) {
+        // one sequence a lane
+        const int li = lane < a.B ? a.lens[lane] : 0;
+        const int n = lane < a.B ? pages_of(li) + extra : 0;
+        int T;
+        const int incl = wave_incl_scan(n, lane, T);
+        per = run_of(T, u0, u1);
+        if (u0 >= T) return;                         // (every wave alike, before any barrier)
+        b = __builtin_ctzll(__ballot(u0 < incl));    // (lanes past the batch hold T)
+        P = __builtin_amdgcn_readlane(incl - n, b);
+        len = __builtin_amdgcn_readlane(li, b);
+    } else {
+        // a run of sequences a lane
+        const int per_lane = (a.B + WAVE - 1) / WAVE;
+        const int b0 = lane * per_lane < a.B ? lane * per_lane : a.B;
+        const int b1 = b0 + per_lane < a.B ? b0 + per_lane : a.B;
+        int mine = 0;
+        for (int i = b0; i < b1; ++i) mine += pages_of(a.lens[i]) + extra;
+        int T;
+        const int incl = wave_incl_scan(mine, lane, T);
+        per = run_of(T, u0, u1);
+        if (u0 >= T) return;
+        int pos = incl - mine, fb = 0, fp = 0, fl = 0;
         const bool holds = u0 >= pos && u0 < incl;
-        int fb = 0, fp = 0, fl = 0;
         if (holds) {
             for (int i = b0; i < b1; ++i) {
-                const int li = a.lens[i], n = units_of(li);
+                const int li = a.lens[i], n = pages_of(li) + extra;
                 if (u0 < pos + n) {
                     fb = i;
                     fp = pos;
@@ -226,71 +349,127 @@ void int4_decode_kernel(const Int4DecodeParams a) {
         P = __builtin_amdgcn_readlane(fp, src);
         len = __builtin_amdgcn_readlane(fl, src);
     }
+    if (u1 <= P + extra) return;                     // (none of its pages)
 
-    const float scale_log2 = a.scale * I4_LOG2E;
-    const int64_t rec = (int64_t)NR * HEAD_DIM + 2 * MAX_NREP;
-    int at = u0;
-    while (true) {
-        const int n = units_of(len);
-        const int s0 = at - P, s1 = u1 - P < n ? u1 - P : n;      // this run's pages of it
-
-        // query rows (past n_rep: row 0, never stored), channels 32 j + 8 g + (0..7)
-        // in the order of the code pairs
-        h8 q[4];
-        {
-            const half_t* row = a.q + (int64_t)b * a.sq_b + (int64_t)h * a.sq_h +
-                                (int64_t)(c < NR ? c : 0) * a.sq_r + 8 * g;
+    // q's sign takes the scale's, so that a larger product is a larger score.
+    const float scale = fabsf(a.scale) * I4_LOG2E;
+    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+    const Splice sp = make_splice();
+    // Query rows (past n_rep: row 0, never stored), channels 32 j + 8 g + (0..7).
+    auto load_q = [&](int bq, u4 (&t)[4]) {
+        const half_t* row = a.q + (int64_t)bq * a.sq_b + (int64_t)h * a.sq_h +
+                            (int64_t)(c < NR ? c : 0) * a.sq_r + 8 * g;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const h8 t = *(const h8*)(row + 32 * j);
-                q[j] = (h8){t[0], t[4], t[1], t[5], t[2], t[6], t[3], t[7]};
-            }
-        }
-        const int32_t* trow = a.tables + (int64_t)b * a.st_b;
+        for (int j = 0; j < 4; ++j) t[j] = *(const u4*)(row + 32 * j);
+    };
+    // A block from the table, -1 where it lies outside the pool.
+    auto valid = [&](int t) { return (unsigned)t < (unsigned)a.p.num_blocks ? t : -1; };
+
+    int s0 = u0 - P - extra;
+    s0 = s0 > 0 ? s0 : 0;
+    u4 q_raw[4];
+    load_q(b, q_raw);
+    // the table entries of the wave's first pair (lanes 0 and 1), past the table's end
+    // the last one's
+    auto first_entries = [&](int bt, int from) {
+        const int p = from + 2 * wv + (lane & 1);
+        return a.tables[(int64_t)bt * a.st_b + (p < a.max_pages ? p : a.max_pages - 1)];
+    };
+    int entry = first_entries(b, s0);
+
+    Int4Page page[2][2];
+    int item[2], blk[2][2];
+    auto request = [&](int slot, int it, int b0, int b1) {
+        item[slot] = it;
+        blk[slot][0] = b0;
+        blk[slot][1] = b1;
+        int4_load(a, page[slot][0], b0, h, g, c);
+        int4_load(a, page[slot][1], b1, h, g, c);
+    };
+    bool requested = false;          // the segment's first pair is on its way
+    while (true) {
+        // ---- this run's pages [s0, s1) of sequence b ----
+        const int n = pages_of(len), start = P + extra;
+        const int s1 = u1 - start < n ? u1 - start : n;
         const int pages = len > 0 ? n : 0;
-        // the wave's pages s0 + wv, + NW, ...; lane i holds the block of its
-        // (base + i)-th (-1: none, or outside the pool)
-        int base = 0, blk_of = -1;
-        auto fill = [&](int from) {
-            base = from;
-            const int64_t pg = s0 + wv + (int64_t)(from + lane) * I4_NW;
-            int t = -1;
-            if (pg < s1 && pg < pages) t = trow[pg];
-            blk_of = t >= 0 && t < a.p.num_blocks ? t : -1;
+        const bool more = P + extra + n + extra < u1;     // the next sequence has pages here
+        auto request_first = [&](int from, int to, int limit) {
+            const int i = from + 2 * wv;
+            const int b0 = valid(__builtin_amdgcn_readlane(entry, 0));
+            const int b1 = valid(__builtin_amdgcn_readlane(entry, 1));
+            request(0, wv, i < to && i < limit ? b0 : -1, i + 1 < to && i + 1 < limit ? b1 : -1);
         };
-        fill(0);
+        if (!requested) request_first(s0, s1, pages);
+        h8 q[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const h8 t = __builtin_bit_cast(h8, (u4)(q_raw[j] ^ flip));
+            q[j] = (h8){t[0], t[4], t[1], t[5], t[2], t[6], t[3], t[7]};
+        }
+        // what the next sequence of the run needs, ahead of its turn
+        const int b_next = more ? b + 1 : b;
+        const int len_next = a.lens[b_next];
+        int entry_next = first_entries(b_next, 0);
+        load_q(b_next, q_raw);
 
         Int4State st;
 #pragma unroll
         for (int t = 0; t < 8; ++t) st.acc[t] = (f4){0.f, 0.f, 0.f, 0.f};
+        st.l = (f4){0.f, 0.f, 0.f, 0.f};
         st.m = neg_inf();
-        st.l = 0.f;
-        const int count = s0 + wv < s1 ? (s1 - s0 - wv + I4_NW - 1) / I4_NW : 0;
-        Int4Page page[2];
-        int blk[2];
-        blk[0] = __builtin_amdgcn_readlane(blk_of, 0);
-        if (count > 0) int4_load(a, page[0], blk[0], h, g, c);
-        for (int k = 0; k < count; k += 2) {
-#pragma unroll
-            for (int z = 0; z < 2; ++z) {
-                if (k + z >= count) break;
-                const int nx = k + z + 1;
-                if (nx < count) {
-                    if (nx - base == WAVE) fill(nx);
-                    blk[z ^ 1] = __builtin_amdgcn_readlane(blk_of, nx - base);
-                    int4_load(a, page[z ^ 1], blk[z ^ 1], h, g, c);
-                }
-                const int pg = s0 + wv + (k + z) * I4_NW;
-                int4_compute(page[z], st, q, pg * PAGE, blk[z] >= 0 ? len : 0, scale_log2, g);
+        const int32_t* trow = a.tables + (int64_t)b * a.st_b;
+        // The pages' blocks in LDS, a run of more than I4_TABLE pages in pieces; the
+        // waves claim pairs of pages one by one (the oldest win memory arbitration: with
+        // static shares the youngest ended 5 us later at B16 x 16K), the first pair of
+        // each fixed, so that it is requested while the table fills.
+        for (int c0 = s0; c0 < s1; c0 += I4_TABLE) {
+            const int n_pg = s1 - c0 < I4_TABLE ? s1 - c0 : I4_TABLE, pairs = (n_pg + 1) / 2;
+            if (c0 != s0) {
+                __syncthreads();                           // the piece before is claimed out
+                entry = first_entries(b, c0);
+                request_first(c0, s1, pages);
             }
+            for (int i = threadIdx.x; i < 2 * pairs; i += WAVE * I4_NW)
+                sm.blk[i] = i < n_pg && c0 + i < pages ? valid(trow[c0 + i]) : -1;
+            if (threadIdx.x == 0) sm.claim = I4_NW;
+            __syncthreads();
+            auto claim = [&]() {
+                int r = 0;
+                if (lane == 0)
+                    r = __hip_atomic_fetch_add(&sm.claim, 1, __ATOMIC_RELAXED,
+                                               __HIP_MEMORY_SCOPE_WORKGROUP);
+                return r;
+            };
+            int next = claim();
+            bool live = item[0] < pairs;
+            while (live) {
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                    if (!live) break;
+                    const int it = __builtin_amdgcn_readfirstlane(next);
+                    next = claim();                        // (read a step later)
+                    if (it < pairs)
+                        request(z ^ 1, it, __builtin_amdgcn_readfirstlane(sm.blk[2 * it]),
+                                __builtin_amdgcn_readfirstlane(sm.blk[2 * it + 1]));
+                    const int lens[2] = {blk[z][0] >= 0 ? len : 0, blk[z][1] >= 0 ? len : 0};
+                    int4_compute(sp, page[z], st, q, (c0 + 2 * item[z]) * PAGE, lens, scale, g);
+                    live = it < pairs;
+                }
+            }
+        }
+        // the next sequence's first pair, on its way while this one is merged
+        entry = entry_next;
+        if (more) {
+            const int n2 = pages_of(len_next), start2 = start + n + extra;
+            request_first(0, u1 - start2 < n2 ? u1 - start2 : n2, len_next > 0 ? n2 : 0);
+            requested = true;
         }
 
         // ---- the waves' states merged in LDS ----
-        const float lrow = group4_sum(st.l);
         if (c < NR) {
             if (g == 0) {
                 sm.m[wv][c] = st.m;
-                sm.l[wv][c] = lrow;
+                sm.l[wv][c] = st.l[0];
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -305,9 +484,12 @@ void int4_decode_kernel(const Int4DecodeParams a) {
         }
         __syncthreads();
         const bool whole = s0 == 0 && s1 == n;
+        const int first = start / per;                     // the sequence's first group
+        const Int4Records R = {a.work + (int64_t)h * a.rec, H * a.rec * (int)sizeof(float), a.groups,
+                               first};
         const int d0 = 4 * (threadIdx.x % 32);
-        float* record = a.work + ((int64_t)(2 * w + (s0 == 0 ? 1 : 0)) * H + h) * rec;
-        half_t* orow = a.out + (int64_t)b * a.so_b + (int64_t)h * a.so_h + d0;
+        float* record = (float*)((char*)R.work + R.at(w - first));
+        half_t* orow = a.out + (int64_t)b * a.so_b + (int64_t)h * a.so_h;
         for (int r = threadIdx.x / 32; r < NR; r += I4_NW * 2) {
             float mg = neg_inf();
 #pragma unroll
@@ -323,57 +505,62 @@ void int4_decode_kernel(const Int4DecodeParams a) {
             if (whole) {
                 const float inv = 1.f / fmaxf(lt, 1e-20f);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) orow[(int64_t)r * a.so_r + e] = (half_t)(acc[e] * inv);
+                for (int e = 0; e < 4; ++e)
+                    orow[(int64_t)r * a.so_r + d0 + e] = (half_t)(acc[e] * inv);
             } else {
                 store_coherent(record + r * HEAD_DIM + d0, acc);
                 if (d0 == 0) store_coherent(record + NR * HEAD_DIM + 2 * r, mg, lt);
             }
         }
         if (!whole) {
-            // ---- the last of the sequence's groups merges their records ----
-            const int first = P / per, last = (P + n - 1) / per;
-            int32_t* counter = a.counters + ((int64_t)first * H + h) * I4_COUNTER_STRIDE;
-            handoff_release();
-            __syncthreads();
-            if (threadIdx.x == 0)
-                sm.is_last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED,
-                                                    __HIP_MEMORY_SCOPE_AGENT) == last - first;
-            __syncthreads();
-            if (sm.is_last) {
-                for (int r = threadIdx.x / 32; r < NR; r += I4_NW * 2) {
-                    float mg = neg_inf(), lt = 0.f;
-                    f4 acc = {0.f, 0.f, 0.f, 0.f};
-                    for (int k = first; k <= last; ++k) {
-                        const float* rk = a.work + ((int64_t)(2 * k + (k == first ? 1 : 0)) * H + h) * rec;
-                        const float mk = load_coherent(rk + NR * HEAD_DIM + 2 * r);
-                        const float lk = load_coherent(rk + NR * HEAD_DIM + 2 * r + 1);
-                        f4 ak;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) ak[e] = load_coherent(rk + r * HEAD_DIM + d0 + e);
-                        const float mn = fmaxf(mg, mk);
-                        const bool none = mn == neg_inf();
-                        const float wa = none ? 0.f : fast_exp2(mg - mn);
-                        const float wb = none ? 0.f : fast_exp2(mk - mn);
-                        lt = lt * wa + lk * wb;
-                        acc = acc * wa + ak * wb;
-                        mg = mn;
-                    }
-                    const float inv = 1.f / fmaxf(lt, 1e-20f);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) orow[(int64_t)r * a.so_r + e] = (half_t)(acc[e] * inv);
+            // ---- the last of the sequence's groups to arrive merges their records ----
+            const int S = (start + n - 1) / per - first + 1;
+            const int k = w - first, cl = k / I4_CLUSTER;
+            const bool tree = S > I4_CLUSTER;
+            // arrival counters: [0] the sequence's, at its first group; [1], [2] of 16
+            // groups, at the first of them (two, since that group may start another
+            // sequence, whose own first 16 count there)
+            auto arrive = [&](int group, int which, int all) {
+                handoff_release();
+                __syncthreads();
+                if (threadIdx.x == 0) {
+                    int32_t* counter = a.counters + ((int64_t)group * H + h) * I4_COUNTER_STRIDE + which;
+                    const int before = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED,
+                                                              __HIP_MEMORY_SCOPE_AGENT);
+                    sm.is_last = before == all - 1;
+                    if (before == all - 1)                 // back to zero for the next launch
+                        __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 }
-                if (threadIdx.x == 0)
-                    __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __syncthreads();
+                return sm.is_last != 0;
+            };
+            int k0 = tree ? cl * I4_CLUSTER : 0, step = 1, count = tree ? S - k0 : S;
+            count = count < I4_CLUSTER ? count : I4_CLUSTER;
+            int which = tree ? (cl == 0 ? 1 : 2) : 0;
+            while (arrive(first + k0, which, count)) {
+                merge_records(R, k0, step, count, NR, which == 0 ? orow : nullptr, a.so_r);
+                if (which == 0) break;
+                which = 0;
+                k0 = 0;
+                step = I4_CLUSTER;
+                count = (S + I4_CLUSTER - 1) / I4_CLUSTER;
             }
         }
-        at = P + n;
-        if (at >= u1) return;
-        ++b;
-        P = at;
-        len = a.lens[b];
+        if (!more) return;
+        P = start + n;
+        s0 = 0;
+        b = b_next;
+        len = len_next;
         __syncthreads();                 // the merge's LDS reads end before the next states
     }
 }
+
+// What starting on a sequence costs a group beside its pages (its first loads, its merge),
+// in pages, where groups start on them often: with pages alone, the groups of short
+// sequences end late (us, 0 -> 16 -> 32 pages, ragged lengths: B250 to 500, 4 heads 35.0
+// -> 23.6 -> 26.6; B48 to 1531, 8 heads 23.3 -> 20.5 -> 25.1; B96 to 16K 61.3 -> 58.4 ->
+// 60.9); where most groups start on none, it would take pages from the ones that do.
+constexpr int I4_EXTRA = 16;
 
 int int4_groups(int batch, int kv_heads, int64_t pages_bound) {
     int64_t most = I4_RESIDENT / kv_heads;
@@ -383,7 +570,10 @@ int int4_groups(int batch, int kv_heads, int64_t pages_bound) {
 }
 
 hipError_t launch_int4_decode(const Int4DecodeParams& a, hipStream_t stream) {
-    hipLaunchKernelGGL(int4_decode_kernel, dim3(a.groups * a.H), dim3(WAVE * I4_NW), 0, stream, a);
+    Int4DecodeParams d = a;
+    d.rec = int4_record_floats(a.NR);
+    d.extra = 4 * a.B > a.groups ? I4_EXTRA : 0;
+    hipLaunchKernelGGL(int4_decode_kernel, dim3(a.groups * a.H), dim3(WAVE * I4_NW), 0, stream, d);
     return hipGetLastError();
 }
 

@@ -66,15 +66,17 @@ struct Int4DecodeParams {
     int32_t* counters;            // [groups * H * I4_COUNTER_STRIDE], zero at rest
     int B, H, NR;
     int groups;                   // workgroups a KV head
+    int rec;                      // floats of a record (set at launch, as the next)
+    int extra;                    // pages that starting on a sequence counts as
     float scale;
 };
 
-constexpr int I4_COUNTER_STRIDE = 2;      // int32 a (group, head)
+constexpr int I4_COUNTER_STRIDE = 4;      // int32 a (group, head)
 constexpr int I4_MAX_GROUPS = 1 << 20;    // groups x heads of a launch, at most
 
 // Workgroups a head for these sizes, and the floats of the split records.
 int int4_groups(int batch, int kv_heads, int64_t pages_bound);
-constexpr int64_t int4_record_floats(int n_rep) { return (int64_t)n_rep * 128 + 2 * 16; }
+constexpr int int4_record_floats(int n_rep) { return n_rep * 128 + 2 * 16; }
 
 hipError_t launch_int4_write(const Int4WriteParams& a, hipStream_t stream);
 hipError_t launch_int4_read(const Int4ReadParams& a, hipStream_t stream);

@@ -182,9 +182,10 @@ int ls_paged_decode_int4(const void* q, const int64_t* q_strides, const void* k_
     if (int rc = check_tables(block_tables, bt_stride, max_pages, seq_lens, batch)) return rc;
     if (n_rep < 1 || n_rep > ls::MAX_NREP)
         return fail(LS_ERR_INVALID, "n_rep must be in [1, 16], got %d", n_rep);
-    if (groups < 1 || (int64_t)groups * kv_heads > ls::I4_MAX_GROUPS)
-        return fail(LS_ERR_INVALID, "groups must be >= 1 and groups x kv_heads at most %d",
-                    ls::I4_MAX_GROUPS);
+    if (groups < 1 || (int64_t)groups * kv_heads > ls::I4_MAX_GROUPS ||
+        ls_int4_decode_workspace_bytes(groups, kv_heads, n_rep) >= (size_t)1 << 31)
+        return fail(LS_ERR_INVALID, "groups must be >= 1, groups x kv_heads at most %d and the "
+                    "workspace below 2^31 bytes", ls::I4_MAX_GROUPS);
     if (!rows_aligned(q, q_strides, 3, 2) || !rows_aligned(out, out_strides, 3, 2))
         return fail(LS_ERR_INVALID, "q and out rows must be 16-byte aligned");
     if (!aligned(workspace, 16) ||

@@ -118,7 +118,7 @@ struct LogprobParams {
 };
 
 // Parts a row is split over, and the floats of a part's record.
-int logprob_parts(int rows, int n, int fp32);
+int logprob_parts(int rows, int n);
 constexpr int logprob_record_floats(int top) { return 4 + 2 * top; }
 hipError_t launch_token_logprobs(const LogprobParams& a, int fp32, hipStream_t stream);
 

@@ -279,16 +279,16 @@ int ls_page_copy(void* const* tensors, const int64_t* page_strides, const int64_
     return LS_OK;
 }
 
-size_t ls_token_logprobs_workspace_bytes(int rows, int n, int top, int elem_bytes) {
+size_t ls_token_logprobs_workspace_bytes(int rows, int n, int top) {
     if (rows < 1 || n < 1 || top < 0 || top > ls::LOGPROB_MAX_TOP) return 0;
-    const int parts = ls::logprob_parts(rows, n, elem_bytes == 4);
+    const int parts = ls::logprob_parts(rows, n);
     if (parts == 1) return 0;
     return (size_t)rows * parts * ls::logprob_record_floats(top) * sizeof(float);
 }
 
-size_t ls_token_logprobs_counter_ints(int rows, int n, int elem_bytes) {
+size_t ls_token_logprobs_counter_ints(int rows, int n) {
     if (rows < 1 || n < 1) return 0;
-    return ls::logprob_parts(rows, n, elem_bytes == 4) == 1 ? 0 : (size_t)rows;
+    return ls::logprob_parts(rows, n) == 1 ? 0 : (size_t)rows;
 }
 
 int ls_token_logprobs(const void* x, int64_t x_stride, int elem_bytes, const int64_t* tokens,
@@ -307,11 +307,11 @@ int ls_token_logprobs(const void* x, int64_t x_stride, int elem_bytes, const int
     if (!aligned(x, elem_bytes)) return fail(LS_ERR_INVALID, "x must be aligned to its elements");
     if (rows == 0) return LS_OK;
     ls::LogprobParams a;
-    a.parts = ls::logprob_parts(rows, n, elem_bytes == 4);
+    a.parts = ls::logprob_parts(rows, n);
     if ((int64_t)rows * a.parts > (1LL << 31) - 1)
         return fail(LS_ERR_INVALID, "rows x n too large for one call");
     if (a.parts > 1) {
-        const size_t need = ls_token_logprobs_workspace_bytes(rows, n, top, elem_bytes);
+        const size_t need = ls_token_logprobs_workspace_bytes(rows, n, top);
         if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
             return fail(LS_ERR_INVALID, "needs a 16-byte aligned workspace of %zu bytes", need);
         if (!counters || !aligned(counters, 4))

@@ -62,13 +62,13 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     if rows:
         lib = _serving.lib()
         size = x.element_size()
-        need = lib.ls_token_logprobs_workspace_bytes(rows, n, top, size)
+        need = lib.ls_token_logprobs_workspace_bytes(rows, n, top)
         with _serving.on(dev):
             work = cnt = None
             if need:
                 work = torch.empty(need, dtype=torch.uint8, device=dev)
                 cnt = _serving.counters(dev, stream,
-                                        lib.ls_token_logprobs_counter_ints(rows, n, size))
+                                        lib.ls_token_logprobs_counter_ints(rows, n))
             rc = lib.ls_token_logprobs(
                 x.data_ptr(), x.stride(0) if rows > 1 else n, size, tok.data_ptr(),
                 tok.stride(0) if rows > 1 else 1, both.data_ptr(), both.data_ptr() + 4 * rows,

@@ -96,7 +96,7 @@ int ls_page_copy(void* const* tensors, const int64_t* page_strides, const int64_
  * `counters` (zero before the first call, left zero) of a log-probability call;
  * 0 where none is needed. */
 size_t ls_token_logprobs_workspace_bytes(int rows, int n, int top);
-size_t ls_token_logprobs_counter_ints(int rows, int n);
+size_t ls_token_logprobs_counter_ints(int rows, int n, int top);
 
 /* Rows of n logits (fp16: elem_bytes 2, fp32: 4; row stride x_stride in
  * elements, unit stride inside): logprob[r] = log softmax(x_r)[tokens[r]]

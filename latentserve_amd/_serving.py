@@ -40,7 +40,7 @@ _SIGNATURES = {
                              _VP],
     "ls_page_copy": [_VP, _I64P, _I64P, _I32, _I64, _I32P, _I32P, _I32, _VP],
     "ls_token_logprobs_workspace_bytes": [_I32, _I32, _I32],
-    "ls_token_logprobs_counter_ints": [_I32, _I32],
+    "ls_token_logprobs_counter_ints": [_I32, _I32, _I32],
     "ls_token_logprobs": [_VP, _I64, _I32, _VP, _I64, _VP, _VP, _VP, _VP, _VP, _SZ, _VP, _I32,
                           _I32, _I32, _VP],
 }

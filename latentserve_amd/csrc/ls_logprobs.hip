@@ -21,12 +21,18 @@
 #include "ls_common.h"
 #include "ls_serving.h"
 
+// (a maximum's product with log2 e is rounded once and used as that value everywhere)
+#pragma clang fp contract(off)
+
 namespace ls {
 
 constexpr int LP_THREADS = 256;
 constexpr int LP_WAVES = LP_THREADS / WAVE;
 // Logits a thread holds: 64, or 16 where that leaves more than half of the CUs idle.
 constexpr int LP_LONG = 64, LP_SHORT = 16;
+// Streaming groups a call aims at: two a CU (us at 512 / 1024 / 2048, 152K logits a row: 1021
+// rows 57 / 61 / 62, 600 rows 39 / 40 / -, 300 rows 24 / 24 / -).
+constexpr int LP_GROUPS = 512;
 constexpr int LP_POOL = LOGPROB_MAX_TOP * LP_LONG;
 constexpr float LP_LOG2E = 1.4426950408889634f, LP_LN2 = 0.6931471805599453f;
 
@@ -41,12 +47,13 @@ __device__ __forceinline__ float key_value(uint32_t k) {
     return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
+template <bool TOP>
 struct LogprobSmem {
     float red[3][LP_WAVES];
     uint32_t wave_bound[LP_WAVES];
-    uint64_t best[LP_THREADS];
-    uint64_t pool[LP_POOL];
-    uint64_t kept[LOGPROB_MAX_TOP];
+    uint64_t best[TOP ? LP_THREADS : 1];
+    uint64_t pool[TOP ? LP_POOL : 1];
+    uint64_t kept[TOP ? LOGPROB_MAX_TOP : 1];
     uint64_t bound;
     int count;
     int is_last;
@@ -57,23 +64,38 @@ __device__ __forceinline__ float wave_max_all(float v) {
     return fmaxf(p.a, p.b);
 }
 
-// Z and E against the maximum m; differences in log2 units (of values,
-// not of scaled ones: a type's lowest value times log2 e need not be finite, and a
-// large maximum's rounding would be in every difference).
+// Z and E against a maximum m, differences in log2 units.  fp16 logits: m itself is in log2
+// units, so that a difference is one fused multiply-add (the rounding of m log2 e is in
+// every difference alike, the results' too, and cancels).  fp32: m is a logit, since a
+// logit times log2 e need not be finite (the type's lowest value, a mask).
+template <bool F32>
 struct Sums {
     float m, z, e;
+    static __device__ __forceinline__ float ref(float x) { return F32 ? x : x * LP_LOG2E; }
+    static __device__ __forceinline__ float diff(float x, float m) {
+        return F32 ? (x - m) * LP_LOG2E : __builtin_fmaf(x, LP_LOG2E, -m);
+    }
     // Against `to`, which is finite; a maximum of -inf (nothing summed) weighs nothing.
     __device__ __forceinline__ void move(float to) {
-        const float d = (m - to) * LP_LOG2E, w = m == neg_inf() ? 0.f : fast_exp2(d);
+        const float d = F32 ? (m - to) * LP_LOG2E : m - to;
+        const float w = m == neg_inf() ? 0.f : fast_exp2(d);
         // (z may be NaN, which stays)
         e = w == 0.f ? 0.f * z : w * (e + z * d);
         z *= w;
         m = to;
     }
+    // A logit against m (finite).
+    __device__ __forceinline__ void add(float x) {
+        const float d = diff(x, m);
+        const float p = fast_exp2(d);
+        z += p;
+        e = __builtin_fmaf(p, fmaxf(d, -1024.f), e);      // (0 for -inf)
+    }
 };
 
 // (m, z, e) of the lanes' sums, in every lane.
-__device__ __forceinline__ Sums wave_sums(Sums s) {
+template <bool F32>
+__device__ __forceinline__ Sums<F32> wave_sums(Sums<F32> s) {
     const float top = wave_max_all(s.m);
     s.move(top == neg_inf() ? 0.f : top);
     s.z = wave_sum_dpp(s.z);
@@ -82,19 +104,21 @@ __device__ __forceinline__ Sums wave_sums(Sums s) {
     return s;
 }
 
-// Ranks the n entries of sm.pool; the k best go to sm.kept in order (0: none).
-__device__ __forceinline__ void rank_pool(LogprobSmem& sm, int n, int k) {
-    const int tid = threadIdx.x;
-    if (tid < k) sm.kept[tid] = 0;
-    __syncthreads();
-    for (int i = tid; i < n; i += LP_THREADS) {
-        const uint64_t key = sm.pool[i];
-        int r = 0;
-#pragma unroll 8
-        for (int j = 0; j < n; ++j) r += sm.pool[j] > key ? 1 : 0;
-        if (r < k) sm.kept[r] = key;
+// A group's sums, in every lane, from its waves'.
+template <bool F32, class Smem>
+__device__ __forceinline__ Sums<F32> group_sums(Smem& sm, Sums<F32> s) {
+    const int lane = threadIdx.x % WAVE, wv = threadIdx.x / WAVE;
+    s = wave_sums(s);
+    if (lane == 0) {
+        sm.red[0][wv] = s.m;
+        sm.red[1][wv] = s.z;
+        sm.red[2][wv] = s.e;
     }
     __syncthreads();
+    const int v = lane % LP_WAVES;
+    s = {sm.red[0][v], sm.red[1][v], sm.red[2][v]};
+    if (lane >= LP_WAVES) s = {neg_inf(), 0.f, 0.f};
+    return wave_sums(s);
 }
 
 // The k-th largest of the wave's keys (0 where fewer than k lanes have one).
@@ -108,13 +132,150 @@ __device__ __forceinline__ uint32_t wave_kth(uint32_t key, int k) {
     return ans;
 }
 
+// The largest of the waves' k-th largest keys, at least 1: no more than the k-th
+// largest of all.  (Two barriers; sm.count is 0 after it.)
+__device__ __forceinline__ uint32_t group_bound(LogprobSmem<true>& sm, uint32_t key, int k) {
+    const uint32_t kth = wave_kth(key, k);
+    __syncthreads();
+    if (threadIdx.x % WAVE == 0) sm.wave_bound[threadIdx.x / WAVE] = kth;
+    if (threadIdx.x == 0) sm.count = 0;
+    __syncthreads();
+    uint32_t bound = 1;
+#pragma unroll
+    for (int v = 0; v < LP_WAVES; ++v) bound = sm.wave_bound[v] > bound ? sm.wave_bound[v] : bound;
+    return bound;
+}
+
+// The k best of the n entries of sm.pool go to sm.kept in order (0: none), ranked by
+// counting after all but a few have been dropped.
+__device__ __forceinline__ void rank_pool(LogprobSmem<true>& sm, int n, int k) {
+    const int tid = threadIdx.x;
+    const uint64_t* list = sm.pool;
+    if (n > WAVE) {
+        uint32_t best = 0;
+        for (int i = tid; i < n; i += LP_THREADS) {
+            const uint32_t key = (uint32_t)(sm.pool[i] >> 32);
+            best = key > best ? key : best;
+        }
+        const uint32_t bound = group_bound(sm, best, k);
+        for (int i = tid; i < n; i += LP_THREADS) {
+            const uint64_t key = sm.pool[i];
+            if ((uint32_t)(key >> 32) >= bound) {
+                const int at = atomicAdd(&sm.count, 1);
+                if (at < LP_THREADS) sm.best[at] = key;
+            }
+        }
+        __syncthreads();
+        if (sm.count <= LP_THREADS) {
+            list = sm.best;
+            n = sm.count;
+        }
+    }
+    if (tid < k) sm.kept[tid] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += LP_THREADS) {
+        const uint64_t key = list[i];
+        int r = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) r += list[j] > key ? 1 : 0;
+        if (r < k) sm.kept[r] = key;
+    }
+    __syncthreads();
+}
+
+// A part's sums s (in every lane), and its k best in sm.kept, to the row's results: at
+// once, or by the last of the row's groups to arrive.
+template <bool TOP, bool F32, class T>
+__device__ __forceinline__ void finish(const LogprobParams& a, LogprobSmem<TOP>& sm, Sums<F32> s,
+                                       const T* xr, int row, int part) {
+    const int tid = threadIdx.x, lane = tid % WAVE, top = TOP ? a.top : 0;
+    if (a.parts > 1) {
+        const int floats = logprob_record_floats(top);
+        float* rec = a.part + ((int64_t)row * a.parts + part) * floats;
+        auto put = [](float* p, float v) {
+            __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        };
+        if (tid == 0) {
+            put(rec, s.m);
+            put(rec + 1, s.z);
+            put(rec + 2, s.e);
+        }
+        if (TOP && tid < top)
+            __hip_atomic_store((uint64_t*)(rec + 4) + tid, sm.kept[tid], __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_AGENT);
+        handoff_release();
+        __syncthreads();
+        if (tid == 0)
+            sm.is_last = __hip_atomic_fetch_add(a.counters + row, 1, __ATOMIC_RELAXED,
+                                                __HIP_MEMORY_SCOPE_AGENT) == a.parts - 1;
+        __syncthreads();
+        if (!sm.is_last) return;
+        if (tid == 0) __hip_atomic_store(a.counters + row, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const float* recs = a.part + (int64_t)row * a.parts * floats;
+        // (every wave the same: a part a lane; the first ones requested ahead of the
+        // entries)
+        auto sums_of = [&](int p) {
+            Sums<F32> t = {neg_inf(), 0.f, 0.f};
+            if (p < a.parts) {
+                const float* rp = recs + (int64_t)p * floats;
+                t = {load_coherent(rp), load_coherent(rp + 1), load_coherent(rp + 2)};
+            }
+            return t;
+        };
+        s = sums_of(lane);
+        if constexpr (TOP) {
+            // rounds: the kept ones so far, then as many parts' as fit
+            const int round = (LP_POOL - LOGPROB_MAX_TOP) / top;
+            for (int p0 = 0; p0 < a.parts; p0 += round) {
+                const int np = a.parts - p0 < round ? a.parts - p0 : round;
+                const int had = p0 == 0 ? 0 : top;
+                if (tid < had) sm.pool[tid] = sm.kept[tid];
+                // (every part's best, then every part's second, ...: a wave's entries are
+                // alike in rank, and the first wave's bound is a good one)
+                for (int i = tid; i < np * top; i += LP_THREADS)
+                    sm.pool[had + i] = load_coherent(
+                        (const uint64_t*)(recs + (int64_t)(p0 + i % np) * floats + 4) + i / np);
+                __syncthreads();
+                // (absent entries are 0 and never rank before a present one)
+                rank_pool(sm, had + np * top, top);
+            }
+        }
+        s = wave_sums(s);
+        for (int p0 = WAVE; p0 < a.parts; p0 += WAVE) {
+            Sums<F32> t = wave_sums(sums_of(p0 + lane));
+            const float m = fmaxf(s.m, t.m), to = m == neg_inf() ? 0.f : m;
+            s.move(to);
+            t.move(to);
+            s = {m, s.z + t.z, s.e + t.e};
+        }
+    }
+
+    // (a row of -inf only: m -inf, z 0)
+    const float mr = s.m == neg_inf() ? 0.f : s.m;
+    const float lz = __builtin_amdgcn_logf(s.z);                   // log2
+    auto logp = [&](float v) {
+        if (v == neg_inf() && s.z == s.z) return neg_inf();
+        return F32 ? (v - mr) - lz * LP_LN2 : (Sums<F32>::diff(v, mr) - lz) * LP_LN2;
+    };
+    if (tid == 0) {
+        const int64_t tok = a.tokens[(int64_t)row * a.s_tok];
+        a.logprob[row] = tok >= 0 && tok < a.n ? logp((float)xr[tok]) : 0.f;
+        a.entropy[row] = s.z == 0.f ? 0.f : (lz - s.e / s.z) * LP_LN2;
+    }
+    if (TOP && tid < top) {
+        const uint64_t key = sm.kept[tid];
+        a.top_val[(int64_t)row * top + tid] = logp(key_value((uint32_t)(key >> 32)));
+        a.top_id[(int64_t)row * top + tid] = (uint32_t)~(uint32_t)key;
+    }
+}
+
 template <bool F32, bool TOP, int HELD>
 __global__ __launch_bounds__(LP_THREADS) void logprob_kernel(const LogprobParams a) {
     constexpr int VEC = F32 ? 4 : 8, CHUNKS = HELD / VEC, PART = LP_THREADS * HELD;
     using T = std::conditional_t<F32, float, half_t>;
     typedef T tv __attribute__((ext_vector_type(VEC)));
-    __shared__ LogprobSmem sm;
-    const int tid = threadIdx.x, lane = tid % WAVE, wv = tid / WAVE;
+    __shared__ LogprobSmem<TOP> sm;
+    const int tid = threadIdx.x;
     const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
     const T* xr = (const T*)a.x + (int64_t)row * a.sx;
     const int top = TOP ? a.top : 0;
@@ -138,7 +299,6 @@ __global__ __launch_bounds__(LP_THREADS) void logprob_kernel(const LogprobParams
             }
         }
     }
-    if (tid == 0) sm.count = 0;
     tv mx = x[0];
 #pragma unroll
     for (int k = 1; k < CHUNKS; ++k) mx = __builtin_elementwise_max(mx, x[k]);
@@ -146,29 +306,18 @@ __global__ __launch_bounds__(LP_THREADS) void logprob_kernel(const LogprobParams
 #pragma unroll
     for (int v = 1; v < VEC; ++v) best = fmaxf(best, (float)mx[v]);
 
-    Sums s = {best, 0.f, 0.f};
-    const float mb = s.m == neg_inf() ? 0.f : s.m;
+    const float mine = Sums<F32>::ref(best);
+    Sums<F32> s = {mine == neg_inf() ? 0.f : mine, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < CHUNKS; ++k)
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const float d = ((float)x[k][v] - mb) * LP_LOG2E;
-            const float p = fast_exp2(d);
-            s.z += p;
-            s.e = __builtin_fmaf(p, fmaxf(d, -1024.f), s.e);      // (0 for -inf)
-        }
-    s = wave_sums(s);
-    if (lane == 0) {
-        sm.red[0][wv] = s.m;
-        sm.red[1][wv] = s.z;
-        sm.red[2][wv] = s.e;
-    }
+        for (int v = 0; v < VEC; ++v) s.add((float)x[k][v]);
+    s.m = mine;
 
-    // the part's k best to sm.kept
-    uint32_t tkey = 0;
-    if (top > 0) {
-        // (the maximum ignores NaN, which ranks first: any NaN makes the thread's key
-        // the largest)
+    s = group_sums(sm, s);
+    if constexpr (TOP) {
+        // (the maximum ignores NaN, which ranks first: a NaN makes the thread's key the
+        // largest)
         bool nan = false, any = false;
 #pragma unroll
         for (int k = 0; k < CHUNKS; ++k) {
@@ -177,45 +326,49 @@ __global__ __launch_bounds__(LP_THREADS) void logprob_kernel(const LogprobParams
 #pragma unroll
             for (int v = 0; v < VEC; ++v) nan = nan || x[k][v] != x[k][v];
         }
-        tkey = nan ? 0xFFFFFFFFu : any ? value_key(best) : 0;
-        const uint32_t kth = wave_kth(tkey, top);
-        if (lane == 0) sm.wave_bound[wv] = kth;
-    }
-    __syncthreads();
-    s = {sm.red[0][lane % LP_WAVES], sm.red[1][lane % LP_WAVES], sm.red[2][lane % LP_WAVES]};
-    if (lane >= LP_WAVES) s = {neg_inf(), 0.f, 0.f};
-    s = wave_sums(s);
-    if (top > 0) {
-        uint32_t bound = 1;
+        const uint32_t mine = nan ? 0xFFFFFFFFu : any ? value_key(best) : 0;
+        const uint32_t bound = group_bound(sm, mine, top);
+        // The entries at or over the bound to the pool (NaN among them; where the bound
+        // stands for none, all): a thread counts its own, so it asks for its place once.
+        if (mine >= bound) {
+            const float value = key_value(bound);
+            uint64_t hits = 0;
 #pragma unroll
-        for (int v = 0; v < LP_WAVES; ++v) bound = sm.wave_bound[v] > bound ? sm.wave_bound[v] : bound;
-        auto collect = [&](uint64_t least) {
+            for (int k = 0; k < CHUNKS; ++k) {
+                const int i0 = base + k * STEP;
+                uint32_t hit = 0;
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) hit |= (float)x[k][v] < value ? 0u : 1u << v;
+                const int from = i0 < 0 ? -i0 : 0, to = a.n - i0 < VEC ? a.n - i0 : VEC;
+                hit &= to > from ? (1u << to) - (1u << from) : 0u;
+                hits |= (uint64_t)hit << (k * VEC);
+            }
+            int at = atomicAdd(&sm.count, __builtin_popcountll(hits));
 #pragma unroll
             for (int k = 0; k < CHUNKS; ++k)
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    const int i = base + k * STEP + v;
-                    const uint64_t key = ((uint64_t)value_key((float)x[k][v]) << 32) | (uint32_t)~i;
-                    if (key >= least && i >= 0 && i < a.n) {
-                        const int at = atomicAdd(&sm.count, 1);
-                        if (at < LP_POOL) sm.pool[at] = key;
+                for (int v = 0; v < VEC; ++v)
+                    if (hits >> (k * VEC + v) & 1) {
+                        const uint32_t i = base + k * STEP + v;
+                        if (at < LP_POOL)
+                            sm.pool[at] = ((uint64_t)value_key((float)x[k][v]) << 32) | ~i;
+                        ++at;
                     }
-                }
-        };
-        if (tkey >= bound) collect((uint64_t)bound << 32);
+        }
         __syncthreads();
         if (sm.count > LP_POOL) {
             // Ties: the bound as the k-th largest of the threads' best (value, index)
             // pairs.  Only the k threads whose best reaches it hold entries over it.
+            auto entry = [&](int k, int v) -> uint64_t {
+                const int i = base + k * STEP + v;
+                if (i < 0 || i >= a.n) return 0;
+                return ((uint64_t)value_key((float)x[k][v]) << 32) | (uint32_t)~i;
+            };
             uint64_t pair = 0;
 #pragma unroll
             for (int k = 0; k < CHUNKS; ++k)
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    const int i = base + k * STEP + v;
-                    const uint64_t key = ((uint64_t)value_key((float)x[k][v]) << 32) | (uint32_t)~i;
-                    if (i >= 0 && i < a.n && key > pair) pair = key;
-                }
+                for (int v = 0; v < VEC; ++v) pair = entry(k, v) > pair ? entry(k, v) : pair;
             sm.best[tid] = pair;
             __syncthreads();
             if (tid == 0) {
@@ -228,111 +381,135 @@ __global__ __launch_bounds__(LP_THREADS) void logprob_kernel(const LogprobParams
             __syncthreads();
             if (pair != 0 && r == top - 1) sm.bound = pair;
             __syncthreads();
-            if (pair >= sm.bound) collect(sm.bound);
+            const uint64_t least = sm.bound;
+            if (pair >= least)
+#pragma unroll
+                for (int k = 0; k < CHUNKS; ++k)
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v)
+                        if (entry(k, v) >= least) sm.pool[atomicAdd(&sm.count, 1)] = entry(k, v);
             __syncthreads();
         }
         rank_pool(sm, sm.count, top);
     }
+    finish<TOP, F32>(a, sm, s, xr, row, part);
+}
 
-    if (a.parts > 1) {
-        const int floats = logprob_record_floats(top);
-        float* rec = a.part + ((int64_t)row * a.parts + part) * floats;
-        auto put = [](float* p, float v) {
-            __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        };
-        if (tid == 0) {
-            put(rec, s.m);
-            put(rec + 1, s.z);
-            put(rec + 2, s.e);
-        }
-        if (tid < top)
-            __hip_atomic_store((uint64_t*)(rec + 4) + tid, sm.kept[tid], __ATOMIC_RELAXED,
-                               __HIP_MEMORY_SCOPE_AGENT);
-        handoff_release();
-        __syncthreads();
-        if (tid == 0)
-            sm.is_last = __hip_atomic_fetch_add(a.counters + row, 1, __ATOMIC_RELAXED,
-                                                __HIP_MEMORY_SCOPE_AGENT) == a.parts - 1;
-        __syncthreads();
-        if (!sm.is_last) return;
-        if (tid == 0) __hip_atomic_store(a.counters + row, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const float* recs = a.part + (int64_t)row * a.parts * floats;
-        // (every wave the same: a part a lane)
-        s = {neg_inf(), 0.f, 0.f};
-        for (int p0 = 0; p0 < a.parts; p0 += WAVE) {
-            Sums t = {neg_inf(), 0.f, 0.f};
-            if (p0 + lane < a.parts) {
-                const float* rp = recs + (int64_t)(p0 + lane) * floats;
-                t = {load_coherent(rp), load_coherent(rp + 1), load_coherent(rp + 2)};
-            }
-            t = wave_sums(t);
-            const float m = fmaxf(s.m, t.m), to = m == neg_inf() ? 0.f : m;
-            s.move(to);
-            t.move(to);
-            s = {m, s.z + t.z, s.e + t.e};
-        }
-        if (top > 0) {
-            // rounds: the kept ones so far, then as many parts' as fit
-            const int round = (LP_POOL - LOGPROB_MAX_TOP) / top;
-            for (int p0 = 0; p0 < a.parts; p0 += round) {
-                const int np = a.parts - p0 < round ? a.parts - p0 : round;
-                const int had = p0 == 0 ? 0 : top;
-                if (tid < had) sm.pool[tid] = sm.kept[tid];
-                for (int i = tid; i < np * top; i += LP_THREADS)
-                    sm.pool[had + i] = load_coherent(
-                        (const uint64_t*)(recs + (int64_t)(p0 + i / top) * floats + 4) + i % top);
-                __syncthreads();
-                // (absent entries are 0 and never rank before a present one)
-                rank_pool(sm, had + np * top, top);
-            }
-        }
-    }
+// Many logits and no alternatives: a group streams its part, so there are few parts to
+// hand over, each thread's sums moving along with its maximum.
+constexpr int LP_AHEAD = 4;          // chunks a thread takes a step; the next ones on their way
 
-    // (a row of -inf only: m -inf, z 0)
-    const float mr = s.m == neg_inf() ? 0.f : s.m;
-    const float lz = __builtin_amdgcn_logf(s.z);                   // log2
-    auto logp = [&](float v) {
-        return v == neg_inf() && s.z == s.z ? neg_inf()
-                                            : (v - mr) - lz * LP_LN2;
+template <bool F32>
+__global__ __launch_bounds__(LP_THREADS) void logprob_stream_kernel(const LogprobParams a) {
+    constexpr int VEC = F32 ? 4 : 8, STEP = LP_THREADS * VEC;
+    using T = std::conditional_t<F32, float, half_t>;
+    typedef T tv __attribute__((ext_vector_type(VEC)));
+    __shared__ LogprobSmem<false> sm;
+    const int tid = threadIdx.x;
+    const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
+    const T* xr = (const T*)a.x + (int64_t)row * a.sx;
+    const int off = (int)(((uintptr_t)xr % 16) / sizeof(T));
+    const int lo = part * a.part_len - off, hi = lo + a.part_len < a.n ? lo + a.part_len : a.n;
+    Sums<F32> s = {neg_inf(), 0.f, 0.f};
+    auto add = [&](const tv (&x)[LP_AHEAD]) {
+        tv mx = x[0];
+#pragma unroll
+        for (int k = 1; k < LP_AHEAD; ++k) mx = __builtin_elementwise_max(mx, x[k]);
+        float best = (float)mx[0];
+#pragma unroll
+        for (int v = 1; v < VEC; ++v) best = fmaxf(best, (float)mx[v]);
+        best = fmaxf(s.m, Sums<F32>::ref(best));
+        const float to = best == neg_inf() ? 0.f : best;
+        if (best != s.m) s.move(to);
+        s.m = to;
+#pragma unroll
+        for (int k = 0; k < LP_AHEAD; ++k)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) s.add((float)x[k][v]);
+        s.m = best;
     };
-    if (tid == 0) {
-        const int64_t tok = a.tokens[(int64_t)row * a.s_tok];
-        a.logprob[row] = tok >= 0 && tok < a.n ? logp((float)xr[tok]) : 0.f;
-        a.entropy[row] = s.z == 0.f ? 0.f : (lz - s.e / s.z) * LP_LN2;
+    tv x[2][LP_AHEAD];
+    // a step that the row's start or the part's end cuts
+    auto cut = [&](int from) {
+#pragma unroll
+        for (int k = 0; k < LP_AHEAD; ++k)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                const int i = from + tid * VEC + k * STEP + v;
+                x[0][k][v] = i >= 0 && i < hi ? xr[i] : (T)neg_inf();
+            }
+        add(x[0]);
+    };
+    auto load = [&](tv (&to)[LP_AHEAD], int from) {
+#pragma unroll
+        for (int k = 0; k < LP_AHEAD; ++k)
+            to[k] = stream_load((const tv*)(xr + from + tid * VEC + k * STEP));
+    };
+    constexpr int ALL = LP_AHEAD * STEP;
+    int at = lo;
+    if (at < 0) {
+        cut(at);
+        at += ALL;
     }
-    if (tid < top) {
-        const uint64_t key = sm.kept[tid];
-        a.top_val[(int64_t)row * top + tid] = logp(key_value((uint32_t)(key >> 32)));
-        a.top_id[(int64_t)row * top + tid] = (uint32_t)~(uint32_t)key;
+    if (at + ALL <= hi) {
+        load(x[0], at);
+        while (true) {
+            const bool one = at + 2 * ALL <= hi;
+            if (one) load(x[1], at + ALL);
+            add(x[0]);
+            at += ALL;
+            if (!one) break;
+            const bool two = at + 2 * ALL <= hi;
+            if (two) load(x[0], at + ALL);
+            add(x[1]);
+            at += ALL;
+            if (!two) break;
+        }
     }
+    if (at < hi) cut(at);
+    finish<false, F32>(a, sm, group_sums(sm, s), xr, row, part);
 }
 
-// Logits a thread holds for these sizes.
-static int held(int rows, int n) {
-    const int64_t part = LP_THREADS * LP_LONG;
-    return rows * ((n + 7 + part - 1) / part) <= 128 ? LP_SHORT : LP_LONG;
-}
-
-int logprob_parts(int rows, int n) {
+// How a call is split: held parts of LP_THREADS times `held` logits, or (held 0) streamed
+// ones of part_len.
+struct LogprobPlan {
+    int held, parts, part_len;
+};
+static LogprobPlan plan(int rows, int n, int top) {
     // (a row that does not start on 16 bytes takes up to 7 entries more)
-    const int part = LP_THREADS * held(rows, n);
-    return (n + 7 + part - 1) / part;
+    const int64_t all = (int64_t)n + 7;
+    auto count = [&](int64_t len) { return (int)((all + len - 1) / len); };
+    const int64_t longs = LP_THREADS * LP_LONG;
+    if (rows * (int64_t)count(longs) <= 128)
+        return {LP_SHORT, count(LP_THREADS * LP_SHORT), LP_THREADS * LP_SHORT};
+    if (top) return {LP_LONG, count(longs), (int)longs};
+    // none of less than a held part
+    int64_t len = all / ((LP_GROUPS + rows - 1) / rows);
+    len = (len + longs - 1) / longs * longs;
+    return {0, count(len), (int)len};
 }
+
+int logprob_parts(int rows, int n, int top) { return plan(rows, n, top).parts; }
 
 template <bool F32, bool TOP>
-static void launch_held(const LogprobParams& a, hipStream_t stream) {
+static void launch_held(const LogprobParams& a, int held, hipStream_t stream) {
     const dim3 grid((unsigned)((int64_t)a.rows * a.parts)), block(LP_THREADS);
-    if (held(a.rows, a.n) == LP_SHORT)
+    if (held == LP_SHORT)
         hipLaunchKernelGGL((logprob_kernel<F32, TOP, LP_SHORT>), grid, block, 0, stream, a);
-    else
+    else if constexpr (TOP)
         hipLaunchKernelGGL((logprob_kernel<F32, TOP, LP_LONG>), grid, block, 0, stream, a);
+    else
+        hipLaunchKernelGGL(logprob_stream_kernel<F32>, grid, block, 0, stream, a);
 }
 
 hipError_t launch_token_logprobs(const LogprobParams& a, int fp32, hipStream_t stream) {
-    if (fp32 && a.top) launch_held<true, true>(a, stream);
-    else if (fp32) launch_held<true, false>(a, stream);
-    else if (a.top) launch_held<false, true>(a, stream);
-    else launch_held<false, false>(a, stream);
+    const LogprobPlan p = plan(a.rows, a.n, a.top);
+    LogprobParams d = a;
+    d.part_len = p.part_len;
+    if (fp32 && a.top) launch_held<true, true>(d, p.held, stream);
+    else if (fp32) launch_held<true, false>(d, p.held, stream);
+    else if (a.top) launch_held<false, true>(d, p.held, stream);
+    else launch_held<false, false>(d, p.held, stream);
     return hipGetLastError();
 }
 

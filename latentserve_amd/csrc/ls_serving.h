@@ -115,10 +115,11 @@ struct LogprobParams {
     float* part;                  // [rows * parts] records
     int32_t* counters;            // [rows], zero at rest
     int rows, n, top, parts;
+    int part_len;                 // of a streamed part (set at launch)
 };
 
 // Parts a row is split over, and the floats of a part's record.
-int logprob_parts(int rows, int n);
+int logprob_parts(int rows, int n, int top);
 constexpr int logprob_record_floats(int top) { return 4 + 2 * top; }
 hipError_t launch_token_logprobs(const LogprobParams& a, int fp32, hipStream_t stream);
 

@@ -281,14 +281,14 @@ int ls_page_copy(void* const* tensors, const int64_t* page_strides, const int64_
 
 size_t ls_token_logprobs_workspace_bytes(int rows, int n, int top) {
     if (rows < 1 || n < 1 || top < 0 || top > ls::LOGPROB_MAX_TOP) return 0;
-    const int parts = ls::logprob_parts(rows, n);
+    const int parts = ls::logprob_parts(rows, n, top);
     if (parts == 1) return 0;
     return (size_t)rows * parts * ls::logprob_record_floats(top) * sizeof(float);
 }
 
-size_t ls_token_logprobs_counter_ints(int rows, int n) {
+size_t ls_token_logprobs_counter_ints(int rows, int n, int top) {
     if (rows < 1 || n < 1) return 0;
-    return ls::logprob_parts(rows, n) == 1 ? 0 : (size_t)rows;
+    return ls::logprob_parts(rows, n, top) == 1 ? 0 : (size_t)rows;
 }
 
 int ls_token_logprobs(const void* x, int64_t x_stride, int elem_bytes, const int64_t* tokens,
@@ -307,7 +307,7 @@ int ls_token_logprobs(const void* x, int64_t x_stride, int elem_bytes, const int
     if (!aligned(x, elem_bytes)) return fail(LS_ERR_INVALID, "x must be aligned to its elements");
     if (rows == 0) return LS_OK;
     ls::LogprobParams a;
-    a.parts = ls::logprob_parts(rows, n);
+    a.parts = ls::logprob_parts(rows, n, top);
     if ((int64_t)rows * a.parts > (1LL << 31) - 1)
         return fail(LS_ERR_INVALID, "rows x n too large for one call");
     if (a.parts > 1) {

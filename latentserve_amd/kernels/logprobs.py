@@ -68,7 +68,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
             if need:
                 work = torch.empty(need, dtype=torch.uint8, device=dev)
                 cnt = _serving.counters(dev, stream,
-                                        lib.ls_token_logprobs_counter_ints(rows, n))
+                                        lib.ls_token_logprobs_counter_ints(rows, n, top))
             rc = lib.ls_token_logprobs(
                 x.data_ptr(), x.stride(0) if rows > 1 else n, size, tok.data_ptr(),
                 tok.stride(0) if rows > 1 else 1, both.data_ptr(), both.data_ptr() + 4 * rows,

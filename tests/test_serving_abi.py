@@ -20,7 +20,7 @@ from latentserve_amd.kernels.hip import page_copy as pc
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 HEADER = os.path.join(ROOT, "include", "latentserve_amd_serving.h")
-DECLARATIONS = (1, "3fc4cc8fe9823459")
+DECLARATIONS = (1, "7a1d70adfe011700")
 
 
 def _text():

@@ -18,7 +18,6 @@ from latentserve_amd import _lib
 
 _VP = ctypes.c_void_p
 _I64P = ctypes.POINTER(ctypes.c_int64)
-_I32P = ctypes.POINTER(ctypes.c_int32)
 _I32 = ctypes.c_int
 _F32 = ctypes.c_float
 _I64 = ctypes.c_int64
@@ -38,7 +37,7 @@ _SIGNATURES = {
     "ls_paged_decode_int4": [_VP, _I64P, _VP, _VP, _VP, _VP, _I64P, _I64, _VP, _I64, _I32, _VP,
                              _VP, _I64P, _VP, _SZ, _VP, _I32, _I32, _I32, _I32, _I32, _I32, _F32,
                              _VP],
-    "ls_page_copy": [_VP, _I64P, _I64P, _I32, _I64, _I32P, _I32P, _I32, _VP],
+    "ls_page_copy": [_VP, _VP, _VP, _I32, _I64, _VP, _VP, _I32, _VP],
     "ls_token_logprobs_workspace_bytes": [_I32, _I32, _I32],
     "ls_token_logprobs_counter_ints": [_I32, _I32, _I32],
     "ls_token_logprobs": [_VP, _I64, _I32, _VP, _I64, _VP, _VP, _VP, _VP, _VP, _SZ, _VP, _I32,
@@ -94,31 +93,35 @@ def _slab(device: torch.device) -> None:
     _slabs[device.index] = [slab, 0]
 
 
+# (what torch.cuda.is_current_stream_capturing and current_device wrap, without their
+# checks that CUDA is initialised: a launch's stream lookup has done that)
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_NOTHING = contextlib.nullcontext()
+
+
 def counters(device: torch.device, stream: int, ints: int) -> torch.Tensor:
     """At least `ints` zeroed counters for one call on `stream` of `device`."""
-    if torch.cuda.is_current_stream_capturing():
+    index = device.index
+    have = _slabs.get(index)
+    if _capturing():
         take = -(-ints // 32) * 32                       # whole 128-byte lines
-        have = _slabs.get(device.index)
         if have is None or have[1] + take > _SLAB_INTS:
             return torch.zeros(ints, dtype=torch.int32, device=device)
         at = have[1]
         have[1] += take
         return have[0][at:at + take]
-    have = _slabs.get(device.index)
     if have is None or 2 * have[1] > _SLAB_INTS:         # room for the captures to come
         _slab(device)
-    key = (device.index, stream)
-    buf = _by_stream.get(key)
+    buf = _by_stream.get((index, stream))
     if buf is None or buf.numel() < ints:
         if buf is not None:
             _kept.append(buf)
         buf = torch.zeros(max(ints, 4096), dtype=torch.int32, device=device)
-        _by_stream[key] = buf
+        _by_stream[index, stream] = buf
     return buf
 
 
 def on(device: torch.device):
     """`device` as the current one for a launch (nothing to do where it is)."""
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    return _NOTHING if device.index == _current_device() else torch.cuda.device(device)

@@ -33,6 +33,7 @@ HEAD_DIM = 128
 PAGE = 16
 GROUP = 32
 MAX_NREP = 16
+_SCALE = 1.0 / math.sqrt(HEAD_DIM)
 
 _SHAPES = ((PAGE, 64), (PAGE, 4, 2), (16, PAGE, 4), (4, 4, 2, 4))
 _INNER = ((64, 1), (8, 2, 1), (64, 4, 1), (32, 8, 4, 1))
@@ -55,8 +56,25 @@ def empty_pools(num_blocks: int, kv_heads: int, device) -> Int4Pools:
 
 def _pools(pools, written: bool = False):
     """(num_blocks, heads, C arguments) of checked pools."""
-    if len(pools) != 4:
-        raise ValueError("4-bit pools are (k_codes, k_affine, v_codes, v_affine)")
+    try:
+        kc, ka, vc, va = pools
+    except (TypeError, ValueError):
+        raise ValueError("4-bit pools are (k_codes, k_affine, v_codes, v_affine)") from None
+    nb, h = kc.shape[:2]
+    if kc.dtype is vc.dtype is torch.uint8 and ka.dtype is va.dtype is torch.float16 \
+            and kc.shape == (nb, h, PAGE, 64) and ka.shape == (nb, h, PAGE, 4, 2) \
+            and vc.shape == (nb, h, 16, PAGE, 4) and va.shape == (nb, h, 4, 4, 2, 4) \
+            and kc.is_contiguous() and ka.is_contiguous() and vc.is_contiguous() \
+            and va.is_contiguous() \
+            and kc.get_device() == ka.get_device() == vc.get_device() == va.get_device():
+        codes, affine = h * 1024, h * 256
+        return nb, h, (kc.data_ptr(), ka.data_ptr(), vc.data_ptr(), va.data_ptr(),
+                       _lib._I64N[4](codes, affine, codes, affine), nb)
+    return _uncommon_pools(pools, written)
+
+
+def _uncommon_pools(pools, written: bool):
+    """The same for pools that are not simply contiguous, or not pools."""
     nb, h = pools[0].shape[:2]
     dev = pools[0].device
     steps = []
@@ -73,35 +91,52 @@ def _pools(pools, written: bool = False):
         if written and nb > 1 and st[0] < h * head:
             raise ValueError(f"{name}: pages that overlap cannot be written")
         steps.append(st[0] * t.element_size())
-    return nb, h, (pools[0].data_ptr(), pools[1].data_ptr(), pools[2].data_ptr(),
-                   pools[3].data_ptr(), _lib._I64N[4](*steps), nb)
+    return nb, h, (*(t.data_ptr() for t in pools), _lib._I64N[4](*steps), nb)
 
 
-def _rows(name: str, t: torch.Tensor) -> None:
-    if t.dtype != torch.float16:
+def _rows(name: str, t: torch.Tensor):
+    """The strides of checked rows [., ., ., 128]; a dimension of one row has none that
+    matters."""
+    if t.dtype is not torch.float16:
         raise ValueError(f"{name} must be float16, got {t.dtype}")
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or any(
-            s % 8 for s, n in zip(t.stride()[:-1], t.shape) if n > 1):
-        raise ValueError(f"{name} rows must be 16-byte aligned and unit-stride")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient, which a 4-bit cache does not carry")
+    s0, s1, s2, unit = t.stride()
+    n0, n1, n2, _ = t.shape
+    s0, s1, s2 = (s0 if n0 > 1 else 0), (s1 if n1 > 1 else 0), (s2 if n2 > 1 else 0)
+    if unit != 1 or t.data_ptr() & 15 or (s0 | s1 | s2) & 7:
+        raise ValueError(f"{name} rows must be 16-byte aligned and unit-stride")
+    return _lib._I64N[3](s0, s1, s2)
 
 
-def _strides(t: torch.Tensor):
-    """The first three strides; a dimension of one row has none that matters."""
-    return _lib._I64N[3](*(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape)))
-
-
-def _tables(block_tables: torch.Tensor, seq_lens: torch.Tensor, b: int, device) -> None:
-    if block_tables.dtype != torch.int32 or seq_lens.dtype != torch.int32 \
-            or block_tables.dim() != 2 or block_tables.stride(-1) != 1 \
-            or (b > 1 and seq_lens.stride(-1) != 1):
+def _tables(block_tables: torch.Tensor, seq_lens: torch.Tensor, b: int, device: int) -> None:
+    if block_tables.dtype is not torch.int32 or seq_lens.dtype is not torch.int32 \
+            or block_tables.dim() != 2 or seq_lens.shape != (b,) or block_tables.stride(1) != 1 \
+            or (b > 1 and seq_lens.stride(0) != 1):
         raise ValueError("block tables [B, pages] and sequence lengths [B] must be unit-stride "
-                         "int32")
-    if block_tables.shape[0] != b or seq_lens.shape != (b,):
-        raise ValueError(f"block tables and sequence lengths must have {b} rows")
-    if block_tables.device != device or seq_lens.device != device:
+                         f"int32, of {b} sequences")
+    if block_tables.shape[0] != b:
+        raise ValueError(f"block tables must have {b} rows")
+    if block_tables.get_device() != device or seq_lens.get_device() != device:
         raise ValueError("block tables and sequence lengths must be on the pools' device")
+
+
+# Launch sizes by a decode's shape: (groups, workspace bytes, counters).
+_SIZES: dict = {}
+
+
+def _sizes(b: int, h: int, n_rep: int, width: int, bound: int):
+    key = (b, h, n_rep, width, bound)
+    got = _SIZES.get(key)
+    if got is None:
+        lib = _serving.lib()
+        groups = lib.ls_int4_decode_groups(b, h, width, bound)
+        got = (groups, lib.ls_int4_decode_workspace_bytes(groups, h, n_rep),
+               lib.ls_int4_decode_counter_ints(groups, h))
+        if len(_SIZES) >= 4096:
+            _SIZES.clear()
+        _SIZES[key] = got
+    return got
 
 
 def write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, pools) -> None:
@@ -117,16 +152,16 @@ def write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, pools) -> None:
     if slots.dtype != torch.int64 or slots.shape != (b * n,) \
             or (b * n > 1 and slots.stride(0) != 1):
         raise ValueError(f"slots must be {b * n} unit-stride int64 values")
-    if k.device != dev or v.device != dev or slots.device != dev:
+    index = pools[0].get_device()
+    if k.get_device() != index or v.get_device() != index or slots.get_device() != index:
         raise ValueError("k, v and slots must be on the pools' device")
     stream = _lib.stream_of(dev)
     if b * n == 0:
         return
-    _rows("k", k)
-    _rows("v", v)
+    ks, vs = _rows("k", k), _rows("v", v)
     with _serving.on(dev):
-        rc = _serving.lib().ls_int4_write(k.data_ptr(), _strides(k), v.data_ptr(), _strides(v),
-                                          slots.data_ptr(), *args, b, h, n, HEAD_DIM, PAGE, stream)
+        rc = _serving.lib().ls_int4_write(k.data_ptr(), ks, v.data_ptr(), vs, slots.data_ptr(),
+                                          *args, b, h, n, HEAD_DIM, PAGE, stream)
     _lib.check(rc, "ls_int4_write")
 
 
@@ -138,13 +173,13 @@ def read(pools, block_tables: torch.Tensor, seq_lens: torch.Tensor,
     nb, h, args = _pools(pools)
     dev = pools[0].device
     b = block_tables.shape[0]
-    _tables(block_tables, seq_lens, b, dev)
+    _tables(block_tables, seq_lens, b, pools[0].get_device())
     length = block_tables.shape[1] * PAGE if length is None else int(length)
     if length < 0:
         raise ValueError(f"length must be >= 0, got {length}")
     stream = _lib.stream_of(dev)
-    k, v = (torch.empty(b, length, h, HEAD_DIM, dtype=torch.float16, device=dev)
-            for _ in range(2))
+    k = torch.empty((b, length, h, HEAD_DIM), dtype=torch.float16, device=dev)
+    v = torch.empty((b, length, h, HEAD_DIM), dtype=torch.float16, device=dev)
     if b * length:
         if block_tables.shape[1] == 0:
             k.zero_(), v.zero_()
@@ -174,34 +209,31 @@ def paged_decode_int4(q: torch.Tensor, pools, block_tables: torch.Tensor, seq_le
             or not 1 <= q.shape[2] <= MAX_NREP:
         raise ValueError(f"q must be [B, {h}, n_rep 1..{MAX_NREP}, {HEAD_DIM}], got "
                          f"{tuple(q.shape)}")
-    if q.device != dev:
+    if q.get_device() != pools[0].get_device():
         raise ValueError("q must be on the pools' device")
     b, _, n_rep, _ = q.shape
-    _tables(block_tables, seq_lens, b, dev)
+    _tables(block_tables, seq_lens, b, pools[0].get_device())
     stream = _lib.stream_of(dev)
-    _rows("q", q)
+    qs = _rows("q", q)
     if out is None:
         out = torch.empty((b, h, n_rep, HEAD_DIM), dtype=torch.float16, device=dev)
-    else:
-        if out.shape != q.shape or out.device != dev:
-            raise ValueError(f"out must be {tuple(q.shape)} on {dev}")
-        _rows("out", out)
+    elif out.shape != q.shape or out.device != dev:
+        raise ValueError(f"out must be {tuple(q.shape)} on {dev}")
+    os = _rows("out", out)
     if b == 0:
         return out
     width = block_tables.shape[1]
     if width == 0:
         return out.zero_()
-    lib = _serving.lib()
-    bound = 0 if max_seq_len is None else max(1, int(max_seq_len))
-    groups = lib.ls_int4_decode_groups(b, h, width, bound)
-    nbytes = lib.ls_int4_decode_workspace_bytes(groups, h, n_rep)
-    scale = 1.0 / math.sqrt(HEAD_DIM) if softmax_scale is None else float(softmax_scale)
+    groups, nbytes, ints = _sizes(b, h, n_rep, width,
+                                  0 if max_seq_len is None else max(1, int(max_seq_len)))
+    scale = _SCALE if softmax_scale is None else float(softmax_scale)
     with _serving.on(dev):
         work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        cnt = _serving.counters(dev, stream, lib.ls_int4_decode_counter_ints(groups, h))
-        rc = lib.ls_paged_decode_int4(
-            q.data_ptr(), _strides(q), *args, block_tables.data_ptr(), block_tables.stride(0),
-            width, seq_lens.data_ptr(), out.data_ptr(), _strides(out), work.data_ptr(), nbytes,
-            cnt.data_ptr(), b, h, n_rep, HEAD_DIM, PAGE, groups, scale, stream)
+        cnt = _serving.counters(dev, stream, ints)
+        rc = _serving.lib().ls_paged_decode_int4(
+            q.data_ptr(), qs, *args, block_tables.data_ptr(), block_tables.stride(0), width,
+            seq_lens.data_ptr(), out.data_ptr(), os, work.data_ptr(), nbytes, cnt.data_ptr(), b, h,
+            n_rep, HEAD_DIM, PAGE, groups, scale, stream)
     _lib.check(rc, "ls_paged_decode_int4")
     return out

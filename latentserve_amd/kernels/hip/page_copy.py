@@ -7,8 +7,8 @@ numbers in the launch's arguments.
 
 from __future__ import annotations
 
-import ctypes
 import operator
+from array import array
 from typing import Sequence
 
 import torch
@@ -37,36 +37,57 @@ def copy_pages(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequenc
     if not tensors:
         return
     first = tensors[0]
-    pages, dev = first.shape[0] if first.dim() else 0, first.device
-    count = len(tensors)
-    ptrs, steps, sizes = ((ctypes.c_int64 * count)() for _ in range(3))
-    for i, t in enumerate(tensors):
-        if t.dim() == 0 or t.shape[0] != pages:
-            raise ValueError(f"every tensor must have {pages} pages, got {tuple(t.shape)}")
-        if t.device != dev:
-            raise ValueError("the tensors must be on one device")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise ValueError("a page copy records no gradient")
-        elems = 1
-        st = t.stride()
-        for k in range(t.dim() - 1, 0, -1):
-            if t.shape[k] != 1 and st[k] != elems and t.numel():
-                raise ValueError("a page's elements must be contiguous")
-            elems *= t.shape[k]
-        size = t.element_size()
-        ptrs[i], steps[i], sizes[i] = t.data_ptr(), st[0] * size, elems * size
+    dev = first.device
+    count, pages = len(tensors), first.shape[0] if first.dim() else 0
+    if any(map(_ndim_0, tensors)) or set(map(len, tensors)) != {pages}:
+        raise ValueError(f"every tensor must have {pages} pages, got "
+                         f"{[tuple(t.shape) for t in tensors][:8]}")
+    if set(map(torch.Tensor.get_device, tensors)) != {first.get_device()}:
+        raise ValueError("the tensors must be on one device")
+    if torch.is_grad_enabled() and any(map(_requires_grad, tensors)):
+        raise ValueError("a page copy records no gradient")
+    if all(map(torch.Tensor.is_contiguous, tensors)):
+        sizes = steps = array("q", [b // pages if pages else 0 for b in map(_nbytes, tensors)])
+    else:
+        steps, sizes = _layouts(tensors)
     stream = _lib.stream_of(dev)
     if n == 0:
         return
     if min(min(src), min(dst)) < 0 or max(max(src), max(dst)) >= pages:
         raise ValueError(f"page numbers must be in [0, {pages})")      # (before 32 bits wrap them)
-    if any(size == 0 for size in sizes):
+    ptrs = array("q", map(torch.Tensor.data_ptr, tensors))
+    if 0 in sizes:
         keep = [i for i in range(count) if sizes[i]]
-        ptrs, steps, sizes = ((ctypes.c_int64 * len(keep))(*(a[i] for i in keep))
-                              for a in (ptrs, steps, sizes))
+        ptrs, steps, sizes = (array("q", [a[i] for i in keep]) for a in (ptrs, steps, sizes))
         count = len(keep)
+    s, d = array("i", src), array("i", dst)
     with _serving.on(dev):
-        rc = _serving.lib().ls_page_copy(ctypes.cast(ptrs, ctypes.c_void_p), steps, sizes, count,
-                                         pages, (ctypes.c_int32 * n)(*src),
-                                         (ctypes.c_int32 * n)(*dst), n, stream)
+        rc = _serving.lib().ls_page_copy(*map(_address, (ptrs, steps, sizes)), count, pages,
+                                         _address(s), _address(d), n, stream)
     _lib.check(rc, "ls_page_copy")
+
+
+_nbytes = operator.attrgetter("nbytes")
+_requires_grad = operator.attrgetter("requires_grad")
+
+
+def _ndim_0(t: torch.Tensor) -> bool:
+    return t.ndim == 0
+
+
+def _address(a: array) -> int:
+    return a.buffer_info()[0]
+
+
+def _layouts(tensors):
+    """Bytes from page to page, and of a page, of tensors that are not all contiguous."""
+    steps, sizes = array("q"), array("q")
+    for t in tensors:
+        elems, st = 1, t.stride()
+        for k in range(t.dim() - 1, 0, -1):
+            if t.shape[k] != 1 and st[k] != elems and t.numel():
+                raise ValueError("a page's elements must be contiguous")
+            elems *= t.shape[k]
+        steps.append(st[0] * t.element_size())
+        sizes.append(elems * t.element_size())
+    return steps, sizes

@@ -37,11 +37,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError("logits must be [..., n]")
     lead, n = logits.shape[:-1], logits.shape[-1]
+    flat = len(lead) == 1
     if tokens.dtype != torch.int64 or tokens.shape != lead:
         raise ValueError(f"tokens must be int64 {tuple(lead)}, got {tokens.dtype} "
                          f"{tuple(tokens.shape)}")
     dev = logits.device
-    if tokens.device != dev:
+    if tokens.get_device() != logits.get_device():
         raise ValueError("tokens must be on the logits' device")
     if logits.requires_grad and torch.is_grad_enabled():
         raise ValueError("logits require a gradient, which token_logprobs does not record")
@@ -49,10 +50,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     if not 0 <= top <= min(MAX_TOP, n):
         raise ValueError(f"top must be in [0, {min(MAX_TOP, n)}], got {top}")
     stream = _lib.stream_of(dev)
-    x = logits.reshape(-1, n)
-    if n > 1 and x.stride(-1) != 1:
+    x = logits if flat else logits.reshape(-1, n)
+    if n > 1 and x.stride(1) != 1:
         x = x.contiguous()
-    tok = tokens.reshape(-1)
+    tok = tokens if flat else tokens.reshape(-1)
     rows = x.shape[0]
     both = torch.empty((2, rows), dtype=torch.float32, device=dev)
     val = ids = None
@@ -60,21 +61,38 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
         val = torch.empty((rows, top), dtype=torch.float32, device=dev)
         ids = torch.empty((rows, top), dtype=torch.int64, device=dev)
     if rows:
-        lib = _serving.lib()
         size = x.element_size()
-        need = lib.ls_token_logprobs_workspace_bytes(rows, n, top)
+        need, ints = _sizes(rows, n, top)
         with _serving.on(dev):
             work = cnt = None
             if need:
                 work = torch.empty(need, dtype=torch.uint8, device=dev)
-                cnt = _serving.counters(dev, stream,
-                                        lib.ls_token_logprobs_counter_ints(rows, n, top))
-            rc = lib.ls_token_logprobs(
+                cnt = _serving.counters(dev, stream, ints)
+            rc = _serving.lib().ls_token_logprobs(
                 x.data_ptr(), x.stride(0) if rows > 1 else n, size, tok.data_ptr(),
                 tok.stride(0) if rows > 1 else 1, both.data_ptr(), both.data_ptr() + 4 * rows,
                 _lib.ptr(val), _lib.ptr(ids), _lib.ptr(work), need, _lib.ptr(cnt), rows, n, top,
                 stream)
         _lib.check(rc, "ls_token_logprobs")
-    return TokenLogprobs(both[0].view(lead), both[1].view(lead),
+    logprob, entropy = both.unbind(0)
+    if flat:
+        return TokenLogprobs(logprob, entropy, val, ids)
+    return TokenLogprobs(logprob.view(lead), entropy.view(lead),
                          None if val is None else val.view(*lead, top),
                          None if ids is None else ids.view(*lead, top))
+
+
+# Workspace bytes and counters by a call's sizes.
+_SIZES: dict = {}
+
+
+def _sizes(rows: int, n: int, top: int):
+    got = _SIZES.get((rows, n, top))
+    if got is None:
+        lib = _serving.lib()
+        got = (lib.ls_token_logprobs_workspace_bytes(rows, n, top),
+               lib.ls_token_logprobs_counter_ints(rows, n, top))
+        if len(_SIZES) >= 4096:
+            _SIZES.clear()
+        _SIZES[rows, n, top] = got
+    return got

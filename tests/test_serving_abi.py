@@ -125,8 +125,8 @@ def test_nothing_to_do_is_no_launch(lib):
 
 def _copy(lib, src, dst, pages=10, stride=4096, size=4096, base=1 << 20):
     n = len(src)
-    one = lambda v: _st(v)  # noqa: E731
-    return lib.ls_page_copy(ctypes.cast(one(base), ctypes.c_void_p), one(stride), one(size), 1, pages,
+    one = lambda v: ctypes.cast(_st(v), ctypes.c_void_p)  # noqa: E731
+    return lib.ls_page_copy(one(base), one(stride), one(size), 1, pages,
                             (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst), n, None)
 
 

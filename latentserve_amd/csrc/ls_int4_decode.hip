@@ -376,6 +376,13 @@ void int4_decode_kernel(const Int4DecodeParams a) {
         return a.tables[(int64_t)bt * a.st_b + (p < a.max_pages ? p : a.max_pages - 1)];
     };
     int entry = first_entries(b, s0);
+    // ... and the group's first ones, a thread each, requested ahead of any page so
+    // that the table need not wait for one
+    auto table_entry = [&](int bt, int from) {
+        const int p = from + (int)threadIdx.x;
+        return a.tables[(int64_t)bt * a.st_b + (p < a.max_pages ? p : a.max_pages - 1)];
+    };
+    int filled = table_entry(b, s0);
 
     Int4Page page[2][2];
     int item[2], blk[2][2];
@@ -409,7 +416,7 @@ void int4_decode_kernel(const Int4DecodeParams a) {
         // what the next sequence of the run needs, ahead of its turn
         const int b_next = more ? b + 1 : b;
         const int len_next = a.lens[b_next];
-        int entry_next = first_entries(b_next, 0);
+        const int entry_next = first_entries(b_next, 0), filled_next = table_entry(b_next, 0);
         load_q(b_next, q_raw);
 
         Int4State st;
@@ -427,9 +434,14 @@ void int4_decode_kernel(const Int4DecodeParams a) {
             if (c0 != s0) {
                 __syncthreads();                           // the piece before is claimed out
                 entry = first_entries(b, c0);
+                filled = table_entry(b, c0);
                 request_first(c0, s1, pages);
             }
-            for (int i = threadIdx.x; i < 2 * pairs; i += WAVE * I4_NW)
+            {
+                const int i = threadIdx.x;
+                if (i < 2 * pairs) sm.blk[i] = i < n_pg && c0 + i < pages ? valid(filled) : -1;
+            }
+            for (int i = threadIdx.x + WAVE * I4_NW; i < 2 * pairs; i += WAVE * I4_NW)
                 sm.blk[i] = i < n_pg && c0 + i < pages ? valid(trow[c0 + i]) : -1;
             if (threadIdx.x == 0) sm.claim = I4_NW;
             __syncthreads();
@@ -448,9 +460,12 @@ void int4_decode_kernel(const Int4DecodeParams a) {
                     if (!live) break;
                     const int it = __builtin_amdgcn_readfirstlane(next);
                     next = claim();                        // (read a step later)
-                    if (it < pairs)
-                        request(z ^ 1, it, __builtin_amdgcn_readfirstlane(sm.blk[2 * it]),
-                                __builtin_amdgcn_readfirstlane(sm.blk[2 * it + 1]));
+                    // (requested past the end too, from no bytes: loads under a branch would
+                    // make the compute wait for them, not for the ones before)
+                    const int at = it < pairs ? it : 0;
+                    const int b0 = __builtin_amdgcn_readfirstlane(sm.blk[2 * at]);
+                    const int b1 = __builtin_amdgcn_readfirstlane(sm.blk[2 * at + 1]);
+                    request(z ^ 1, it, it < pairs ? b0 : -1, it < pairs ? b1 : -1);
                     const int lens[2] = {blk[z][0] >= 0 ? len : 0, blk[z][1] >= 0 ? len : 0};
                     int4_compute(sp, page[z], st, q, (c0 + 2 * item[z]) * PAGE, lens, scale, g);
                     live = it < pairs;
@@ -459,6 +474,7 @@ void int4_decode_kernel(const Int4DecodeParams a) {
         }
         // the next sequence's first pair, on its way while this one is merged
         entry = entry_next;
+        filled = filled_next;
         if (more) {
             const int n2 = pages_of(len_next), start2 = start + n + extra;
             request_first(0, u1 - start2 < n2 ? u1 - start2 : n2, len_next > 0 ? n2 : 0);

@@ -169,7 +169,7 @@ def read(pools, block_tables: torch.Tensor, seq_lens: torch.Tensor,
          length: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """(k, v) [B, H, length, 128] fp16: the values that each sequence's first
     `length` entries stand for (default: the table's width), zeros past its
-    end.  Views of [B, length, H, 128] buffers, as paged_gather.read's."""
+    end.  Views of one [2, B, length, H, 128] buffer."""
     nb, h, args = _pools(pools)
     dev = pools[0].device
     b = block_tables.shape[0]
@@ -178,19 +178,19 @@ def read(pools, block_tables: torch.Tensor, seq_lens: torch.Tensor,
     if length < 0:
         raise ValueError(f"length must be >= 0, got {length}")
     stream = _lib.stream_of(dev)
-    k = torch.empty((b, length, h, HEAD_DIM), dtype=torch.float16, device=dev)
-    v = torch.empty((b, length, h, HEAD_DIM), dtype=torch.float16, device=dev)
+    kv = torch.empty((2, b, length, h, HEAD_DIM), dtype=torch.float16, device=dev)
     if b * length:
         if block_tables.shape[1] == 0:
-            k.zero_(), v.zero_()
+            kv.zero_()
         else:
+            at = kv.data_ptr()
             with _serving.on(dev):
                 rc = _serving.lib().ls_int4_read(
                     *args, block_tables.data_ptr(), block_tables.stride(0),
-                    block_tables.shape[1], seq_lens.data_ptr(), k.data_ptr(), v.data_ptr(), b, h,
+                    block_tables.shape[1], seq_lens.data_ptr(), at, at + kv.nbytes // 2, b, h,
                     HEAD_DIM, PAGE, length, stream)
             _lib.check(rc, "ls_int4_read")
-    return k.permute(0, 2, 1, 3), v.permute(0, 2, 1, 3)
+    return kv.transpose(2, 3).unbind(0)
 
 
 def paged_decode_int4(q: torch.Tensor, pools, block_tables: torch.Tensor, seq_lens: torch.Tensor,
@@ -217,9 +217,11 @@ def paged_decode_int4(q: torch.Tensor, pools, block_tables: torch.Tensor, seq_le
     qs = _rows("q", q)
     if out is None:
         out = torch.empty((b, h, n_rep, HEAD_DIM), dtype=torch.float16, device=dev)
-    elif out.shape != q.shape or out.device != dev:
-        raise ValueError(f"out must be {tuple(q.shape)} on {dev}")
-    os = _rows("out", out)
+        os = _lib._I64N[3](h * n_rep * HEAD_DIM, n_rep * HEAD_DIM, HEAD_DIM)
+    else:
+        if out.shape != q.shape or out.device != dev:
+            raise ValueError(f"out must be {tuple(q.shape)} on {dev}")
+        os = _rows("out", out)
     if b == 0:
         return out
     width = block_tables.shape[1]

@@ -39,7 +39,8 @@ def copy_pages(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequenc
     first = tensors[0]
     dev = first.device
     count, pages = len(tensors), first.shape[0] if first.dim() else 0
-    if any(map(_ndim_0, tensors)) or set(map(len, tensors)) != {pages}:
+    if not first.dim() or any(map(_ndim_0, tensors)) \
+            or set(map(torch.Tensor.size, tensors, (0,) * count)) != {pages}:
         raise ValueError(f"every tensor must have {pages} pages, got "
                          f"{[tuple(t.shape) for t in tensors][:8]}")
     if set(map(torch.Tensor.get_device, tensors)) != {first.get_device()}:

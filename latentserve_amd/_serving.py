@@ -8,8 +8,8 @@ the scratch that their calls take.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import threading
 from typing import Dict, List, Optional
 
 import torch
@@ -73,55 +73,54 @@ def lib() -> ctypes.CDLL:
     return handle
 
 
-# Arrival counters (int32, zero at rest: every call leaves its own at zero).
-# Two calls that may run at once may not share them: a device's streams have one
-# buffer each, and a call recorded into a graph, which may be replayed beside
-# anything, has a slice of its own for good.  Slices come from zero-filled slabs
-# made outside captures; a capture that finds none left has its counters
-# zeroed by the graph itself.
+# Scratch of a call: records (any contents) and arrival counters (int32, zero at rest:
+# every call leaves its own at zero).  Two calls that may run at once may not share
+# it: a device's streams have their own, kept and grown, and a call recorded into a
+# graph, which may be replayed beside anything, has records of the graph's own and a
+# slice of counters for good.  Slices come from zero-filled slabs made outside
+# captures; a capture that finds none left has its counters zeroed by the graph itself.
 _SLAB_INTS = 1 << 18
-_by_stream: Dict[tuple, torch.Tensor] = {}
+_by_stream: Dict[tuple, tuple] = {}   # (device index, stream) -> (records, counters)
 _slabs: Dict[int, List] = {}          # device index -> [newest slab, ints taken]
-_kept: List[torch.Tensor] = []        # slabs and outgrown buffers: graphs may hold their addresses
-
-
-def _slab(device: torch.device) -> None:
-    slab = torch.zeros(_SLAB_INTS, dtype=torch.int32, device=device)
-    # (the fill is on this stream; a graph that takes a slice may replay on any)
-    torch.cuda.current_stream(device).synchronize()
-    _kept.append(slab)
-    _slabs[device.index] = [slab, 0]
-
-
+_kept: List[torch.Tensor] = []        # slabs, whose addresses graphs hold
+_lock = threading.Lock()              # two captures at once may not get one slice
 # (what torch.cuda.is_current_stream_capturing and current_device wrap, without their
 # checks that CUDA is initialised: a launch's stream lookup has done that)
 _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None)
-_current_device = getattr(torch._C, "_cuda_getDevice", None)
-_NOTHING = contextlib.nullcontext()
+current_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
-def counters(device: torch.device, stream: int, ints: int) -> torch.Tensor:
-    """At least `ints` zeroed counters for one call on `stream` of `device`."""
-    index = device.index
-    have = _slabs.get(index)
-    if _capturing():
-        take = -(-ints // 32) * 32                       # whole 128-byte lines
+def _captured_scratch(device: torch.device, nbytes: int, ints: int):
+    work = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    have = _slabs.get(device.index)
+    take = -(-ints // 32) * 32                               # whole 128-byte lines
+    with _lock:
         if have is None or have[1] + take > _SLAB_INTS:
-            return torch.zeros(ints, dtype=torch.int32, device=device)
+            return work, torch.zeros(ints, dtype=torch.int32, device=device)
         at = have[1]
         have[1] += take
-        return have[0][at:at + take]
-    if have is None or 2 * have[1] > _SLAB_INTS:         # room for the captures to come
-        _slab(device)
-    buf = _by_stream.get((index, stream))
-    if buf is None or buf.numel() < ints:
-        if buf is not None:
-            _kept.append(buf)
-        buf = torch.zeros(max(ints, 4096), dtype=torch.int32, device=device)
-        _by_stream[index, stream] = buf
-    return buf
+    return work, have[0][at:at + take]
 
 
-def on(device: torch.device):
-    """`device` as the current one for a launch (nothing to do where it is)."""
-    return _NOTHING if device.index == _current_device() else torch.cuda.device(device)
+def scratch(device: torch.device, stream: int, nbytes: int, ints: int):
+    """(records, counters) tensors of at least these sizes for one call on `stream`, the
+    current one of the current device."""
+    if _capturing():
+        return _captured_scratch(device, nbytes, ints)
+    index = device.index
+    have = _slabs.get(index)
+    if have is None or 2 * have[1] > _SLAB_INTS:             # room for the captures to come
+        slab = torch.zeros(_SLAB_INTS, dtype=torch.int32, device=device)
+        # (filled on this stream; a graph that takes a slice may replay on any)
+        torch.cuda.current_stream(device).synchronize()
+        _kept.append(slab)
+        _slabs[index] = [slab, 0]
+    got = _by_stream.get((index, stream))
+    if got is None or got[0].numel() < nbytes or got[1].numel() < ints:
+        # (an outgrown pair goes back to the allocator, which hands it on in this
+        # stream's order)
+        old = got or (torch.empty(0, dtype=torch.uint8), torch.empty(0, dtype=torch.int32))
+        got = (torch.empty(max(nbytes, old[0].numel(), 1 << 16), dtype=torch.uint8, device=device),
+               torch.zeros(max(ints, old[1].numel(), 4096), dtype=torch.int32, device=device))
+        _by_stream[index, stream] = got
+    return got

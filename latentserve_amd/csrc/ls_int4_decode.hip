@@ -297,7 +297,7 @@ void int4_decode_kernel(const Int4DecodeParams a) {
     // reads: its group stores the zeros.)
     const int extra = a.extra;
     auto pages_of = [&](int len) {
-        int p = len > 0 ? (len + PAGE - 1) / PAGE : 1;
+        int p = len > 0 ? (len - 1) / PAGE + 1 : 1;
         return p < a.max_pages ? p : a.max_pages;
     };
     auto run_of = [&](int T, int& u0, int& u1) {

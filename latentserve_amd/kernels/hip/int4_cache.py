@@ -54,6 +54,9 @@ def empty_pools(num_blocks: int, kv_heads: int, device) -> Int4Pools:
                        for s, d in zip(_SHAPES, _DTYPES)))
 
 
+_STEPS: dict = {}               # contiguous pools' page strides by their heads
+
+
 def _pools(pools, written: bool = False):
     """(num_blocks, heads, C arguments) of checked pools."""
     try:
@@ -67,9 +70,10 @@ def _pools(pools, written: bool = False):
             and kc.is_contiguous() and ka.is_contiguous() and vc.is_contiguous() \
             and va.is_contiguous() \
             and kc.get_device() == ka.get_device() == vc.get_device() == va.get_device():
-        codes, affine = h * 1024, h * 256
-        return nb, h, (kc.data_ptr(), ka.data_ptr(), vc.data_ptr(), va.data_ptr(),
-                       _lib._I64N[4](codes, affine, codes, affine), nb)
+        steps = _STEPS.get(h)
+        if steps is None:
+            steps = _STEPS[h] = _lib._I64N[4](h * 1024, h * 256, h * 1024, h * 256)
+        return nb, h, (kc.data_ptr(), ka.data_ptr(), vc.data_ptr(), va.data_ptr(), steps, nb)
     return _uncommon_pools(pools, written)
 
 
@@ -107,6 +111,12 @@ def _rows(name: str, t: torch.Tensor):
     if unit != 1 or t.data_ptr() & 15 or (s0 | s1 | s2) & 7:
         raise ValueError(f"{name} rows must be 16-byte aligned and unit-stride")
     return _lib._I64N[3](s0, s1, s2)
+
+
+def _span(t: torch.Tensor):
+    """First byte of t and the one behind its last (the gaps between rows included)."""
+    last = sum(s * (n - 1) for s, n in zip(t.stride(), t.shape))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
 def _tables(block_tables: torch.Tensor, seq_lens: torch.Tensor, b: int, device: int) -> None:
@@ -159,9 +169,11 @@ def write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, pools) -> None:
     if b * n == 0:
         return
     ks, vs = _rows("k", k), _rows("v", v)
-    with _serving.on(dev):
-        rc = _serving.lib().ls_int4_write(k.data_ptr(), ks, v.data_ptr(), vs, slots.data_ptr(),
-                                          *args, b, h, n, HEAD_DIM, PAGE, stream)
+    if index != _serving.current_device():
+        with torch.cuda.device(index):
+            return write(k, v, slots, pools)
+    rc = _serving.lib().ls_int4_write(k.data_ptr(), ks, v.data_ptr(), vs, slots.data_ptr(), *args,
+                                      b, h, n, HEAD_DIM, PAGE, stream)
     _lib.check(rc, "ls_int4_write")
 
 
@@ -178,18 +190,19 @@ def read(pools, block_tables: torch.Tensor, seq_lens: torch.Tensor,
     if length < 0:
         raise ValueError(f"length must be >= 0, got {length}")
     stream = _lib.stream_of(dev)
+    if dev.index != _serving.current_device():
+        with torch.cuda.device(dev):
+            return read(pools, block_tables, seq_lens, length)
+    width = block_tables.shape[1]
     kv = torch.empty((2, b, length, h, HEAD_DIM), dtype=torch.float16, device=dev)
-    if b * length:
-        if block_tables.shape[1] == 0:
-            kv.zero_()
-        else:
-            at = kv.data_ptr()
-            with _serving.on(dev):
-                rc = _serving.lib().ls_int4_read(
-                    *args, block_tables.data_ptr(), block_tables.stride(0),
-                    block_tables.shape[1], seq_lens.data_ptr(), at, at + kv.nbytes // 2, b, h,
-                    HEAD_DIM, PAGE, length, stream)
-            _lib.check(rc, "ls_int4_read")
+    if width == 0:
+        kv.zero_()
+    elif b * length:
+        at = kv.data_ptr()
+        rc = _serving.lib().ls_int4_read(
+            *args, block_tables.data_ptr(), block_tables.stride(0), width, seq_lens.data_ptr(), at,
+            at + kv.nbytes // 2, b, h, HEAD_DIM, PAGE, length, stream)
+        _lib.check(rc, "ls_int4_read")
     return kv.transpose(2, 3).unbind(0)
 
 
@@ -201,7 +214,7 @@ def paged_decode_int4(q: torch.Tensor, pools, block_tables: torch.Tensor, seq_le
 
     max_seq_len: the longest sequence expected (a graph's bucket); it only sizes
     the launch, a longer one is attended whole.  Sequences of no tokens give
-    zeros.  Each call has its own scratch, so calls may run at once on several
+    zeros, and blocks outside the pool are skipped.  out may not overlap q.  Each call has its own scratch, so calls may run at once on several
     streams and from several graphs."""
     nb, h, args = _pools(pools)
     dev = pools[0].device
@@ -222,20 +235,22 @@ def paged_decode_int4(q: torch.Tensor, pools, block_tables: torch.Tensor, seq_le
         if out.shape != q.shape or out.device != dev:
             raise ValueError(f"out must be {tuple(q.shape)} on {dev}")
         os = _rows("out", out)
-    if b == 0:
-        return out
+        if b and _span(out)[0] < _span(q)[1] and _span(q)[0] < _span(out)[1]:
+            raise ValueError("out may not overlap q, which other workgroups still read")
+    if dev.index != _serving.current_device():
+        with torch.cuda.device(dev):
+            return paged_decode_int4(q, pools, block_tables, seq_lens, max_seq_len, softmax_scale,
+                                     out)
     width = block_tables.shape[1]
-    if width == 0:
+    if b == 0 or width == 0:
         return out.zero_()
     groups, nbytes, ints = _sizes(b, h, n_rep, width,
                                   0 if max_seq_len is None else max(1, int(max_seq_len)))
     scale = _SCALE if softmax_scale is None else float(softmax_scale)
-    with _serving.on(dev):
-        work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        cnt = _serving.counters(dev, stream, ints)
-        rc = _serving.lib().ls_paged_decode_int4(
-            q.data_ptr(), qs, *args, block_tables.data_ptr(), block_tables.stride(0), width,
-            seq_lens.data_ptr(), out.data_ptr(), os, work.data_ptr(), nbytes, cnt.data_ptr(), b, h,
-            n_rep, HEAD_DIM, PAGE, groups, scale, stream)
+    work, cnt = _serving.scratch(dev, stream, nbytes, ints)
+    rc = _serving.lib().ls_paged_decode_int4(
+        q.data_ptr(), qs, *args, block_tables.data_ptr(), block_tables.stride(0), width,
+        seq_lens.data_ptr(), out.data_ptr(), os, work.data_ptr(), nbytes, cnt.data_ptr(), b, h,
+        n_rep, HEAD_DIM, PAGE, groups, scale, stream)
     _lib.check(rc, "ls_paged_decode_int4")
     return out

@@ -62,9 +62,11 @@ def copy_pages(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequenc
         ptrs, steps, sizes = (array("q", [a[i] for i in keep]) for a in (ptrs, steps, sizes))
         count = len(keep)
     s, d = array("i", src), array("i", dst)
-    with _serving.on(dev):
-        rc = _serving.lib().ls_page_copy(*map(_address, (ptrs, steps, sizes)), count, pages,
-                                         _address(s), _address(d), n, stream)
+    if dev.index != _serving.current_device():
+        with torch.cuda.device(dev):
+            return copy_pages(tensors, src, dst)
+    rc = _serving.lib().ls_page_copy(*map(_address, (ptrs, steps, sizes)), count, pages,
+                                     _address(s), _address(d), n, stream)
     _lib.check(rc, "ls_page_copy")
 
 

@@ -50,31 +50,30 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     if not 0 <= top <= min(MAX_TOP, n):
         raise ValueError(f"top must be in [0, {min(MAX_TOP, n)}], got {top}")
     stream = _lib.stream_of(dev)
+    if dev.index != _serving.current_device():
+        with torch.cuda.device(dev):
+            return token_logprobs(logits, tokens, top)
     x = logits if flat else logits.reshape(-1, n)
     if n > 1 and x.stride(1) != 1:
         x = x.contiguous()
     tok = tokens if flat else tokens.reshape(-1)
     rows = x.shape[0]
-    both = torch.empty((2, rows), dtype=torch.float32, device=dev)
+    logprob = torch.empty((rows,), dtype=torch.float32, device=dev)
+    entropy = torch.empty((rows,), dtype=torch.float32, device=dev)
     val = ids = None
     if top:
         val = torch.empty((rows, top), dtype=torch.float32, device=dev)
         ids = torch.empty((rows, top), dtype=torch.int64, device=dev)
     if rows:
-        size = x.element_size()
         need, ints = _sizes(rows, n, top)
-        with _serving.on(dev):
-            work = cnt = None
-            if need:
-                work = torch.empty(need, dtype=torch.uint8, device=dev)
-                cnt = _serving.counters(dev, stream, ints)
-            rc = _serving.lib().ls_token_logprobs(
-                x.data_ptr(), x.stride(0) if rows > 1 else n, size, tok.data_ptr(),
-                tok.stride(0) if rows > 1 else 1, both.data_ptr(), both.data_ptr() + 4 * rows,
-                _lib.ptr(val), _lib.ptr(ids), _lib.ptr(work), need, _lib.ptr(cnt), rows, n, top,
-                stream)
+        work = cnt = None
+        if need:
+            work, cnt = _serving.scratch(dev, stream, need, ints)
+        rc = _serving.lib().ls_token_logprobs(
+            x.data_ptr(), x.stride(0) if rows > 1 else n, x.element_size(), tok.data_ptr(),
+            tok.stride(0) if rows > 1 else 1, logprob.data_ptr(), entropy.data_ptr(),
+            _lib.ptr(val), _lib.ptr(ids), _lib.ptr(work), need, _lib.ptr(cnt), rows, n, top, stream)
         _lib.check(rc, "ls_token_logprobs")
-    logprob, entropy = both.unbind(0)
     if flat:
         return TokenLogprobs(logprob, entropy, val, ids)
     return TokenLogprobs(logprob.view(lead), entropy.view(lead),

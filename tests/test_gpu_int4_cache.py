@@ -338,3 +338,69 @@ def test_captured_steps_replay_beside_each_other_and_eager_calls():
             check(st["out"], q, a, t, l, rep)
         q, a, t, l, _ = state[0]["host"]
         check(eager, q, a, t, l - 1, "eager")
+
+
+def test_decode_of_runs_longer_than_the_table_in_lds():
+    """More heads than workgroups, so that one takes a whole sequence: runs of thousands of
+    pages, in pieces.  The tables name a few blocks over and over."""
+    h, pages = 520, [2100, 4097, 1, 2048]
+    arrays = ref.random_pools(5, h, 60)
+    g = np.random.default_rng(61)
+    tables = g.integers(0, 5, (4, 4097)).astype(np.int32)
+    ln = np.array([16 * n - 5 for n in pages], np.int32)
+    q = g.standard_normal((4, h, 1, 128)).astype(np.float16)
+    out = i4().paged_decode_int4(dev(q), pools_of(arrays), dev(tables), dev(ln))
+    for hh in (0, 257, 519):
+        part = [np.ascontiguousarray(a[:, hh:hh + 1]) for a in arrays]
+        check(out[:, hh:hh + 1], q[:, hh:hh + 1], part, tables, ln, hh)
+
+
+def test_decode_of_lengths_past_the_table_and_below_zero():
+    q, arrays, tables, ln = attend_case([64, 64, 64], seed=62)
+    for lens in ([1000, 64, 65], [-3, 5, -(1 << 31)]):
+        ln = np.array(lens, np.int32)
+        out = i4().paged_decode_int4(dev(q), pools_of(arrays), dev(tables), dev(ln))
+        check(out, q, arrays, tables, ln, lens)
+
+
+def test_decode_refuses_an_out_that_overlaps_q():
+    q, arrays, tables, ln = attend_case([20, 3], seed=63)
+    x = dev(q)
+    args = (pools_of(arrays), dev(tables), dev(ln))
+    with pytest.raises(ValueError):
+        i4().paged_decode_int4(x, *args, out=x)
+    both = torch.cat((x, x, x))
+    with pytest.raises(ValueError):
+        i4().paged_decode_int4(both[0:2], *args, out=both[1:3])
+
+
+def test_a_row_with_a_nan_query_leaves_the_others():
+    q, arrays, tables, ln = attend_case([700, 40], seed=64)
+    bad = q.copy()
+    bad[0, 1, 2, 5] = np.nan
+    out = i4().paged_decode_int4(dev(bad), pools_of(arrays), dev(tables), dev(ln))
+    assert torch.isnan(out[0, 1, 2]).all()
+    clean = i4().paged_decode_int4(dev(q), pools_of(arrays), dev(tables), dev(ln))
+    out[0, 1, 2] = clean[0, 1, 2]
+    check(out, q, arrays, tables, ln, "nan")
+
+
+def test_many_captures_have_their_own_counters():
+    """More captured calls than one slab of counters holds; all replay rightly."""
+    q, arrays, tables, ln = attend_case([2000, 300], seed=65)
+    args = (dev(q), pools_of(arrays), dev(tables), dev(ln))
+    i4().paged_decode_int4(*args)
+    graphs = []
+    for _ in range(3):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs = [i4().paged_decode_int4(*args) for _ in range(150)]
+        graphs.append((g, outs))
+    for _ in range(2):
+        for g, _ in graphs:
+            g.replay()
+        i4().paged_decode_int4(*args)
+    torch.cuda.synchronize()
+    for _, outs in graphs:
+        for o in (outs[0], outs[77], outs[-1]):
+            check(o, q, arrays, tables, ln, "captures")

@@ -97,8 +97,8 @@ struct PageCopyParams {
 
 // vec: bytes a lane moves at once (16, 8, 4, 2 or 1; every base, stride and
 // size a multiple of it).
-hipError_t launch_page_copy(const PageCopyParams& a, int tensors, int pairs, int max_bytes,
-                            int vec, hipStream_t stream);
+hipError_t launch_page_copy(const PageCopyParams& a, int tensors, int pairs, int vec,
+                            hipStream_t stream);
 
 // ---- token log probabilities ----------------------------------------------------
 constexpr int LOGPROB_MAX_TOP = 32;

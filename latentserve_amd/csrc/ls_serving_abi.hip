@@ -258,20 +258,18 @@ int ls_page_copy(void* const* tensors, const int64_t* page_strides, const int64_
     for (int k0 = 0; k0 < num_tensors; k0 += ls::COPY_TENSORS) {
         const int nt = std::min(num_tensors - k0, ls::COPY_TENSORS);
         uint64_t bits = 16;
-        int most = 0;
         for (int k = 0; k < nt; ++k) {
             a.base[k] = (char*)tensors[k0 + k];
             a.stride[k] = page_strides[k0 + k];
             a.bytes[k] = (int)page_bytes[k0 + k];
             bits |= (uint64_t)(uintptr_t)a.base[k] | (uint64_t)a.stride[k] | (uint64_t)a.bytes[k];
-            most = std::max(most, a.bytes[k]);
         }
         const int vec = (int)(bits & (~bits + 1));          // the lowest bit set: at most 16
         for (int p0 = 0; p0 < pairs; p0 += ls::COPY_PAIRS) {
             const int np = std::min(pairs - p0, ls::COPY_PAIRS);
             std::copy(src + p0, src + p0 + np, a.src);
             std::copy(dst + p0, dst + p0 + np, a.dst);
-            if (int rc = hip_status(ls::launch_page_copy(a, nt, np, most, vec, (hipStream_t)stream),
+            if (int rc = hip_status(ls::launch_page_copy(a, nt, np, vec, (hipStream_t)stream),
                                     "ls_page_copy"))
                 return rc;
         }

@@ -39,8 +39,7 @@ def copy_pages(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequenc
     first = tensors[0]
     dev = first.device
     count, pages = len(tensors), first.shape[0] if first.dim() else 0
-    if not first.dim() or any(map(_ndim_0, tensors)) \
-            or set(map(torch.Tensor.size, tensors, (0,) * count)) != {pages}:
+    if any(shape[:1] != (pages,) for shape in set(map(_shape, tensors))):
         raise ValueError(f"every tensor must have {pages} pages, got "
                          f"{[tuple(t.shape) for t in tensors][:8]}")
     if set(map(torch.Tensor.get_device, tensors)) != {first.get_device()}:
@@ -70,12 +69,9 @@ def copy_pages(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequenc
     _lib.check(rc, "ls_page_copy")
 
 
+_shape = operator.attrgetter("shape")
 _nbytes = operator.attrgetter("nbytes")
 _requires_grad = operator.attrgetter("requires_grad")
-
-
-def _ndim_0(t: torch.Tensor) -> bool:
-    return t.ndim == 0
 
 
 def _address(a: array) -> int:

@@ -111,7 +111,7 @@ __device__ __forceinline__ void int4_load(const Int4DecodeParams& a, Int4Page& d
 }
 
 // Two adjacent pages, the first one's first token tok0; token tok0 + i counts if it is
-// below len[i / 16].  scale >= 0.
+// below len[i / 16].  scale > 0.
 __device__ __forceinline__ void int4_compute(const Splice& sp, const Int4Page (&d)[2],
                                              Int4State& st, const h8 (&q)[4], int tok0,
                                              const int (&len)[2], float scale, int g) {
@@ -153,15 +153,14 @@ __device__ __forceinline__ void int4_compute(const Splice& sp, const Int4Page (&
     top = fmaxf(fmaxf(top, s[0][3]), s[1][0]);
     top = fmaxf(fmaxf(top, s[1][1]), fmaxf(s[1][2], s[1][3]));
     top = group4_max(top);
-    // (a row of -inf only, nothing valid yet: -inf also where scale is 0)
-    const float m_new = fmaxf(st.m, top == neg_inf() ? top : top * scale);
+    // (a row of -inf only has nothing valid yet)
+    const float m_new = fmaxf(st.m, top * scale);
     const float m_use = m_new == neg_inf() ? 0.f : m_new;
     const float alpha = fast_exp2(st.m - m_use);
     h8 pb;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float x = s[i / 4][i % 4];
-        pb[i] = (half_t)fast_exp2(x == neg_inf() ? x : __builtin_fmaf(x, scale, -m_use));
+        pb[i] = (half_t)fast_exp2(__builtin_fmaf(s[i / 4][i % 4], scale, -m_use));
     }
     if (__any(alpha != 1.f)) {
         st.l *= alpha;
@@ -351,10 +350,13 @@ void int4_decode_kernel(const Int4DecodeParams a) {
     }
     if (u1 <= P + extra) return;                     // (none of its pages)
 
-    // q's sign takes the scale's, so that a larger product is a larger score.
-    const float scale = fabsf(a.scale) * I4_LOG2E;
+    // q's sign takes the scale's, so that a larger product is a larger score; a scale of
+    // 0 is the smallest there is (of -inf, a masked score, nothing else would stay -inf).
+    const float scale = fmaxf(fabsf(a.scale) * I4_LOG2E, 0x1p-126f);
     const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
     const Splice sp = make_splice();
+    int mine = 0;                                    // 0, which the compiler does not know
+    asm("" : "+v"(mine));
     // Query rows (past n_rep: row 0, never stored), channels 32 j + 8 g + (0..7).
     auto load_q = [&](int bq, u4 (&t)[4]) {
         const half_t* row = a.q + (int64_t)bq * a.sq_b + (int64_t)h * a.sq_h +
@@ -443,32 +445,42 @@ void int4_decode_kernel(const Int4DecodeParams a) {
             }
             for (int i = threadIdx.x + WAVE * I4_NW; i < 2 * pairs; i += WAVE * I4_NW)
                 sm.blk[i] = i < n_pg && c0 + i < pages ? valid(trow[c0 + i]) : -1;
-            if (threadIdx.x == 0) sm.claim = I4_NW;
+            if (threadIdx.x == 0) sm.claim = 2 * I4_NW;
             __syncthreads();
+            // A step takes the pair whose blocks the step before read from the table,
+            // requests it, computes the one requested before, and meanwhile the pair
+            // after has its blocks read and the one after that is claimed: no step
+            // waits for LDS.
             auto claim = [&]() {
                 int r = 0;
+                // (an address of the lane's own: of one known to be the same in every
+                // lane the compiler would add for the wave and wait for it at once)
                 if (lane == 0)
-                    r = __hip_atomic_fetch_add(&sm.claim, 1, __ATOMIC_RELAXED,
+                    r = __hip_atomic_fetch_add(&sm.claim + mine, 1, __ATOMIC_RELAXED,
                                                __HIP_MEMORY_SCOPE_WORKGROUP);
                 return r;
             };
-            int next = claim();
+            auto blocks = [&](int it) { return *(const u2*)&sm.blk[2 * (it < pairs ? it : 0)]; };
+            int ahead = wv + I4_NW;
+            u2 ahead_blk = blocks(ahead);
+            int claimed = claim();
             bool live = item[0] < pairs;
             while (live) {
 #pragma unroll
                 for (int z = 0; z < 2; ++z) {
                     if (!live) break;
-                    const int it = __builtin_amdgcn_readfirstlane(next);
-                    next = claim();                        // (read a step later)
                     // (requested past the end too, from no bytes: loads under a branch would
                     // make the compute wait for them, not for the ones before)
-                    const int at = it < pairs ? it : 0;
-                    const int b0 = __builtin_amdgcn_readfirstlane(sm.blk[2 * at]);
-                    const int b1 = __builtin_amdgcn_readfirstlane(sm.blk[2 * at + 1]);
-                    request(z ^ 1, it, it < pairs ? b0 : -1, it < pairs ? b1 : -1);
+                    const bool there = ahead < pairs;
+                    const int b0 = __builtin_amdgcn_readfirstlane(ahead_blk.x);
+                    const int b1 = __builtin_amdgcn_readfirstlane(ahead_blk.y);
+                    request(z ^ 1, ahead, there ? b0 : -1, there ? b1 : -1);
+                    ahead = __builtin_amdgcn_readfirstlane(claimed);
+                    ahead_blk = blocks(ahead);
+                    claimed = claim();
                     const int lens[2] = {blk[z][0] >= 0 ? len : 0, blk[z][1] >= 0 ? len : 0};
                     int4_compute(sp, page[z], st, q, (c0 + 2 * item[z]) * PAGE, lens, scale, g);
-                    live = it < pairs;
+                    live = there;
                 }
             }
         }

@@ -221,8 +221,8 @@ int ls_page_copy(void* const* tensors, const int64_t* page_strides, const int64_
                  int pairs, void* stream) {
     if (num_tensors < 0 || pairs < 0 || num_pages < 0)
         return fail(LS_ERR_INVALID, "bad num_tensors, num_pages or pairs");
-    if (num_tensors == 0 || pairs == 0) return LS_OK;
-    if (!tensors || !page_strides || !page_bytes || !src || !dst)
+    if (pairs == 0) return LS_OK;
+    if (!src || !dst || (num_tensors > 0 && (!tensors || !page_strides || !page_bytes)))
         return fail(LS_ERR_INVALID, "null pointer argument");
     for (int k = 0; k < num_tensors; ++k) {
         if (!tensors[k]) return fail(LS_ERR_INVALID, "null pointer argument");

@@ -194,16 +194,19 @@ def read(pools, block_tables: torch.Tensor, seq_lens: torch.Tensor,
         with torch.cuda.device(dev):
             return read(pools, block_tables, seq_lens, length)
     width = block_tables.shape[1]
-    kv = torch.empty((2, b, length, h, HEAD_DIM), dtype=torch.float16, device=dev)
+    token = h * HEAD_DIM
+    kv = torch.empty_strided((2, b, h, length, HEAD_DIM),
+                             (b * length * token, length * token, HEAD_DIM, token, 1),
+                             dtype=torch.float16, device=dev)
     if width == 0:
         kv.zero_()
     elif b * length:
         at = kv.data_ptr()
         rc = _serving.lib().ls_int4_read(
             *args, block_tables.data_ptr(), block_tables.stride(0), width, seq_lens.data_ptr(), at,
-            at + kv.nbytes // 2, b, h, HEAD_DIM, PAGE, length, stream)
+            at + 2 * b * length * token, b, h, HEAD_DIM, PAGE, length, stream)
         _lib.check(rc, "ls_int4_read")
-    return kv.transpose(2, 3).unbind(0)
+    return kv.unbind(0)
 
 
 def paged_decode_int4(q: torch.Tensor, pools, block_tables: torch.Tensor, seq_lens: torch.Tensor,
@@ -229,7 +232,7 @@ def paged_decode_int4(q: torch.Tensor, pools, block_tables: torch.Tensor, seq_le
     stream = _lib.stream_of(dev)
     qs = _rows("q", q)
     if out is None:
-        out = torch.empty((b, h, n_rep, HEAD_DIM), dtype=torch.float16, device=dev)
+        out = torch.empty(b, h, n_rep, HEAD_DIM, dtype=torch.float16, device=dev)
         os = _lib._I64N[3](h * n_rep * HEAD_DIM, n_rep * HEAD_DIM, HEAD_DIM)
     else:
         if out.shape != q.shape or out.device != dev:

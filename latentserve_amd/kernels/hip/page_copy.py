@@ -28,9 +28,9 @@ def copy_pages(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequenc
     try:
         if any(isinstance(p, torch.Tensor) and p.device.type != "cpu" for p in (src, dst)):
             raise TypeError
-        src, dst = (list(map(operator.index, p)) for p in (src, dst))
-    except TypeError:
-        raise ValueError("page numbers must be whole numbers on the host") from None
+        src, dst = array("i", src), array("i", dst)
+    except (TypeError, OverflowError):
+        raise ValueError("page numbers must be whole numbers on the host, below 2^31") from None
     n = len(src)
     if len(dst) != n:
         raise ValueError(f"{n} source pages for {len(dst)} destinations")
@@ -53,19 +53,16 @@ def copy_pages(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequenc
     stream = _lib.stream_of(dev)
     if n == 0:
         return
-    if min(min(src), min(dst)) < 0 or max(max(src), max(dst)) >= pages:
-        raise ValueError(f"page numbers must be in [0, {pages})")      # (before 32 bits wrap them)
     ptrs = array("q", map(torch.Tensor.data_ptr, tensors))
     if 0 in sizes:
         keep = [i for i in range(count) if sizes[i]]
         ptrs, steps, sizes = (array("q", [a[i] for i in keep]) for a in (ptrs, steps, sizes))
         count = len(keep)
-    s, d = array("i", src), array("i", dst)
     if dev.index != _serving.current_device():
         with torch.cuda.device(dev):
             return copy_pages(tensors, src, dst)
     rc = _serving.lib().ls_page_copy(*map(_address, (ptrs, steps, sizes)), count, pages,
-                                     _address(s), _address(d), n, stream)
+                                     _address(src), _address(dst), n, stream)
     _lib.check(rc, "ls_page_copy")
 
 

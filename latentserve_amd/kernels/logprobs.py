@@ -58,12 +58,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
         x = x.contiguous()
     tok = tokens if flat else tokens.reshape(-1)
     rows = x.shape[0]
-    logprob = torch.empty((rows,), dtype=torch.float32, device=dev)
-    entropy = torch.empty((rows,), dtype=torch.float32, device=dev)
+    logprob = torch.empty(rows, dtype=torch.float32, device=dev)
+    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
     val = ids = None
     if top:
-        val = torch.empty((rows, top), dtype=torch.float32, device=dev)
-        ids = torch.empty((rows, top), dtype=torch.int64, device=dev)
+        val = torch.empty(rows, top, dtype=torch.float32, device=dev)
+        ids = torch.empty(rows, top, dtype=torch.int64, device=dev)
     if rows:
         need, ints = _sizes(rows, n, top)
         work = cnt = None

@@ -80,6 +80,10 @@ def test_refused_calls_copy_nothing():
             copy([t], src, dst)
     with pytest.raises(ValueError):
         copy([t, t.cpu()], [0], [1])
+    with pytest.raises(ValueError):
+        copy([t[:, :0]], [0], [10])
+    with pytest.raises(ValueError):
+        copy([t[:0]], [0], [1])
     torch.cuda.synchronize()
     assert torch.equal(t, w)
 

@@ -4,10 +4,15 @@
 //   M = max x, Z = sum exp(x - M), E = sum exp(x - M) (x - M)
 //   logprob(t) = x_t - M - log Z, entropy = log Z - E / Z
 //
-// with 2^x for the exponentials and fp32 sums.  A row is split over workgroups of 256 threads that hold their part in
-// registers; each thread sums against its own maximum, so nothing is exchanged before
-// the sums are made.  Bound by the logits' read and by a quarter-rate exponential a
-// logit, about alike.
+// with 2^x for the exponentials and fp32 sums.  A row is split over workgroups of 256
+// threads that hold their part in registers (one read serves the maximum, the sums and
+// the alternatives); each thread sums against its own maximum, so nothing is exchanged
+// before the sums are made.  Without alternatives a large call streams instead.
+//
+// 1021 fp16 rows of 151936: 57 us, 5.4 TB/s, as a large copy runs; bound by the read.
+// 16 rows with 20 alternatives: 12.0 us (0.9 us of bytes), 1 row without 4.4 us: bound by
+// what each group does once, in turn (load, two exchanges, the ranking, the hand-over to
+// the row's last group and its merge).
 //
 // Top k of a part: the k-th largest of a wave's 64 thread maxima bounds the k-th largest
 // logit from below, so the logits at or over the largest such bound hold the k best;
@@ -28,8 +33,10 @@ namespace ls {
 
 constexpr int LP_THREADS = 256;
 constexpr int LP_WAVES = LP_THREADS / WAVE;
-// Logits a thread holds: 64, or 16 where that leaves more than half of the CUs idle.
-constexpr int LP_LONG = 64, LP_SHORT = 16;
+// Logits a thread holds: 64, or 16 where that makes at most LP_FEW groups, a quarter of the
+// CUs (us with 16 / 64, 20 alternatives: 1 row of 152K 10.0 / 11.6, 4 rows 11.1 / 11.7, 8 rows
+// 13.1 / 11.9; 32 rows of 32K 10.1 / 10.6, 64 rows 11.6 / 10.8).
+constexpr int LP_LONG = 64, LP_SHORT = 16, LP_FEW = 64;
 // Streaming groups a call aims at: two a CU (us at 512 / 1024 / 2048, 152K logits a row: 1021
 // rows 57 / 61 / 62, 600 rows 39 / 40 / -, 300 rows 24 / 24 / -).
 constexpr int LP_GROUPS = 512;
@@ -46,6 +53,11 @@ __device__ __forceinline__ float key_value(uint32_t k) {
     if (k == 0xFFFFFFFFu) return __builtin_nanf("");
     return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
+
+// Keys of fp16 values differ only above these bits, which are 0, or all 1 in negative ones:
+// a bound without them lies at most one value lower.
+template <bool F32>
+constexpr int LOW_BITS = F32 ? 0 : 13;
 
 template <bool TOP>
 struct LogprobSmem {
@@ -121,11 +133,13 @@ __device__ __forceinline__ Sums<F32> group_sums(Smem& sm, Sums<F32> s) {
     return wave_sums(s);
 }
 
-// The k-th largest of the wave's keys (0 where fewer than k lanes have one).
+// The k-th largest of the wave's keys (0 where fewer than k lanes have one), its bits
+// below LOW left 0.
+template <int LOW>
 __device__ __forceinline__ uint32_t wave_kth(uint32_t key, int k) {
     uint32_t ans = 0;
 #pragma unroll
-    for (int bit = 31; bit >= 0; --bit) {
+    for (int bit = 31; bit >= LOW; --bit) {
         const uint32_t cand = ans | (1u << bit);
         if (__builtin_popcountll(__ballot(key >= cand)) >= k) ans = cand;
     }
@@ -134,8 +148,9 @@ __device__ __forceinline__ uint32_t wave_kth(uint32_t key, int k) {
 
 // The largest of the waves' k-th largest keys, at least 1: no more than the k-th
 // largest of all.  (Two barriers; sm.count is 0 after it.)
+template <int LOW>
 __device__ __forceinline__ uint32_t group_bound(LogprobSmem<true>& sm, uint32_t key, int k) {
-    const uint32_t kth = wave_kth(key, k);
+    const uint32_t kth = wave_kth<LOW>(key, k);
     __syncthreads();
     if (threadIdx.x % WAVE == 0) sm.wave_bound[threadIdx.x / WAVE] = kth;
     if (threadIdx.x == 0) sm.count = 0;
@@ -148,6 +163,7 @@ __device__ __forceinline__ uint32_t group_bound(LogprobSmem<true>& sm, uint32_t 
 
 // The k best of the n entries of sm.pool go to sm.kept in order (0: none), ranked by
 // counting after all but a few have been dropped.
+template <int LOW>
 __device__ __forceinline__ void rank_pool(LogprobSmem<true>& sm, int n, int k) {
     const int tid = threadIdx.x;
     const uint64_t* list = sm.pool;
@@ -157,7 +173,7 @@ __device__ __forceinline__ void rank_pool(LogprobSmem<true>& sm, int n, int k) {
             const uint32_t key = (uint32_t)(sm.pool[i] >> 32);
             best = key > best ? key : best;
         }
-        const uint32_t bound = group_bound(sm, best, k);
+        const uint32_t bound = group_bound<LOW>(sm, best, k);
         for (int i = tid; i < n; i += LP_THREADS) {
             const uint64_t key = sm.pool[i];
             if ((uint32_t)(key >> 32) >= bound) {
@@ -237,7 +253,7 @@ __device__ __forceinline__ void finish(const LogprobParams& a, LogprobSmem<TOP>&
                         (const uint64_t*)(recs + (int64_t)(p0 + i % np) * floats + 4) + i / np);
                 __syncthreads();
                 // (absent entries are 0 and never rank before a present one)
-                rank_pool(sm, had + np * top, top);
+                rank_pool<LOW_BITS<F32>>(sm, had + np * top, top);
             }
         }
         s = wave_sums(s);
@@ -306,54 +322,50 @@ __global__ __launch_bounds__(LP_THREADS) void logprob_kernel(const LogprobParams
 #pragma unroll
     for (int v = 1; v < VEC; ++v) best = fmaxf(best, (float)mx[v]);
 
-    const float mine = Sums<F32>::ref(best);
-    Sums<F32> s = {mine == neg_inf() ? 0.f : mine, 0.f, 0.f};
+    const float ref = Sums<F32>::ref(best);
+    Sums<F32> s = {ref == neg_inf() ? 0.f : ref, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < CHUNKS; ++k)
 #pragma unroll
         for (int v = 0; v < VEC; ++v) s.add((float)x[k][v]);
-    s.m = mine;
+    s.m = ref;
 
+    // (the maximum ignores NaN, which ranks first: a thread whose sum is NaN, by one or by
+    // an infinity, counts as holding the largest, a bound made of such threads takes in
+    // all)
+    const bool nan = s.z != s.z;
     s = group_sums(sm, s);
     if constexpr (TOP) {
-        // (the maximum ignores NaN, which ranks first: a NaN makes the thread's key the
-        // largest)
-        bool nan = false, any = false;
+        bool any = false;
 #pragma unroll
         for (int k = 0; k < CHUNKS; ++k) {
             const int i0 = base + k * STEP;
             any = any || (i0 + VEC > 0 && i0 < a.n);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) nan = nan || x[k][v] != x[k][v];
         }
         const uint32_t mine = nan ? 0xFFFFFFFFu : any ? value_key(best) : 0;
-        const uint32_t bound = group_bound(sm, mine, top);
+        const uint32_t bound = group_bound<LOW_BITS<F32>>(sm, mine, top);
         // The entries at or over the bound to the pool (NaN among them; where the bound
         // stands for none, all): a thread counts its own, so it asks for its place once.
         if (mine >= bound) {
-            const float value = key_value(bound);
+            const T value = (T)key_value(bound);         // (of one of the logits, or NaN)
             uint64_t hits = 0;
 #pragma unroll
             for (int k = 0; k < CHUNKS; ++k) {
                 const int i0 = base + k * STEP;
                 uint32_t hit = 0;
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) hit |= (float)x[k][v] < value ? 0u : 1u << v;
+                for (int v = 0; v < VEC; ++v) hit |= x[k][v] < value ? 0u : 1u << v;
                 const int from = i0 < 0 ? -i0 : 0, to = a.n - i0 < VEC ? a.n - i0 : VEC;
                 hit &= to > from ? (1u << to) - (1u << from) : 0u;
                 hits |= (uint64_t)hit << (k * VEC);
             }
             int at = atomicAdd(&sm.count, __builtin_popcountll(hits));
-#pragma unroll
-            for (int k = 0; k < CHUNKS; ++k)
-#pragma unroll
-                for (int v = 0; v < VEC; ++v)
-                    if (hits >> (k * VEC + v) & 1) {
-                        const uint32_t i = base + k * STEP + v;
-                        if (at < LP_POOL)
-                            sm.pool[at] = ((uint64_t)value_key((float)x[k][v]) << 32) | ~i;
-                        ++at;
-                    }
+            // (read again, from a cache: a register cannot be picked by a lane's number)
+            for (; hits && at < LP_POOL; hits &= hits - 1, ++at) {
+                const int j = __builtin_ctzll(hits);
+                const uint32_t i = base + j / VEC * STEP + j % VEC;
+                sm.pool[at] = ((uint64_t)value_key((float)xr[i]) << 32) | ~i;
+            }
         }
         __syncthreads();
         if (sm.count > LP_POOL) {
@@ -390,7 +402,7 @@ __global__ __launch_bounds__(LP_THREADS) void logprob_kernel(const LogprobParams
                         if (entry(k, v) >= least) sm.pool[atomicAdd(&sm.count, 1)] = entry(k, v);
             __syncthreads();
         }
-        rank_pool(sm, sm.count, top);
+        rank_pool<LOW_BITS<F32>>(sm, sm.count, top);
     }
     finish<TOP, F32>(a, sm, s, xr, row, part);
 }
@@ -480,7 +492,7 @@ static LogprobPlan plan(int rows, int n, int top) {
     const int64_t all = (int64_t)n + 7;
     auto count = [&](int64_t len) { return (int)((all + len - 1) / len); };
     const int64_t longs = LP_THREADS * LP_LONG;
-    if (rows * (int64_t)count(longs) <= 128)
+    if (rows * (int64_t)count(longs) <= LP_FEW)
         return {LP_SHORT, count(LP_THREADS * LP_SHORT), LP_THREADS * LP_SHORT};
     if (top) return {LP_LONG, count(longs), (int)longs};
     // none of less than a held part

@@ -31,7 +31,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
 
     A token outside [0, n) is padding and gets 0.  Logits of -inf have probability
     0 (their log probability is -inf); a row of nothing else has entropy 0.  A NaN
-    or +inf makes its row NaN.  No gradient is recorded."""
+    or +inf makes its row NaN (NaN ranks first).  No gradient is recorded."""
     if logits.dtype not in (torch.float16, torch.float32):
         raise ValueError(f"logits must be float16 or float32, got {logits.dtype}")
     if logits.dim() < 1 or logits.shape[-1] < 1:

@@ -137,6 +137,35 @@ def test_padding_tokens_and_nan():
     np.testing.assert_array_equal(out.top_ids[keep].cpu().numpy(), want[3])
 
 
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("n,every", [(50, 7), (5003, 3), (40000, 1), (40000, 611), (151936, 9001)])
+def test_nan_and_infinity_rank_first(n, every, dtype):
+    """NaN, then +inf, then the rest, of each the lower numbers first."""
+    x = logits(3, n, n, np.float32)
+    x[0, ::every] = np.nan
+    x[1, ::every] = np.inf
+    x[1, n - 2] = np.nan
+    x[2, ::every] = np.inf
+    x[2, :n // 2] -= 40                            # negative ones
+    x = x.astype(dtype)
+    out = score(torch.from_numpy(x).cuda(), torch.zeros(3, dtype=torch.int64, device="cuda"), 32)
+    rank = np.where(np.isnan(x), np.inf, np.where(np.isinf(x), 1e30, x.astype(np.float64)))
+    want = np.argsort(-rank, axis=1, kind="stable")[:, :32]
+    np.testing.assert_array_equal(out.top_ids.cpu().numpy(), want)
+    for t in (out.logprob, out.entropy, out.top_logprobs):
+        assert torch.isnan(t).all()
+
+
+@pytest.mark.parametrize("n", [300, 151936])
+def test_negative_halves(n):
+    """Neighbouring negative fp16 values: where a bound of fewer bits takes in one more."""
+    x = -(1 + np.random.default_rng(n).integers(0, 1024, (4, n)) / 1024).astype(np.float16)
+    x[1] *= np.float16(2.0 ** -15)                 # subnormal ones
+    x[2] = -x[2]
+    x[3] *= np.float16(8192)
+    check(x, np.array([0, 1, 2, n - 1]), 32)
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 def test_strides_shapes_and_odd_starts(dtype):
     g = torch.Generator(device="cuda").manual_seed(5)

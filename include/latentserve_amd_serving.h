@@ -74,7 +74,7 @@ size_t ls_int4_decode_counter_ints(int groups, int kv_heads);
 /* Decode attention over 4-bit pools: q [batch, kv_heads, n_rep, 128] fp16,
  * q_strides[3] = (b, h, r); out the same shape, out_strides[3]; n_rep in
  * 1..16.  Sequences of no tokens give zeros; blocks outside the pool are
- * skipped.  batch * max_pages < 2^31. */
+ * skipped.  batch * (max_pages + 16) + groups < 2^31. */
 int ls_paged_decode_int4(const void* q, const int64_t* q_strides, const void* k_codes,
                          const void* k_affine, const void* v_codes, const void* v_affine,
                          const int64_t* page_strides, int64_t num_blocks,

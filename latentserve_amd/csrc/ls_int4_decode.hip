@@ -36,6 +36,13 @@ constexpr int I4_ROW = HEAD_DIM + 4;     // LDS row: 16 rows written at once fal
 constexpr int I4_RESIDENT = 512;         // groups resident at once: two a CU
 // Fewest pages a run has: a pair a wave.
 constexpr int I4_MIN_PAGES = 2 * I4_NW;
+// Runs of at least this many pages (all groups have one then) differ, where two groups
+// share each CU: loads of the older group's waves go first, and of even runs its own
+// ended 5 us early at B16 x 16K; of 5 to 3 parts they end together.  (us, even /
+// 5 to 3: B16 x 16K 24.4 / 23.6, B16 x 64K 66.0 / 62.4, 2 x 100K 22.9 / 21.0, B64 ragged to
+// 4096 of 8 heads 41.5 / 38.9, B96 ragged to 16K 54.6 / 51.0.  A rule of speed only: any
+// group may run anywhere.)
+constexpr int I4_LONG_RUN = 24;
 // Pages whose blocks a group holds in LDS at once.
 constexpr int I4_TABLE = 2048;
 // Records that one group merges.
@@ -287,8 +294,6 @@ void int4_decode_kernel(const Int4DecodeParams a) {
     const int H = a.H, NR = a.NR;
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE;
     const int g = lane >> 4, c = lane & 15;
-    const int u = xcd_major(blockIdx.x, gridDim.x);
-    const int w = u / H, h = u - w * H;          // this group's run and head
 
     // ---- its run of the head's page list, and the sequence that run starts in ----
     // A sequence weighs its pages and `extra` (what starting on it costs a group, in
@@ -299,21 +304,52 @@ void int4_decode_kernel(const Int4DecodeParams a) {
         int p = len > 0 ? (len - 1) / PAGE + 1 : 1;
         return p < a.max_pages ? p : a.max_pages;
     };
-    auto run_of = [&](int T, int& u0, int& u1) {
-        int per = (T + a.groups - 1) / a.groups;
-        per = per > I4_MIN_PAGES ? per : I4_MIN_PAGES;
-        u0 = (int64_t)w * per < T ? w * per : T;
-        u1 = T - u0 < per ? T : u0 + per;
-        return per;
+    auto div = [](int n, Divisor d) { return (int)((uint64_t)(uint32_t)n * d.mul >> d.shift); };
+    // This group's run and head: neighbouring runs on one XCD, whose L2 has their tables
+    // and queries.
+    int w, h;
+    auto place = [&](int u) {
+        w = div(u, a.by_heads);
+        h = u - w * H;
     };
-    int per, b, P, len, u0, u1;          // weight of a run; the sequence, its start, length
+    place(xcd_major(blockIdx.x, gridDim.x));
+    // A run's pages `per`; with `skew` runs take more and fewer, `big` and 2 per - big, in
+    // turn.
+    int per, big;
+    bool skew;
+    auto run_of = [&](int T, int& u0, int& u1) {
+        per = div(T + a.groups - 1, a.by_groups);
+        per = per > I4_MIN_PAGES ? per : I4_MIN_PAGES;
+        skew = a.skew != 0 && per >= I4_LONG_RUN;
+        big = per;
+        if (skew) {
+            big += per / 4;
+            const int L = blockIdx.x, half = gridDim.x / 2;
+            place(L < half ? L : L - half);
+            w = 2 * w + (L < half ? 0 : 1);
+        } else if (per == I4_MIN_PAGES) {
+            // (lengths below the bound's: the groups that have a run, over all XCDs)
+            const int L = blockIdx.x, used = (T + I4_MIN_PAGES - 1) / I4_MIN_PAGES * H;
+            if (used < (int)gridDim.x) place(L < used ? xcd_major(L, used) : L);
+        }
+        const int64_t at = (int64_t)(w / 2) * 2 * per + (w & 1 ? big : 0);
+        const int mine = w & 1 ? 2 * per - big : big;
+        u0 = at < T ? at : T;
+        u1 = T - u0 < mine ? T : u0 + mine;
+    };
+    auto group_of = [&](int page) {
+        if (!skew) return page / per;
+        const int pair = page / (2 * per);
+        return 2 * pair + (page - pair * 2 * per < big ? 0 : 1);
+    };
+    int b, P, len, u0, u1;           // the first sequence, its start, length; the run
     if (a.B <= WAVE) {
         // one sequence a lane
         const int li = lane < a.B ? a.lens[lane] : 0;
         const int n = lane < a.B ? pages_of(li) + extra : 0;
         int T;
         const int incl = wave_incl_scan(n, lane, T);
-        per = run_of(T, u0, u1);
+        run_of(T, u0, u1);
         if (u0 >= T) return;                         // (every wave alike, before any barrier)
         b = __builtin_ctzll(__ballot(u0 < incl));    // (lanes past the batch hold T)
         P = __builtin_amdgcn_readlane(incl - n, b);
@@ -327,7 +363,7 @@ void int4_decode_kernel(const Int4DecodeParams a) {
         for (int i = b0; i < b1; ++i) mine += pages_of(a.lens[i]) + extra;
         int T;
         const int incl = wave_incl_scan(mine, lane, T);
-        per = run_of(T, u0, u1);
+        run_of(T, u0, u1);
         if (u0 >= T) return;
         int pos = incl - mine, fb = 0, fp = 0, fl = 0;
         const bool holds = u0 >= pos && u0 < incl;
@@ -512,7 +548,7 @@ void int4_decode_kernel(const Int4DecodeParams a) {
         }
         __syncthreads();
         const bool whole = s0 == 0 && s1 == n;
-        const int first = start / per;                     // the sequence's first group
+        const int first = group_of(start);                   // the sequence's first group
         const Int4Records R = {a.work + (int64_t)h * a.rec, H * a.rec * (int)sizeof(float), a.groups,
                                first};
         const int d0 = 4 * (threadIdx.x % 32);
@@ -542,7 +578,7 @@ void int4_decode_kernel(const Int4DecodeParams a) {
         }
         if (!whole) {
             // ---- the last of the sequence's groups to arrive merges their records ----
-            const int S = (start + n - 1) / per - first + 1;
+            const int S = group_of(start + n - 1) - first + 1;
             const int k = w - first, cl = k / I4_CLUSTER;
             const bool tree = S > I4_CLUSTER;
             // arrival counters: [0] the sequence's, at its first group; [1], [2] of 16
@@ -600,6 +636,10 @@ int int4_groups(int batch, int kv_heads, int64_t pages_bound) {
 hipError_t launch_int4_decode(const Int4DecodeParams& a, hipStream_t stream) {
     Int4DecodeParams d = a;
     d.rec = int4_record_floats(a.NR);
+    d.by_groups = make_divisor(a.groups);
+    d.by_heads = make_divisor(a.H);
+    // (pairs of runs to the blocks L and L + 256, which the dispatcher gives one CU)
+    d.skew = a.groups * a.H == I4_RESIDENT && a.groups % 2 == 0;
     d.extra = 4 * a.B > a.groups ? I4_EXTRA : 0;
     hipLaunchKernelGGL(int4_decode_kernel, dim3(a.groups * a.H), dim3(WAVE * I4_NW), 0, stream, d);
     return hipGetLastError();

@@ -52,6 +52,19 @@ struct Int4ReadParams {
     int B, H, L;
 };
 
+// Division by a number that the host knows: n / d = n * mul >> shift for 0 <= n < 2^31
+// (mul = floor(2^shift / d) + 1 and 2^(shift - 31) >= d: mul d exceeds 2^shift by at most
+// d, so n mul d / 2^shift exceeds n by less than 1).
+struct Divisor {
+    uint32_t mul;
+    int shift;
+};
+inline Divisor make_divisor(uint32_t d) {
+    int l = 0;
+    while (l < 31 && (1u << l) < d) ++l;
+    return {(uint32_t)((((uint64_t)1 << (31 + l)) / d) + 1), 31 + l};
+}
+
 struct Int4DecodeParams {
     const _Float16* q;
     int64_t sq_b, sq_h, sq_r;
@@ -68,6 +81,8 @@ struct Int4DecodeParams {
     int groups;                   // workgroups a KV head
     int rec;                      // floats of a record (set at launch, as the next)
     int extra;                    // pages that starting on a sequence counts as
+    int skew;                     // long runs may differ (int4_decode_kernel)
+    Divisor by_groups, by_heads;
     float scale;
 };
 

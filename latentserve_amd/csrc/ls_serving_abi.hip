@@ -186,6 +186,9 @@ int ls_paged_decode_int4(const void* q, const int64_t* q_strides, const void* k_
         ls_int4_decode_workspace_bytes(groups, kv_heads, n_rep) >= (size_t)1 << 31)
         return fail(LS_ERR_INVALID, "groups must be >= 1, groups x kv_heads at most %d and the "
                     "workspace below 2^31 bytes", ls::I4_MAX_GROUPS);
+    // (what a head's pages and the starts on sequences weigh together: 32-bit places)
+    if ((int64_t)batch * ((int64_t)max_pages + 16) + groups >= (1LL << 31))
+        return fail(LS_ERR_INVALID, "batch x (max_pages + 16) + groups must be below 2^31");
     if (!rows_aligned(q, q_strides, 3, 2) || !rows_aligned(out, out_strides, 3, 2))
         return fail(LS_ERR_INVALID, "q and out rows must be 16-byte aligned");
     if (!aligned(workspace, 16) ||

@@ -161,6 +161,26 @@ def test_decode_matches_64_bits(lens, h, r):
     check(out, q, arrays, tables, ln, (lens, h, r))
 
 
+@pytest.mark.parametrize("h,r,lens", [(256, 1, [900]), (256, 1, [767]), (128, 2, [1537, 31]),
+                                      (32, 2, [12000]), (32, 6, [7001, 1, 0, 5000, 300, 17]),
+                                      (16, 16, [16000, 9, 8000]), (8, 4, [2000] * 13)])
+def test_decode_of_runs_that_differ(h, r, lens):
+    """A full launch with long runs: they take more and fewer pages in turn."""
+    print(f"decode lens={lens[:7]} h={h} r={r}", flush=True)
+    q, arrays, tables, ln = attend_case(lens, h, r, seed=len(lens) + h)
+    out = i4().paged_decode_int4(dev(q), pools_of(arrays), dev(tables), dev(ln))
+    check(out, q, arrays, tables, ln, (lens, h, r))
+
+
+@pytest.mark.parametrize("h", [1, 2, 3, 8, 32])
+def test_decode_far_below_the_bound(h):
+    """A launch sized for long sequences serves short ones, by some of its groups."""
+    for lens in ([1], [128], [129, 0], [500, 2000, 7], [3, 1500]):
+        q, arrays, tables, ln = attend_case(lens, h, 4, seed=h, width=400 if h < 8 else 140)
+        out = i4().paged_decode_int4(dev(q), pools_of(arrays), dev(tables), dev(ln))
+        check(out, q, arrays, tables, ln, (lens, h))
+
+
 @pytest.mark.parametrize("bound", [1, 100, 4096, 100000])
 def test_decode_takes_any_expected_length(bound):
     q, arrays, tables, ln = attend_case([3000, 40], seed=11)

@@ -116,6 +116,11 @@ def test_decode_refuses(lib, over, needle):
     assert needle in lib.ls_last_error().decode()
 
 
+def test_decode_refuses_more_pages_than_its_places(lib):
+    assert _decode(lib, b=65535, mp=32767) == 1        # below 2^31 as a table
+    assert "+ 16" in lib.ls_last_error().decode()
+
+
 def test_nothing_to_do_is_no_launch(lib):
     assert _write(lib, b=0) == _write(lib, n=0) == _read(lib, b=0) == _read(lib, n=0) == 0
     assert _decode(lib, b=0) == 0

@@ -45,7 +45,8 @@ int ls_serving_abi_version(void);
  * v_strides[3] = (b, h, t) in elements, quantized into flat slots [batch *
  * tokens] int64 (block * 16 + offset; outside the pool: not written).  Slots
  * are distinct; of two tokens with one slot, either's codes may end up there.
- * Other tokens of a page are left as they are. */
+ * Other tokens of a page are left as they are.  A group that holds a NaN or an
+ * infinity reads back as NaN. */
 int ls_int4_write(const void* k, const int64_t* k_strides, const void* v,
                   const int64_t* v_strides, const int64_t* slots, void* k_codes, void* k_affine,
                   void* v_codes, void* v_affine, const int64_t* page_strides, int64_t num_blocks,

@@ -21,7 +21,7 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 constexpr int I4_THREADS = 256;
 constexpr int I4_LANES = HEAD_DIM / 8;      // lanes a (token, head)
 
-// Minimum / maximum over the lane's quad.
+// Minimum / maximum / sum over the lane's quad.
 __device__ __forceinline__ float quad_min(float v) {
     v = fminf(v, dpp_move<0xB1>(v));
     return fminf(v, dpp_move<0x4E>(v));
@@ -29,6 +29,11 @@ __device__ __forceinline__ float quad_min(float v) {
 __device__ __forceinline__ float quad_max(float v) {
     v = fmaxf(v, dpp_move<0xB1>(v));
     return fmaxf(v, dpp_move<0x4E>(v));
+}
+
+__device__ __forceinline__ float quad_sum(float v) {
+    v += dpp_move<0xB1>(v);
+    return v + dpp_move<0x4E>(v);
 }
 
 // (blockIdx.y: K, V)
@@ -43,14 +48,19 @@ __global__ __launch_bounds__(I4_THREADS) void int4_write_kernel(const Int4WriteP
     const int64_t slot = a.slots[(int64_t)b * a.N + t_new];
     const h8 x = *(const h8*)(a.src[z] + b * a.ss_b[z] + h * a.ss_h[z] + t_new * a.ss_t[z] + 16 * o);
     if (slot < 0 || slot >= (int64_t)a.p.num_blocks * PAGE) return;
-    float lo = (float)x[0], hi = lo;
+    float lo = (float)x[0], hi = lo, sum = lo;
 #pragma unroll
     for (int e = 1; e < 8; ++e) {
         lo = fminf(lo, (float)x[e]);
         hi = fmaxf(hi, (float)x[e]);
+        sum += (float)x[e];
     }
     lo = quad_min(lo);
     hi = quad_max(hi);
+    // (min and max pass over a NaN; a sum of fp16 values is finite only if all are.  One
+    // that is not makes m NaN, and so all of the group's entries)
+    sum = quad_sum(sum);
+    lo = sum - sum != 0.f ? __builtin_nanf("") : lo;
     half_t s = (half_t)((hi - lo) / 15.f);
     // (65520 is where fp16 rounds to infinity; s is then over 4000, and a step of it
     // less takes 15 s below max)
@@ -61,7 +71,7 @@ __global__ __launch_bounds__(I4_THREADS) void int4_write_kernel(const Int4WriteP
     // so only one within 2^-16 of a border between two codes is taken again in 64 bits,
     // where the difference is exact (fp16 operands span 40 bits) and the quotient's
     // rounding is far finer than the distance of a border (4 x 2048 tokens: every
-    // quotient in 64 bits 7.9 us, so 6.3).
+    // quotient in 64 bits 7.9 us, so 6.6).
     uint32_t word = 0, near = 0;
     const float sf = (float)s, inv = sf > 0.f ? 1.f / sf : 0.f;
 #pragma unroll

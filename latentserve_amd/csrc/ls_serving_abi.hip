@@ -6,6 +6,7 @@
 #include <stdio.h>
 
 #include <algorithm>
+#include <cmath>
 #include <new>
 
 #include "../../include/latentserve_amd.h"
@@ -133,7 +134,8 @@ int ls_int4_read(const void* k_codes, const void* k_affine, const void* v_codes,
     if (!aligned(k_out, 16) || !aligned(v_out, 16))
         return fail(LS_ERR_INVALID, "k_out and v_out must be 16-byte aligned");
     if (length < 0) return fail(LS_ERR_INVALID, "length must be >= 0");
-    if (batch > 0 && length > ((1LL << 31) - 1) * 16 / kv_heads / batch)
+    // (16 threads each, below 2^32)
+    if (batch > 0 && length > ((1LL << 28) - 1) / kv_heads / batch)
         return fail(LS_ERR_INVALID, "batch x heads x length too large for one read");
     if (batch == 0 || length == 0) return LS_OK;
     a.tables = block_tables;
@@ -189,6 +191,7 @@ int ls_paged_decode_int4(const void* q, const int64_t* q_strides, const void* k_
     // (what a head's pages and the starts on sequences weigh together: 32-bit places)
     if ((int64_t)batch * ((int64_t)max_pages + 16) + groups >= (1LL << 31))
         return fail(LS_ERR_INVALID, "batch x (max_pages + 16) + groups must be below 2^31");
+    if (!std::isfinite(softmax_scale)) return fail(LS_ERR_INVALID, "softmax_scale must be finite");
     if (!rows_aligned(q, q_strides, 3, 2) || !rows_aligned(out, out_strides, 3, 2))
         return fail(LS_ERR_INVALID, "q and out rows must be 16-byte aligned");
     if (!aligned(workspace, 16) ||
@@ -309,7 +312,7 @@ int ls_token_logprobs(const void* x, int64_t x_stride, int elem_bytes, const int
     if (rows == 0) return LS_OK;
     ls::LogprobParams a;
     a.parts = ls::logprob_parts(rows, n, top);
-    if ((int64_t)rows * a.parts > (1LL << 31) - 1)
+    if ((int64_t)rows * a.parts >= 1LL << 24)                  // (256 threads each, below 2^32)
         return fail(LS_ERR_INVALID, "rows x n too large for one call");
     if (a.parts > 1) {
         const size_t need = ls_token_logprobs_workspace_bytes(rows, n, top);

@@ -33,6 +33,7 @@ HEAD_DIM = 128
 PAGE = 16
 GROUP = 32
 MAX_NREP = 16
+_MAX_WIDTH = 1 << 24            # pages of a block table
 _SCALE = 1.0 / math.sqrt(HEAD_DIM)
 
 _SHAPES = ((PAGE, 64), (PAGE, 4, 2), (16, PAGE, 4), (4, 4, 2, 4))
@@ -139,6 +140,8 @@ def _sizes(b: int, h: int, n_rep: int, width: int, bound: int):
     key = (b, h, n_rep, width, bound)
     got = _SIZES.get(key)
     if got is None:
+        if width > _MAX_WIDTH:
+            raise ValueError(f"block tables of {width} pages are too wide")
         lib = _serving.lib()
         groups = lib.ls_int4_decode_groups(b, h, width, bound)
         got = (groups, lib.ls_int4_decode_workspace_bytes(groups, h, n_rep),
@@ -152,7 +155,8 @@ def _sizes(b: int, h: int, n_rep: int, width: int, bound: int):
 def write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, pools) -> None:
     """k, v [B, H, n, 128] fp16 (any strides of whole 16 bytes) quantized into flat
     token slots [B * n] int64 (block * 16 + offset; outside the pool: not
-    written).  Slots are distinct.  Other tokens keep their entries."""
+    written).  Slots are distinct.  Other tokens keep their entries.  A group of 32
+    channels that holds a NaN or an infinity reads back as NaN."""
     nb, h, args = _pools(pools, written=True)
     dev = pools[0].device
     if k.dim() != 4 or k.shape != v.shape or k.shape[1] != h or k.shape[3] != HEAD_DIM:
@@ -194,6 +198,8 @@ def read(pools, block_tables: torch.Tensor, seq_lens: torch.Tensor,
         with torch.cuda.device(dev):
             return read(pools, block_tables, seq_lens, length)
     width = block_tables.shape[1]
+    if width > _MAX_WIDTH:
+        raise ValueError(f"block tables of {width} pages are too wide")
     token = h * HEAD_DIM
     kv = torch.empty_strided((2, b, h, length, HEAD_DIM),
                              (b * length * token, length * token, HEAD_DIM, token, 1),
@@ -217,8 +223,9 @@ def paged_decode_int4(q: torch.Tensor, pools, block_tables: torch.Tensor, seq_le
 
     max_seq_len: the longest sequence expected (a graph's bucket); it only sizes
     the launch, a longer one is attended whole.  Sequences of no tokens give
-    zeros, and blocks outside the pool are skipped.  out may not overlap q.  Each call has its own scratch, so calls may run at once on several
-    streams and from several graphs."""
+    zeros, and blocks outside the pool are skipped.  out may not overlap q.  Each
+    call has its own scratch, so calls may run at once on several streams and from
+    several graphs."""
     nb, h, args = _pools(pools)
     dev = pools[0].device
     if q.dim() != 4 or q.shape[1] != h or q.shape[3] != HEAD_DIM \

@@ -88,6 +88,8 @@ _SIZES: dict = {}
 def _sizes(rows: int, n: int, top: int):
     got = _SIZES.get((rows, n, top))
     if got is None:
+        if max(rows, n) >= 1 << 31:                       # (C ints)
+            raise ValueError(f"{rows} rows of {n} logits are too many for one call")
         lib = _serving.lib()
         got = (lib.ls_token_logprobs_workspace_bytes(rows, n, top),
                lib.ls_token_logprobs_counter_ints(rows, n, top))

@@ -412,6 +412,8 @@ class _PagedBase:
         if len(set(children)) != len(children):
             raise ValueError(f"slots {children}: a child is named twice")
         for c in children:
+            if not 0 <= c < len(self.tables):
+                raise ValueError(f"slot {c} is not one of {len(self.tables)}")
             if self.tables[c].length or self.tables[c].blocks:
                 raise ValueError(f"slot {c} already holds a sequence")
         pages = t.blocks[:self.allocator.blocks_for_tokens(t.length)]

@@ -98,7 +98,7 @@ def test_fork_at_a_page_border_and_of_nothing():
 def test_fork_refuses():
     c = cache()
     grow(c, [0, 1], [[1], [2]])
-    for children in ([1], [0], [2, 2], [2, 1]):
+    for children in ([1], [0], [2, 2], [2, 1], [-1], [1000]):
         with pytest.raises(ValueError):
             c.fork(0, children)
     check_refs(c, [[1], [2], [], [], [], []])

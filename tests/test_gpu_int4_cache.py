@@ -84,6 +84,24 @@ def test_write_is_bit_exact_and_leaves_the_rest(b, h, n):
         np.testing.assert_array_equal(got, exp, err_msg=name)
 
 
+def test_a_group_with_a_nan_or_an_infinity_reads_back_as_nan():
+    x = rows((1, 2, 6, 128), 9)
+    bad = np.zeros((6, 4), bool)
+    for t, (c, value) in enumerate([(0, np.nan), (63, np.inf), (100, -np.inf), (37, np.nan)]):
+        x[0, 1, t, c] = value
+        bad[t, c // 32] = True
+    x[0, 1, 4, 64:96], x[0, 1, 5, 2:4] = np.nan, (np.inf, -np.inf)
+    bad[4, 2] = bad[5, 0] = True
+    pools = i4().empty_pools(1, 2, "cuda")
+    i4().write(dev(x), dev(x), torch.arange(6, device="cuda"), pools)
+    table, lens = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.tensor([6], device="cuda").int()
+    for got in i4().read(pools, table, lens, 6):
+        nan = torch.isnan(got).cpu().numpy().reshape(2, 6, 4, 32)
+        assert not nan[0].any()
+        np.testing.assert_array_equal(nan[1].all(-1), bad)
+        np.testing.assert_array_equal(nan[1].any(-1), bad)
+
+
 def test_write_takes_strided_rows_and_skips_slots_outside():
     b, h, n, nb = 2, 2, 3, 4
     x = dev(rows((b, n, 2 * h, 128), 5))

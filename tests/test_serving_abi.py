@@ -74,12 +74,12 @@ def _read(lib, **over):
 def _decode(lib, **over):
     a = dict(POOL, q=1 << 12, qs=_st(1536, 768, 128), t=64, ts=4, mp=4, l=64, o=1 << 13,
              os=_st(1536, 768, 128), w=1 << 14, wb=1 << 30, c=64, b=2, h=2, r=6, d=128, page=16,
-             g=4)
+             g=4, scale=0.088)
     a.update(over)
     return lib.ls_paged_decode_int4(a["q"], a["qs"], a["kc"], a["ka"], a["vc"], a["va"], a["ps"],
                                     a["nb"], a["t"], a["ts"], a["mp"], a["l"], a["o"], a["os"],
                                     a["w"], a["wb"], a["c"], a["b"], a["h"], a["r"], a["d"],
-                                    a["page"], a["g"], 0.088, None)
+                                    a["page"], a["g"], a["scale"], None)
 
 
 BAD_POOLS = [(dict(kc=None), "null"), (dict(va=None), "null"), (dict(ps=None), "null"),
@@ -114,6 +114,17 @@ def test_read_refuses(lib, over, needle):
 def test_decode_refuses(lib, over, needle):
     assert _decode(lib, **over) == 1
     assert needle in lib.ls_last_error().decode()
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf")])
+def test_decode_refuses_a_scale_that_is_not_finite(lib, scale):
+    assert _decode(lib, scale=scale) == 1
+    assert "finite" in lib.ls_last_error().decode()
+
+
+def test_sizes_past_a_launch_are_refused(lib):
+    assert _read(lib, b=4, h=64, n=1 << 20) == 1 and "too large" in lib.ls_last_error().decode()
+    assert _score(lib, rows=1 << 24, n=1, top=0) == 1 and "too large" in lib.ls_last_error().decode()
 
 
 def test_decode_refuses_more_pages_than_its_places(lib):

@@ -8,8 +8,11 @@
 //
 // Sixteen lanes take a (token, head)'s 16 octets of channels, so a group of 32 is
 // a quad of lanes and its minimum and maximum two lane exchanges; a lane reads 16
-// bytes and writes one word of codes.  Both kernels are bound by their loads
-// and stores.
+// bytes and writes one word of codes.
+//
+// Both are bound by memory, and small calls by the launch and one round trip.  4 x 2048
+// tokens, 2 heads: write 6.8 us for 11 MB, read 5.2 (2 us at a large copy's rate; copies of
+// this size are as far from it); 16 tokens of 2 heads: 3.1 and 3.0.
 
 #include "ls_common.h"
 #include "ls_serving.h"
@@ -39,12 +42,11 @@ __device__ __forceinline__ float quad_sum(float v) {
 // (blockIdx.y: K, V)
 __global__ __launch_bounds__(I4_THREADS) void int4_write_kernel(const Int4WriteParams a) {
     const int z = blockIdx.y;
-    const int64_t i = (int64_t)blockIdx.x * I4_THREADS + threadIdx.x;
     const int o = threadIdx.x % I4_LANES;
-    const int item = (int)(i / I4_LANES);               // (sequence, head, token)
+    const int item = blockIdx.x * (I4_THREADS / I4_LANES) + threadIdx.x / I4_LANES;
     if (item >= a.B * a.H * a.N) return;                // (whole groups of 16 lanes)
-    const int bh = item / a.N, t_new = item - bh * a.N;
-    const int b = bh / a.H, h = bh - b * a.H;
+    const int bh = divide(item, a.by_tokens), t_new = item - bh * a.N;     // (b, h, t)
+    const int b = divide(bh, a.by_heads), h = bh - b * a.H;
     const int64_t slot = a.slots[(int64_t)b * a.N + t_new];
     const h8 x = *(const h8*)(a.src[z] + b * a.ss_b[z] + h * a.ss_h[z] + t_new * a.ss_t[z] + 16 * o);
     if (slot < 0 || slot >= (int64_t)a.p.num_blocks * PAGE) return;
@@ -61,32 +63,36 @@ __global__ __launch_bounds__(I4_THREADS) void int4_write_kernel(const Int4WriteP
     // that is not makes m NaN, and so all of the group's entries)
     sum = quad_sum(sum);
     lo = sum - sum != 0.f ? __builtin_nanf("") : lo;
-    half_t s = (half_t)((hi - lo) / 15.f);
+    // ((hi - lo) / 15 rounded once: a product with 1 / 15 corrected by its remainder, exact
+    // fused steps; checked over all fp32 significands)
+    constexpr float FIFTEENTH = 1.f / 15.f;
+    const float span = hi - lo, near15 = span * FIFTEENTH;
+    half_t s = (half_t)__builtin_fmaf(__builtin_fmaf(-15.f, near15, span), FIFTEENTH, near15);
     // (65520 is where fp16 rounds to infinity; s is then over 4000, and a step of it
     // less takes 15 s below max)
     if (lo + 15.f * (float)s >= 65520.f && hi <= 65504.f)
         s = __builtin_bit_cast(half_t, (uint16_t)(__builtin_bit_cast(uint16_t, s) - 1));
     // The nearest whole number to (x - m) / s, decided exactly: the fp32 quotient is off by
-    // at most 16 * 2^-22 (the difference, the reciprocal and the product round once each),
-    // so only one within 2^-16 of a border between two codes is taken again in 64 bits,
-    // where the difference is exact (fp16 operands span 40 bits) and the quotient's
-    // rounding is far finer than the distance of a border (4 x 2048 tokens: every
-    // quotient in 64 bits 7.9 us, so 6.6).
-    uint32_t word = 0, near = 0;
-    const float sf = (float)s, inv = sf > 0.f ? 1.f / sf : 0.f;
+    // at most 16 * 2^-22 (the difference, the reciprocal and the product round once each,
+    // the reciprocal by up to a step), so only where one lies within 2^-16 of a border
+    // between two codes are a lane's eight taken again in 64 bits, where the difference is
+    // exact (fp16 operands span 40 bits) and the quotient's rounding is far finer than the
+    // distance of a border (4 x 2048 tokens, all in 64 bits: 1.3 us more).
+    uint32_t word = 0;
+    float off = 0.f;
+    const float sf = (float)s, inv = sf > 0.f ? __builtin_amdgcn_rcpf(sf) : 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const float r = ((float)x[e] - lo) * inv, c = rintf(r);
-        near |= fabsf(r - c) > 0.5f - 0x1p-16f ? 1u << e : 0u;
+        off = fmaxf(off, fabsf(r - c));
         word |= (uint32_t)(c < 15.f ? c : 15.f) << (4 * e);
     }
-    if (near) {
+    if (off > 0.5f - 0x1p-16f) {
+        word = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            if (near >> e & 1) {
-                const double c = rint(((double)(float)x[e] - (double)lo) / (double)sf);
-                word = (word & ~(15u << (4 * e))) | (uint32_t)(c < 15. ? c : 15.) << (4 * e);
-            }
+            const double c = rint(((double)(float)x[e] - (double)lo) / (double)sf);
+            word |= (uint32_t)(c < 15. ? c : 15.) << (4 * e);
         }
     }
     const int64_t blk = slot / PAGE;
@@ -111,12 +117,17 @@ __global__ __launch_bounds__(I4_THREADS) void int4_write_kernel(const Int4WriteP
 }
 
 // The eight entries of a word: fp16(m + s * code), each pair one fused multiply-add.
+// (Codes become fp16 by a splice under the exponent of 1024: 1024 + code, less 1024.)
 __device__ __forceinline__ h8 word_values(uint32_t w, half_t s, half_t m) {
+    const h2 ss = {s, s}, mm = {m, m}, bias = {(half_t)1024.f, (half_t)1024.f};
     h8 r;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const half_t c = (half_t)(float)((w >> (4 * e)) & 15);
-        r[e] = __builtin_fmaf16(c, s, m);
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t two = w >> (4 * i) & 0x000F000Fu;           // codes i and i + 4
+        const h2 c = __builtin_bit_cast(h2, two | 0x64006400u) - bias;
+        const h2 y = __builtin_elementwise_fma(c, ss, mm);
+        r[i] = y[0];
+        r[i + 4] = y[1];
     }
     return r;
 }
@@ -124,13 +135,11 @@ __device__ __forceinline__ h8 word_values(uint32_t w, half_t s, half_t m) {
 // (blockIdx.y: K, V)  Items (sequence, token, head), 16 lanes each.
 __global__ __launch_bounds__(I4_THREADS) void int4_read_kernel(const Int4ReadParams a) {
     const int z = blockIdx.y;
-    const int64_t i = (int64_t)blockIdx.x * I4_THREADS + threadIdx.x;
     const int o = threadIdx.x % I4_LANES;
-    const int64_t item = i / I4_LANES;
-    if (item >= (int64_t)a.B * a.L * a.H) return;
-    const int64_t bt = item / a.H;
-    const int h = (int)(item - bt * a.H);
-    const int b = (int)(bt / a.L), pos = (int)(bt - (int64_t)b * a.L);
+    const int item = blockIdx.x * (I4_THREADS / I4_LANES) + threadIdx.x / I4_LANES;
+    if (item >= a.B * a.L * a.H) return;                // (below 2^28)
+    const int bt = divide(item, a.by_heads), h = item - bt * a.H;
+    const int b = divide(bt, a.by_length), pos = bt - b * a.L;
     h8 y = {};
     const int page = pos / PAGE, t = pos % PAGE;
     const int len = a.lens[b];
@@ -150,17 +159,23 @@ __global__ __launch_bounds__(I4_THREADS) void int4_read_kernel(const Int4ReadPar
             }
         }
     }
-    *(h8*)(a.out[z] + item * HEAD_DIM + 8 * o) = y;
+    *(h8*)(a.out[z] + (int64_t)item * HEAD_DIM + 8 * o) = y;
 }
 
-hipError_t launch_int4_write(const Int4WriteParams& a, hipStream_t stream) {
+hipError_t launch_int4_write(const Int4WriteParams& p, hipStream_t stream) {
+    Int4WriteParams a = p;
+    a.by_tokens = make_divisor(a.N);
+    a.by_heads = make_divisor(a.H);
     const int64_t lanes = (int64_t)a.B * a.H * a.N * I4_LANES;
     hipLaunchKernelGGL(int4_write_kernel, dim3((unsigned)((lanes + I4_THREADS - 1) / I4_THREADS), 2),
                        dim3(I4_THREADS), 0, stream, a);
     return hipGetLastError();
 }
 
-hipError_t launch_int4_read(const Int4ReadParams& a, hipStream_t stream) {
+hipError_t launch_int4_read(const Int4ReadParams& p, hipStream_t stream) {
+    Int4ReadParams a = p;
+    a.by_heads = make_divisor(a.H);
+    a.by_length = make_divisor(a.L);
     const int64_t lanes = (int64_t)a.B * a.L * a.H * I4_LANES;
     hipLaunchKernelGGL(int4_read_kernel, dim3((unsigned)((lanes + I4_THREADS - 1) / I4_THREADS), 2),
                        dim3(I4_THREADS), 0, stream, a);

@@ -34,24 +34,6 @@ struct Int4Pools {
     int num_blocks;
 };
 
-struct Int4WriteParams {
-    const char* src[2];           // k, v [B, H, N, 128] fp16
-    int64_t ss_b[2], ss_h[2], ss_t[2];   // strides, bytes
-    const int64_t* slots;         // [B * N]
-    Int4Pools p;
-    int B, H, N;
-};
-
-struct Int4ReadParams {
-    Int4Pools p;
-    const int32_t* tables;
-    int64_t st_b;
-    int max_pages;
-    const int32_t* lens;
-    _Float16* out[2];             // [B, L, H, 128], contiguous
-    int B, H, L;
-};
-
 // Division by a number that the host knows: n / d = n * mul >> shift for 0 <= n < 2^31
 // (mul = floor(2^shift / d) + 1 and 2^(shift - 31) >= d: mul d exceeds 2^shift by at most
 // d, so n mul d / 2^shift exceeds n by less than 1).
@@ -64,6 +46,29 @@ inline Divisor make_divisor(uint32_t d) {
     while (l < 31 && (1u << l) < d) ++l;
     return {(uint32_t)((((uint64_t)1 << (31 + l)) / d) + 1), 31 + l};
 }
+__device__ __forceinline__ int divide(int n, Divisor d) {
+    return (int)((uint64_t)(uint32_t)n * d.mul >> d.shift);
+}
+
+struct Int4WriteParams {
+    const char* src[2];           // k, v [B, H, N, 128] fp16
+    int64_t ss_b[2], ss_h[2], ss_t[2];   // strides, bytes
+    const int64_t* slots;         // [B * N]
+    Int4Pools p;
+    int B, H, N;
+    Divisor by_tokens, by_heads;  // set at launch
+};
+
+struct Int4ReadParams {
+    Int4Pools p;
+    const int32_t* tables;
+    int64_t st_b;
+    int max_pages;
+    const int32_t* lens;
+    _Float16* out[2];             // [B, L, H, 128], contiguous
+    int B, H, L;
+    Divisor by_heads, by_length;  // set at launch
+};
 
 struct Int4DecodeParams {
     const _Float16* q;

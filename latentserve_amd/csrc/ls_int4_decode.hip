@@ -20,8 +20,8 @@
 //    words of two tokens are first spliced by halves, so that a pair is two tokens
 //    of one channel, the operand V^T needs.
 //  * Bound: 160 bytes a token and head from HBM, and the codes' way to fp16 beside it
-//    (3.3 vector instructions a pair of entries; the MFMAs a fifth of that).  B16 x 16K, 2
-//    heads, 84 MB: 21 to 23 us, 4.0 TB/s; its loads alone take 18 us and its arithmetic
+//    (372 vector instructions a wave and two pages, 17 MFMAs).  B16 x 16K, 2 heads, 84 MB:
+//    21 to 23 us, 4.0 TB/s; its loads alone take 18 us and its arithmetic
 //    alone 17, of each 8 before the first page and after the last (lengths, table, pages;
 //    records, arrival, records).  B1 x 2048 is that chain, 7.4 us.
 //  * Online softmax in the log2 domain; a step in which no row's maximum moved skips

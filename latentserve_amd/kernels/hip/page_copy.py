@@ -8,6 +8,7 @@ numbers in the launch's arguments.
 from __future__ import annotations
 
 import operator
+import struct
 from array import array
 from typing import Sequence
 
@@ -39,7 +40,7 @@ def copy_pages(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequenc
     first = tensors[0]
     dev = first.device
     count, pages = len(tensors), first.shape[0] if first.dim() else 0
-    if any(shape[:1] != (pages,) for shape in set(map(_shape, tensors))):
+    if set(map(_length, tensors)) != {pages}:
         raise ValueError(f"every tensor must have {pages} pages, got "
                          f"{[tuple(t.shape) for t in tensors][:8]}")
     if set(map(torch.Tensor.get_device, tensors)) != {first.get_device()}:
@@ -47,26 +48,29 @@ def copy_pages(tensors: Sequence[torch.Tensor], src: Sequence[int], dst: Sequenc
     if torch.is_grad_enabled() and any(map(_requires_grad, tensors)):
         raise ValueError("a page copy records no gradient")
     if all(map(torch.Tensor.is_contiguous, tensors)):
-        sizes = steps = array("q", [b // pages if pages else 0 for b in map(_nbytes, tensors)])
+        sizes = steps = [b // pages if pages else 0 for b in map(_nbytes, tensors)]
     else:
         steps, sizes = _layouts(tensors)
     stream = _lib.stream_of(dev)
     if n == 0:
         return
-    ptrs = array("q", map(torch.Tensor.data_ptr, tensors))
+    ptrs = list(map(torch.Tensor.data_ptr, tensors))
     if 0 in sizes:
         keep = [i for i in range(count) if sizes[i]]
-        ptrs, steps, sizes = (array("q", [a[i] for i in keep]) for a in (ptrs, steps, sizes))
+        ptrs, steps, sizes = ([a[i] for i in keep] for a in (ptrs, steps, sizes))
         count = len(keep)
     if dev.index != _serving.current_device():
         with torch.cuda.device(dev):
             return copy_pages(tensors, src, dst)
-    rc = _serving.lib().ls_page_copy(*map(_address, (ptrs, steps, sizes)), count, pages,
-                                     _address(src), _address(dst), n, stream)
+    int64s = struct.Struct(f"{count}q").pack
+    size = int64s(*sizes)
+    rc = _serving.lib().ls_page_copy(int64s(*ptrs), size if steps is sizes else int64s(*steps), size,
+                                     count, pages, _address(src), _address(dst), n, stream)
     _lib.check(rc, "ls_page_copy")
 
 
-_shape = operator.attrgetter("shape")
+# (the C slot, past len()'s Python wrapper: a tensor without dimensions has 0)
+_length = torch._C.TensorBase.__len__
 _nbytes = operator.attrgetter("nbytes")
 _requires_grad = operator.attrgetter("requires_grad")
 
@@ -77,7 +81,7 @@ def _address(a: array) -> int:
 
 def _layouts(tensors):
     """Bytes from page to page, and of a page, of tensors that are not all contiguous."""
-    steps, sizes = array("q"), array("q")
+    steps, sizes = [], []
     for t in tensors:
         elems, st = 1, t.stride()
         for k in range(t.dim() - 1, 0, -1):

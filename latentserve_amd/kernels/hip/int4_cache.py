@@ -226,28 +226,28 @@ def paged_decode_int4(q: torch.Tensor, pools, block_tables: torch.Tensor, seq_le
     zeros, and blocks outside the pool are skipped.  out may not overlap q.  Each
     call has its own scratch, so calls may run at once on several streams and from
     several graphs."""
-    nb, h, args = _pools(pools)
-    dev = pools[0].device
-    if q.dim() != 4 or q.shape[1] != h or q.shape[3] != HEAD_DIM \
-            or not 1 <= q.shape[2] <= MAX_NREP:
+    _, h, args = _pools(pools)
+    shape, dev, index = q.shape, q.device, q.get_device()
+    if len(shape) != 4 or shape[1] != h or shape[3] != HEAD_DIM \
+            or not 1 <= shape[2] <= MAX_NREP:
         raise ValueError(f"q must be [B, {h}, n_rep 1..{MAX_NREP}, {HEAD_DIM}], got "
-                         f"{tuple(q.shape)}")
-    if q.get_device() != pools[0].get_device():
+                         f"{tuple(shape)}")
+    if index != pools[0].get_device():
         raise ValueError("q must be on the pools' device")
-    b, _, n_rep, _ = q.shape
-    _tables(block_tables, seq_lens, b, pools[0].get_device())
+    b, _, n_rep, _ = shape
+    _tables(block_tables, seq_lens, b, index)
     stream = _lib.stream_of(dev)
     qs = _rows("q", q)
     if out is None:
         out = torch.empty(b, h, n_rep, HEAD_DIM, dtype=torch.float16, device=dev)
         os = _lib._I64N[3](h * n_rep * HEAD_DIM, n_rep * HEAD_DIM, HEAD_DIM)
     else:
-        if out.shape != q.shape or out.device != dev:
-            raise ValueError(f"out must be {tuple(q.shape)} on {dev}")
+        if out.shape != shape or out.device != dev:
+            raise ValueError(f"out must be {tuple(shape)} on {dev}")
         os = _rows("out", out)
         if b and _span(out)[0] < _span(q)[1] and _span(q)[0] < _span(out)[1]:
             raise ValueError("out may not overlap q, which other workgroups still read")
-    if dev.index != _serving.current_device():
+    if index != _serving.current_device():
         with torch.cuda.device(dev):
             return paged_decode_int4(q, pools, block_tables, seq_lens, max_seq_len, softmax_scale,
                                      out)

@@ -159,11 +159,12 @@ def write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, pools) -> None:
     channels that holds a NaN or an infinity reads back as NaN."""
     nb, h, args = _pools(pools, written=True)
     dev = pools[0].device
-    if k.dim() != 4 or k.shape != v.shape or k.shape[1] != h or k.shape[3] != HEAD_DIM:
-        raise ValueError(f"k and v must be [B, {h}, n, {HEAD_DIM}], got {tuple(k.shape)} and "
+    shape = k.shape
+    if len(shape) != 4 or shape != v.shape or shape[1] != h or shape[3] != HEAD_DIM:
+        raise ValueError(f"k and v must be [B, {h}, n, {HEAD_DIM}], got {tuple(shape)} and "
                          f"{tuple(v.shape)}")
-    b, _, n, _ = k.shape
-    if slots.dtype != torch.int64 or slots.shape != (b * n,) \
+    b, _, n, _ = shape
+    if slots.dtype is not torch.int64 or slots.shape != (b * n,) \
             or (b * n > 1 and slots.stride(0) != 1):
         raise ValueError(f"slots must be {b * n} unit-stride int64 values")
     index = pools[0].get_device()
@@ -185,7 +186,7 @@ def read(pools, block_tables: torch.Tensor, seq_lens: torch.Tensor,
          length: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """(k, v) [B, H, length, 128] fp16: the values that each sequence's first
     `length` entries stand for (default: the table's width), zeros past its
-    end.  Views of one [2, B, length, H, 128] buffer."""
+    end.  Token-major in memory, as [B, length, H, 128]."""
     nb, h, args = _pools(pools)
     dev = pools[0].device
     b = block_tables.shape[0]
@@ -201,18 +202,17 @@ def read(pools, block_tables: torch.Tensor, seq_lens: torch.Tensor,
     if width > _MAX_WIDTH:
         raise ValueError(f"block tables of {width} pages are too wide")
     token = h * HEAD_DIM
-    kv = torch.empty_strided((2, b, h, length, HEAD_DIM),
-                             (b * length * token, length * token, HEAD_DIM, token, 1),
-                             dtype=torch.float16, device=dev)
+    shape, steps = (b, h, length, HEAD_DIM), (length * token, HEAD_DIM, token, 1)
+    k = torch.empty_strided(shape, steps, dtype=torch.float16, device=dev)
+    v = torch.empty_strided(shape, steps, dtype=torch.float16, device=dev)
     if width == 0:
-        kv.zero_()
-    elif b * length:
-        at = kv.data_ptr()
+        return k.zero_(), v.zero_()
+    if b * length:
         rc = _serving.lib().ls_int4_read(
-            *args, block_tables.data_ptr(), block_tables.stride(0), width, seq_lens.data_ptr(), at,
-            at + 2 * b * length * token, b, h, HEAD_DIM, PAGE, length, stream)
+            *args, block_tables.data_ptr(), block_tables.stride(0), width, seq_lens.data_ptr(),
+            k.data_ptr(), v.data_ptr(), b, h, HEAD_DIM, PAGE, length, stream)
         _lib.check(rc, "ls_int4_read")
-    return kv.unbind(0)
+    return k, v
 
 
 def paged_decode_int4(q: torch.Tensor, pools, block_tables: torch.Tensor, seq_lens: torch.Tensor,

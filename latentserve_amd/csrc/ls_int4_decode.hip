@@ -14,11 +14,11 @@
 //    eight 16x16x32 MFMAs (one a channel group and page); PV: O^T[128 ch x 16 rows]
 //    += V^T . P^T, eight more.  The QK result is already the PV operand's layout, as
 //    in the fp16 walk (ls_decode.hip).
-//  * Codes to fp16: two of a word's codes at once are spliced under the exponent
-//    of 1024.0h (bits 0..3 of a half) or 64.0h (bits 4..7), the bias subtracted
-//    exactly, then one packed fused multiply-add gives fp16(m + s * code).  V's
-//    words of two tokens are first spliced by halves, so that a pair is two tokens
-//    of one channel, the operand V^T needs.
+//  * Codes to fp16: a nibble in a byte is an fp8 value, converted two at once, then one
+//    packed fused multiply-add gives fp16(m + s * code).  V's words of two tokens are
+//    first interleaved by bytes, so that a pair is two tokens of one channel, the
+//    operand V^T needs.  (Spliced under fp16 exponents, two instructions a pair, B16 x
+//    64K took 63.3 us, not 60.3.)
 //  * Bound: 160 bytes a token and head from HBM, and the codes' way to fp16 beside it
 //    (372 vector instructions a wave and two pages, 17 MFMAs).  B16 x 16K, 2 heads, 84 MB:
 //    21 to 23 us, 4.0 TB/s; its loads alone take 18 us and its arithmetic
@@ -75,26 +75,15 @@ struct Int4State {
 __device__ __forceinline__ h2 as_h2(uint32_t x) { return __builtin_bit_cast(h2, x); }
 __device__ __forceinline__ uint32_t bits(h2 v) { return __builtin_bit_cast(uint32_t, v); }
 
-// The splice's constants in registers (masks scalar, exponents vector), where one
-// v_and_or_b32 takes both; as literals each would be an instruction of its own.
-struct Splice {
-    uint32_t lo, hi, e1024, e64;
-};
-__device__ __forceinline__ Splice make_splice() {
-    Splice s = {0x000F000Fu, 0x00F000F0u, 0x64006400u, 0x54005400u};
-    asm("" : "+s"(s.lo), "+s"(s.hi), "+v"(s.e1024), "+v"(s.e64));
-    return s;
-}
-
-// Four pairs of codes: pair i is codes i and i + 4 of the word (of each half of
-// the dword), as fp16, exactly.
-__device__ __forceinline__ void code_pairs(const Splice& k, uint32_t x, h2 (&p)[4]) {
-    const h2 b1024 = {(half_t)1024.f, (half_t)1024.f}, b64 = {(half_t)64.f, (half_t)64.f};
-    const uint32_t y = x >> 8;
-    p[0] = as_h2((x & k.lo) | k.e1024) - b1024;
-    p[1] = as_h2((x & k.hi) | k.e64) - b64;
-    p[2] = as_h2((y & k.lo) | k.e1024) - b1024;
-    p[3] = as_h2((y & k.hi) | k.e64) - b64;
+// Four pairs of a word's codes as fp16, exactly: (0, 2), (1, 3), (4, 6), (5, 7).  A byte
+// 0 .. 15 is that many times 2^-9 as fp8 (e4m3: 0 .. 7 its subnormals, 8 .. 15 the first
+// normal ones), which the conversion multiplies by its power of two.
+__device__ __forceinline__ void code_pairs(uint32_t x, h2 (&p)[4]) {
+    const uint32_t lo = x & 0x0F0F0F0Fu, hi = (x >> 4) & 0x0F0F0F0Fu;
+    p[0] = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.f, false));
+    p[1] = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.f, false));
+    p[2] = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 512.f, true));
+    p[3] = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 512.f, true));
 }
 
 __device__ __forceinline__ h2 splat_lo(uint32_t x) {
@@ -124,7 +113,7 @@ __device__ __forceinline__ void int4_load(const Int4DecodeParams& a, Int4Page& d
 
 // Two adjacent pages, the first one's first token tok0; token tok0 + i counts if it is
 // below len[i / 16].  scale > 0.
-__device__ __forceinline__ void int4_compute(const Splice& sp, const Int4Page (&d)[2],
+__device__ __forceinline__ void int4_compute(const Int4Page (&d)[2],
                                              Int4State& st, const h8 (&q)[4], int tok0,
                                              const int (&len)[2], float scale, int g) {
     f4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -133,7 +122,7 @@ __device__ __forceinline__ void int4_compute(const Splice& sp, const Int4Page (&
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
             h2 p[4];
-            code_pairs(sp, d[z].kc[j], p);
+            code_pairs(d[z].kc[j], p);
             const h2 ks = splat_lo(d[z].ka[j]), km = splat_hi(d[z].ka[j]);
             u4 w;
 #pragma unroll
@@ -185,14 +174,15 @@ __device__ __forceinline__ void int4_compute(const Splice& sp, const Int4Page (&
 
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-        // this half's four codes of tokens 4g, 4g + 1 (and 4g + 2, 4g + 3)
-        const uint32_t sel = half ? 0x07060302u : 0x05040100u;
+        // this half's four codes of tokens 4g, 4g + 1 (and 4g + 2, 4g + 3), their bytes in
+        // turn: a pair is one code of both
+        const uint32_t sel = half ? 0x07030602u : 0x05010400u;
         u4 w[4];
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
             h2 p01[4], p23[4];
-            code_pairs(sp, __builtin_amdgcn_perm(d[z].vc.y, d[z].vc.x, sel), p01);
-            code_pairs(sp, __builtin_amdgcn_perm(d[z].vc.w, d[z].vc.z, sel), p23);
+            code_pairs(__builtin_amdgcn_perm(d[z].vc.y, d[z].vc.x, sel), p01);
+            code_pairs(__builtin_amdgcn_perm(d[z].vc.w, d[z].vc.z, sel), p23);
             const h2 s01 = as_h2(va[z].x), s23 = as_h2(va[z].y), m01 = as_h2(va[z].z),
                      m23 = as_h2(va[z].w);
 #pragma unroll
@@ -394,7 +384,6 @@ void int4_decode_kernel(const Int4DecodeParams a) {
     // 0 is the smallest there is (of -inf, a masked score, nothing else would stay -inf).
     const float scale = fmaxf(fabsf(a.scale) * I4_LOG2E, 0x1p-126f);
     const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
-    const Splice sp = make_splice();
     int mine = 0;                                    // 0, which the compiler does not know
     asm("" : "+v"(mine));
     // Query rows (past n_rep: row 0, never stored), channels 32 j + 8 g + (0..7).
@@ -453,7 +442,7 @@ void int4_decode_kernel(const Int4DecodeParams a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const h8 t = __builtin_bit_cast(h8, (u4)(q_raw[j] ^ flip));
-            q[j] = (h8){t[0], t[4], t[1], t[5], t[2], t[6], t[3], t[7]};
+            q[j] = (h8){t[0], t[2], t[1], t[3], t[4], t[6], t[5], t[7]};
         }
         // what the next sequence of the run needs, ahead of its turn
         const int b_next = more ? b + 1 : b;
@@ -519,7 +508,7 @@ void int4_decode_kernel(const Int4DecodeParams a) {
                     ahead_blk = blocks(ahead);
                     claimed = claim();
                     const int lens[2] = {blk[z][0] >= 0 ? len : 0, blk[z][1] >= 0 ? len : 0};
-                    int4_compute(sp, page[z], st, q, (c0 + 2 * item[z]) * PAGE, lens, scale, g);
+                    int4_compute(page[z], st, q, (c0 + 2 * item[z]) * PAGE, lens, scale, g);
                     live = there;
                 }
             }

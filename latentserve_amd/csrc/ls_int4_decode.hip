@@ -20,10 +20,10 @@
 //    operand V^T needs.  (Spliced under fp16 exponents, two instructions a pair, B16 x
 //    64K took 63.3 us, not 60.3.)
 //  * Bound: 160 bytes a token and head from HBM, and the codes' way to fp16 beside it
-//    (372 vector instructions a wave and two pages, 17 MFMAs).  B16 x 16K, 2 heads, 84 MB:
-//    21 to 23 us, 4.0 TB/s; its loads alone take 18 us and its arithmetic
-//    alone 17, of each 8 before the first page and after the last (lengths, table, pages;
-//    records, arrival, records).  B1 x 2048 is that chain, 7.4 us.
+//    (339 vector instructions a wave and two pages, 17 MFMAs).  B16 x 16K, 2 heads, 84 MB:
+//    21.0 us, 4.0 TB/s; its loads alone take 18 us and its arithmetic alone 16, of each 8
+//    before the first page and after the last (lengths, table, pages; records, arrival,
+//    records).  B16 x 64K 61.5 us, 5.5 TB/s; B1 x 2048 is that chain, 7.4 us.
 //  * Online softmax in the log2 domain; a step in which no row's maximum moved skips
 //    the rescale.  Maxima and sums are fp32; the weights are rounded to fp16 for the
 //    MFMA as the fp16 walk rounds them, and summed as rounded, by an MFMA with ones.

@@ -79,7 +79,7 @@ def lib() -> ctypes.CDLL:
 # graph, which may be replayed beside anything, has records of the graph's own and a
 # slice of counters for good.  Slices come from zero-filled slabs made outside
 # captures; a capture that finds none left has its counters zeroed by the graph itself.
-_SLAB_INTS = 1 << 18
+_SLAB_INTS = 1 << 20                  # (a full decode takes 2048: over 250 layers captured at once)
 _by_stream: Dict[tuple, tuple] = {}   # (device index, stream) -> (records, counters)
 _slabs: Dict[int, List] = {}          # device index -> [newest slab, ints taken]
 _kept: List[torch.Tensor] = []        # slabs, whose addresses graphs hold

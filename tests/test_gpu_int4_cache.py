@@ -442,3 +442,27 @@ def test_many_captures_have_their_own_counters():
     for _, outs in graphs:
         for o in (outs[0], outs[77], outs[-1]):
             check(o, q, arrays, tables, ln, "captures")
+
+
+def test_a_capture_without_counters_left_zeroes_its_own(monkeypatch):
+    """Every slice of the slab taken: the graph clears its counters itself, each replay."""
+    from latentserve_amd import _serving
+
+    q, arrays, tables, ln = attend_case([3000, 300, 40], seed=66)
+    args = (dev(q), pools_of(arrays), dev(tables), dev(ln))
+    eager = i4().paged_decode_int4(*args)
+    slab = _serving._slabs[0][0]
+    monkeypatch.setitem(_serving._slabs, 0, [slab, _serving._SLAB_INTS])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = [i4().paged_decode_int4(*args) for _ in range(3)]
+    monkeypatch.undo()
+    for _ in range(4):
+        for o in outs:
+            o.zero_()
+        g.replay()
+        i4().paged_decode_int4(*args)
+        torch.cuda.synchronize()
+        for o in outs:
+            check(o, q, arrays, tables, ln, "replay")
+    check(eager, q, arrays, tables, ln, "eager")

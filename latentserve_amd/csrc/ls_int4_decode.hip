@@ -25,8 +25,11 @@
 //    before the first page and after the last (lengths, table, pages; records, arrival,
 //    records).  B16 x 64K 61.5 us, 5.5 TB/s; B1 x 2048 is that chain, 7.4 us.
 //  * Online softmax in the log2 domain; a step in which no row's maximum moved skips
-//    the rescale.  Maxima and sums are fp32; the weights are rounded to fp16 for the
-//    MFMA as the fp16 walk rounds them, and summed as rounded, by an MFMA with ones.
+//    the rescale.  Maxima and sums are fp32; a weight is two fp16 numbers, 21 bits and more
+//    (one, as the fp16 walk has it, put a rounding of 2^-12 a weight beside the result's
+//    own, and lost those below 2^-25 of the largest), summed as they are by an MFMA with
+//    ones.  Up to 8 rows the second one takes matrix columns that were idle (B16 x 64K 62.6 ->
+//    63.2 us, B48 ragged to 1531 of 8 heads 19.0 -> 19.2; as products of their own 67.6, 19.5).
 
 #include "ls_common.h"
 #include "ls_serving.h"
@@ -36,6 +39,11 @@ namespace ls {
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
 constexpr float I4_LOG2E = 1.4426950408889634f;
+// The largest weight is 2^I4_TOP (it cancels in the division by their sum): the least that
+// fp16 holds is then 2^-39 of it.  Against 1, all below 2^-25 vanished, a long tail under a
+// large score with them.
+constexpr float I4_TOP = 15.f;
+constexpr int I4_PAIRED = MAX_NREP / 2;
 constexpr int I4_NW = 4;                 // waves a group
 constexpr int I4_ROW = HEAD_DIM + 4;     // LDS row: 16 rows written at once fall in different banks
 constexpr int I4_RESIDENT = 512;         // groups resident at once: two a CU
@@ -99,6 +107,12 @@ __device__ __forceinline__ f4 mfma32(u4 a, h8 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), b, c, 0, 0, 0);
 }
 
+// Two weights as fp16, towards zero: one over fp16's largest value is that value, not an
+// infinity.
+__device__ __forceinline__ h2 truncated(float a, float b) {
+    return __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(a, b));
+}
+
 // blk < 0: zeros, without a memory request.
 __device__ __forceinline__ void int4_load(const Int4DecodeParams& a, Int4Page& d, int blk, int h,
                                           int g, int c) {
@@ -113,9 +127,15 @@ __device__ __forceinline__ void int4_load(const Int4DecodeParams& a, Int4Page& d
 
 // Two adjacent pages, the first one's first token tok0; token tok0 + i counts if it is
 // below len[i / 16].  scale > 0.
+//
+// A weight p goes into the products as two fp16 numbers, itself truncated and what that
+// leaves, 21 bits or more of it.  Up to 8 rows: in columns c and c + 8, which hold one
+// row's scores (`take` is 0 in the first, -1 in the second), so they cost no product.  More
+// rows (WIDE, take -1): a second product each.
+template <bool WIDE>
 __device__ __forceinline__ void int4_compute(const Int4Page (&d)[2],
                                              Int4State& st, const h8 (&q)[4], int tok0,
-                                             const int (&len)[2], float scale, int g) {
+                                             const int (&len)[2], float scale, int g, float take) {
     f4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -155,13 +175,21 @@ __device__ __forceinline__ void int4_compute(const Int4Page (&d)[2],
     top = fmaxf(fmaxf(top, s[1][1]), fmaxf(s[1][2], s[1][3]));
     top = group4_max(top);
     // (a row of -inf only has nothing valid yet)
-    const float m_new = fmaxf(st.m, top * scale);
+    const float m_new = fmaxf(st.m, __builtin_fmaf(top, scale, -I4_TOP));
     const float m_use = m_new == neg_inf() ? 0.f : m_new;
     const float alpha = fast_exp2(st.m - m_use);
-    h8 pb;
+    h8 hi, part;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        pb[i] = (half_t)fast_exp2(__builtin_fmaf(s[i / 4][i % 4], scale, -m_use));
+    for (int i = 0; i < 4; ++i) {
+        const float p0 = fast_exp2(__builtin_fmaf(s[i / 2][2 * (i % 2)], scale, -m_use));
+        const float p1 = fast_exp2(__builtin_fmaf(s[i / 2][2 * (i % 2) + 1], scale, -m_use));
+        const h2 a = truncated(p0, p1);
+        const h2 b = truncated(__builtin_fmaf((float)a[0], take, p0),
+                               __builtin_fmaf((float)a[1], take, p1));
+        hi[2 * i] = a[0];
+        hi[2 * i + 1] = a[1];
+        part[2 * i] = b[0];
+        part[2 * i + 1] = b[1];
     }
     if (__any(alpha != 1.f)) {
         st.l *= alpha;
@@ -170,7 +198,8 @@ __device__ __forceinline__ void int4_compute(const Int4Page (&d)[2],
     }
     st.m = m_new;
     constexpr uint32_t ONES = 0x3C003C00u;
-    st.l = mfma32((u4){ONES, ONES, ONES, ONES}, pb, st.l);
+    st.l = mfma32((u4){ONES, ONES, ONES, ONES}, part, st.l);
+    if constexpr (WIDE) st.l = mfma32((u4){ONES, ONES, ONES, ONES}, hi, st.l);
 
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -192,7 +221,10 @@ __device__ __forceinline__ void int4_compute(const Int4Page (&d)[2],
             }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) st.acc[4 * half + i] = mfma32(w[i], pb, st.acc[4 * half + i]);
+        for (int i = 0; i < 4; ++i) st.acc[4 * half + i] = mfma32(w[i], part, st.acc[4 * half + i]);
+        if constexpr (WIDE)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) st.acc[4 * half + i] = mfma32(w[i], hi, st.acc[4 * half + i]);
     }
 }
 
@@ -209,6 +241,15 @@ __device__ __forceinline__ int wave_incl_scan(int x, int lane, int& total) {
     total = r0 + r1 + r2 + r3;
     const int row = lane >> 4;
     return x + (row > 0 ? r0 : 0) + (row > 1 ? r1 : 0) + (row > 2 ? r2 : 0);
+}
+
+// Lanes c and c ^ 8 of 16 added: a row rotation of 8 as part of the addition (every lane
+// has a source; the sum stays where it is made, not under a later branch, apart from the move).
+__device__ __forceinline__ float add_paired(float v) {
+    float r = v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+                                                0, __builtin_bit_cast(int, v), 0x128, 0xF, 0xF, true));
+    asm("" : "+v"(r));
+    return r;
 }
 
 __device__ __forceinline__ void store_coherent(float* p, f4 v) {
@@ -283,6 +324,8 @@ __device__ __forceinline__ void merge_records(const Int4Records& R, int k0, int 
     }
 }
 
+// WIDE: more than I4_PAIRED rows (int4_compute).
+template <bool WIDE>
 __global__ __launch_bounds__(WAVE* I4_NW) __attribute__((amdgpu_waves_per_eu(2)))
 void int4_decode_kernel(const Int4DecodeParams a) {
     __shared__ Int4Smem sm;
@@ -386,10 +429,13 @@ void int4_decode_kernel(const Int4DecodeParams a) {
     const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
     int mine = 0;                                    // 0, which the compiler does not know
     asm("" : "+v"(mine));
-    // Query rows (past n_rep: row 0, never stored), channels 32 j + 8 g + (0..7).
+    // Lane c's query row (past n_rep: row 0, never stored), channels 32 j + 8 g + (0..7).
+    const int row_of = WIDE ? c : c % I4_PAIRED;
+    float take = WIDE || c >= I4_PAIRED ? -1.f : 0.f;
+    if constexpr (WIDE) asm("" : "+s"(take));        // (of a known -1, two instructions)
     auto load_q = [&](int bq, u4 (&t)[4]) {
         const half_t* row = a.q + (int64_t)bq * a.sq_b + (int64_t)h * a.sq_h +
-                            (int64_t)(c < NR ? c : 0) * a.sq_r + 8 * g;
+                            (int64_t)(row_of < NR ? row_of : 0) * a.sq_r + 8 * g;
 #pragma unroll
         for (int j = 0; j < 4; ++j) t[j] = *(const u4*)(row + 32 * j);
     };
@@ -508,10 +554,18 @@ void int4_decode_kernel(const Int4DecodeParams a) {
                     ahead_blk = blocks(ahead);
                     claimed = claim();
                     const int lens[2] = {blk[z][0] >= 0 ? len : 0, blk[z][1] >= 0 ? len : 0};
-                    int4_compute(page[z], st, q, (c0 + 2 * item[z]) * PAGE, lens, scale, g);
+                    int4_compute<WIDE>(page[z], st, q, (c0 + 2 * item[z]) * PAGE, lens, scale, g, take);
                     live = there;
                 }
             }
+        }
+        // both parts of each weight (ahead of the next loads, whose registers this takes)
+        if constexpr (!WIDE) {
+            st.l[0] = add_paired(st.l[0]);
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) st.acc[t][i] = add_paired(st.acc[t][i]);
         }
         // the next sequence's first pair, on its way while this one is merged
         entry = entry_next;
@@ -634,7 +688,9 @@ hipError_t launch_int4_decode(const Int4DecodeParams& a, hipStream_t stream) {
     // (pairs of runs to the blocks L and L + 256, which the dispatcher gives one CU)
     d.skew = a.groups * a.H == I4_RESIDENT && a.groups % 2 == 0;
     d.extra = 4 * a.B > a.groups ? I4_EXTRA : 0;
-    hipLaunchKernelGGL(int4_decode_kernel, dim3(a.groups * a.H), dim3(WAVE * I4_NW), 0, stream, d);
+    const dim3 grid(a.groups * a.H), block(WAVE * I4_NW);
+    if (a.NR > I4_PAIRED) hipLaunchKernelGGL(int4_decode_kernel<true>, grid, block, 0, stream, d);
+    else hipLaunchKernelGGL(int4_decode_kernel<false>, grid, block, 0, stream, d);
     return hipGetLastError();
 }
 

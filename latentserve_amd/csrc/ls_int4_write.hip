@@ -69,8 +69,10 @@ __global__ __launch_bounds__(I4_THREADS) void int4_write_kernel(const Int4WriteP
     const float span = hi - lo, near15 = span * FIFTEENTH;
     half_t s = (half_t)__builtin_fmaf(__builtin_fmaf(-15.f, near15, span), FIFTEENTH, near15);
     // (65520 is where fp16 rounds to infinity; s is then over 4000, and a step of it
-    // less takes 15 s below max)
-    if (lo + 15.f * (float)s >= 65520.f && hi <= 65504.f)
+    // less takes 15 s below max.  On this side the difference is exact wherever it comes
+    // near lo, 15 s being a multiple of 2^-8 at least there; lo + 15 s is not: -2^-24 +
+    // 65520 rounds to 65520.  Checked over all lo and all hi from 60000)
+    if (lo >= 65520.f - 15.f * (float)s && hi <= 65504.f)
         s = __builtin_bit_cast(half_t, (uint16_t)(__builtin_bit_cast(uint16_t, s) - 1));
     // The nearest whole number to (x - m) / s, decided exactly: the fp32 quotient is off by
     // at most 16 * 2^-22 (the difference, the reciprocal and the product round once each,

@@ -38,8 +38,9 @@ class Int4PagedKVCache(_PagedBase):
     def advance(self, n: int, batch_size: Optional[int] = None,
                 slots: Optional[Sequence[int]] = None) -> None:
         """Reserve n more tokens for each active sequence and publish the
-        step's kernel inputs."""
-        self._publish(n, self._grow(n, batch_size, slots))
+        step's kernel inputs.  OutOfBlocks leaves everything as it was."""
+        self._room_for_step(n, batch_size, slots)
+        self._publish(n, self._grow(n))
 
     def rewind(self, length: int, slots: Optional[Sequence[int]] = None) -> None:
         """Shorten sequences to `length` tokens, keeping their pages."""

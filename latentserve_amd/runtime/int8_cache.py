@@ -151,13 +151,10 @@ class Int8PagedKVCache(_PagedBase):
     # ---- steps ----------------------------------------------------------------
     def advance(self, n: int, batch_size: Optional[int] = None,
                 slots: Optional[Sequence[int]] = None) -> None:
-        if slots is not None:
-            self.set_active(slots)
-        elif batch_size is not None:
-            self.set_active(range(batch_size))
+        self._room_for_step(n, batch_size, slots)
         if n > 0:
             self._pool_full_last_pages(self._active)
-        starts = self._grow(n, None, None)
+        starts = self._grow(n)
         self._starts = starts
         bs = self.block_size
         extra = {"res_row": list(self._active)}

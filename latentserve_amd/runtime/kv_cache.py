@@ -102,13 +102,17 @@ class BlockAllocator:
         cache holds alone."""
         return len(self._stack) + (self.reclaimable() if self.reclaimable else 0)
 
-    def allocate(self, count: int) -> List[int]:
-        count = int(count)
+    def ensure(self, count: int) -> None:
+        """`count` blocks free, reclaimed where it takes that; else OutOfBlocks."""
         if count > len(self._stack) and self.reclaimer is not None:
             self.reclaimer(count - len(self._stack))
         if count > len(self._stack):
             raise OutOfBlocks(f"cannot allocate {count} blocks: only {len(self._stack)} of "
                               f"{self.num_blocks} are free")
+
+    def allocate(self, count: int) -> List[int]:
+        count = int(count)
+        self.ensure(count)
         taken = self._stack[len(self._stack) - count:][::-1]
         del self._stack[len(self._stack) - count:]
         self.alloc_calls += 1
@@ -425,31 +429,42 @@ class _PagedBase:
             child.version += 1
             child.lineage += 1
 
-    def _own_pages(self, seqs: Sequence[int], n: int) -> None:
-        """Before n tokens are written: the pages they go to that other sequences
-        (or a prefix cache) hold too are replaced by pages of their own, with
-        the tokens they keep."""
+    def _make_room(self, seqs: Sequence[int], n: int) -> None:
+        """Pages for n more tokens of each sequence, lengths unchanged; and of the pages
+        they go to, those that other sequences (or a prefix cache) hold too are
+        replaced by pages of their own, with the tokens they keep.  All or
+        nothing: where the pool has not the blocks for all of it (OutOfBlocks),
+        or a sequence would outgrow the cache, nothing has changed."""
         bs, refs = self.block_size, self.allocator.ref_count
-        todo, left = [], {}
+        todo, left, grown = [], {}, 0
         for s in seqs:
             t = self.tables[s]
-            first = t.length // bs
-            for page in range(first, min(len(t.blocks), -(-(t.length + n) // bs))):
+            first, have, end = t.length // bs, len(t.blocks), -(-(t.length + n) // bs)
+            if end > have:
+                if end > self.capacity_pages:
+                    raise RuntimeError(f"the sequence in slot {s} would hold {end} pages; the "
+                                       f"cache was sized for {self.capacity_pages}")
+                grown += end - have
+            for page in range(first, min(have, end)):
                 blk = t.blocks[page]
                 count = left.get(blk, refs(blk))
                 if count > 1:
                     left[blk] = count - 1              # the last to write keeps the page
                     todo.append((t, page, blk, page == first and t.length % bs > 0))
-        if not todo:
-            return
-        fresh = self.allocator.allocate(len(todo))     # (OutOfBlocks: nothing has changed)
-        kept = [(blk, new) for (_, _, blk, keeps), new in zip(todo, fresh) if keeps]
-        self._copy_rows(self._page_tensors(), [a for a, _ in kept], [b for _, b in kept])
-        for (t, page, blk, _), new in zip(todo, fresh):
-            t.blocks[page] = new
-            t.version += 1
-            t.lineage += 1
-        self.allocator.free([blk for _, _, blk, _ in todo])
+        if grown or todo:
+            self.allocator.ensure(grown + len(todo))
+        if todo:
+            fresh = self.allocator.allocate(len(todo))
+            kept = [(blk, new) for (_, _, blk, keeps), new in zip(todo, fresh) if keeps]
+            self._copy_rows(self._page_tensors(), [a for a, _ in kept], [b for _, b in kept])
+            for (t, page, blk, _), new in zip(todo, fresh):
+                t.blocks[page] = new
+                t.version += 1
+                t.lineage += 1
+            self.allocator.free([blk for _, _, blk, _ in todo])
+        if grown:
+            for s in seqs:
+                self.tables[s].reserve(n)
 
     def compact(self) -> Dict[int, int]:
         """Move the held pages to the pool's lowest blocks, so that they are blocks
@@ -492,16 +507,20 @@ class _PagedBase:
         self.inputs.forget_rows()
 
     # ---- per-step inputs --------------------------------------------------
-    def _grow(self, n: int, batch_size, slots) -> List[int]:
-        """Extend the active sequences by n tokens; returns their old lengths."""
-        if slots is not None:
-            self.set_active(slots)
-        elif batch_size is not None:
-            self.set_active(range(batch_size))
+    def _room_for_step(self, n: int, batch_size, slots) -> None:
+        """The sequences that a step extends become the active ones, with room for n more
+        tokens each; where there is none, nothing has changed."""
+        seqs = list(slots) if slots is not None else \
+            self._active if batch_size is None else list(range(batch_size))
+        self._make_room(seqs, n)
+        self._active = seqs
+
+    def _grow(self, n: int) -> List[int]:
+        """Extend the active sequences by n tokens, which there is room for; returns
+        their old lengths."""
         starts = [self.tables[s].length for s in self._active]
-        self._own_pages(self._active, n)
         for s in self._active:
-            self.tables[s].append(n)
+            self.tables[s].length += n
         return starts
 
     def _publish(self, n: int, starts: List[int], extra: Optional[dict] = None) -> None:
@@ -584,9 +603,10 @@ class PagedKVCache(_PagedBase):
     def advance(self, n: int, batch_size: Optional[int] = None,
                 slots: Optional[Sequence[int]] = None) -> None:
         """Reserve n more tokens for each active sequence (paged_cache.py:
-        235-271) and publish the step's kernel inputs."""
-        starts = self._grow(n, batch_size, slots)
-        self._publish(n, starts)
+        235-271) and publish the step's kernel inputs.  OutOfBlocks leaves
+        every sequence, and which are active, as they were."""
+        self._room_for_step(n, batch_size, slots)
+        self._publish(n, self._grow(n))
 
     def rewind(self, length: int, slots: Optional[Sequence[int]] = None) -> None:
         """Shorten sequences to `length` tokens, keeping their pages
@@ -596,7 +616,8 @@ class PagedKVCache(_PagedBase):
         self._shorten(length, seqs)
         if self.kmin is not None and length % self.block_size:
             try:
-                self._own_pages(seqs, 0)      # (its bounds change: no one else's may)
+                # (its bounds change: no one else's may)
+                self._make_room(seqs, 0)
             except OutOfBlocks:
                 for s, n in zip(seqs, before):
                     self.tables[s].length = n

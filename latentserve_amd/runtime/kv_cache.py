@@ -512,6 +512,8 @@ class _PagedBase:
         tokens each; where there is none, nothing has changed."""
         seqs = list(slots) if slots is not None else \
             self._active if batch_size is None else list(range(batch_size))
+        if len(set(seqs)) != len(seqs):
+            raise ValueError(f"slots {seqs}: a sequence is named twice")
         self._make_room(seqs, n)
         self._active = seqs
 
@@ -617,7 +619,7 @@ class PagedKVCache(_PagedBase):
         if self.kmin is not None and length % self.block_size:
             try:
                 # (its bounds change: no one else's may)
-                self._make_room(seqs, 0)
+                self._make_room(list(dict.fromkeys(seqs)), 0)
             except OutOfBlocks:
                 for s, n in zip(seqs, before):
                     self.tables[s].length = n

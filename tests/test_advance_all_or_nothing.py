@@ -78,6 +78,28 @@ def test_a_sequence_past_the_capacity(kind):
     c.advance(12, slots=[0, 1])
 
 
+@pytest.mark.parametrize("kind", CACHES)
+def test_a_sequence_named_twice_is_refused(kind):
+    c = of(kind, 20)
+    c.advance(5, slots=[0, 1])
+    before = state(c)
+    for slots in ([0, 0], [1, 0, 1]):
+        with pytest.raises(ValueError):
+            c.advance(1, slots=slots)
+        same(state(c), before)
+
+
+def test_a_page_of_bounds_owned_once_where_a_rewind_names_a_sequence_twice(monkeypatch):
+    c = cache()
+    grow(c, [0], [list(range(20))])
+    c.fork(0, [1, 2])
+    c.kmin = c.kmax = []                             # (page bounds are the GPU's to keep)
+    monkeypatch.setattr(c, "_bound_partial_page", lambda *a: None)
+    c.rewind(18, slots=[1, 1])
+    base = list(range(20))
+    check_refs(c, [base, base[:18], base, [], [], []])
+
+
 def test_blocks_that_a_prefix_cache_holds_alone_count():
     """A step takes what reclaiming gives, copies and pages together; one more is too many."""
     for blocks, fits in ((6, True), (5, False)):

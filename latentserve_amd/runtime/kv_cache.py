@@ -410,15 +410,17 @@ class _PagedBase:
         holds the same tokens, on the same pages, and grows its own way from
         there.  Nothing is copied now: a page that several sequences hold is
         copied when one of them is about to write it (advance()).  Between
-        steps only: the tokens of the last advance() must have been written."""
+        steps only: the tokens of the last advance() must have been written
+        (the caller's to see to: a replayed graph's writes pass the cache by)."""
         children = list(children)
+        for s in [index] + children:
+            if not 0 <= s < len(self.tables):
+                raise ValueError(f"slot {s} is not one of {len(self.tables)}")
         t = self.tables[index]
         if len(set(children)) != len(children):
             raise ValueError(f"slots {children}: a child is named twice")
         for c in children:
-            if not 0 <= c < len(self.tables):
-                raise ValueError(f"slot {c} is not one of {len(self.tables)}")
-            if self.tables[c].length or self.tables[c].blocks:
+            if c == index or self.tables[c].length or self.tables[c].blocks:
                 raise ValueError(f"slot {c} already holds a sequence")
         pages = t.blocks[:self.allocator.blocks_for_tokens(t.length)]
         for c in children:

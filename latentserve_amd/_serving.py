@@ -8,8 +8,11 @@ the scratch that their calls take.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import threading
+import weakref
+from collections import deque
 from typing import Dict, List, Optional
 
 import torch
@@ -75,14 +78,22 @@ def lib() -> ctypes.CDLL:
 
 # Scratch of a call: records (any contents) and arrival counters (int32, zero at rest:
 # every call leaves its own at zero).  Two calls that may run at once may not share
-# it: a device's streams have their own, kept and grown, and a call recorded into a
-# graph, which may be replayed beside anything, has records of the graph's own and a
-# slice of counters for good.  Slices come from zero-filled slabs made outside
-# captures; a capture that finds none left has its counters zeroed by the graph itself.
+# it.  A device's streams have their own, kept and grown up to a bound (a stream is
+# known by its handle, as to torch's allocator: work of a destroyed stream has ended
+# before its handle is used again).  A call recorded into a graph, which may be
+# replayed beside anything, has records of the graph's own and a slice of counters
+# that goes back when the graph is gone (counters_of), or is the call's for good where
+# nobody says which graph that is.  Slices come from zero-filled slabs made
+# outside captures; a capture that finds none left has its counters zeroed by the
+# graph itself.
 _SLAB_INTS = 1 << 20                  # (a full decode takes 2048: over 250 layers captured at once)
+_KEPT_BYTES, _KEPT_INTS = 16 << 20, 1 << 18          # a larger call's go back to the allocator
 _by_stream: Dict[tuple, tuple] = {}   # (device index, stream) -> (records, counters)
 _slabs: Dict[int, List] = {}          # device index -> [newest slab, ints taken]
 _kept: List[torch.Tensor] = []        # slabs, whose addresses graphs hold
+_free: Dict[tuple, List] = {}         # (device index, ints) -> slices that no graph holds
+_returned: deque = deque()            # (device index, slices) of graphs that are gone
+_owner = threading.local()            # .slices: where this thread's captured calls list theirs
 _lock = threading.Lock()              # two captures at once may not get one slice
 # (what torch.cuda.is_current_stream_capturing and current_device wrap, without their
 # checks that CUDA is initialised: a launch's stream lookup has done that)
@@ -90,16 +101,71 @@ _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None)
 current_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
+def _room(device: torch.device) -> None:
+    """A slab with room for the captures to come."""
+    have = _slabs.get(device.index)
+    if have is None or 2 * have[1] > _SLAB_INTS:
+        slab = torch.zeros(_SLAB_INTS, dtype=torch.int32, device=device)
+        # (filled on this stream; a graph that takes a slice may replay on any)
+        torch.cuda.current_stream(device).synchronize()
+        _kept.append(slab)
+        _slabs[device.index] = [slab, 0]
+
+
+@contextlib.contextmanager
+def counters_of(graph: torch.cuda.CUDAGraph):
+    """Around a capture: the counters that its calls take go back once `graph` is gone.
+
+        with counters_of(g), torch.cuda.graph(g):
+            ...
+    """
+    index = torch.cuda.current_device()
+    if _returned:
+        # (a graph may be dropped while its last replay runs)
+        gone = [_returned.popleft() for _ in range(len(_returned))]
+        for i in {i for i, _ in gone}:
+            torch.cuda.synchronize(i)
+        with _lock:
+            for i, slices in gone:
+                for cnt in slices:
+                    _free.setdefault((i, cnt.numel()), []).append(cnt)
+    _room(torch.device("cuda", index))
+    outer, _owner.slices = getattr(_owner, "slices", None), []
+    try:
+        yield
+    finally:
+        slices, _owner.slices = _owner.slices, outer
+        if slices:
+            # (a finalizer may run anywhere, under the lock too: it takes none)
+            weakref.finalize(graph, _returned.append, (index, slices)).atexit = False
+
+
 def _captured_scratch(device: torch.device, nbytes: int, ints: int):
     work = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    have = _slabs.get(device.index)
+    cnt = _slice_for_capture(device.index, ints)
+    return work, torch.zeros(ints, dtype=torch.int32, device=device) if cnt is None else cnt
+
+
+def _slice_for_capture(index: int, ints: int) -> Optional[torch.Tensor]:
     take = -(-ints // 32) * 32                               # whole 128-byte lines
     with _lock:
-        if have is None or have[1] + take > _SLAB_INTS:
-            return work, torch.zeros(ints, dtype=torch.int32, device=device)
-        at = have[1]
-        have[1] += take
-    return work, have[0][at:at + take]
+        cnt = _slice(index, take)
+    slices = getattr(_owner, "slices", None)
+    if cnt is not None and slices is not None:
+        slices.append(cnt)
+    return cnt
+
+
+def _slice(index: int, take: int) -> Optional[torch.Tensor]:
+    free = _free.get((index, take))
+    if free:
+        return free.pop()
+    have = _slabs.get(index)
+    if have is None or have[1] + take > _SLAB_INTS:
+        return None
+    at = have[1]
+    have[1] += take
+    return have[0][at:at + take]
 
 
 def scratch(device: torch.device, stream: int, nbytes: int, ints: int):
@@ -109,14 +175,13 @@ def scratch(device: torch.device, stream: int, nbytes: int, ints: int):
         return _captured_scratch(device, nbytes, ints)
     index = device.index
     have = _slabs.get(index)
-    if have is None or 2 * have[1] > _SLAB_INTS:             # room for the captures to come
-        slab = torch.zeros(_SLAB_INTS, dtype=torch.int32, device=device)
-        # (filled on this stream; a graph that takes a slice may replay on any)
-        torch.cuda.current_stream(device).synchronize()
-        _kept.append(slab)
-        _slabs[index] = [slab, 0]
+    if have is None or 2 * have[1] > _SLAB_INTS:
+        _room(device)
     got = _by_stream.get((index, stream))
     if got is None or got[0].numel() < nbytes or got[1].numel() < ints:
+        if nbytes > _KEPT_BYTES or ints > _KEPT_INTS:
+            return (torch.empty(nbytes, dtype=torch.uint8, device=device),
+                    torch.zeros(ints, dtype=torch.int32, device=device))
         # (an outgrown pair goes back to the allocator, which hands it on in this
         # stream's order)
         old = got or (torch.empty(0, dtype=torch.uint8), torch.empty(0, dtype=torch.int32))

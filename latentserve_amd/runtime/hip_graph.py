@@ -35,6 +35,7 @@ from typing import Dict, Optional, Sequence, Tuple
 
 import torch
 
+from latentserve_amd._serving import counters_of
 from latentserve_amd.kernels import fused_elementwise as fe
 from latentserve_amd.kernels.logprobs import TokenLogprobs, token_logprobs
 
@@ -128,7 +129,7 @@ class CapturedDecode:
                     self._forward()
             torch.cuda.current_stream().wait_stream(side)
             g = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(g, pool=pool):
+            with counters_of(g), torch.cuda.graph(g, pool=pool):
                 self.logits_buf, self.next_buf, self.logprobs_buf = self._forward()
         self.graph = g
 

@@ -37,7 +37,7 @@ import torch
 
 from latentserve_amd._serving import counters_of
 from latentserve_amd.kernels import fused_elementwise as fe
-from latentserve_amd.kernels.logprobs import TokenLogprobs, token_logprobs
+from latentserve_amd.kernels.logprobs import MAX_TOP, TokenLogprobs, token_logprobs
 
 DEFAULT_BUCKETS = (1024, 2048, 4096, 8192, 16384, 32768)
 
@@ -160,6 +160,10 @@ class GraphedDecoder:
         if logprobs is not None and not greedy:
             raise ValueError("logprobs are of the greedy steps' tokens: GraphedDecoder(..., "
                              "greedy=True)")
+        # (here, not by the first step, which has advanced the cache by then)
+        most = MAX_TOP if logprobs is None else min(MAX_TOP, model.cfg.vocab_size)
+        if logprobs is not None and not 0 <= int(logprobs) <= most:
+            raise ValueError(f"logprobs must be in [0, {most}], got {logprobs}")
         self.model = model
         self.greedy = greedy
         self.logprobs = logprobs

@@ -516,7 +516,8 @@ class _PagedBase:
             self._active if batch_size is None else list(range(batch_size))
         if len(set(seqs)) != len(seqs):
             raise ValueError(f"slots {seqs}: a sequence is named twice")
-        self._make_room(seqs, n)
+        if n:                              # (a step of none writes no page: it shares on)
+            self._make_room(seqs, n)
         self._active = seqs
 
     def _grow(self, n: int) -> List[int]:

@@ -100,6 +100,20 @@ def test_a_page_of_bounds_owned_once_where_a_rewind_names_a_sequence_twice(monke
     check_refs(c, [base, base[:18], base, [], [], []])
 
 
+@pytest.mark.parametrize("kind", CACHES)
+def test_a_step_of_no_tokens_copies_no_page(kind):
+    """advance(0) publishes the sequences; their shared pages stay shared, and no block is
+    asked for."""
+    c = of(kind, 2)
+    c.advance(20, slots=[0])
+    c.fork(0, [1, 2])
+    c.advance(0, slots=[0, 2])
+    assert c.allocator.num_used == 2 and c.active_slots == [0, 2]
+    assert c.tables[0].blocks == c.tables[1].blocks == c.tables[2].blocks
+    assert c.seq_lens_tensor(2).tolist() == [20, 20]
+    assert c.block_tables_tensor(2)[:, :2].tolist() == [c.tables[0].blocks] * 2
+
+
 def test_blocks_that_a_prefix_cache_holds_alone_count():
     """A step takes what reclaiming gives, copies and pages together; one more is too many."""
     for blocks, fits in ((6, True), (5, False)):

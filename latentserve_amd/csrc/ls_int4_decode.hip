@@ -10,7 +10,8 @@
 //    sequence that crosses runs leaves one record a run (acc, m, l), merged by the
 //    last of its groups to arrive (over 16 runs: by the last of each 16, then the
 //    last of those): one launch.
-//  * The waves of a group claim pairs of pages.  QK: S^T[32 tok x 16 rows] = K . Q^T,
+//  * The waves of a group claim pairs of pages (so two calls on the same operands can differ
+//    by a rounding: a wave sums other pages).  QK: S^T[32 tok x 16 rows] = K . Q^T,
 //    eight 16x16x32 MFMAs (one a channel group and page); PV: O^T[128 ch x 16 rows]
 //    += V^T . P^T, eight more.  The QK result is already the PV operand's layout, as
 //    in the fp16 walk (ls_decode.hip).
@@ -18,12 +19,13 @@
 //    packed fused multiply-add gives fp16(m + s * code).  V's words of two tokens are
 //    first interleaved by bytes, so that a pair is two tokens of one channel, the
 //    operand V^T needs.  (Spliced under fp16 exponents, two instructions a pair, B16 x
-//    64K took 63.3 us, not 60.3.)
+//    64K took 3 us more.)
 //  * Bound: 160 bytes a token and head from HBM, and the codes' way to fp16 beside it
-//    (339 vector instructions a wave and two pages, 17 MFMAs).  B16 x 16K, 2 heads, 84 MB:
-//    21.0 us, 4.0 TB/s; its loads alone take 18 us and its arithmetic alone 16, of each 8
-//    before the first page and after the last (lengths, table, pages; records, arrival,
-//    records).  B16 x 64K 61.5 us, 5.5 TB/s; B1 x 2048 is that chain, 7.4 us.
+//    (351 vector instructions a wave and two pages, 17 MFMAs).  B16 x 16K, 2 heads, 84 MB:
+//    22.9 us in a graph, 3.7 TB/s (a plain read of as many bytes 12.6); its loads alone take
+//    18 us and its arithmetic alone 16, of each 8 before the first page and after the last
+//    (lengths, table, pages; records, arrival, records).  B16 x 64K 62.6 us, 5.4 TB/s; B1 x
+//    2048 is that chain, 7.4 us.
 //  * Online softmax in the log2 domain; a step in which no row's maximum moved skips
 //    the rescale.  Maxima and sums are fp32; a weight is two fp16 numbers, 21 bits and more
 //    (one, as the fp16 walk has it, put a rounding of 2^-12 a weight beside the result's
@@ -50,9 +52,10 @@ constexpr int I4_RESIDENT = 512;         // groups resident at once: two a CU
 // Fewest pages a run has: a pair a wave.
 constexpr int I4_MIN_PAGES = 2 * I4_NW;
 // Runs of at least this many pages (all groups have one then) differ, where two groups
-// share each CU: loads of the older group's waves go first, and of even runs its own
+// share each CU (512 groups in all, so head counts that divide 512; 3, 5, 6 or 7 heads make
+// 510 or 511, and their runs stay even): loads of the older group's waves go first, and of even runs its own
 // ended 5 us early at B16 x 16K; of 5 to 3 parts they end together.  (us, even /
-// 5 to 3: B16 x 16K 24.4 / 23.6, B16 x 64K 66.0 / 62.4, 2 x 100K 22.9 / 21.0, B64 ragged to
+// 5 to 3, of one machine and with the walk as it was then: B16 x 16K 24.4 / 23.6, B16 x 64K 66.0 / 62.4, 2 x 100K 22.9 / 21.0, B64 ragged to
 // 4096 of 8 heads 41.5 / 38.9, B96 ragged to 16K 54.6 / 51.0.  A rule of speed only: any
 // group may run anywhere.)
 constexpr int I4_LONG_RUN = 24;

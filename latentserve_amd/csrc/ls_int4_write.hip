@@ -10,9 +10,10 @@
 // a quad of lanes and its minimum and maximum two lane exchanges; a lane reads 16
 // bytes and writes one word of codes.
 //
-// Both are bound by memory, and small calls by the launch and one round trip.  4 x 2048
-// tokens, 2 heads: write 6.8 us for 11 MB, read 5.2 (2 us at a large copy's rate; copies of
-// this size are as far from it); 16 tokens of 2 heads: 3.1 and 3.0.
+// Small calls are bound by the launch and one round trip (16 tokens of 2 heads: 3.1 and 2.9
+// us), large ones by their accesses: an item a thread, V's codes 4 bytes and its steps 2 at
+// a place.  4 x 2048 tokens, 2 heads, 11 MB: write 6.9 us, read 5.3, a plain copy of as many
+// bytes 3.0.
 
 #include "ls_common.h"
 #include "ls_serving.h"

@@ -9,7 +9,8 @@
 // the alternatives); each thread sums against its own maximum, so nothing is exchanged
 // before the sums are made.  Without alternatives a large call streams instead.
 //
-// 1021 fp16 rows of 151936: 57 us, 5.4 TB/s, as a large copy runs; bound by the read.
+// 1021 fp16 rows of 151936: 58 us, 5.3 TB/s; bound by the read (a plain one of as many bytes
+// runs at 7.0).
 // 16 rows with 20 alternatives: 12.0 us (0.9 us of bytes), 1 row without 4.4 us: bound by
 // what each group does once, in turn (load, two exchanges, the ranking, the hand-over to
 // the row's last group and its merge).

@@ -1,8 +1,8 @@
 // Pages copied to other pages of the same pools: t[dst[i]] = t[src[i]] for every
 // tensor t (all layers' K and V pools, scales, bounds) in one launch.
 //
-// Bound by HBM (160 pages of 56 pools, 147 MB read and written: 26.2 us, 5.6 TB/s), and
-// for a few pages by the launch itself (8 pages: 2.7 us): the pointers, strides and page
+// Bound by HBM (160 pages of 56 pools, 147 MB read and written: 26.4 us, 5.6 TB/s), and
+// for a few pages by the launch itself (8 pages: 2.6 us): the pointers, strides and page
 // numbers travel in the kernel's arguments, so a branch of a sequence costs one launch
 // and no transfer.
 
@@ -23,8 +23,8 @@ __global__ __launch_bounds__(COPY_THREADS) void page_copy_kernel(const PageCopyP
     const int n = a.bytes[k] / (int)sizeof(T);
     // Two pieces a thread at a time; the source past the caches (read once, unless it
     // goes to several pages, then the lines are there for a while all the same), the
-    // copy through them: the next step's attention reads it.  160 pages of 8 KB by 56
-    // tensors: 31.7 us -> 26.9 (5.5 TB/s read and written).
+    // copy through them: the next step's attention reads it.  (One piece, through the
+    // caches: 160 pages of 8 KB by 56 tensors take 5 us more.)
     for (int e = threadIdx.x; e < n; e += 2 * COPY_THREADS) {
         const int e2 = e + COPY_THREADS;
         const T v = stream_load(src + e), v2 = stream_load(src + (e2 < n ? e2 : e));

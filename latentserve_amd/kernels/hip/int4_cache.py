@@ -225,7 +225,8 @@ def paged_decode_int4(q: torch.Tensor, pools, block_tables: torch.Tensor, seq_le
     the launch, a longer one is attended whole.  Sequences of no tokens give
     zeros, and blocks outside the pool are skipped.  out may not overlap q.  Each
     call has its own scratch, so calls may run at once on several streams and from
-    several graphs."""
+    several graphs.  Sums are fp32, of weights of 21 bits and more; their order may differ
+    from call to call, and the result by a rounding."""
     _, h, args = _pools(pools)
     shape, dev, index = q.shape, q.device, q.get_device()
     if len(shape) != 4 or shape[1] != h or shape[3] != HEAD_DIM \

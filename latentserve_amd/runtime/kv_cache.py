@@ -371,7 +371,8 @@ class _PagedBase:
         """Start the empty slot `index` on `blocks`, whole pages already
         written by another sequence with the same first num_tokens tokens
         (cache/paged_cache.py:199-217).  The slot takes a reference to each;
-        pages are append-only, so a shared page is never written again."""
+        a step that would write a page that others hold too (a rewound or forked
+        sequence's) gives its sequence a copy first (_make_room())."""
         t = self.tables[index]
         if t.length or t.blocks:
             raise ValueError(f"slot {index} already holds a sequence")

@@ -228,6 +228,22 @@ __device__ __forceinline__ _Float16 rope_h(_Float16 x, _Float16 c, _Float16 y, _
 // on the same decode; these loads +0.65 us (49.5 -> 50.2 us), over the
 // plain loads an earlier form used, which were right only while the
 // reader's L2 held no copy of the partials' lines.
+
+// Device-coherent stores: sixteen bytes with the write-through policy (sc1) that the
+// compiler gives a relaxed agent-scope store, one vector store a lane, so a wave
+// writes whole lines instead of four partial passes over them.
+__device__ __forceinline__ void store_coherent4(float* p, f4 v) {
+    asm volatile("global_store_dwordx4 %0, %1, off sc1" : : "v"(p), "v"(v) : "memory");
+}
+
+// Eight bytes the same way.
+__device__ __forceinline__ void store_coherent2(float* p, float x, float y) {
+    u2 v;
+    v.x = __builtin_bit_cast(uint32_t, x);
+    v.y = __builtin_bit_cast(uint32_t, y);
+    asm volatile("global_store_dwordx2 %0, %1, off sc1" : : "v"(p), "v"(v) : "memory");
+}
+
 // Device-coherent loads (sc1: served from memory or a coherent copy, never
 // from a stale line in this XCD's L2), as relaxed agent-scope atomic loads.
 template <class T>

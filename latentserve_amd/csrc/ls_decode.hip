@@ -360,25 +360,6 @@ __device__ __forceinline__ void compute_page(const PageBuf& buf, WaveState& st, 
 // and splits 16-byte aligned), VEC 1 as four scalar loads.
 constexpr int CMB_CHUNK = 16;
 
-__device__ __forceinline__ void store_coherent(float* p, float v) {
-    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
-// Sixteen bytes with the same write-through policy (sc1) the compiler gives
-// the relaxed agent-scope store above: one vector store a lane, so a wave
-// writes whole lines instead of four partial passes over them.
-__device__ __forceinline__ void store_coherent4(float* p, f4 v) {
-    asm volatile("global_store_dwordx4 %0, %1, off sc1" : : "v"(p), "v"(v) : "memory");
-}
-
-// Eight bytes the same way.
-__device__ __forceinline__ void store_coherent2(float* p, float x, float y) {
-    u2 v;
-    v.x = __builtin_bit_cast(uint32_t, x);
-    v.y = __builtin_bit_cast(uint32_t, y);
-    asm volatile("global_store_dwordx2 %0, %1, off sc1" : : "v"(p), "v"(v) : "memory");
-}
-
 // The standalone split merge (ls_combine_splits): VEC 4, 16-byte loads; 1,
 // scalar loads.
 template <int VEC>

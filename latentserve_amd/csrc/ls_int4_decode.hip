@@ -255,16 +255,6 @@ __device__ __forceinline__ float add_paired(float v) {
     return r;
 }
 
-__device__ __forceinline__ void store_coherent(float* p, f4 v) {
-    asm volatile("global_store_dwordx4 %0, %1, off sc1" : : "v"(p), "v"(v) : "memory");
-}
-__device__ __forceinline__ void store_coherent(float* p, float x, float y) {
-    u2 v;
-    v.x = __builtin_bit_cast(uint32_t, x);
-    v.y = __builtin_bit_cast(uint32_t, y);
-    asm volatile("global_store_dwordx2 %0, %1, off sc1" : : "v"(p), "v"(v) : "memory");
-}
-
 // The records of a sequence of a KV head: its first group's among those of sequences
 // that start in their group, the others' among those that go on.
 struct Int4Records {
@@ -321,8 +311,8 @@ __device__ __forceinline__ void merge_records(const Int4Records& R, int k0, int 
             for (int e = 0; e < 4; ++e) o[e] = (half_t)(acc[e] * inv);
         } else {
             float* rk = (float*)((char*)R.work + R.at(k0));
-            store_coherent(rk + r * HEAD_DIM + d0, acc);
-            if (j == 0) store_coherent(rk + NR * HEAD_DIM + 2 * r, mg, lt);
+            store_coherent4(rk + r * HEAD_DIM + d0, acc);
+            if (j == 0) store_coherent2(rk + NR * HEAD_DIM + 2 * r, mg, lt);
         }
     }
 }
@@ -622,8 +612,8 @@ void int4_decode_kernel(const Int4DecodeParams a) {
                 for (int e = 0; e < 4; ++e)
                     orow[(int64_t)r * a.so_r + d0 + e] = (half_t)(acc[e] * inv);
             } else {
-                store_coherent(record + r * HEAD_DIM + d0, acc);
-                if (d0 == 0) store_coherent(record + NR * HEAD_DIM + 2 * r, mg, lt);
+                store_coherent4(record + r * HEAD_DIM + d0, acc);
+                if (d0 == 0) store_coherent2(record + NR * HEAD_DIM + 2 * r, mg, lt);
             }
         }
         if (!whole) {

@@ -120,16 +120,9 @@ def counters_of(graph: torch.cuda.CUDAGraph):
             ...
     """
     index = torch.cuda.current_device()
-    if _returned:
-        # (a graph may be dropped while its last replay runs)
-        gone = [_returned.popleft() for _ in range(len(_returned))]
-        for i in {i for i, _ in gone}:
-            torch.cuda.synchronize(i)
-        with _lock:
-            for i, slices in gone:
-                for cnt in slices:
-                    _free.setdefault((i, cnt.numel()), []).append(cnt)
-    _room(torch.device("cuda", index))
+    if not _capturing():                                     # (entered inside it: later captures)
+        _recycle()
+        _room(torch.device("cuda", index))
     outer, _owner.slices = getattr(_owner, "slices", None), []
     try:
         yield
@@ -138,6 +131,22 @@ def counters_of(graph: torch.cuda.CUDAGraph):
         if slices:
             # (a finalizer may run anywhere, under the lock too: it takes none)
             weakref.finalize(graph, _returned.append, (index, slices)).atexit = False
+
+
+def _recycle() -> None:
+    """The slices of graphs that are gone become free ones."""
+    gone = []
+    while True:
+        try:
+            gone.append(_returned.popleft())
+        except IndexError:
+            break
+    for i in {i for i, _ in gone}:
+        torch.cuda.synchronize(i)            # (a graph may be dropped while its last replay runs)
+    with _lock:
+        for i, slices in gone:
+            for cnt in slices:
+                _free.setdefault((i, cnt.numel()), []).append(cnt)
 
 
 def _captured_scratch(device: torch.device, nbytes: int, ints: int):

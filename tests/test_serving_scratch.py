@@ -23,6 +23,7 @@ def slabs(monkeypatch):
     _serving._returned.clear()
     synced = []
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(_serving, "_capturing", lambda: False)
     monkeypatch.setattr(torch.cuda, "synchronize", synced.append)
 
     def room(device):
@@ -125,3 +126,21 @@ def test_no_slice_left(slabs):
     g = Graph()
     got = capture(g, [2048, 2048, 32])
     assert got[0] is not None and got[1] is not None and got[2] is None
+
+
+def test_entered_inside_a_capture(slabs, monkeypatch):
+    """Nothing that a capture forbids (a synchronisation, a new slab); the slices are listed
+    all the same."""
+    _serving._room(Dev)
+    gone = Graph()
+    a = capture(gone, [32])
+    del gone
+    gc.collect()
+    monkeypatch.setattr(_serving, "_capturing", lambda: True)
+    monkeypatch.setattr(_serving, "_room", lambda device: pytest.fail("a slab in a capture"))
+    g = Graph()
+    b = capture(g, [32])
+    assert not slabs and apart(a + b)
+    del g
+    gc.collect()
+    assert len(_serving._returned) == 2

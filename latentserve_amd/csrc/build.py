@@ -24,7 +24,8 @@ LIB = os.path.join(PKG, "liblatentserve_hip.so")
 SOURCES = ["ls_abi.hip", "ls_decode.hip", "ls_sparse_index.hip", "ls_int8_write.hip",
            "ls_gather.hip", "ls_elementwise.hip", "ls_gemm.hip", "ls_gemm_plain.hip",
            "ls_gemm_glu.hip", "ls_gemm_rope.hip", "ls_serving_abi.hip", "ls_int4_write.hip",
-           "ls_int4_decode.hip", "ls_page_copy.hip", "ls_logprobs.hip"]
+           "ls_int4_decode.hip", "ls_page_copy.hip", "ls_logprobs.hip", "ls_tree_abi.hip",
+           "ls_tree_attention.hip", "ls_tree_weights.hip", "ls_tree_move.hip"]
 ARCH = os.environ.get("LS_OFFLOAD_ARCH", "gfx950")
 
 # Packed-fp32 VALU forms are disabled for every device pass; fp32 division

@@ -34,10 +34,11 @@ __device__ __forceinline__ f16v mfma3216(u4 a, u4 b, f16v c) {
                                                   __builtin_bit_cast(h8, b), c, 0, 0, 0);
 }
 
-__device__ __forceinline__ void load_to_lds(const char* src, char* dst) {
-    __builtin_amdgcn_global_load_lds(
-        (const void __attribute__((address_space(1)))*)src,
-        (void __attribute__((address_space(3)))*)dst, 16, 0, 0);
+// (buffer loads: after a global load to LDS the compiler waits for all LDS reads where it
+// needs one)
+typedef void __attribute__((address_space(3)))* lds_ptr;
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, uint32_t off, int soff, char* dst) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)dst, 16, off, soff, 0, 0);
 }
 
 __device__ __forceinline__ u2 read_transposed(const char* p) {
@@ -45,19 +46,29 @@ __device__ __forceinline__ u2 read_transposed(const char* p) {
         u2, __builtin_amdgcn_ds_read_tr16_b64_v4f16((g4 __attribute__((address_space(3)))*)p));
 }
 
-// Where a lane reads a tile's K and V, in bytes (every other offset is a constant).
+// Where a lane reads a tile's K and V, and what it loads of it, in bytes.  A tile starts
+// on 1 KB and a row is 256 bytes, so a swizzled place inside a row is one exclusive or:
+//   K of step j:         k ^ (32 j)        (piece 2 j + half of key lane % 32)
+//   V of channels 32 c:  v ^ (64 c)        (see values_of)
+//   loads i of a page:   (4 i + lane / 16) rows, pieces k_in ^ (64 i), v_in ^ (128 (i % 2))
 struct LanePlaces {
-    int k[8], v[4];
+    uint32_t k, v, k_in, v_in;
 };
 __device__ __forceinline__ LanePlaces lane_places(int lane) {
     LanePlaces p;
-    const int key = lane & 31, half = lane >> 5;
-#pragma unroll
-    for (int s = 0; s < 8; ++s) p.k[s] = key * 256 + 16 * ((2 * s + half) ^ (key & 15));
-    const int quarter = lane >> 4, r = 4 * (quarter >> 1) + ((lane & 15) >> 2);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) p.v[c] = r * 256 + 32 * ((2 * c + (quarter & 1)) ^ r) + 8 * (lane & 3);
+    const int key = lane & 31, half = lane >> 5, quarter = lane >> 4, pp = lane & 15;
+    const int r = 4 * (quarter >> 1) + ((lane & 15) >> 2);
+    p.k = key * 256 + 16 * (half ^ (key & 15));
+    p.v = r * 256 + 32 * ((quarter & 1) ^ r) + 8 * (lane & 3);
+    p.k_in = 16 * (pp ^ quarter);
+    p.v_in = 32 * ((pp >> 1) ^ quarter) + 16 * (pp & 1);
     return p;
+}
+// The same value, made anew where it is used: what follows from it is computed there, not
+// kept in registers through the loop.
+__device__ __forceinline__ uint32_t here(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
 }
 
 struct RowState {
@@ -103,6 +114,18 @@ __device__ __forceinline__ uint32_t seen_bits(const TreeParams& a, const uint64_
     return rel0 < 0 ? (t << (int)(-rel0)) | ctx : t;
 }
 
+// What the scheduler is to keep: `first` LDS reads ahead, then one product and `per`
+// reads in turn (left to itself it reads an operand and waits for it, product by product).
+template <int FIRST, int PER, int READS, int PRODUCTS>
+__device__ __forceinline__ void reads_ahead() {
+    __builtin_amdgcn_sched_group_barrier(0x100, FIRST, 0);
+#pragma unroll
+    for (int i = 0; i < PRODUCTS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        if (FIRST + i * PER < READS) __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+    }
+}
+
 // Scores of a tile of 32 KB keys for the wave's 32 rows.
 template <int KB>
 __device__ __forceinline__ void scores_of(const char* kt, const LanePlaces& at, const u4 (&q)[8],
@@ -111,76 +134,105 @@ __device__ __forceinline__ void scores_of(const char* kt, const LanePlaces& at, 
     for (int z = 0; z < KB; ++z)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[z][i] = 0.f;
+    u4 k[8][KB];
+    const uint32_t lane_k = here(at.k);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int z = 0; z < KB; ++z)
-            s[z] = mfma3216(*(const u4*)(kt + at.k[j] + z * 8192), q[j], s[z]);
+        for (int z = 0; z < KB; ++z) k[j][z] = *(const u4*)(kt + (lane_k ^ (32 * j)) + z * 8192);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int z = 0; z < KB; ++z) s[z] = mfma3216(k[j][z], q[j], s[z]);
+    reads_ahead<4, 1, 8 * KB, 8 * KB>();
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 template <int KB>
 __device__ __forceinline__ void mask_scores(f16v (&s)[KB], const uint32_t (&bits)[KB], int half) {
+    const uint32_t shift = here(4 * half);
 #pragma unroll
     for (int z = 0; z < KB; ++z) {
-        const uint32_t b = bits[z] >> (4 * half);
+        const uint32_t b = bits[z] >> shift;
 #pragma unroll
         for (int i = 0; i < 16; ++i)
             s[z][i] = (b >> (8 * (i / 4) + i % 4)) & 1 ? s[z][i] : neg_inf();
     }
 }
 
-// Softmax weights of the tile as fp16 pairs, the state's maximum and sum brought up to date.
+// The row's maximum with the tile's scores, in log2 units.
 template <int KB>
-__device__ __forceinline__ void weights_of(const f16v (&s)[KB], RowState& st, float scale2,
-                                           u4 (&p)[2 * KB]) {
+__device__ __forceinline__ float top_of(const f16v (&s)[KB], const RowState& st, float scale2) {
     float top = neg_inf();
 #pragma unroll
     for (int z = 0; z < KB; ++z)
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[z][i]);
     const LanePair o = swap32(top);
-    const float m_new = fmaxf(st.m, fmaxf(o.a, o.b) * scale2);
-    // (wave-uniform; weights stay below 2^15 as long as nothing outgrows the maximum by more)
-    if (__any(m_new > st.m + TREE_LAZY)) {
-        const float alpha = fast_exp2(st.m - (m_new == neg_inf() ? 0.f : m_new));
-        st.l *= alpha;
+    return fmaxf(st.m, fmaxf(o.a, o.b) * scale2);
+}
+// Whether weights could pass 2^15: a score outgrew the maximum (the same in every lane).
+__device__ __forceinline__ bool outgrown(const RowState& st, float top) {
+    return __any(top > st.m + TREE_LAZY);
+}
+__device__ __forceinline__ void rescale(RowState& st, float top) {
+    const float alpha = fast_exp2(st.m - (top == neg_inf() ? 0.f : top));
+    st.l *= alpha;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) st.acc[c] *= alpha;
-        st.m = m_new;
-    }
+    for (int c = 0; c < 4; ++c) st.acc[c] *= alpha;
+    st.m = top;
+}
+
+// Softmax weights of the tile as fp16 pairs, and their sum.
+template <int KB>
+__device__ __forceinline__ void weights_of(const f16v (&s)[KB], RowState& st, float scale2,
+                                           u4 (&p)[2 * KB]) {
     const float off = TREE_TOP - (st.m == neg_inf() ? 0.f : st.m);
+    float l[4] = {0.f, 0.f, 0.f, 0.f};        // (four sums: shorter chains)
 #pragma unroll
     for (int z = 0; z < KB; ++z)
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
             const float w0 = fast_exp2(__builtin_fmaf(s[z][i], scale2, off));
             const float w1 = fast_exp2(__builtin_fmaf(s[z][i + 1], scale2, off));
-            st.l += w0 + w1;
+            l[i % 4] += w0;
+            l[i % 4 + 1] += w1;
             const h2 w = {(half_t)w0, (half_t)w1};
             p[2 * z + i / 8][i / 2 % 4] = __builtin_bit_cast(uint32_t, w);
         }
+    st.l += (l[0] + l[1]) + (l[2] + l[3]);
 }
 
 // V^T of 16 keys (step j of the tile) and 32 channels (c).
-__device__ __forceinline__ u4 values_of(const char* vt, const LanePlaces& at, int j, int c) {
-    const u2 a = read_transposed(vt + at.v[c] + j * 4096);
-    const u2 b = read_transposed(vt + at.v[c] + j * 4096 + 2048);
+__device__ __forceinline__ u4 values_of(const char* vt, uint32_t lane_v, int j, int c) {
+    const u2 a = read_transposed(vt + (lane_v ^ (64 * c)) + j * 4096);
+    const u2 b = read_transposed(vt + (lane_v ^ (64 * c)) + j * 4096 + 2048);
     return (u4){a.x, a.y, b.x, b.y};
 }
 
 template <int KB>
 __device__ __forceinline__ void add_values(const char* vt, const LanePlaces& at, RowState& st,
                                            const u4 (&p)[2 * KB]) {
+    u4 v[2 * KB][4];
+    const uint32_t lane_v = here(at.v);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int j = 0; j < 2 * KB; ++j)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) st.acc[c] = mfma3216(values_of(vt, at, j, c), p[j], st.acc[c]);
+        for (int c = 0; c < 4; ++c) v[j][c] = values_of(vt, lane_v, j, c);
+#pragma unroll
+    for (int j = 0; j < 2 * KB; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) st.acc[c] = mfma3216(v[j][c], p[j], st.acc[c]);
+    reads_ahead<10, 2, 16 * KB, 8 * KB>();
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 // Halves of a V operand's keys 16 j + 4 half + (0..3) and + 8 cleared where `keep` (bits of the
 // 32 keys) has a 0.
 __device__ __forceinline__ u4 keep_keys(u4 v, uint32_t keep, int j, int half) {
-    const uint32_t b = keep >> (16 * (j & 1) + 4 * half);
+    const uint32_t b = keep >> here(16 * (j & 1) + 4 * half);
     auto pair = [&](int i) {
         return ((b >> i) & 1 ? 0xFFFFu : 0u) | ((b >> (i + 1)) & 1 ? 0xFFFF0000u : 0u);
     };
@@ -190,50 +242,71 @@ __device__ __forceinline__ u4 keep_keys(u4 v, uint32_t keep, int j, int half) {
     v.w &= pair(10);
     return v;
 }
-__device__ __forceinline__ bool finite(uint32_t w) {
-    return (w & 0x7C00u) != 0x7C00u && (w & 0x7C000000u) != 0x7C000000u;
+// V rows of a 32-key block whose keys do not exist (not `live`) become zeros in LDS: what lies
+// there may be anything, and a weight of 0 removes no NaN.  (Waves that share the block all
+// write the same zeros.)
+__device__ __forceinline__ void clear_values(char* vt, uint32_t live, int lane_) {
+    const uint32_t lane = here(lane_);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (!((live >> (4 * i + (lane >> 4))) & 1)) *(u4*)(vt + i * 1024 + lane * 16) = (u4){0, 0, 0, 0};
 }
 
-// The same for a 32-key block that meets the tree or the end.  bits: what the lane's row sees
-// of it; live: the keys that exist (the same in every lane): other V rows count as zeros.
-// A key that exists may be hidden from a row and hold an infinity or a NaN, which a
-// weight of 0 does not remove: such a block's products are made a row at a time, of the
-// keys that the row sees.
-__device__ __forceinline__ void add_values_masked(const char* vt, const LanePlaces& at, RowState& st,
-                                                  const u4 (&p)[2], uint32_t bits, uint32_t live,
-                                                  int half) {
-    bool odd = false;
+// The largest magnitude of an operand's halves so far, as bits (an infinity or a NaN: 0x7C00 and
+// more).
+typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ us2 magnitude(us2 m, u4 v) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int i = 0; i < 4; ++i)
+        m = __builtin_elementwise_max(m, __builtin_bit_cast(us2, v[i] & 0x7FFF7FFFu));
+    return m;
+}
+
+// Whether V of a tile holds an infinity or a NaN.
+template <int KB>
+__device__ __forceinline__ bool odd_values(const char* vt, const LanePlaces& at) {
+    const uint32_t lane_v = here(at.v);
+    us2 m = {0, 0};
+#pragma unroll 1
+    for (int j = 0; j < 2 * KB; ++j) {
+        u4 v[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const u4 v = keep_keys(values_of(vt, at, j, c), live, j, half);
-            odd |= !(finite(v.x) && finite(v.y) && finite(v.z) && finite(v.w));
-        }
-    asm volatile("" ::: "memory");            // (read again below: not kept in registers)
-    if (!__any(odd)) {
+        for (int c = 0; c < 4; ++c) v[c] = values_of(vt + j * 4096, lane_v, 0, c);
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                st.acc[c] = mfma3216(keep_keys(values_of(vt, at, j, c), live, j, half), p[j], st.acc[c]);
-        return;
+        for (int c = 0; c < 4; ++c) m = magnitude(m, v[c]);
     }
-    const int row = __lane_id() & 31;
-    for (int x = 0; x < 32; ++x) {
-        const uint32_t seen = (uint32_t)__builtin_amdgcn_readlane((int)bits, x) & live;
+    return __any(m.x >= 0x7C00 || m.y >= 0x7C00);
+}
+
+// A tile whose V holds an infinity or a NaN, which some rows see and others do not: products a
+// row at a time, of the keys that the row sees.  bits: what the lane's row sees.
+template <int KB>
+__device__ __forceinline__ void add_values_by_row(const char* vt, const LanePlaces& at, RowState& st,
+                                                  const u4 (&p)[2 * KB], const uint32_t (&bits)[KB],
+                                                  int half) {
+    const int row = (int)here(__lane_id()) & 31;
+    // (loops that stay loops: this is rare, and registers are the common path's)
+#pragma unroll 1
+    for (int z = 0; z < KB; ++z) {
+        const u4 p0 = z ? p[2 * KB - 2] : p[0], p1 = z ? p[2 * KB - 1] : p[1];
+        const uint32_t b = z ? bits[KB - 1] : bits[0];
+#pragma unroll 1
+        for (int x = 0; x < 32; ++x) {
+            const uint32_t seen = (uint32_t)__builtin_amdgcn_readlane((int)b, x);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            f16v y;
+            for (int c = 0; c < 4; ++c) {
+                const uint32_t lane_v = here(at.v);
+                f16v y;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) y[i] = 0.f;
+                for (int i = 0; i < 16; ++i) y[i] = 0.f;
+                y = mfma3216(keep_keys(values_of(vt + z * 8192, lane_v, 0, c), seen, 0, half), p0, y);
+                y = mfma3216(keep_keys(values_of(vt + z * 8192, lane_v, 1, c), seen, 1, half), p1, y);
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-                y = mfma3216(keep_keys(values_of(vt, at, j, c), seen, j, half), p[j], y);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) st.acc[c][i] = row == x ? st.acc[c][i] + y[i] : st.acc[c][i];
+                for (int i = 0; i < 16; ++i) st.acc[c][i] += row == x ? y[i] : 0.f;
+                __builtin_amdgcn_sched_barrier(0);
+                asm volatile("" ::: "memory");        // (one quarter's registers at a time)
+            }
         }
-        asm volatile("" ::: "memory");
     }
 }
 
@@ -258,52 +331,131 @@ __device__ __forceinline__ int steps_of(const TreeParams& a, int len, int step_k
     return n > 0 ? (n - 1) / step_keys + 1 : 1;
 }
 
-// The total of all units' places, and (find) the unit that place u0 lies in.
-__device__ __forceinline__ int total_places(const TreeParams& a, int step_keys, int lane) {
-    int mine = 0;
-    for (int b = lane; b < a.B; b += WAVE)
-        mine += (steps_of(a, length_of(a, b), step_keys) + a.extra) * a.H;
-    // (each half's lanes, then the halves; whole numbers below 2^31)
-#pragma unroll
-    for (int d = 1; d < WAVE; d *= 2) mine += __shfl_xor(mine, d);
-    return __builtin_amdgcn_readfirstlane(mine);
+// Inclusive prefix sum over the wave's lanes, and its total (row shifts inside 16 lanes, whose
+// missing sources add 0, then the rows' totals).
+template <int CTRL>
+__device__ __forceinline__ int dpp_add(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, false);
 }
-__device__ __forceinline__ Unit find_unit(const TreeParams& a, int step_keys, int lane, int u0) {
-    Unit u = {0, 0, 0, 0, 1};
+__device__ __forceinline__ int scan(int x, int lane, int& total) {
+    x = dpp_add<0x118>(dpp_add<0x114>(dpp_add<0x112>(dpp_add<0x111>(x))));
+    const int r0 = __builtin_amdgcn_readlane(x, 15), r1 = __builtin_amdgcn_readlane(x, 31),
+              r2 = __builtin_amdgcn_readlane(x, 47), r3 = __builtin_amdgcn_readlane(x, 63);
+    total = r0 + r1 + r2 + r3;
+    const int row = lane >> 4;
+    return x + (row > 0 ? r0 : 0) + (row > 1 ? r1 : 0) + (row > 2 ? r2 : 0);
+}
+
+// Which steps of which units group g takes.
+//
+// Units no more than groups (one sequence a lane): a group has a part of one unit, so it
+// starts and joins once.  Parts are as long as the groups suffice for: the smallest length
+// `per` whose parts, ceil(steps / per) a unit, are no more than the groups; a unit's parts
+// are then made even.
+//
+// More units: all units' steps in a row, each unit's behind `extra` places that starting on
+// it counts as, cut into even runs; a group's run may end one unit and start others.
+struct Runs {
+    bool dealt;
+    int per;                              // of a run
+    int u0, u1;                           // the run (dealt: the unit's steps s0, s1)
+    int first, last;                      // dealt: the unit's groups
+};
+__device__ __forceinline__ Unit find_run(const TreeParams& a, int step_keys, int lane, int g, Runs& r) {
+    Unit u = {a.B, 0, 0, 0, 1};
+    const int units = a.B * a.H;
+    r.dealt = a.B <= WAVE && units <= a.groups;
+    if (r.dealt) {
+        const int len = lane < a.B ? length_of(a, lane) : 0;
+        const int steps = lane < a.B ? steps_of(a, len, step_keys) : 0;
+        int total;
+        scan(steps, lane, total);
+        total *= a.H;
+        // parts of length per: at most total / per + units
+        int lo = (total + a.groups - 1) / a.groups, hi = total;
+        if (a.groups > units) hi = (total + a.groups - units - 1) / (a.groups - units);
+        lo = __builtin_amdgcn_readfirstlane(lo < 1 ? 1 : lo);
+        hi = __builtin_amdgcn_readfirstlane(hi < lo ? lo : hi);
+        auto parts_of = [&](int per) {
+            // (an estimate by the reciprocal, put right)
+            int n = (int)((float)steps * __builtin_amdgcn_rcpf((float)per));
+            n += n * per < steps ? 1 : 0;
+            n += n * per < steps ? 1 : 0;
+            return n;
+        };
+        while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            int sum;
+            scan(parts_of(mid), lane, sum);
+            if (sum * a.H <= a.groups)
+                hi = mid;
+            else
+                lo = mid + 1;
+        }
+        const int n = parts_of(lo);
+        int all;
+        const int incl = scan(n * a.H, lane, all);
+        if (g >= all) return u;
+        const int src = __builtin_ctzll(__ballot(g < incl));
+        const int parts = __builtin_amdgcn_readlane(n, src);
+        const int at = g - __builtin_amdgcn_readlane(incl - n * a.H, src);
+        u.b = src;
+        u.len = __builtin_amdgcn_readlane(len, src);
+        u.steps = __builtin_amdgcn_readlane(steps, src);
+        u.h = __builtin_amdgcn_readfirstlane(at / parts);
+        const int part = at - u.h * parts;
+        const int even = __builtin_amdgcn_readfirstlane(u.steps / parts), more = u.steps - even * parts;
+        r.u0 = part * even + (part < more ? part : more);
+        r.u1 = r.u0 + even + (part < more ? 1 : 0);
+        r.first = g - part;
+        r.last = r.first + parts - 1;
+        return u;
+    }
+    // (two passes over the lengths: the total, then where the run starts)
+    int total = 0;
+    for (int b0 = 0; b0 < a.B; b0 += WAVE) {
+        const int b = b0 + lane;
+        int sum;
+        scan(b < a.B ? (steps_of(a, length_of(a, b), step_keys) + a.extra) * a.H : 0, lane, sum);
+        total += sum;
+    }
+    r.per = __builtin_amdgcn_readfirstlane((total + a.groups - 1) / a.groups);
+    const int64_t from = (int64_t)g * r.per;
+    if (from >= total) return u;
+    r.u0 = (int)from;
+    r.u1 = total - r.u0 < r.per ? total : r.u0 + r.per;
     int before = 0;
     for (int b0 = 0; b0 < a.B; b0 += WAVE) {
         const int b = b0 + lane;
         const int len = b < a.B ? length_of(a, b) : 0;
         const int n = b < a.B ? (steps_of(a, len, step_keys) + a.extra) * a.H : 0;
-        int incl = n;
-#pragma unroll
-        for (int d = 1; d < WAVE; d *= 2) {
-            const int o = __shfl_up(incl, d);
-            if (lane >= d) incl += o;
-        }
-        const uint64_t hit = __ballot(b < a.B && u0 < before + incl);
-        if (hit) {
-            const int src = __builtin_ctzll(hit);
+        int sum;
+        const int incl = scan(n, lane, sum);
+        if (r.u0 < before + sum) {
+            const int src = __builtin_ctzll(__ballot(r.u0 < before + incl));
             u.b = b0 + src;
             u.len = __builtin_amdgcn_readlane(len, src);
             u.steps = steps_of(a, u.len, step_keys);
             const int first = before + __builtin_amdgcn_readlane(incl - n, src);
-            u.h = __builtin_amdgcn_readfirstlane((u0 - first) / (u.steps + a.extra));
+            u.h = __builtin_amdgcn_readfirstlane((r.u0 - first) / (u.steps + a.extra));
             u.start = first + u.h * (u.steps + a.extra) + a.extra;
             return u;
         }
-        before += __builtin_amdgcn_readlane(incl, WAVE - 1);
+        before += sum;
     }
-    u.b = a.B;
     return u;
 }
-__device__ __forceinline__ void next_unit(const TreeParams& a, int step_keys, Unit& u) {
+// The next unit of a run (false: none).
+__device__ __forceinline__ bool next_unit(const TreeParams& a, int step_keys, const Runs& r, Unit& u) {
+    if (r.dealt) return false;
     u.start += u.steps + a.extra;
-    if (++u.h < a.H) return;
-    u.h = 0;
-    if (++u.b >= a.B) return;
-    u.len = length_of(a, u.b);
-    u.steps = steps_of(a, u.len, step_keys);
+    if (++u.h == a.H) {
+        u.h = 0;
+        if (++u.b >= a.B) return false;
+        u.len = length_of(a, u.b);
+        u.steps = steps_of(a, u.len, step_keys);
+    }
+    return u.start - a.extra < r.u1;
 }
 
 // WR row groups of 32 rows by 8 / WR key groups.
@@ -325,33 +477,37 @@ void tree_kernel(const TreeParams a) {
     const int v = xcd_major(blockIdx.x, gridDim.x);
     const int g = __builtin_amdgcn_readfirstlane(v / a.row_tiles), rt = v - g * a.row_tiles;
 
-    const int total = total_places(a, STEP, lane);
-    const int per = __builtin_amdgcn_readfirstlane((total + a.groups - 1) / a.groups);
-    const int64_t lo = (int64_t)g * per;
-    if (lo >= total) return;
-    const int u0 = (int)lo, u1 = total - u0 < per ? total : u0 + per;
+    Runs run;
+    Unit u = find_run(a, STEP, lane, g, run);
+    if (u.b >= a.B) return;                                // (every wave alike, before any barrier)
 
     const LanePlaces at = lane_places(lane);
     const int R = a.N * a.NR;
-    const int row = (rt * WR + rg) * 32 + (lane & 31);
-    const bool is_row = row < R;
-    const int node = is_row ? row / a.NR : 0, rep = is_row ? row - node * a.NR : 0;
+    // the lane's row, worked out where it is used (in registers it would cost the loop some)
+    struct Row {
+        int node, rep;
+        bool is;
+    };
+    auto row_of = [&] {
+        const int row = (rt * WR + rg) * 32 + (int)here(lane & 31);
+        Row o;
+        o.is = row < R;
+        o.node = o.is ? row / a.NR : 0;
+        o.rep = o.is ? row - o.node * a.NR : 0;
+        return o;
+    };
 
     // this wave's part of a tile's loads: LOADS instructions of four rows, K and V each
     constexpr int LOADS = KEYS / 4 / WR;
-    int src_k[LOADS], src_v[LOADS];                        // bytes inside a (page, head)
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-        const int r = (rg * LOADS + i) * 4 + (lane >> 4), pp = lane & 15;
-        src_k[i] = (int)((r & 15) * a.sp_t) + 16 * (pp ^ (r & 15));
-        src_v[i] = (int)((r & 15) * a.sp_t) + 32 * ((pp >> 1) ^ (r & 7)) + 16 * (pp & 1);
-    }
+    const uint32_t row_in = (uint32_t)(lane >> 4) * (uint32_t)a.sp_t;
 
-    Unit u = find_unit(a, STEP, lane, u0);
-    for (; u.b < a.B && u.start - a.extra < u1; next_unit(a, STEP, u)) {
-        const int s0 = u0 > u.start ? u0 - u.start : 0;
-        const int s1 = u1 - u.start < u.steps ? u1 - u.start : u.steps;
-        if (s0 >= s1) continue;                            // (only what starting counts as)
+    do {
+        int s0 = run.u0, s1 = run.u1;
+        if (!run.dealt) {
+            s0 = s0 > u.start ? s0 - u.start : 0;
+            s1 = s1 - u.start < u.steps ? s1 - u.start : u.steps;
+            if (s0 >= s1) continue;                        // (only what starting counts as)
+        }
         const int keys = keys_of(a, u.len);
         const int ctx = u.len > a.N ? u.len - a.N : 0;
         int nodes = a.N;
@@ -360,57 +516,46 @@ void tree_kernel(const TreeParams a) {
             nodes = n < nodes ? (n > 0 ? n : 0) : nodes;
         }
         nodes = nodes < u.len ? nodes : u.len;
-        const bool seeing = is_row && node < nodes;
-        const uint64_t* row_mask =
-            a.masks && is_row ? a.masks + ((int64_t)u.b * a.N + node) * a.words : nullptr;
         const int32_t* table = a.tables + u.b * a.st_b;
-        const int pages = (keys + PAGE - 1) / PAGE;
+        const int pages = (keys + PAGE - 1) / PAGE, last_page = pages > 0 ? pages - 1 : 0;
 
         u4 q[8];
-        {
-            const half_t* p = a.q + u.b * a.sq_b + node * a.sq_n + u.h * a.sq_h + rep * a.sq_r + 8 * half;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) q[j] = is_row ? *(const u4*)(p + 16 * j) : (u4){0, 0, 0, 0};
-        }
         RowState st;
-        clear(st);
 
-        // block of page `lane` of a step's tile, -1: none
+        // Blocks of a step's tile, a lane a page (past the sequence's last page, it again: keys
+        // there do not count).
         auto ids_of = [&](int step) {
-            const int64_t page = ((int64_t)step * WK + kg) * (KEYS / PAGE) + lane;
-            int id = -1;
-            if (lane < KEYS / PAGE && page < pages) {
-                id = table[page];
-                if ((unsigned)id >= (unsigned)a.num_blocks) id = -1;
-            }
-            return id;
+            int i = (int)here(lane);
+            i = (step * WK + kg) * (KEYS / PAGE) + (i < KEYS / PAGE ? i : KEYS / PAGE - 1);
+            return table[i < pages ? i : last_page];
         };
+        // its pages that are not in the pool
         auto bad_of = [&](int ids) {
-            return (uint32_t)__ballot(lane < KEYS / PAGE && ids < 0);
+            return (uint32_t)__ballot((unsigned)ids >= (unsigned)a.num_blocks) & ((1u << (KEYS / PAGE)) - 1);
         };
-        // a page outside the pool is read as zeros
+        // (a page outside the pool is not requested: what its rows hold then counts as nothing)
         auto load = [&](int z, int ids, char* t) {
             constexpr int SAME = LOADS < 4 ? LOADS : 4;    // instructions of one page
+            const uint32_t row = here(row_in), k_in = here(at.k_in), v_in = here(at.v_in);
 #pragma unroll
             for (int i0 = 0; i0 < LOADS; i0 += SAME) {
                 const int first = (rg * LOADS + i0) * 4;
                 const int id = __builtin_amdgcn_readlane(ids, first / PAGE);
-                if (id >= 0) {
-                    const char* from = a.pool[z] + id * a.sp_b + u.h * a.sp_h;
+                const bool in = (unsigned)id < (unsigned)a.num_blocks;
+                const __amdgpu_buffer_rsrc_t from =
+                    page_rsrc(a.pool[z] + (in ? id : 0) * a.sp_b + u.h * a.sp_h, in);
 #pragma unroll
-                    for (int i = i0; i < i0 + SAME; ++i)
-                        load_to_lds(from + (z ? src_v[i] : src_k[i]), t + (first + 4 * (i - i0)) * 256);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < SAME; ++i)
-                        *(u4*)(t + (first + 4 * i) * 256 + lane * 16) = (u4){0, 0, 0, 0};
+                for (int i = 0; i < SAME; ++i) {
+                    const int n = LOADS < 4 ? (rg * LOADS + i) & 3 : i;       // of the page's four
+                    const uint32_t off = z ? v_in ^ (128 * (n & 1)) : k_in ^ (64 * n);
+                    load_to_lds(from, row + off, 4 * n * (int)a.sp_t, t + (first + 4 * i) * 256);
                 }
             }
         };
         // a block's scores, in log2 units
         auto store_scores = [&](const f16v& s, int64_t k0) {
-            if (!is_row) return;
-            float* to = a.scores + ((int64_t)(u.b * a.H + u.h) * R + row) * a.score_len + k0 + 4 * half;
+            if ((lane & 31) >= R || k0 >= keys) return;
+            float* to = a.scores + ((int64_t)(u.b * a.H + u.h) * R + (lane & 31)) * a.score_len + k0 + 4 * half;
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
                 const f4 x = {s[4 * n] * a.scale2, s[4 * n + 1] * a.scale2, s[4 * n + 2] * a.scale2,
@@ -418,34 +563,45 @@ void tree_kernel(const TreeParams a) {
                 *(f4*)(to + 8 * n) = x;
             }
         };
-        // keys of the context only; bad: pages of the tile that are not there
-        auto mask_pages = [&](f16v (&s)[KB], uint32_t bad) {
-            uint32_t bits[KB];
+        // What the row sees of a step's tile (bits), and which of its keys exist (live, the same in
+        // every lane).  Steps of the context alone, with all their pages, need neither.
+        uint32_t bits[KB], live[KB];
+        auto look = [&](int step, uint32_t bad) {
+            const Row row = row_of();
+            const bool seeing = row.is && row.node < nodes;
+            const uint64_t* row_mask =
+                a.masks ? a.masks + ((int64_t)u.b * a.N + row.node) * a.words : nullptr;
 #pragma unroll
-            for (int z = 0; z < KB; ++z)
-                bits[z] = ((bad >> (2 * z)) & 1 ? 0u : 0xFFFFu) |
-                          ((bad >> (2 * z + 1)) & 1 ? 0u : 0xFFFF0000u);
-            mask_scores<KB>(s, bits, half);
-        };
-        // a tile that meets the tree or the end, a block at a time
-        auto compute_masked = [&](int step, uint32_t bad, const char* kt, const char* vt) {
             for (int z = 0; z < KB; ++z) {
                 const int64_t k0 = ((int64_t)step * WK + kg) * KEYS + 32 * z;
                 const int64_t left = (ctx + nodes < keys ? ctx + nodes : keys) - k0;
-                if (left <= 0) return;
-                uint32_t live = left >= 32 ? ~0u : (1u << (int)left) - 1;
-                if ((bad >> (2 * z)) & 1) live &= 0xFFFF0000u;
-                if ((bad >> (2 * z + 1)) & 1) live &= 0x0000FFFFu;
-                const uint32_t bits[1] = {
-                    seeing ? seen_bits(a, row_mask, node, k0 - ctx, nodes) & live : 0u};
-                f16v s[1];
-                u4 p[2];
-                scores_of<1>(kt + z * 8192, at, q, s);
-                mask_scores<1>(s, bits, half);
-                if constexpr (SCORES) store_scores(s[0], k0);
-                weights_of<1>(s, st, a.scale2, p);
-                add_values_masked(vt + z * 8192, at, st, p, bits[0], live, half);
+                uint32_t l = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << (int)left) - 1;
+                if ((bad >> (2 * z)) & 1) l &= 0xFFFF0000u;
+                if ((bad >> (2 * z + 1)) & 1) l &= 0x0000FFFFu;
+                live[z] = l;
+                bits[z] = seeing && l ? seen_bits(a, row_mask, row.node, k0 - ctx, nodes) & l : 0u;
             }
+        };
+        // A step that meets the tree or the end, that raises a maximum, or the first one.
+        auto other_step = [&](int step, bool masked, const char* kt, char* vt, auto&& between) {
+            f16v s[KB];
+            u4 p[2 * KB];
+            scores_of<KB>(kt, at, q, s);
+            if (masked) mask_scores<KB>(s, bits, half);
+            if constexpr (SCORES) store_scores(s[0], ((int64_t)step * WK + kg) * KEYS);
+            between();
+            const float top = top_of<KB>(s, st, a.scale2);
+            if (outgrown(st, top)) rescale(st, top);
+            weights_of<KB>(s, st, a.scale2, p);
+            if (masked) {
+#pragma unroll 1
+                for (int z = 0; z < KB; ++z) clear_values(vt + z * 8192, z ? live[KB - 1] : live[0], lane);
+                if (odd_values<KB>(vt, at)) {
+                    add_values_by_row<KB>(vt, at, st, p, bits, half);
+                    return;
+                }
+            }
+            add_values<KB>(vt, at, st, p);
         };
 
         char* const kt0 = k0_ + kg * TILE;
@@ -453,48 +609,73 @@ void tree_kernel(const TreeParams a) {
         // steps of the context alone, then the others
         const int sf = s1 < ctx / STEP ? s1 : (s0 > ctx / STEP ? s0 : ctx / STEP);
         int ids = ids_of(s0);
+        {
+            // (a lane past the last row takes the first one's: its results go nowhere)
+            const Row row = row_of();
+            const half_t* p = a.q + u.b * a.sq_b + row.node * a.sq_n + u.h * a.sq_h +
+                              row.rep * a.sq_r + 8 * half;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) q[j] = *(const u4*)(p + 16 * j);
+        }
+        clear(st);
+
+        uint32_t bad = bad_of(ids);
+        load(0, ids, kt0);
+        load(1, ids, vt0);
+        // Steps go round a loop of plain ones, in which a row's state is one set of registers (a
+        // branch in it that rescales, or adds otherwise, copies all of them every step); the
+        // others leave it.
         if constexpr (TWO) {
             char* const kt1 = k1_ + kg * TILE;
             char* const vt1 = v1_ + kg * TILE;
-            uint32_t bad = bad_of(ids);
-            load(0, ids, kt0);
-            load(1, ids, vt0);
-            ids = s0 + 1 < s1 ? ids_of(s0 + 1) : -1;
+            ids = s0 + 1 < s1 ? ids_of(s0 + 1) : 0;
+            bool masked;
             // a step's loads have come and everyone is done with the step before: the next
             // one's go out
             auto turn = [&](int step, char* kn, char* vn) {
+                masked = step >= sf || bad != 0;
+                if (masked) look(step, bad);               // (its loads come with the tile's)
                 wait_vm_lds<0>();
                 __syncthreads();
-                const uint32_t now = bad;
                 if (step + 1 < s1) {
                     bad = bad_of(ids);
                     load(0, ids, kn);
                     load(1, ids, vn);
                     if (step + 2 < s1) ids = ids_of(step + 2);
                 }
-                return now;
             };
-            auto compute = [&](uint32_t now, const char* kt, const char* vt) {
+            auto plain_step = [&](const char* kt, const char* vt) {
                 f16v s[KB];
                 u4 p[2 * KB];
                 scores_of<KB>(kt, at, q, s);
-                if (now) mask_pages(s, now);
+                if (outgrown(st, top_of<KB>(s, st, a.scale2))) return false;
                 weights_of<KB>(s, st, a.scale2, p);
                 add_values<KB>(vt, at, st, p);
+                return true;
             };
             int step = s0;
-            while (step < sf) {
-                uint32_t now = turn(step, kt1, vt1);
-                compute(now, kt0, vt0);
-                if (++step >= sf) break;
-                now = turn(step, kt0, vt0);
-                compute(now, kt1, vt1);
-                ++step;
-            }
-            for (; step < s1; ++step) {
-                const bool odd = (step - s0) & 1;
-                const uint32_t now = odd ? turn(step, kt0, vt0) : turn(step, kt1, vt1);
-                compute_masked(step, now, odd ? kt1 : kt0, odd ? vt1 : vt0);
+            bool second = false;                           // which buffers hold the step
+            turn(step, kt1, vt1);
+            while (true) {
+                other_step(step, masked, second ? kt1 : kt0, second ? vt1 : vt0, [] {});
+                if (++step >= s1) break;
+                second = !second;
+                if (second) {
+                    turn(step, kt0, vt0);
+                    if (masked || !plain_step(kt1, vt1)) continue;
+                    if (++step >= s1) break;
+                }
+                while (true) {
+                    second = false;
+                    turn(step, kt1, vt1);
+                    if (masked || !plain_step(kt0, vt0)) break;
+                    if (++step >= s1) break;
+                    second = true;
+                    turn(step, kt0, vt0);
+                    if (masked || !plain_step(kt1, vt1)) break;
+                    if (++step >= s1) break;
+                }
+                if (step >= s1) break;
             }
         } else {
             // one buffer of a wave's own, K and V in turn: each is requested again as soon as
@@ -503,40 +684,53 @@ void tree_kernel(const TreeParams a) {
                 __builtin_amdgcn_s_waitcnt(0xC07F);        // lgkmcnt 0
                 asm volatile("" ::: "memory");
             };
-            uint32_t bad = bad_of(ids);
-            load(0, ids, kt0);
-            load(1, ids, vt0);
             int step = s0;
-            for (; step < sf; ++step) {
-                const bool more = step + 1 < s1;
-                int next = -1;
-                if (more) next = ids_of(step + 1);
+            bool more = step + 1 < s1;
+            if (more) ids = ids_of(step + 1);
+            wait_vm_lds<0>();
+            while (true) {
+                // (loads of the step have come; `ids`: the next one's blocks)
+                const bool masked = step >= sf || bad != 0;
+                if (masked) look(step, bad);
+                other_step(step, masked, kt0, vt0, [&] {
+                    reads_done();
+                    if (more) load(0, ids, kt0);
+                });
+                reads_done();
+                if (!more) break;
+                load(1, ids, vt0);
+                bad = bad_of(ids);
+                ++step;
+                more = step + 1 < s1;
+                if (more) ids = ids_of(step + 1);
                 wait_vm_lds<0>();
-                f16v s[KB];
-                u4 p[2 * KB];
-                scores_of<KB>(kt0, at, q, s);
-                if (bad) mask_pages(s, bad);
-                reads_done();
-                if (more) load(0, next, kt0);
-                weights_of<KB>(s, st, a.scale2, p);
-                add_values<KB>(vt0, at, st, p);
-                reads_done();
-                if (more) load(1, next, vt0);
-                if constexpr (SCORES) store_scores(s[0], ((int64_t)step * WK + kg) * KEYS);
-                ids = next;
-                bad = bad_of(next);
-            }
-            for (; step < s1; ++step) {
-                wait_vm_lds<0>();
-                reads_done();
-                compute_masked(step, bad, kt0, vt0);
-                reads_done();
-                if (step + 1 < s1) {
-                    ids = ids_of(step + 1);
-                    bad = bad_of(ids);
-                    load(0, ids, kt0);
+                bool plain = true;
+                while (plain && step < sf && bad == 0) {
+                    f16v s[KB];
+                    u4 p[2 * KB];
+                    scores_of<KB>(kt0, at, q, s);
+                    if (outgrown(st, top_of<KB>(s, st, a.scale2))) {
+                        plain = false;
+                        break;
+                    }
+                    reads_done();
+                    if (more) load(0, ids, kt0);
+                    if constexpr (SCORES) store_scores(s[0], ((int64_t)step * WK + kg) * KEYS);
+                    weights_of<KB>(s, st, a.scale2, p);
+                    add_values<KB>(vt0, at, st, p);
+                    reads_done();
+                    if (!more) {
+                        ++step;
+                        break;
+                    }
                     load(1, ids, vt0);
+                    bad = bad_of(ids);
+                    ++step;
+                    more = step + 1 < s1;
+                    if (more) ids = ids_of(step + 1);
+                    wait_vm_lds<0>();
                 }
+                if (step >= s1) break;
             }
         }
 
@@ -555,11 +749,12 @@ void tree_kernel(const TreeParams a) {
             };
             __syncthreads();
             char* mine = place(wave);
+            const uint32_t lane16 = here(lane * 16);
 #pragma unroll
             for (int n = 0; n < 16; ++n) {
                 const f4 x = {st.acc[n / 4][4 * (n % 4)], st.acc[n / 4][4 * (n % 4) + 1],
                               st.acc[n / 4][4 * (n % 4) + 2], st.acc[n / 4][4 * (n % 4) + 3]};
-                *(f4*)(mine + n * 1024 + lane * 16) = x;
+                *(f4*)(mine + n * 1024 + lane16) = x;
             }
             if (half == 0) ml_[wave][lane] = make_float2(m, l);
             __syncthreads();
@@ -577,7 +772,7 @@ void tree_kernel(const TreeParams a) {
                 const char* from = place(k * WR + rg);
 #pragma unroll
                 for (int n = 0; n < QUADS; ++n)
-                    y[n] += *(const f4*)(from + (kg * QUADS + n) * 1024 + lane * 16) * w;
+                    y[n] += *(const f4*)(from + (kg * QUADS + n) * 1024 + lane16) * w;
             }
             m = top;
             l = sum;
@@ -589,10 +784,12 @@ void tree_kernel(const TreeParams a) {
                             st.acc[n / 4][4 * (n % 4) + 2], st.acc[n / 4][4 * (n % 4) + 3]};
             __syncthreads();
         }
+        const Row row = row_of();
         if (whole) {
+            const bool seeing = row.is && row.node < nodes;
             const float inv = seeing && l != 0.f ? 1.f / l : 0.f;
-            if (is_row) {
-                half_t* o = a.out + u.b * a.so_b + node * a.so_n + u.h * a.so_h + rep * a.so_r;
+            if (row.is) {
+                half_t* o = a.out + u.b * a.so_b + row.node * a.so_n + u.h * a.so_h + row.rep * a.so_r;
 #pragma unroll
                 for (int n = 0; n < QUADS; ++n) {
                     const int quad = kg * QUADS + n;
@@ -602,7 +799,7 @@ void tree_kernel(const TreeParams a) {
                     *(h4*)(o + 8 * quad + 4 * half) = x;
                 }
                 if (a.lse && kg == 0 && half == 0)
-                    a.lse[((int64_t)(u.b * a.N + node) * a.H + u.h) * a.NR + rep] =
+                    a.lse[((int64_t)(u.b * a.N + row.node) * a.H + u.h) * a.NR + row.rep] =
                         seeing && m != neg_inf()
                             ? (m - TREE_TOP + __builtin_amdgcn_logf(l)) * 0.69314718055994531f
                             : neg_inf();
@@ -614,8 +811,10 @@ void tree_kernel(const TreeParams a) {
             if (kg == 0 && half == 0) *(float2*)(rec + 4096 + 2 * lane) = make_float2(m, l);
         }
         if (s0 == 0 && rt == 0 && threadIdx.x == 0)
-            a.info[u.b * a.H + u.h] = make_int2(u.start / per, (u.start + u.steps - 1) / per);
-    }
+            a.info[u.b * a.H + u.h] =
+                run.dealt ? make_int2(run.first, run.last)
+                          : make_int2(u.start / run.per, (u.start + u.steps - 1) / run.per);
+    } while (next_unit(a, STEP, run, u));
 }
 
 // Records of a unit made its output: a workgroup a (unit, 32 rows, CQ channel quads), its

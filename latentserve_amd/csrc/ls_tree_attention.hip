@@ -76,6 +76,12 @@ struct RowState {
     float m, l;                           // running maximum (log2 units), this half's sum
 };
 
+// Keeps the sums in one set of registers where branches join (the compiler otherwise takes them
+// apart there and copies all 64, in every step).
+__device__ __forceinline__ void pin(RowState& st) {
+    asm volatile("" : "+v"(st.acc[0]), "+v"(st.acc[1]), "+v"(st.acc[2]), "+v"(st.acc[3]));
+}
+
 __device__ __forceinline__ void clear(RowState& st) {
 #pragma unroll
     for (int c = 0; c < 4; ++c)
@@ -182,6 +188,7 @@ __device__ __forceinline__ void rescale(RowState& st, float top) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) st.acc[c] *= alpha;
     st.m = top;
+    pin(st);
 }
 
 // Softmax weights of the tile as fp16 pairs, and their sum.
@@ -582,26 +589,39 @@ void tree_kernel(const TreeParams a) {
                 bits[z] = seeing && l ? seen_bits(a, row_mask, row.node, k0 - ctx, nodes) & l : 0u;
             }
         };
-        // A step that meets the tree or the end, that raises a maximum, or the first one.
-        auto other_step = [&](int step, bool masked, const char* kt, char* vt, auto&& between) {
+        // A step's products; false, with nothing done, where V holds an infinity or a NaN that a row
+        // may not see.  (between: what is done once K has been read)
+        auto add_step = [&](int step, bool masked, const char* kt, char* vt, auto&& between) {
             f16v s[KB];
             u4 p[2 * KB];
             scores_of<KB>(kt, at, q, s);
-            if (masked) mask_scores<KB>(s, bits, half);
-            if constexpr (SCORES) store_scores(s[0], ((int64_t)step * WK + kg) * KEYS);
-            between();
-            const float top = top_of<KB>(s, st, a.scale2);
-            if (outgrown(st, top)) rescale(st, top);
-            weights_of<KB>(s, st, a.scale2, p);
             if (masked) {
+                mask_scores<KB>(s, bits, half);
 #pragma unroll 1
                 for (int z = 0; z < KB; ++z) clear_values(vt + z * 8192, z ? live[KB - 1] : live[0], lane);
-                if (odd_values<KB>(vt, at)) {
-                    add_values_by_row<KB>(vt, at, st, p, bits, half);
-                    return;
-                }
+                if (odd_values<KB>(vt, at)) return false;
             }
+            between();
+            if constexpr (SCORES) store_scores(s[0], ((int64_t)step * WK + kg) * KEYS);
+            const float top = top_of<KB>(s, st, a.scale2);
+            if (outgrown(st, top)) rescale(st, top);
+            pin(st);
+            weights_of<KB>(s, st, a.scale2, p);
             add_values<KB>(vt, at, st, p);
+            return true;
+        };
+        auto add_step_by_row = [&](int step, const char* kt, const char* vt, auto&& between) {
+            f16v s[KB];
+            u4 p[2 * KB];
+            scores_of<KB>(kt, at, q, s);
+            between();
+            mask_scores<KB>(s, bits, half);
+            if constexpr (SCORES) store_scores(s[0], ((int64_t)step * WK + kg) * KEYS);
+            const float top = top_of<KB>(s, st, a.scale2);
+            if (outgrown(st, top)) rescale(st, top);
+            pin(st);
+            weights_of<KB>(s, st, a.scale2, p);
+            add_values_by_row<KB>(vt, at, st, p, bits, half);
         };
 
         char* const kt0 = k0_ + kg * TILE;
@@ -622,9 +642,8 @@ void tree_kernel(const TreeParams a) {
         uint32_t bad = bad_of(ids);
         load(0, ids, kt0);
         load(1, ids, vt0);
-        // Steps go round a loop of plain ones, in which a row's state is one set of registers (a
-        // branch in it that rescales, or adds otherwise, copies all of them every step); the
-        // others leave it.
+        // (A step of infinities leaves the loop for its products by row and comes back: as a branch
+        // inside it, it would cost every step copies of the sums.)
         if constexpr (TWO) {
             char* const kt1 = k1_ + kg * TILE;
             char* const vt1 = v1_ + kg * TILE;
@@ -644,38 +663,25 @@ void tree_kernel(const TreeParams a) {
                     if (step + 2 < s1) ids = ids_of(step + 2);
                 }
             };
-            auto plain_step = [&](const char* kt, const char* vt) {
-                f16v s[KB];
-                u4 p[2 * KB];
-                scores_of<KB>(kt, at, q, s);
-                if (outgrown(st, top_of<KB>(s, st, a.scale2))) return false;
-                weights_of<KB>(s, st, a.scale2, p);
-                add_values<KB>(vt, at, st, p);
-                return true;
-            };
             int step = s0;
             bool second = false;                           // which buffers hold the step
-            turn(step, kt1, vt1);
             while (true) {
-                other_step(step, masked, second ? kt1 : kt0, second ? vt1 : vt0, [] {});
-                if (++step >= s1) break;
-                second = !second;
-                if (second) {
-                    turn(step, kt0, vt0);
-                    if (masked || !plain_step(kt1, vt1)) continue;
-                    if (++step >= s1) break;
-                }
                 while (true) {
-                    second = false;
-                    turn(step, kt1, vt1);
-                    if (masked || !plain_step(kt0, vt0)) break;
-                    if (++step >= s1) break;
-                    second = true;
+                    if (!second) {
+                        turn(step, kt1, vt1);
+                        if (!add_step(step, masked, kt0, vt0, [] {})) break;
+                        second = true;
+                        if (++step >= s1) break;
+                    }
                     turn(step, kt0, vt0);
-                    if (masked || !plain_step(kt1, vt1)) break;
+                    if (!add_step(step, masked, kt1, vt1, [] {})) break;
+                    second = false;
                     if (++step >= s1) break;
                 }
                 if (step >= s1) break;
+                add_step_by_row(step, second ? kt1 : kt0, second ? vt1 : vt0, [] {});
+                second = !second;
+                if (++step >= s1) break;
             }
         } else {
             // one buffer of a wave's own, K and V in turn: each is requested again as soon as
@@ -685,52 +691,34 @@ void tree_kernel(const TreeParams a) {
                 asm volatile("" ::: "memory");
             };
             int step = s0;
-            bool more = step + 1 < s1;
-            if (more) ids = ids_of(step + 1);
-            wait_vm_lds<0>();
-            while (true) {
-                // (loads of the step have come; `ids`: the next one's blocks)
-                const bool masked = step >= sf || bad != 0;
-                if (masked) look(step, bad);
-                other_step(step, masked, kt0, vt0, [&] {
-                    reads_done();
-                    if (more) load(0, ids, kt0);
-                });
-                reads_done();
-                if (!more) break;
-                load(1, ids, vt0);
-                bad = bad_of(ids);
-                ++step;
+            bool more, masked;
+            auto turn = [&] {
                 more = step + 1 < s1;
+                masked = step >= sf || bad != 0;
+                if (masked) look(step, bad);
                 if (more) ids = ids_of(step + 1);
                 wait_vm_lds<0>();
-                bool plain = true;
-                while (plain && step < sf && bad == 0) {
-                    f16v s[KB];
-                    u4 p[2 * KB];
-                    scores_of<KB>(kt0, at, q, s);
-                    if (outgrown(st, top_of<KB>(s, st, a.scale2))) {
-                        plain = false;
-                        break;
-                    }
-                    reads_done();
-                    if (more) load(0, ids, kt0);
-                    if constexpr (SCORES) store_scores(s[0], ((int64_t)step * WK + kg) * KEYS);
-                    weights_of<KB>(s, st, a.scale2, p);
-                    add_values<KB>(vt0, at, st, p);
-                    reads_done();
-                    if (!more) {
-                        ++step;
-                        break;
-                    }
-                    load(1, ids, vt0);
-                    bad = bad_of(ids);
-                    ++step;
-                    more = step + 1 < s1;
-                    if (more) ids = ids_of(step + 1);
-                    wait_vm_lds<0>();
+            };
+            auto next_k = [&] {
+                reads_done();
+                if (more) load(0, ids, kt0);
+            };
+            auto next_v = [&] {
+                reads_done();
+                if (more) load(1, ids, vt0);
+                bad = bad_of(ids);
+            };
+            while (true) {
+                while (true) {
+                    turn();
+                    if (!add_step(step, masked, kt0, vt0, next_k)) break;
+                    next_v();
+                    if (++step >= s1) break;
                 }
                 if (step >= s1) break;
+                add_step_by_row(step, kt0, vt0, next_k);
+                next_v();
+                if (++step >= s1) break;
             }
         }
 

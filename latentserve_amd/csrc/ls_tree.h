@@ -9,13 +9,11 @@ namespace ls {
 
 // ---- attention of several new tokens over the fp16 pools --------------------------
 constexpr int TREE_MAX_NODES = 256;
-constexpr int TREE_NW = 8;                // waves a workgroup
-constexpr int TREE_BLOCK = 32;            // rows, and keys, of a product
 
-// How a launch is cut: a workgroup's eight waves are WR row groups of 32 rows by
-// 8 / WR key groups, which take a step's 32 KB keys each.
+// How a launch is cut: a workgroup's nw waves are wr row groups of 32 rows by nw / wr key
+// groups, which take a step's 32 kb keys each.
 struct TreeShape {
-    int wr, kb;                           // row groups; 32-key blocks a key group and step
+    int nw, wr, kb;
     int row_tiles;                        // workgroups that share a run of keys
     int groups;                           // runs
 };

@@ -465,19 +465,20 @@ __device__ __forceinline__ bool next_unit(const TreeParams& a, int step_keys, co
     return u.start - a.extra < r.u1;
 }
 
-// WR row groups of 32 rows by 8 / WR key groups.
+// NW waves: WR row groups of 32 rows by NW / WR key groups.
 // SCORES: the scores are stored too (one tile of rows).
-template <int WR, int KB, bool SCORES>
-__global__ __launch_bounds__(WAVE* TREE_NW) __attribute__((amdgpu_waves_per_eu(2)))
+// (Bounds of eight waves for four too: with more than 256 registers to give, the compiler
+// keeps the sums in the accumulation registers and moves them for every other use.)
+template <int NW, int WR, int KB, bool SCORES>
+__global__ __launch_bounds__(WAVE * 8) __attribute__((amdgpu_waves_per_eu(2)))
 void tree_kernel(const TreeParams a) {
-    constexpr int WK = TREE_NW / WR, KEYS = 32 * KB, STEP = KEYS * WK;
+    constexpr int WK = NW / WR, KEYS = 32 * KB, STEP = KEYS * WK;
     constexpr int TILE = KEYS * 256;                       // bytes of K, and of V
-    constexpr bool TWO = WR > 1;                           // two buffers; one wave's tile: one
     __shared__ __attribute__((aligned(1024))) char k0_[WK * TILE];
     __shared__ __attribute__((aligned(1024))) char v0_[WK * TILE];
-    __shared__ __attribute__((aligned(1024))) char k1_[TWO ? WK * TILE : 16];
-    __shared__ __attribute__((aligned(1024))) char v1_[TWO ? WK * TILE : 16];
-    __shared__ float2 ml_[TREE_NW][32];
+    __shared__ __attribute__((aligned(1024))) char k1_[WK * TILE];
+    __shared__ __attribute__((aligned(1024))) char v1_[WK * TILE];
+    __shared__ float2 ml_[NW][32];
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE;
     const int rg = wave % WR, kg = wave / WR, half = lane >> 5;
@@ -590,8 +591,8 @@ void tree_kernel(const TreeParams a) {
             }
         };
         // A step's products; false, with nothing done, where V holds an infinity or a NaN that a row
-        // may not see.  (between: what is done once K has been read)
-        auto add_step = [&](int step, bool masked, const char* kt, char* vt, auto&& between) {
+        // may not see.
+        auto add_step = [&](int step, bool masked, const char* kt, char* vt) {
             f16v s[KB];
             u4 p[2 * KB];
             scores_of<KB>(kt, at, q, s);
@@ -601,7 +602,6 @@ void tree_kernel(const TreeParams a) {
                 for (int z = 0; z < KB; ++z) clear_values(vt + z * 8192, z ? live[KB - 1] : live[0], lane);
                 if (odd_values<KB>(vt, at)) return false;
             }
-            between();
             if constexpr (SCORES) store_scores(s[0], ((int64_t)step * WK + kg) * KEYS);
             const float top = top_of<KB>(s, st, a.scale2);
             if (outgrown(st, top)) rescale(st, top);
@@ -610,11 +610,10 @@ void tree_kernel(const TreeParams a) {
             add_values<KB>(vt, at, st, p);
             return true;
         };
-        auto add_step_by_row = [&](int step, const char* kt, const char* vt, auto&& between) {
+        auto add_step_by_row = [&](int step, const char* kt, const char* vt) {
             f16v s[KB];
             u4 p[2 * KB];
             scores_of<KB>(kt, at, q, s);
-            between();
             mask_scores<KB>(s, bits, half);
             if constexpr (SCORES) store_scores(s[0], ((int64_t)step * WK + kg) * KEYS);
             const float top = top_of<KB>(s, st, a.scale2);
@@ -627,7 +626,8 @@ void tree_kernel(const TreeParams a) {
         char* const kt0 = k0_ + kg * TILE;
         char* const vt0 = v0_ + kg * TILE;
         // steps of the context alone, then the others
-        const int sf = s1 < ctx / STEP ? s1 : (s0 > ctx / STEP ? s0 : ctx / STEP);
+        const int plain = (ctx < keys ? ctx : keys) / STEP;
+        const int sf = s1 < plain ? s1 : plain;
         int ids = ids_of(s0);
         {
             // (a lane past the last row takes the first one's: its results go nowhere)
@@ -644,82 +644,48 @@ void tree_kernel(const TreeParams a) {
         load(1, ids, vt0);
         // (A step of infinities leaves the loop for its products by row and comes back: as a branch
         // inside it, it would cost every step copies of the sums.)
-        if constexpr (TWO) {
-            char* const kt1 = k1_ + kg * TILE;
-            char* const vt1 = v1_ + kg * TILE;
-            ids = s0 + 1 < s1 ? ids_of(s0 + 1) : 0;
-            bool masked;
-            // a step's loads have come and everyone is done with the step before: the next
-            // one's go out
-            auto turn = [&](int step, char* kn, char* vn) {
-                masked = step >= sf || bad != 0;
-                if (masked) look(step, bad);               // (its loads come with the tile's)
-                wait_vm_lds<0>();
+        char* const kt1 = k1_ + kg * TILE;
+        char* const vt1 = v1_ + kg * TILE;
+        ids = s0 + 1 < s1 ? ids_of(s0 + 1) : 0;
+        bool masked;
+        // a step's loads have come and everyone is done with the step before: the next
+        // one's go out
+        auto turn = [&](int step, char* kn, char* vn) {
+            masked = step >= sf || bad != 0;
+            if (masked) look(step, bad);               // (its loads come with the tile's)
+            wait_vm_lds<0>();
+            if constexpr (WR > 1) {
                 __syncthreads();
-                if (step + 1 < s1) {
-                    bad = bad_of(ids);
-                    load(0, ids, kn);
-                    load(1, ids, vn);
-                    if (step + 2 < s1) ids = ids_of(step + 2);
-                }
-            };
-            int step = s0;
-            bool second = false;                           // which buffers hold the step
-            while (true) {
-                while (true) {
-                    if (!second) {
-                        turn(step, kt1, vt1);
-                        if (!add_step(step, masked, kt0, vt0, [] {})) break;
-                        second = true;
-                        if (++step >= s1) break;
-                    }
-                    turn(step, kt0, vt0);
-                    if (!add_step(step, masked, kt1, vt1, [] {})) break;
-                    second = false;
-                    if (++step >= s1) break;
-                }
-                if (step >= s1) break;
-                add_step_by_row(step, second ? kt1 : kt0, second ? vt1 : vt0, [] {});
-                second = !second;
-                if (++step >= s1) break;
-            }
-        } else {
-            // one buffer of a wave's own, K and V in turn: each is requested again as soon as
-            // it has been read
-            auto reads_done = [&] {
+            } else {                                       // (a tile of the wave's own)
                 __builtin_amdgcn_s_waitcnt(0xC07F);        // lgkmcnt 0
                 asm volatile("" ::: "memory");
-            };
-            int step = s0;
-            bool more, masked;
-            auto turn = [&] {
-                more = step + 1 < s1;
-                masked = step >= sf || bad != 0;
-                if (masked) look(step, bad);
-                if (more) ids = ids_of(step + 1);
-                wait_vm_lds<0>();
-            };
-            auto next_k = [&] {
-                reads_done();
-                if (more) load(0, ids, kt0);
-            };
-            auto next_v = [&] {
-                reads_done();
-                if (more) load(1, ids, vt0);
+            }
+            if (step + 1 < s1) {
                 bad = bad_of(ids);
-            };
+                load(0, ids, kn);
+                load(1, ids, vn);
+                if (step + 2 < s1) ids = ids_of(step + 2);
+            }
+        };
+        int step = s0;
+        bool second = false;                           // which buffers hold the step
+        while (true) {
             while (true) {
-                while (true) {
-                    turn();
-                    if (!add_step(step, masked, kt0, vt0, next_k)) break;
-                    next_v();
+                if (!second) {
+                    turn(step, kt1, vt1);
+                    if (!add_step(step, masked, kt0, vt0)) break;
+                    second = true;
                     if (++step >= s1) break;
                 }
-                if (step >= s1) break;
-                add_step_by_row(step, kt0, vt0, next_k);
-                next_v();
+                turn(step, kt0, vt0);
+                if (!add_step(step, masked, kt1, vt1)) break;
+                second = false;
                 if (++step >= s1) break;
             }
+            if (step >= s1) break;
+            add_step_by_row(step, second ? kt1 : kt0, second ? vt1 : vt0);
+            second = !second;
+            if (++step >= s1) break;
         }
 
         // ---- the key groups' results made one, then the output or a record ----
@@ -730,7 +696,7 @@ void tree_kernel(const TreeParams a) {
         f4 y[QUADS];
         if constexpr (WK > 1) {
             // 16 KB a wave, over the tiles' arrays
-            constexpr int PER = (TWO ? WK * TILE : WK * TILE) / 16384;
+            constexpr int PER = WK * TILE / 16384;
             auto place = [&](int w) -> char* {
                 char* arr = w / PER == 0 ? k0_ : w / PER == 1 ? v0_ : w / PER == 2 ? k1_ : v1_;
                 return arr + (w % PER) * 16384;
@@ -882,10 +848,9 @@ __global__ __launch_bounds__(WAVE* COMBINE_NW) void tree_combine_kernel(const Tr
                 : neg_inf();
 }
 
-template <int WR, int KB, bool SCORES>
+template <int NW, int WR, int KB, bool SCORES>
 hipError_t launch(const TreeParams& a, hipStream_t stream) {
-    tree_kernel<WR, KB, SCORES>
-        <<<dim3(a.groups * a.row_tiles), dim3(WAVE * TREE_NW), 0, stream>>>(a);
+    tree_kernel<NW, WR, KB, SCORES><<<dim3(a.groups * a.row_tiles), dim3(WAVE * NW), 0, stream>>>(a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int blocks = (a.N * a.NR + 31) / 32;
@@ -900,9 +865,10 @@ constexpr int TREE_CUS = 256;
 TreeShape tree_shape(int batch, int kv_heads, int rows, int64_t keys_bound) {
     TreeShape s;
     s.wr = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
+    s.nw = s.wr == 1 ? 4 : 8;
     s.kb = s.wr >= 4 ? 2 : 1;
     s.row_tiles = (rows + 32 * s.wr - 1) / (32 * s.wr);
-    const int64_t step = 32 * s.kb * (TREE_NW / s.wr);
+    const int64_t step = 32 * s.kb * (s.nw / s.wr);
     const int64_t units = (int64_t)batch * kv_heads;
     const int64_t places = units * ((keys_bound + step - 1) / step + TREE_EXTRA);
     int64_t most = (TREE_CUS + s.row_tiles - 1) / s.row_tiles;
@@ -921,12 +887,12 @@ hipError_t launch_tree_attention(const TreeParams& p, const TreeShape& s, hipStr
     a.groups = s.groups;
     a.row_tiles = s.row_tiles;
     a.extra = TREE_EXTRA;
-    if (a.scores) return launch<1, 1, true>(a, stream);
+    if (a.scores) return launch<4, 1, 1, true>(a, stream);
     switch (s.wr) {
-        case 1: return launch<1, 1, false>(a, stream);
-        case 2: return launch<2, 1, false>(a, stream);
-        case 4: return launch<4, 2, false>(a, stream);
-        default: return launch<8, 2, false>(a, stream);
+        case 1: return launch<4, 1, 1, false>(a, stream);
+        case 2: return launch<8, 2, 1, false>(a, stream);
+        case 4: return launch<8, 4, 2, false>(a, stream);
+        default: return launch<8, 8, 2, false>(a, stream);
     }
 }
 

@@ -10,10 +10,10 @@ namespace ls {
 // ---- attention of several new tokens over the fp16 pools --------------------------
 constexpr int TREE_MAX_NODES = 256;
 
-// How a launch is cut: a workgroup's nw waves are wr row groups of 32 rows by nw / wr key
+// How a launch is cut: a workgroup's nw waves are wr row groups of `rows` rows by nw / wr key
 // groups, which take a step's 32 kb keys each.
 struct TreeShape {
-    int nw, wr, kb;
+    int rows, nw, wr, kb;
     int row_tiles;                        // workgroups that share a run of keys
     int groups;                           // runs
 };
@@ -51,11 +51,10 @@ struct TreeParams {
 };
 
 constexpr int TREE_EXTRA = 1;
-constexpr int TREE_RECORD = 32 * 128 + 64;        // floats of a row group's record
 
 TreeShape tree_shape(int batch, int kv_heads, int rows, int64_t keys_bound);
 size_t tree_record_bytes(const TreeShape& s);
-// With scores (up to 32 rows): they are kept, and lse is written.
+// With scores (up to 16 rows): they are kept, and lse is written.
 hipError_t launch_tree_attention(const TreeParams& a, const TreeShape& s, hipStream_t stream);
 
 // ---- weight sums of accepted paths ---------------------------------------------------

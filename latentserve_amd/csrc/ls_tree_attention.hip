@@ -29,11 +29,6 @@ namespace {
 // full precision down to 2^-21 of the running maximum's.
 constexpr float TREE_TOP = 7.f, TREE_LAZY = 8.f;
 
-__device__ __forceinline__ f16v mfma3216(u4 a, u4 b, f16v c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a),
-                                                  __builtin_bit_cast(h8, b), c, 0, 0, 0);
-}
-
 // (buffer loads: after a global load to LDS the compiler waits for all LDS reads where it
 // needs one)
 typedef void __attribute__((address_space(3)))* lds_ptr;
@@ -46,20 +41,45 @@ __device__ __forceinline__ u2 read_transposed(const char* p) {
         u2, __builtin_amdgcn_ds_read_tr16_b64_v4f16((g4 __attribute__((address_space(3)))*)p));
 }
 
+// Products are of ROWS rows: 32 (32x32x16), or 16 (16x16x32) where a head has no more, for half
+// the arithmetic.  A lane holds row lane % ROWS, its part h = lane / ROWS of HB.
+template <int ROWS>
+struct Form;
+template <>
+struct Form<32> {
+    typedef f16v Acc;
+    static constexpr int PARTS = 4;       // of the channels, an accumulator each
+    static __device__ __forceinline__ f16v mfma(u4 a, u4 b, f16v c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a),
+                                                      __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    }
+};
+template <>
+struct Form<16> {
+    typedef f4 Acc;
+    static constexpr int PARTS = 8;
+    static __device__ __forceinline__ f4 mfma(u4 a, u4 b, f4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a),
+                                                      __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    }
+};
+
 // Where a lane reads a tile's K and V, and what it loads of it, in bytes.  A tile starts
 // on 1 KB and a row is 256 bytes, so a swizzled place inside a row is one exclusive or:
-//   K of step j:         k ^ (32 j)        (piece 2 j + half of key lane % 32)
-//   V of channels 32 c:  v ^ (64 c)        (see values_of)
+//   K of step j:         k ^ (16 HB j)     (piece HB j + h of key lane % ROWS)
+//   V of part c:         v ^ (256 / PARTS c)
 //   loads i of a page:   (4 i + lane / 16) rows, pieces k_in ^ (64 i), v_in ^ (128 (i % 2))
 struct LanePlaces {
     uint32_t k, v, k_in, v_in;
 };
+template <int ROWS>
 __device__ __forceinline__ LanePlaces lane_places(int lane) {
     LanePlaces p;
-    const int key = lane & 31, half = lane >> 5, quarter = lane >> 4, pp = lane & 15;
-    const int r = 4 * (quarter >> 1) + ((lane & 15) >> 2);
-    p.k = key * 256 + 16 * (half ^ (key & 15));
-    p.v = r * 256 + 32 * ((quarter & 1) ^ r) + 8 * (lane & 3);
+    const int key = lane % ROWS, h = lane / ROWS, quarter = lane >> 4, pp = lane & 15;
+    p.k = key * 256 + 16 * (h ^ (key & 15));
+    // a transposing read's 16 lanes take four keys' 16 channels and get a channel's four keys
+    const int r = 4 * h + ((lane & 15) >> 2), unit = ROWS == 32 ? quarter & 1 : 0;
+    p.v = r * 256 + 32 * (unit ^ (r & 7)) + 8 * (lane & 3);
     p.k_in = 16 * (pp ^ quarter);
     p.v_in = 32 * ((pp >> 1) ^ quarter) + 16 * (pp & 1);
     return p;
@@ -71,28 +91,248 @@ __device__ __forceinline__ uint32_t here(uint32_t x) {
     return x;
 }
 
-struct RowState {
-    f16v acc[4];                          // O^T: channel 32 c + 8 (i / 4) + 4 half + i % 4
-    float m, l;                           // running maximum (log2 units), this half's sum
+// Of ROWS rows and 32 KB keys a tile.
+template <int ROWS, int KB>
+struct Tile {
+    typedef Form<ROWS> F;
+    typedef typename F::Acc Acc;
+    static constexpr int HB = 64 / ROWS, PARTS = F::PARTS;
+    static constexpr int STEPS = 16 / HB;               // of the first product (128 channels)
+    static constexpr int SN = ROWS / 2;                 // scores a lane and 32 keys
+    static constexpr int NP = KB * SN / 8;              // steps of the second product
+    static constexpr int EL = sizeof(Acc) / 4;
+    static constexpr int QUADS = ROWS / 2;              // four adjacent channels each
+
+    u4 q[STEPS];
+    Acc acc[PARTS];                                     // O^T
+    float m, l;                                         // maximum (log2 units), this part's sum
+    float s[KB][SN];                                    // scores: see key_of
+    u4 p[NP];                                           // weights, fp16
+    LanePlaces at;
+    int h;                                              // lane / ROWS
+
+    // the key of score i, and the channel of quad n's first value, but for 4 h
+    static constexpr int key_of(int i) { return 128 / SN * (i / 4) + i % 4; }
+    static constexpr int channel_of(int n) { return 128 / QUADS * n; }
+    __device__ __forceinline__ f4 quad(int n) const {
+        const Acc& x = acc[4 * n / EL];
+        const int i = 4 * n % EL;
+        return (f4){x[i], x[i + 1], x[i + 2], x[i + 3]};
+    }
+
+    // Keeps the sums in one set of registers where branches join (the compiler otherwise takes
+    // them apart there and copies all of them, in every step).
+    __device__ __forceinline__ void pin() {
+        if constexpr (PARTS == 4)
+            asm volatile("" : "+v"(acc[0]), "+v"(acc[1]), "+v"(acc[2]), "+v"(acc[3]));
+        else
+            asm volatile("" : "+v"(acc[0]), "+v"(acc[1]), "+v"(acc[2]), "+v"(acc[3]), "+v"(acc[4]),
+                              "+v"(acc[5]), "+v"(acc[6]), "+v"(acc[7]));
+    }
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int c = 0; c < PARTS; ++c)
+#pragma unroll
+            for (int i = 0; i < EL; ++i) acc[c][i] = 0.f;
+        m = neg_inf();
+        l = 0.f;
+    }
+
+    // What the scheduler is to keep: `FIRST` LDS reads ahead, then one product and `PER`
+    // reads in turn (left to itself it reads an operand and waits for it, product by product).
+    template <int FIRST, int PER, int READS, int PRODUCTS>
+    static __device__ __forceinline__ void reads_ahead() {
+        __builtin_amdgcn_sched_group_barrier(0x100, FIRST, 0);
+#pragma unroll
+        for (int i = 0; i < PRODUCTS; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            if (FIRST + i * PER < READS) __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+        }
+    }
+
+    __device__ __forceinline__ void scores(const char* kt) {
+        constexpr int NZ = KB * 32 / ROWS;              // ROWS keys each
+        Acc x[NZ];
+#pragma unroll
+        for (int z = 0; z < NZ; ++z)
+#pragma unroll
+            for (int i = 0; i < EL; ++i) x[z][i] = 0.f;
+        u4 k[STEPS][NZ];
+        const uint32_t lane_k = here(at.k);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < STEPS; ++j)
+#pragma unroll
+            for (int z = 0; z < NZ; ++z)
+                k[j][z] = *(const u4*)(kt + (lane_k ^ (16 * HB * j)) + z * ROWS * 256);
+#pragma unroll
+        for (int j = 0; j < STEPS; ++j)
+#pragma unroll
+            for (int z = 0; z < NZ; ++z) x[z] = F::mfma(k[j][z], q[j], x[z]);
+        reads_ahead<4, 1, STEPS * NZ, STEPS * NZ>();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int z = 0; z < KB; ++z)
+#pragma unroll
+            for (int i = 0; i < SN; ++i) s[z][i] = x[(z * SN + i) / EL][i % EL];
+    }
+
+    // bits: what the row sees of each 32 keys
+    __device__ __forceinline__ void mask(const uint32_t (&bits)[KB]) {
+        const uint32_t shift = here(4 * h);
+#pragma unroll
+        for (int z = 0; z < KB; ++z) {
+            const uint32_t b = bits[z] >> shift;
+#pragma unroll
+            for (int i = 0; i < SN; ++i) s[z][i] = (b >> key_of(i)) & 1 ? s[z][i] : neg_inf();
+        }
+    }
+
+    // Softmax weights of the scores, the maximum and the sum brought up to date.
+    __device__ __forceinline__ void weights(float scale2) {
+        float top = neg_inf();
+#pragma unroll
+        for (int z = 0; z < KB; ++z)
+#pragma unroll
+            for (int i = 0; i < SN; ++i) top = fmaxf(top, s[z][i]);
+        if constexpr (HB == 2) {
+            const LanePair o = swap32(top);
+            top = fmaxf(o.a, o.b);
+        } else {
+            top = group4_max(top);
+        }
+        top = fmaxf(m, top * scale2);
+        // (wave-uniform: weights stay below 2^15 while no score outgrows the maximum by more)
+        if (__any(top > m + TREE_LAZY)) {
+            const float alpha = fast_exp2(m - (top == neg_inf() ? 0.f : top));
+            l *= alpha;
+#pragma unroll
+            for (int c = 0; c < PARTS; ++c) acc[c] *= alpha;
+            m = top;
+            pin();
+        }
+        pin();
+        const float off = TREE_TOP - (m == neg_inf() ? 0.f : m);
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};            // (four: shorter chains)
+#pragma unroll
+        for (int z = 0; z < KB; ++z)
+#pragma unroll
+            for (int i = 0; i < SN; i += 2) {
+                const float w0 = fast_exp2(__builtin_fmaf(s[z][i], scale2, off));
+                const float w1 = fast_exp2(__builtin_fmaf(s[z][i + 1], scale2, off));
+                sum[i % 4] += w0;
+                sum[i % 4 + 1] += w1;
+                const h2 w = {(half_t)w0, (half_t)w1};
+                p[z * (SN / 8) + i / 8][i / 2 % 4] = __builtin_bit_cast(uint32_t, w);
+            }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    }
+
+    // V^T of step j's keys (256 / ROWS of them... 16 or 32) and part c's channels, its keys in the
+    // order of the scores.
+    static constexpr int STEP_BYTES = 65536 / SN;       // 16 keys, or 32
+    __device__ __forceinline__ u4 values_of(const char* vt, uint32_t lane_v, int j, int c) const {
+        const char* at = vt + (lane_v ^ (256 / PARTS * c)) + j * STEP_BYTES;
+        const u2 a = read_transposed(at), b = read_transposed(at + STEP_BYTES / 2);
+        return (u4){a.x, a.y, b.x, b.y};
+    }
+
+    __device__ __forceinline__ void values(const char* vt) {
+        u4 v[NP][PARTS];
+        const uint32_t lane_v = here(at.v);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < NP; ++j)
+#pragma unroll
+            for (int c = 0; c < PARTS; ++c) v[j][c] = values_of(vt, lane_v, j, c);
+#pragma unroll
+        for (int j = 0; j < NP; ++j)
+#pragma unroll
+            for (int c = 0; c < PARTS; ++c) acc[c] = F::mfma(v[j][c], p[j], acc[c]);
+        reads_ahead<10, 2, 2 * NP * PARTS, NP * PARTS>();
+        __builtin_amdgcn_sched_barrier(0);
+    }
+
+    // The largest magnitude of an operand's halves so far, as bits (an infinity or a NaN: 0x7C00
+    // and more).
+    typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+
+    // Whether V of the tile holds an infinity or a NaN.
+    __device__ __forceinline__ bool odd(const char* vt) const {
+        const uint32_t lane_v = here(at.v);
+        us2 top = {0, 0};
+#pragma unroll 1
+        for (int j = 0; j < NP; ++j) {
+            u4 v[PARTS];
+#pragma unroll
+            for (int c = 0; c < PARTS; ++c) v[c] = values_of(vt + j * STEP_BYTES, lane_v, 0, c);
+#pragma unroll
+            for (int c = 0; c < PARTS; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    top = __builtin_elementwise_max(top, __builtin_bit_cast(us2, v[c][i] & 0x7FFF7FFFu));
+        }
+        return __any(top.x >= 0x7C00 || top.y >= 0x7C00);
+    }
+
+    // A V operand whose keys outside `keep` (bits of the 32 keys) are zeros; j: its step of them.
+    __device__ __forceinline__ u4 keep_keys(u4 v, uint32_t keep, int j) const {
+        const uint32_t b = keep >> here((SN == 16 ? 16 * j : 0) + 4 * h);
+        auto pair = [&](int i) {
+            return ((b >> i) & 1 ? 0xFFFFu : 0u) | ((b >> (i + 1)) & 1 ? 0xFFFF0000u : 0u);
+        };
+        v.x &= pair(0);
+        v.y &= pair(2);
+        v.z &= pair(key_of(4));
+        v.w &= pair(key_of(4) + 2);
+        return v;
+    }
+
+    // The second product of a tile whose V holds an infinity or a NaN, which some rows see and
+    // others do not: a row at a time, of the keys that the row sees.  bits: what the lane's sees.
+    __device__ __forceinline__ void values_by_row(const char* vt, const uint32_t (&bits)[KB]) {
+        const int row = (int)here(__lane_id()) % ROWS;
+        // (loops that stay loops: this is rare, and registers are the common path's)
+#pragma unroll 1
+        for (int z = 0; z < KB; ++z) {
+            const u4 p0 = z ? p[NP - SN / 8] : p[0], p1 = z ? p[NP - 1] : p[SN / 8 - 1];
+            const uint32_t b = z ? bits[KB - 1] : bits[0];
+#pragma unroll 1
+            for (int x = 0; x < ROWS; ++x) {
+                const uint32_t seen = (uint32_t)__builtin_amdgcn_readlane((int)b, x);
+#pragma unroll
+                for (int c = 0; c < PARTS; ++c) {
+                    const uint32_t lane_v = here(at.v);
+                    Acc y;
+#pragma unroll
+                    for (int i = 0; i < EL; ++i) y[i] = 0.f;
+                    y = F::mfma(keep_keys(values_of(vt + z * 8192, lane_v, 0, c), seen, 0), p0, y);
+                    if constexpr (SN == 16)
+                        y = F::mfma(keep_keys(values_of(vt + z * 8192, lane_v, 1, c), seen, 1), p1, y);
+#pragma unroll
+                    for (int i = 0; i < EL; ++i) acc[c][i] += row == x ? y[i] : 0.f;
+                    pin();
+                    __builtin_amdgcn_sched_barrier(0);
+                    asm volatile("" ::: "memory");      // (one part's registers at a time)
+                }
+            }
+        }
+    }
 };
 
-// Keeps the sums in one set of registers where branches join (the compiler otherwise takes them
-// apart there and copies all 64, in every step).
-__device__ __forceinline__ void pin(RowState& st) {
-    asm volatile("" : "+v"(st.acc[0]), "+v"(st.acc[1]), "+v"(st.acc[2]), "+v"(st.acc[3]));
-}
-
-__device__ __forceinline__ void clear(RowState& st) {
+// V rows of 32 keys that do not exist (not `live`) become zeros in LDS: what lies there may be
+// anything, and a weight of 0 removes no NaN.  (Waves that share the keys all write the same
+// zeros.)
+__device__ __forceinline__ void clear_values(char* vt, uint32_t live, int lane_) {
+    const uint32_t lane = here(lane_);
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) st.acc[c][i] = 0.f;
-    st.m = neg_inf();
-    st.l = 0.f;
+    for (int i = 0; i < 8; ++i)
+        if (!((live >> (4 * i + (lane >> 4))) & 1)) *(u4*)(vt + i * 1024 + lane * 16) = (u4){0, 0, 0, 0};
 }
 
 // The 32 bits of what `row` sees of keys key0 .. key0 + 31 (bit: key - key0), for a tile
-// that meets the tree or the end.  `ok`: keys that exist.
+// that meets the tree or the end.
 __device__ __forceinline__ uint32_t seen_bits(const TreeParams& a, const uint64_t* row_mask, int node,
                                               int64_t rel0, int nodes) {
     // keys of the context
@@ -118,203 +358,6 @@ __device__ __forceinline__ uint32_t seen_bits(const TreeParams& a, const uint64_
     uint32_t t = (uint32_t)w;
     if (left < 32) t &= left <= 0 ? 0u : (1u << left) - 1;
     return rel0 < 0 ? (t << (int)(-rel0)) | ctx : t;
-}
-
-// What the scheduler is to keep: `first` LDS reads ahead, then one product and `per`
-// reads in turn (left to itself it reads an operand and waits for it, product by product).
-template <int FIRST, int PER, int READS, int PRODUCTS>
-__device__ __forceinline__ void reads_ahead() {
-    __builtin_amdgcn_sched_group_barrier(0x100, FIRST, 0);
-#pragma unroll
-    for (int i = 0; i < PRODUCTS; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-        if (FIRST + i * PER < READS) __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
-    }
-}
-
-// Scores of a tile of 32 KB keys for the wave's 32 rows.
-template <int KB>
-__device__ __forceinline__ void scores_of(const char* kt, const LanePlaces& at, const u4 (&q)[8],
-                                          f16v (&s)[KB]) {
-#pragma unroll
-    for (int z = 0; z < KB; ++z)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[z][i] = 0.f;
-    u4 k[8][KB];
-    const uint32_t lane_k = here(at.k);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int z = 0; z < KB; ++z) k[j][z] = *(const u4*)(kt + (lane_k ^ (32 * j)) + z * 8192);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int z = 0; z < KB; ++z) s[z] = mfma3216(k[j][z], q[j], s[z]);
-    reads_ahead<4, 1, 8 * KB, 8 * KB>();
-    __builtin_amdgcn_sched_barrier(0);
-}
-
-template <int KB>
-__device__ __forceinline__ void mask_scores(f16v (&s)[KB], const uint32_t (&bits)[KB], int half) {
-    const uint32_t shift = here(4 * half);
-#pragma unroll
-    for (int z = 0; z < KB; ++z) {
-        const uint32_t b = bits[z] >> shift;
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            s[z][i] = (b >> (8 * (i / 4) + i % 4)) & 1 ? s[z][i] : neg_inf();
-    }
-}
-
-// The row's maximum with the tile's scores, in log2 units.
-template <int KB>
-__device__ __forceinline__ float top_of(const f16v (&s)[KB], const RowState& st, float scale2) {
-    float top = neg_inf();
-#pragma unroll
-    for (int z = 0; z < KB; ++z)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[z][i]);
-    const LanePair o = swap32(top);
-    return fmaxf(st.m, fmaxf(o.a, o.b) * scale2);
-}
-// Whether weights could pass 2^15: a score outgrew the maximum (the same in every lane).
-__device__ __forceinline__ bool outgrown(const RowState& st, float top) {
-    return __any(top > st.m + TREE_LAZY);
-}
-__device__ __forceinline__ void rescale(RowState& st, float top) {
-    const float alpha = fast_exp2(st.m - (top == neg_inf() ? 0.f : top));
-    st.l *= alpha;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) st.acc[c] *= alpha;
-    st.m = top;
-    pin(st);
-}
-
-// Softmax weights of the tile as fp16 pairs, and their sum.
-template <int KB>
-__device__ __forceinline__ void weights_of(const f16v (&s)[KB], RowState& st, float scale2,
-                                           u4 (&p)[2 * KB]) {
-    const float off = TREE_TOP - (st.m == neg_inf() ? 0.f : st.m);
-    float l[4] = {0.f, 0.f, 0.f, 0.f};        // (four sums: shorter chains)
-#pragma unroll
-    for (int z = 0; z < KB; ++z)
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-            const float w0 = fast_exp2(__builtin_fmaf(s[z][i], scale2, off));
-            const float w1 = fast_exp2(__builtin_fmaf(s[z][i + 1], scale2, off));
-            l[i % 4] += w0;
-            l[i % 4 + 1] += w1;
-            const h2 w = {(half_t)w0, (half_t)w1};
-            p[2 * z + i / 8][i / 2 % 4] = __builtin_bit_cast(uint32_t, w);
-        }
-    st.l += (l[0] + l[1]) + (l[2] + l[3]);
-}
-
-// V^T of 16 keys (step j of the tile) and 32 channels (c).
-__device__ __forceinline__ u4 values_of(const char* vt, uint32_t lane_v, int j, int c) {
-    const u2 a = read_transposed(vt + (lane_v ^ (64 * c)) + j * 4096);
-    const u2 b = read_transposed(vt + (lane_v ^ (64 * c)) + j * 4096 + 2048);
-    return (u4){a.x, a.y, b.x, b.y};
-}
-
-template <int KB>
-__device__ __forceinline__ void add_values(const char* vt, const LanePlaces& at, RowState& st,
-                                           const u4 (&p)[2 * KB]) {
-    u4 v[2 * KB][4];
-    const uint32_t lane_v = here(at.v);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int j = 0; j < 2 * KB; ++j)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) v[j][c] = values_of(vt, lane_v, j, c);
-#pragma unroll
-    for (int j = 0; j < 2 * KB; ++j)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) st.acc[c] = mfma3216(v[j][c], p[j], st.acc[c]);
-    reads_ahead<10, 2, 16 * KB, 8 * KB>();
-    __builtin_amdgcn_sched_barrier(0);
-}
-
-// Halves of a V operand's keys 16 j + 4 half + (0..3) and + 8 cleared where `keep` (bits of the
-// 32 keys) has a 0.
-__device__ __forceinline__ u4 keep_keys(u4 v, uint32_t keep, int j, int half) {
-    const uint32_t b = keep >> here(16 * (j & 1) + 4 * half);
-    auto pair = [&](int i) {
-        return ((b >> i) & 1 ? 0xFFFFu : 0u) | ((b >> (i + 1)) & 1 ? 0xFFFF0000u : 0u);
-    };
-    v.x &= pair(0);
-    v.y &= pair(2);
-    v.z &= pair(8);
-    v.w &= pair(10);
-    return v;
-}
-// V rows of a 32-key block whose keys do not exist (not `live`) become zeros in LDS: what lies
-// there may be anything, and a weight of 0 removes no NaN.  (Waves that share the block all
-// write the same zeros.)
-__device__ __forceinline__ void clear_values(char* vt, uint32_t live, int lane_) {
-    const uint32_t lane = here(lane_);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (!((live >> (4 * i + (lane >> 4))) & 1)) *(u4*)(vt + i * 1024 + lane * 16) = (u4){0, 0, 0, 0};
-}
-
-// The largest magnitude of an operand's halves so far, as bits (an infinity or a NaN: 0x7C00 and
-// more).
-typedef uint16_t us2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ us2 magnitude(us2 m, u4 v) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        m = __builtin_elementwise_max(m, __builtin_bit_cast(us2, v[i] & 0x7FFF7FFFu));
-    return m;
-}
-
-// Whether V of a tile holds an infinity or a NaN.
-template <int KB>
-__device__ __forceinline__ bool odd_values(const char* vt, const LanePlaces& at) {
-    const uint32_t lane_v = here(at.v);
-    us2 m = {0, 0};
-#pragma unroll 1
-    for (int j = 0; j < 2 * KB; ++j) {
-        u4 v[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) v[c] = values_of(vt + j * 4096, lane_v, 0, c);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) m = magnitude(m, v[c]);
-    }
-    return __any(m.x >= 0x7C00 || m.y >= 0x7C00);
-}
-
-// A tile whose V holds an infinity or a NaN, which some rows see and others do not: products a
-// row at a time, of the keys that the row sees.  bits: what the lane's row sees.
-template <int KB>
-__device__ __forceinline__ void add_values_by_row(const char* vt, const LanePlaces& at, RowState& st,
-                                                  const u4 (&p)[2 * KB], const uint32_t (&bits)[KB],
-                                                  int half) {
-    const int row = (int)here(__lane_id()) & 31;
-    // (loops that stay loops: this is rare, and registers are the common path's)
-#pragma unroll 1
-    for (int z = 0; z < KB; ++z) {
-        const u4 p0 = z ? p[2 * KB - 2] : p[0], p1 = z ? p[2 * KB - 1] : p[1];
-        const uint32_t b = z ? bits[KB - 1] : bits[0];
-#pragma unroll 1
-        for (int x = 0; x < 32; ++x) {
-            const uint32_t seen = (uint32_t)__builtin_amdgcn_readlane((int)b, x);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const uint32_t lane_v = here(at.v);
-                f16v y;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) y[i] = 0.f;
-                y = mfma3216(keep_keys(values_of(vt + z * 8192, lane_v, 0, c), seen, 0, half), p0, y);
-                y = mfma3216(keep_keys(values_of(vt + z * 8192, lane_v, 1, c), seen, 1, half), p1, y);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) st.acc[c][i] += row == x ? y[i] : 0.f;
-                __builtin_amdgcn_sched_barrier(0);
-                asm volatile("" ::: "memory");        // (one quarter's registers at a time)
-            }
-        }
-    }
 }
 
 // ---- the run of a group -------------------------------------------------------------
@@ -465,23 +508,24 @@ __device__ __forceinline__ bool next_unit(const TreeParams& a, int step_keys, co
     return u.start - a.extra < r.u1;
 }
 
-// NW waves: WR row groups of 32 rows by NW / WR key groups.
-// SCORES: the scores are stored too (one tile of rows).
+// NW waves: WR row groups of ROWS rows by NW / WR key groups.
+// SCORES: the scores are stored too (one row group).
 // (Bounds of eight waves for four too: with more than 256 registers to give, the compiler
 // keeps the sums in the accumulation registers and moves them for every other use.)
-template <int NW, int WR, int KB, bool SCORES>
+template <int ROWS, int NW, int WR, int KB, bool SCORES>
 __global__ __launch_bounds__(WAVE * 8) __attribute__((amdgpu_waves_per_eu(2)))
 void tree_kernel(const TreeParams a) {
+    typedef Tile<ROWS, KB> T;
     constexpr int WK = NW / WR, KEYS = 32 * KB, STEP = KEYS * WK;
     constexpr int TILE = KEYS * 256;                       // bytes of K, and of V
     __shared__ __attribute__((aligned(1024))) char k0_[WK * TILE];
     __shared__ __attribute__((aligned(1024))) char v0_[WK * TILE];
     __shared__ __attribute__((aligned(1024))) char k1_[WK * TILE];
     __shared__ __attribute__((aligned(1024))) char v1_[WK * TILE];
-    __shared__ float2 ml_[NW][32];
+    __shared__ float2 ml_[NW][ROWS];
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE;
-    const int rg = wave % WR, kg = wave / WR, half = lane >> 5;
+    const int rg = wave % WR, kg = wave / WR;
     const int v = xcd_major(blockIdx.x, gridDim.x);
     const int g = __builtin_amdgcn_readfirstlane(v / a.row_tiles), rt = v - g * a.row_tiles;
 
@@ -489,15 +533,19 @@ void tree_kernel(const TreeParams a) {
     Unit u = find_run(a, STEP, lane, g, run);
     if (u.b >= a.B) return;                                // (every wave alike, before any barrier)
 
-    const LanePlaces at = lane_places(lane);
+    T t;
+    t.at = lane_places<ROWS>(lane);
+    t.h = lane / ROWS;
     const int R = a.N * a.NR;
+    // (a row group past the last row only loads)
+    const bool works = (rt * WR + rg) * ROWS < R;
     // the lane's row, worked out where it is used (in registers it would cost the loop some)
     struct Row {
         int node, rep;
         bool is;
     };
     auto row_of = [&] {
-        const int row = (rt * WR + rg) * 32 + (int)here(lane & 31);
+        const int row = (rt * WR + rg) * ROWS + (int)here(lane % ROWS);
         Row o;
         o.is = row < R;
         o.node = o.is ? row / a.NR : 0;
@@ -527,9 +575,6 @@ void tree_kernel(const TreeParams a) {
         const int32_t* table = a.tables + u.b * a.st_b;
         const int pages = (keys + PAGE - 1) / PAGE, last_page = pages > 0 ? pages - 1 : 0;
 
-        u4 q[8];
-        RowState st;
-
         // Blocks of a step's tile, a lane a page (past the sequence's last page, it again: keys
         // there do not count).
         auto ids_of = [&](int step) {
@@ -542,9 +587,9 @@ void tree_kernel(const TreeParams a) {
             return (uint32_t)__ballot((unsigned)ids >= (unsigned)a.num_blocks) & ((1u << (KEYS / PAGE)) - 1);
         };
         // (a page outside the pool is not requested: what its rows hold then counts as nothing)
-        auto load = [&](int z, int ids, char* t) {
+        auto load = [&](int z, int ids, char* to) {
             constexpr int SAME = LOADS < 4 ? LOADS : 4;    // instructions of one page
-            const uint32_t row = here(row_in), k_in = here(at.k_in), v_in = here(at.v_in);
+            const uint32_t row = here(row_in), k_in = here(t.at.k_in), v_in = here(t.at.v_in);
 #pragma unroll
             for (int i0 = 0; i0 < LOADS; i0 += SAME) {
                 const int first = (rg * LOADS + i0) * 4;
@@ -556,19 +601,20 @@ void tree_kernel(const TreeParams a) {
                 for (int i = 0; i < SAME; ++i) {
                     const int n = LOADS < 4 ? (rg * LOADS + i) & 3 : i;       // of the page's four
                     const uint32_t off = z ? v_in ^ (128 * (n & 1)) : k_in ^ (64 * n);
-                    load_to_lds(from, row + off, 4 * n * (int)a.sp_t, t + (first + 4 * i) * 256);
+                    load_to_lds(from, row + off, 4 * n * (int)a.sp_t, to + (first + 4 * i) * 256);
                 }
             }
         };
-        // a block's scores, in log2 units
-        auto store_scores = [&](const f16v& s, int64_t k0) {
-            if ((lane & 31) >= R || k0 >= keys) return;
-            float* to = a.scores + ((int64_t)(u.b * a.H + u.h) * R + (lane & 31)) * a.score_len + k0 + 4 * half;
+        // the scores of a tile (KB 1), in log2 units
+        auto store_scores = [&](int64_t k0) {
+            const int row = lane % ROWS;
+            if (row >= R || k0 >= keys) return;
+            float* to = a.scores + ((int64_t)(u.b * a.H + u.h) * R + row) * a.score_len + k0 + 4 * t.h;
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                const f4 x = {s[4 * n] * a.scale2, s[4 * n + 1] * a.scale2, s[4 * n + 2] * a.scale2,
-                              s[4 * n + 3] * a.scale2};
-                *(f4*)(to + 8 * n) = x;
+            for (int i = 0; i < T::SN; i += 4) {
+                const f4 x = {t.s[0][i] * a.scale2, t.s[0][i + 1] * a.scale2, t.s[0][i + 2] * a.scale2,
+                              t.s[0][i + 3] * a.scale2};
+                *(f4*)(to + T::key_of(i)) = x;
             }
         };
         // What the row sees of a step's tile (bits), and which of its keys exist (live, the same in
@@ -593,38 +639,31 @@ void tree_kernel(const TreeParams a) {
         // A step's products; false, with nothing done, where V holds an infinity or a NaN that a row
         // may not see.
         auto add_step = [&](int step, bool masked, const char* kt, char* vt) {
-            f16v s[KB];
-            u4 p[2 * KB];
-            scores_of<KB>(kt, at, q, s);
+            if (!works) return true;
+            t.scores(kt);
             if (masked) {
-                mask_scores<KB>(s, bits, half);
+                t.mask(bits);
 #pragma unroll 1
                 for (int z = 0; z < KB; ++z) clear_values(vt + z * 8192, z ? live[KB - 1] : live[0], lane);
-                if (odd_values<KB>(vt, at)) return false;
+                if (t.odd(vt)) return false;
             }
-            if constexpr (SCORES) store_scores(s[0], ((int64_t)step * WK + kg) * KEYS);
-            const float top = top_of<KB>(s, st, a.scale2);
-            if (outgrown(st, top)) rescale(st, top);
-            pin(st);
-            weights_of<KB>(s, st, a.scale2, p);
-            add_values<KB>(vt, at, st, p);
+            if constexpr (SCORES) store_scores(((int64_t)step * WK + kg) * KEYS);
+            t.weights(a.scale2);
+            t.values(vt);
             return true;
         };
         auto add_step_by_row = [&](int step, const char* kt, const char* vt) {
-            f16v s[KB];
-            u4 p[2 * KB];
-            scores_of<KB>(kt, at, q, s);
-            mask_scores<KB>(s, bits, half);
-            if constexpr (SCORES) store_scores(s[0], ((int64_t)step * WK + kg) * KEYS);
-            const float top = top_of<KB>(s, st, a.scale2);
-            if (outgrown(st, top)) rescale(st, top);
-            pin(st);
-            weights_of<KB>(s, st, a.scale2, p);
-            add_values_by_row<KB>(vt, at, st, p, bits, half);
+            t.scores(kt);
+            t.mask(bits);
+            if constexpr (SCORES) store_scores(((int64_t)step * WK + kg) * KEYS);
+            t.weights(a.scale2);
+            t.values_by_row(vt, bits);
         };
 
         char* const kt0 = k0_ + kg * TILE;
         char* const vt0 = v0_ + kg * TILE;
+        char* const kt1 = k1_ + kg * TILE;
+        char* const vt1 = v1_ + kg * TILE;
         // steps of the context alone, then the others
         const int plain = (ctx < keys ? ctx : keys) / STEP;
         const int sf = s1 < plain ? s1 : plain;
@@ -633,26 +672,21 @@ void tree_kernel(const TreeParams a) {
             // (a lane past the last row takes the first one's: its results go nowhere)
             const Row row = row_of();
             const half_t* p = a.q + u.b * a.sq_b + row.node * a.sq_n + u.h * a.sq_h +
-                              row.rep * a.sq_r + 8 * half;
+                              row.rep * a.sq_r + 8 * t.h;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) q[j] = *(const u4*)(p + 16 * j);
+            for (int j = 0; j < T::STEPS; ++j) t.q[j] = *(const u4*)(p + 8 * T::HB * j);
         }
-        clear(st);
-
+        t.clear();
         uint32_t bad = bad_of(ids);
         load(0, ids, kt0);
         load(1, ids, vt0);
-        // (A step of infinities leaves the loop for its products by row and comes back: as a branch
-        // inside it, it would cost every step copies of the sums.)
-        char* const kt1 = k1_ + kg * TILE;
-        char* const vt1 = v1_ + kg * TILE;
         ids = s0 + 1 < s1 ? ids_of(s0 + 1) : 0;
         bool masked;
         // a step's loads have come and everyone is done with the step before: the next
         // one's go out
         auto turn = [&](int step, char* kn, char* vn) {
             masked = step >= sf || bad != 0;
-            if (masked) look(step, bad);               // (its loads come with the tile's)
+            if (masked) look(step, bad);                   // (its loads come with the tile's)
             wait_vm_lds<0>();
             if constexpr (WR > 1) {
                 __syncthreads();
@@ -667,8 +701,10 @@ void tree_kernel(const TreeParams a) {
                 if (step + 2 < s1) ids = ids_of(step + 2);
             }
         };
+        // (A step of infinities leaves the loop for its products by row and comes back: as a branch
+        // inside it, it would cost every step copies of the sums.)
         int step = s0;
-        bool second = false;                           // which buffers hold the step
+        bool second = false;                               // which buffers hold the step
         while (true) {
             while (true) {
                 if (!second) {
@@ -690,36 +726,37 @@ void tree_kernel(const TreeParams a) {
 
         // ---- the key groups' results made one, then the output or a record ----
         const bool whole = s0 == 0 && s1 == u.steps;
-        const LanePair lp = swap32(st.l);
-        float l = lp.a + lp.b, m = st.m;
-        constexpr int QUADS = 16 / WK;                     // of 16 channel quads, this wave's
+        float l, m = t.m;
+        if constexpr (T::HB == 2) {
+            const LanePair lp = swap32(t.l);
+            l = lp.a + lp.b;
+        } else {
+            l = group4_sum(t.l);
+        }
+        constexpr int QUADS = T::QUADS / WK;               // of the row group's, this wave's
         f4 y[QUADS];
         if constexpr (WK > 1) {
-            // 16 KB a wave, over the tiles' arrays
-            constexpr int PER = WK * TILE / 16384;
+            // over the tiles' arrays
+            constexpr int BYTES = T::QUADS * 1024, PER = WK * TILE / BYTES;
             auto place = [&](int w) -> char* {
                 char* arr = w / PER == 0 ? k0_ : w / PER == 1 ? v0_ : w / PER == 2 ? k1_ : v1_;
-                return arr + (w % PER) * 16384;
+                return arr + (w % PER) * BYTES;
             };
             __syncthreads();
             char* mine = place(wave);
             const uint32_t lane16 = here(lane * 16);
 #pragma unroll
-            for (int n = 0; n < 16; ++n) {
-                const f4 x = {st.acc[n / 4][4 * (n % 4)], st.acc[n / 4][4 * (n % 4) + 1],
-                              st.acc[n / 4][4 * (n % 4) + 2], st.acc[n / 4][4 * (n % 4) + 3]};
-                *(f4*)(mine + n * 1024 + lane16) = x;
-            }
-            if (half == 0) ml_[wave][lane] = make_float2(m, l);
+            for (int n = 0; n < T::QUADS; ++n) *(f4*)(mine + n * 1024 + lane16) = t.quad(n);
+            if (t.h == 0) ml_[wave][lane] = make_float2(m, l);
             __syncthreads();
             float top = neg_inf();
 #pragma unroll
-            for (int k = 0; k < WK; ++k) top = fmaxf(top, ml_[k * WR + rg][lane & 31].x);
+            for (int k = 0; k < WK; ++k) top = fmaxf(top, ml_[k * WR + rg][lane % ROWS].x);
             float sum = 0.f;
 #pragma unroll
             for (int n = 0; n < QUADS; ++n) y[n] = (f4){0.f, 0.f, 0.f, 0.f};
             for (int k = 0; k < WK; ++k) {
-                const float2 o = ml_[k * WR + rg][lane & 31];
+                const float2 o = ml_[k * WR + rg][lane % ROWS];
                 const float w = o.x == neg_inf() ? 0.f : fast_exp2(o.x - top);
                 // (a part that saw nothing holds zeros)
                 sum += w * o.y;
@@ -730,14 +767,11 @@ void tree_kernel(const TreeParams a) {
             }
             m = top;
             l = sum;
-            __syncthreads();                               // (before the next unit's loads)
         } else {
 #pragma unroll
-            for (int n = 0; n < QUADS; ++n)
-                y[n] = (f4){st.acc[n / 4][4 * (n % 4)], st.acc[n / 4][4 * (n % 4) + 1],
-                            st.acc[n / 4][4 * (n % 4) + 2], st.acc[n / 4][4 * (n % 4) + 3]};
-            __syncthreads();
+            for (int n = 0; n < QUADS; ++n) y[n] = t.quad(n);
         }
+        __syncthreads();                                   // (before the next unit's loads)
         const Row row = row_of();
         if (whole) {
             const bool seeing = row.is && row.node < nodes;
@@ -746,23 +780,22 @@ void tree_kernel(const TreeParams a) {
                 half_t* o = a.out + u.b * a.so_b + row.node * a.so_n + u.h * a.so_h + row.rep * a.so_r;
 #pragma unroll
                 for (int n = 0; n < QUADS; ++n) {
-                    const int quad = kg * QUADS + n;
                     h4 x;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) x[e] = seeing ? (half_t)(y[n][e] * inv) : (half_t)0.f;
-                    *(h4*)(o + 8 * quad + 4 * half) = x;
+                    *(h4*)(o + T::channel_of(kg * QUADS + n) + 4 * t.h) = x;
                 }
-                if (a.lse && kg == 0 && half == 0)
+                if (a.lse && kg == 0 && t.h == 0)
                     a.lse[((int64_t)(u.b * a.N + row.node) * a.H + u.h) * a.NR + row.rep] =
                         seeing && m != neg_inf()
                             ? (m - TREE_TOP + __builtin_amdgcn_logf(l)) * 0.69314718055994531f
                             : neg_inf();
             }
-        } else {
-            float* rec = a.work + ((((int64_t)g * 2 + (s0 == 0)) * a.row_tiles + rt) * WR + rg) * TREE_RECORD;
+        } else if (row.is) {
+            float* rec = a.work + ((((int64_t)g * 2 + (s0 == 0)) * a.row_tiles + rt) * WR + rg) * (ROWS * 130);
 #pragma unroll
             for (int n = 0; n < QUADS; ++n) *(f4*)(rec + (kg * QUADS + n) * 256 + lane * 4) = y[n];
-            if (kg == 0 && half == 0) *(float2*)(rec + 4096 + 2 * lane) = make_float2(m, l);
+            if (kg == 0 && t.h == 0) *(float2*)(rec + ROWS * 128 + 2 * lane) = make_float2(m, l);
         }
         if (s0 == 0 && rt == 0 && threadIdx.x == 0)
             a.info[u.b * a.H + u.h] =
@@ -771,39 +804,47 @@ void tree_kernel(const TreeParams a) {
     } while (next_unit(a, STEP, run, u));
 }
 
-// Records of a unit made its output: a workgroup a (unit, 32 rows, CQ channel quads), its
-// waves take the records in turn.
+// Records of a unit made its output: a workgroup a (unit, ROWS rows, CQ channel quads), its
+// waves take the records in turn, AHEAD at once.
 constexpr int COMBINE_NW = 8;
-template <int CQ>
+template <int ROWS, int CQ>
 __global__ __launch_bounds__(WAVE* COMBINE_NW) void tree_combine_kernel(const TreeParams a, int wr) {
+    constexpr int PARTS = ROWS / 2 / CQ, AHEAD = CQ == 1 ? 4 : 1;
     __shared__ float sums[COMBINE_NW][CQ * 4 + 2][WAVE];
-    const int parts = 16 / CQ, blocks = gridDim.y / parts;
-    const int unit = blockIdx.x, rb = blockIdx.y / parts, part = blockIdx.y % parts;
-    (void)blocks;
+    const int unit = blockIdx.x, rb = blockIdx.y / PARTS, part = blockIdx.y % PARTS;
     const int2 gs = a.info[unit];
     if (gs.x == gs.y) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE;
     const int rt = rb / wr, rg = rb % wr, count = gs.y - gs.x + 1;
     auto record = [&](int k) {
         const int64_t slot = (int64_t)(gs.x + k) * 2 + (k == 0);
-        return a.work + ((slot * a.row_tiles + rt) * wr + rg) * TREE_RECORD;
+        return a.work + ((slot * a.row_tiles + rt) * wr + rg) * (ROWS * 130);
     };
     float m = neg_inf(), l = 0.f;
     f4 y[CQ];
 #pragma unroll
     for (int n = 0; n < CQ; ++n) y[n] = (f4){0.f, 0.f, 0.f, 0.f};
-    for (int k = wave; k < count; k += COMBINE_NW) {
-        const float* rec = record(k);
-        const float2 o = *(const float2*)(rec + 4096 + 2 * (lane & 31));
-        f4 x[CQ];
+    for (int k0 = wave; k0 < count; k0 += COMBINE_NW * AHEAD) {
+        float2 o[AHEAD];
+        f4 x[AHEAD][CQ];
 #pragma unroll
-        for (int n = 0; n < CQ; ++n) x[n] = *(const f4*)(rec + (part * CQ + n) * 256 + lane * 4);
-        const float top = fmaxf(m, o.x), use = top == neg_inf() ? 0.f : top;
-        const float keep = fast_exp2(m - use), w = fast_exp2(o.x - use);
-        l = l * keep + o.y * w;
+        for (int i = 0; i < AHEAD; ++i) {
+            const int k = k0 + i * COMBINE_NW;
+            const float* rec = record(k < count ? k : k0);
+            o[i] = *(const float2*)(rec + ROWS * 128 + 2 * (lane % ROWS));
 #pragma unroll
-        for (int n = 0; n < CQ; ++n) y[n] = y[n] * keep + x[n] * w;
-        m = top;
+            for (int n = 0; n < CQ; ++n) x[i][n] = *(const f4*)(rec + (part * CQ + n) * 256 + lane * 4);
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (k0 + i * COMBINE_NW >= count) break;
+            const float top = fmaxf(m, o[i].x), use = top == neg_inf() ? 0.f : top;
+            const float keep = fast_exp2(m - use), w = fast_exp2(o[i].x - use);
+            l = l * keep + o[i].y * w;
+#pragma unroll
+            for (int n = 0; n < CQ; ++n) y[n] = y[n] * keep + x[i][n] * w;
+            m = top;
+        }
     }
 #pragma unroll
     for (int n = 0; n < CQ; ++n)
@@ -824,7 +865,7 @@ __global__ __launch_bounds__(WAVE* COMBINE_NW) void tree_combine_kernel(const Tr
 #pragma unroll
         for (int e = 0; e < 4; ++e) z[e] += f * sums[w][4 * wave + e][lane];
     }
-    const int row = rb * 32 + (lane & 31), half = lane >> 5;
+    const int row = rb * ROWS + lane % ROWS, h4_ = 4 * (lane / ROWS);
     if (row >= a.N * a.NR) return;
     const int node = row / a.NR, rep = row - node * a.NR, b = unit / a.H, h = unit - b * a.H;
     int nodes = a.N;
@@ -839,22 +880,28 @@ __global__ __launch_bounds__(WAVE* COMBINE_NW) void tree_combine_kernel(const Tr
     h4 x;
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = seeing ? (half_t)(z[e] * inv) : (half_t)0.f;
-    *(h4*)(a.out + b * a.so_b + node * a.so_n + h * a.so_h + rep * a.so_r + 8 * (part * CQ + wave) +
-           4 * half) = x;
-    if (a.lse && part == 0 && wave == 0 && half == 0)
+    *(h4*)(a.out + b * a.so_b + node * a.so_n + h * a.so_h + rep * a.so_r +
+           256 / ROWS * (part * CQ + wave) + h4_) = x;
+    if (a.lse && part == 0 && wave == 0 && lane < ROWS)
         a.lse[((int64_t)(b * a.N + node) * a.H + h) * a.NR + rep] =
             seeing && top != neg_inf()
                 ? (top - TREE_TOP + __builtin_amdgcn_logf(total)) * 0.69314718055994531f
                 : neg_inf();
 }
 
-template <int NW, int WR, int KB, bool SCORES>
+template <int ROWS, int NW, int WR, int KB, bool SCORES>
 hipError_t launch(const TreeParams& a, hipStream_t stream) {
-    tree_kernel<NW, WR, KB, SCORES><<<dim3(a.groups * a.row_tiles), dim3(WAVE * NW), 0, stream>>>(a);
+    tree_kernel<ROWS, NW, WR, KB, SCORES>
+        <<<dim3(a.groups * a.row_tiles), dim3(WAVE * NW), 0, stream>>>(a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const int blocks = (a.N * a.NR + 31) / 32;
-    tree_combine_kernel<4><<<dim3(a.B * a.H, blocks * 4), dim3(WAVE * COMBINE_NW), 0, stream>>>(a, WR);
+    // few of them: a quad a workgroup, so that the records are read by the whole chip
+    const int blocks = (a.N * a.NR + ROWS - 1) / ROWS, units = a.B * a.H;
+    const dim3 threads(WAVE * COMBINE_NW);
+    if (units * blocks * (ROWS / 8) >= 256)
+        tree_combine_kernel<ROWS, 4><<<dim3(units, blocks * (ROWS / 8)), threads, 0, stream>>>(a, WR);
+    else
+        tree_combine_kernel<ROWS, 1><<<dim3(units, blocks * (ROWS / 2)), threads, 0, stream>>>(a, WR);
     return hipGetLastError();
 }
 
@@ -864,10 +911,11 @@ constexpr int TREE_CUS = 256;
 
 TreeShape tree_shape(int batch, int kv_heads, int rows, int64_t keys_bound) {
     TreeShape s;
+    s.rows = rows <= 16 ? 16 : 32;
     s.wr = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
     s.nw = s.wr == 1 ? 4 : 8;
     s.kb = s.wr >= 4 ? 2 : 1;
-    s.row_tiles = (rows + 32 * s.wr - 1) / (32 * s.wr);
+    s.row_tiles = (rows + s.rows * s.wr - 1) / (s.rows * s.wr);
     const int64_t step = 32 * s.kb * (s.nw / s.wr);
     const int64_t units = (int64_t)batch * kv_heads;
     const int64_t places = units * ((keys_bound + step - 1) / step + TREE_EXTRA);
@@ -879,7 +927,7 @@ TreeShape tree_shape(int batch, int kv_heads, int rows, int64_t keys_bound) {
 }
 
 size_t tree_record_bytes(const TreeShape& s) {
-    return (size_t)s.groups * 2 * s.row_tiles * s.wr * TREE_RECORD * sizeof(float);
+    return (size_t)s.groups * 2 * s.row_tiles * s.wr * s.rows * 130 * sizeof(float);
 }
 
 hipError_t launch_tree_attention(const TreeParams& p, const TreeShape& s, hipStream_t stream) {
@@ -887,12 +935,13 @@ hipError_t launch_tree_attention(const TreeParams& p, const TreeShape& s, hipStr
     a.groups = s.groups;
     a.row_tiles = s.row_tiles;
     a.extra = TREE_EXTRA;
-    if (a.scores) return launch<4, 1, 1, true>(a, stream);
+    if (a.scores) return launch<16, 4, 1, 1, true>(a, stream);
     switch (s.wr) {
-        case 1: return launch<4, 1, 1, false>(a, stream);
-        case 2: return launch<8, 2, 1, false>(a, stream);
-        case 4: return launch<8, 4, 2, false>(a, stream);
-        default: return launch<8, 8, 2, false>(a, stream);
+        case 1: return s.rows == 16 ? launch<16, 4, 1, 1, false>(a, stream)
+                                    : launch<32, 4, 1, 1, false>(a, stream);
+        case 2: return launch<32, 8, 2, 1, false>(a, stream);
+        case 4: return launch<32, 8, 4, 2, false>(a, stream);
+        default: return launch<32, 8, 8, 2, false>(a, stream);
     }
 }
 

@@ -12,8 +12,8 @@
 // product (whose k order is free as long as V's is the same).
 //
 // K and V go to LDS by direct loads, whole rows of 256 bytes (16 lanes a row): K's 16-byte
-// piece p of key r at place p ^ (r % 16), V's 32-byte unit u of key r at u ^ (r % 8), so
-// that neither the row reads of K nor the transposing reads of V meet in a bank.
+// piece p of key r at place p ^ (r % 16), V's 32-byte units swapped by row too, so that
+// neither the row reads of K nor the transposing reads of V meet in a bank.
 #include "ls_common.h"
 #include "ls_tree.h"
 
@@ -29,11 +29,34 @@ namespace {
 // full precision down to 2^-21 of the running maximum's.
 constexpr float TREE_TOP = 7.f, TREE_LAZY = 8.f;
 
-// (buffer loads: after a global load to LDS the compiler waits for all LDS reads where it
-// needs one)
-typedef void __attribute__((address_space(3)))* lds_ptr;
-__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, uint32_t off, int soff, char* dst) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)dst, 16, off, soff, 0, 0);
+typedef char __attribute__((address_space(3)))* lds_ptr;
+
+// Sixteen bytes a lane from a resource to LDS at `to` + 16 lane (to: the same in every lane).
+// In assembly, since the compiler, where it knows of such a load, waits for all of them before
+// the next LDS read of the array; the waits are this file's own (wait_loads).  It writes no
+// register.  K and V are read once: the policy of the decode's page loads (against none:
+// a decode step of 16 x 16K 76.8 -> 69.5 us, 16 nodes of 16 x 16K 69.6 -> 68.2).
+__device__ __forceinline__ void load_to_lds(u4 rsrc, uint32_t off, uint32_t soff, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %3\n\t"
+                 "s_nop 0\n\t"
+                 "buffer_load_dwordx4 %0, %1, %2 offen sc0 nt lds"
+                 :: "v"(off), "s"(rsrc), "s"(soff), "s"(to) : "memory", "m0");
+}
+// Until at most N vector memory operations of this wave are outstanding.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+__device__ __forceinline__ u4 rsrc_of(const char* base, bool there) {
+    const uint64_t x = (uint64_t)base;
+    u4 r;
+    r.x = __builtin_amdgcn_readfirstlane((uint32_t)x);
+    r.y = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32) & 0xFFFFu);
+    r.z = __builtin_amdgcn_readfirstlane(there ? 0x7fffffffu : 0u);    // (none: no request)
+    r.w = 0x00020000u;
+    return r;
 }
 
 __device__ __forceinline__ u2 read_transposed(const char* p) {
@@ -68,10 +91,16 @@ struct Form<16> {
 // on 1 KB and a row is 256 bytes, so a swizzled place inside a row is one exclusive or:
 //   K of step j:         k ^ (16 HB j)     (piece HB j + h of key lane % ROWS)
 //   V of part c:         v ^ (256 / PARTS c)
-//   loads i of a page:   (4 i + lane / 16) rows, pieces k_in ^ (64 i), v_in ^ (128 (i % 2))
+//   loads i of a page:   (4 i + lane / 16) rows, pieces k_in ^ (64 i), v_in ^ v_turn(i)
+// V's unit u of row r lies at u ^ v_swap(r): a transposing read's 32 lanes take eight units
+// (of four rows, or of eight), which then lie in all eight places of a row's 256 bytes.
 struct LanePlaces {
     uint32_t k, v, k_in, v_in;
 };
+template <int ROWS>
+constexpr __device__ __forceinline__ int v_swap(int r) { return ROWS == 32 ? 2 * (r & 3) : r & 7; }
+template <int ROWS>
+constexpr __device__ __forceinline__ int v_turn(int i) { return ROWS == 32 ? 0 : 128 * (i & 1); }
 template <int ROWS>
 __device__ __forceinline__ LanePlaces lane_places(int lane) {
     LanePlaces p;
@@ -79,9 +108,9 @@ __device__ __forceinline__ LanePlaces lane_places(int lane) {
     p.k = key * 256 + 16 * (h ^ (key & 15));
     // a transposing read's 16 lanes take four keys' 16 channels and get a channel's four keys
     const int r = 4 * h + ((lane & 15) >> 2), unit = ROWS == 32 ? quarter & 1 : 0;
-    p.v = r * 256 + 32 * (unit ^ (r & 7)) + 8 * (lane & 3);
+    p.v = r * 256 + 32 * (unit ^ v_swap<ROWS>(r)) + 8 * (lane & 3);
     p.k_in = 16 * (pp ^ quarter);
-    p.v_in = 32 * ((pp >> 1) ^ quarter) + 16 * (pp & 1);
+    p.v_in = 32 * ((pp >> 1) ^ v_swap<ROWS>(quarter)) + 16 * (pp & 1);
     return p;
 }
 // The same value, made anew where it is used: what follows from it is computed there, not
@@ -518,10 +547,9 @@ void tree_kernel(const TreeParams a) {
     typedef Tile<ROWS, KB> T;
     constexpr int WK = NW / WR, KEYS = 32 * KB, STEP = KEYS * WK;
     constexpr int TILE = KEYS * 256;                       // bytes of K, and of V
-    __shared__ __attribute__((aligned(1024))) char k0_[WK * TILE];
-    __shared__ __attribute__((aligned(1024))) char v0_[WK * TILE];
-    __shared__ __attribute__((aligned(1024))) char k1_[WK * TILE];
-    __shared__ __attribute__((aligned(1024))) char v1_[WK * TILE];
+    // a step's tiles: K of every key group, then V; as many steps as 128 KB hold
+    constexpr int STEP_BYTES = 2 * WK * TILE, NBUF = 131072 / STEP_BYTES;
+    __shared__ __attribute__((aligned(1024))) char tiles_[NBUF * STEP_BYTES];
     __shared__ float2 ml_[NW][ROWS];
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE;
@@ -553,8 +581,6 @@ void tree_kernel(const TreeParams a) {
         return o;
     };
 
-    // this wave's part of a tile's loads: LOADS instructions of four rows, K and V each
-    constexpr int LOADS = KEYS / 4 / WR;
     const uint32_t row_in = (uint32_t)(lane >> 4) * (uint32_t)a.sp_t;
 
     do {
@@ -575,36 +601,62 @@ void tree_kernel(const TreeParams a) {
         const int32_t* table = a.tables + u.b * a.st_b;
         const int pages = (keys + PAGE - 1) / PAGE, last_page = pages > 0 ? pages - 1 : 0;
 
-        // Blocks of a step's tile, a lane a page (past the sequence's last page, it again: keys
-        // there do not count).
+        {
+            // (A lane past the last row takes the first one's: its results go nowhere.  Before the
+            // blocks: a wait for these does not then wait for the tiles.)
+            const Row row = row_of();
+            const half_t* p = a.q + u.b * a.sq_b + row.node * a.sq_n + u.h * a.sq_h +
+                              row.rep * a.sq_r + 8 * t.h;
+#pragma unroll
+            for (int j = 0; j < T::STEPS; ++j) t.q[j] = *(const u4*)(p + 8 * T::HB * j);
+        }
+        // Blocks of the pages of SPB steps' tiles, a lane a page (past the sequence's last page, it
+        // again: keys there do not count), and which of them are not in the pool.
+        constexpr int PPT = KEYS / PAGE, SPB = 64 / PPT;
         auto ids_of = [&](int step) {
             int i = (int)here(lane);
-            i = (step * WK + kg) * (KEYS / PAGE) + (i < KEYS / PAGE ? i : KEYS / PAGE - 1);
+            i = ((step + i / PPT) * WK + kg) * PPT + i % PPT;
             return table[i < pages ? i : last_page];
         };
-        // its pages that are not in the pool
-        auto bad_of = [&](int ids) {
-            return (uint32_t)__ballot((unsigned)ids >= (unsigned)a.num_blocks) & ((1u << (KEYS / PAGE)) - 1);
-        };
-        // (a page outside the pool is not requested: what its rows hold then counts as nothing)
-        auto load = [&](int z, int ids, char* to) {
+        int ids = ids_of(s0), ids_next = 0;
+        uint64_t bad = 0;
+        uint32_t bad_ring = 0;                             // 4 bits a step, the last eight
+        // this wave's part of a tile: LOADS instructions of four rows, K and V each
+        constexpr int LOADS = KEYS / 4 / WR;
+        const uint32_t lds = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_ptr)tiles_);
+        auto load = [&](int z, int step) {
             constexpr int SAME = LOADS < 4 ? LOADS : 4;    // instructions of one page
-            const uint32_t row = here(row_in), k_in = here(t.at.k_in), v_in = here(t.at.v_in);
+            const int at = (step - s0) % SPB * PPT;
+            const uint32_t to = lds + step % NBUF * STEP_BYTES + z * WK * TILE + kg * TILE;
+            const uint32_t row = here(row_in), in0 = here(z ? t.at.v_in : t.at.k_in);
 #pragma unroll
             for (int i0 = 0; i0 < LOADS; i0 += SAME) {
                 const int first = (rg * LOADS + i0) * 4;
-                const int id = __builtin_amdgcn_readlane(ids, first / PAGE);
+                const int id = __builtin_amdgcn_readlane(ids, at + first / PAGE);
+                // (a page outside the pool is not requested: what its rows hold counts as nothing)
                 const bool in = (unsigned)id < (unsigned)a.num_blocks;
-                const __amdgpu_buffer_rsrc_t from =
-                    page_rsrc(a.pool[z] + (in ? id : 0) * a.sp_b + u.h * a.sp_h, in);
+                const u4 from = rsrc_of(a.pool[z] + (in ? id : 0) * a.sp_b + u.h * a.sp_h, in);
 #pragma unroll
                 for (int i = 0; i < SAME; ++i) {
                     const int n = LOADS < 4 ? (rg * LOADS + i) & 3 : i;       // of the page's four
-                    const uint32_t off = z ? v_in ^ (128 * (n & 1)) : k_in ^ (64 * n);
-                    load_to_lds(from, row + off, 4 * n * (int)a.sp_t, to + (first + 4 * i) * 256);
+                    load_to_lds(from, row + (in0 ^ (z ? v_turn<ROWS>(n) : 64 * n)), 4 * n * (uint32_t)a.sp_t,
+                                to + (first + 4 * i) * 256);
                 }
             }
         };
+        // before a step's loads: its blocks at hand
+        auto blocks = [&](int step) {
+            const int n = step - s0;
+            if (n % SPB == 0) {
+                if (n) ids = ids_next;
+                bad = __ballot((unsigned)ids >= (unsigned)a.num_blocks);
+                if (step + SPB < s1) ids_next = ids_of(step + SPB);
+            }
+            const int sh = 4 * (step & 7);
+            bad_ring = (bad_ring & ~(15u << sh)) |
+                       ((uint32_t)(bad >> (n % SPB * PPT)) & ((1u << PPT) - 1)) << sh;
+        };
+        auto bad_of = [&](int step) { return bad_ring >> (4 * (step & 7)) & 15u; };
         // the scores of a tile (KB 1), in log2 units
         auto store_scores = [&](int64_t k0) {
             const int row = lane % ROWS;
@@ -638,7 +690,8 @@ void tree_kernel(const TreeParams a) {
         };
         // A step's products; false, with nothing done, where V holds an infinity or a NaN that a row
         // may not see.
-        auto add_step = [&](int step, bool masked, const char* kt, char* vt) {
+        // (k_read: what is done once K has been read)
+        auto add_step = [&](int step, bool masked, char* kt, char* vt, auto&& k_read) {
             if (!works) return true;
             t.scores(kt);
             if (masked) {
@@ -647,81 +700,121 @@ void tree_kernel(const TreeParams a) {
                 for (int z = 0; z < KB; ++z) clear_values(vt + z * 8192, z ? live[KB - 1] : live[0], lane);
                 if (t.odd(vt)) return false;
             }
+            k_read();
             if constexpr (SCORES) store_scores(((int64_t)step * WK + kg) * KEYS);
             t.weights(a.scale2);
             t.values(vt);
             return true;
         };
-        auto add_step_by_row = [&](int step, const char* kt, const char* vt) {
+        auto add_step_by_row = [&](int step, char* kt, const char* vt, auto&& k_read) {
             t.scores(kt);
             t.mask(bits);
+            k_read();
             if constexpr (SCORES) store_scores(((int64_t)step * WK + kg) * KEYS);
             t.weights(a.scale2);
             t.values_by_row(vt, bits);
         };
 
-        char* const kt0 = k0_ + kg * TILE;
-        char* const vt0 = v0_ + kg * TILE;
-        char* const kt1 = k1_ + kg * TILE;
-        char* const vt1 = v1_ + kg * TILE;
         // steps of the context alone, then the others
         const int plain = (ctx < keys ? ctx : keys) / STEP;
         const int sf = s1 < plain ? s1 : plain;
-        int ids = ids_of(s0);
-        {
-            // (a lane past the last row takes the first one's: its results go nowhere)
-            const Row row = row_of();
-            const half_t* p = a.q + u.b * a.sq_b + row.node * a.sq_n + u.h * a.sq_h +
-                              row.rep * a.sq_r + 8 * t.h;
-#pragma unroll
-            for (int j = 0; j < T::STEPS; ++j) t.q[j] = *(const u4*)(p + 8 * T::HB * j);
-        }
         t.clear();
-        uint32_t bad = bad_of(ids);
-        load(0, ids, kt0);
-        load(1, ids, vt0);
-        ids = s0 + 1 < s1 ? ids_of(s0 + 1) : 0;
-        bool masked;
-        // a step's loads have come and everyone is done with the step before: the next
-        // one's go out
-        auto turn = [&](int step, char* kn, char* vn) {
-            masked = step >= sf || bad != 0;
-            if (masked) look(step, bad);                   // (its loads come with the tile's)
-            wait_vm_lds<0>();
-            if constexpr (WR > 1) {
-                __syncthreads();
-            } else {                                       // (a tile of the wave's own)
-                __builtin_amdgcn_s_waitcnt(0xC07F);        // lgkmcnt 0
-                asm volatile("" ::: "memory");
-            }
-            if (step + 1 < s1) {
-                bad = bad_of(ids);
-                load(0, ids, kn);
-                load(1, ids, vn);
-                if (step + 2 < s1) ids = ids_of(step + 2);
-            }
-        };
-        // (A step of infinities leaves the loop for its products by row and comes back: as a branch
-        // inside it, it would cost every step copies of the sums.)
         int step = s0;
-        bool second = false;                               // which buffers hold the step
-        while (true) {
+        bool masked;
+        char *kt, *vt;
+        auto at_step = [&] {
+            kt = tiles_ + step % NBUF * STEP_BYTES + kg * TILE;
+            vt = kt + WK * TILE;
+        };
+        if constexpr (WR > 1) {
+            // Tiles that row groups share: AHEAD steps are requested; a step's loads have come
+            // and everyone is done with the step before, whose place then takes the next.
+            constexpr int AHEAD = NBUF - 1;
+            for (int i = s0; i < s0 + AHEAD && i < s1; ++i) {
+                blocks(i);
+                load(0, i);
+                load(1, i);
+            }
+            auto turn = [&] {
+                const uint32_t b = bad_of(step);
+                masked = step >= sf || b != 0;
+                if (masked) look(step, b);                 // (its loads come with the tile's)
+                if (AHEAD > 1 && step + AHEAD <= s1)
+                    wait_loads<2 * LOADS*(AHEAD - 1)>();
+                else
+                    wait_loads<0>();
+                __syncthreads();
+                if (step + AHEAD < s1) {
+                    blocks(step + AHEAD);
+                    load(0, step + AHEAD);
+                    load(1, step + AHEAD);
+                }
+                at_step();
+            };
+            auto none = [] {};
+            // (A step of infinities leaves the loop for its products by row and comes back: as a
+            // branch inside it, it would cost every step copies of the sums.)
             while (true) {
-                if (!second) {
-                    turn(step, kt1, vt1);
-                    if (!add_step(step, masked, kt0, vt0)) break;
-                    second = true;
+                while (true) {
+                    turn();
+                    if (!add_step(step, masked, kt, vt, none)) break;
                     if (++step >= s1) break;
                 }
-                turn(step, kt0, vt0);
-                if (!add_step(step, masked, kt1, vt1)) break;
-                second = false;
+                if (step >= s1) break;
+                add_step_by_row(step, kt, vt, none);
                 if (++step >= s1) break;
             }
-            if (step >= s1) break;
-            add_step_by_row(step, second ? kt1 : kt0, second ? vt1 : vt0);
-            second = !second;
-            if (++step >= s1) break;
+        } else {
+            // Tiles of the wave's own: nobody to wait for, and a tile's K and V are replaced by
+            // those two steps on as soon as each has been read, so that a wave waits with
+            // two tiles requested.
+            static_assert(NBUF == 2, "");
+            auto reads_done = [&] {
+                __builtin_amdgcn_s_waitcnt(0xC07F);        // lgkmcnt 0
+                asm volatile("" ::: "memory");
+            };
+            blocks(s0);
+            load(0, s0);
+            load(1, s0);
+            if (s0 + 1 < s1) {
+                blocks(s0 + 1);
+                load(0, s0 + 1);
+                load(1, s0 + 1);
+            }
+            auto turn = [&] {
+                const uint32_t b = bad_of(step);
+                masked = step >= sf || b != 0;
+                if (masked) look(step, b);
+                // (behind the step's own: the next one's 2 LOADS, and maybe more)
+                if (step + 1 < s1)
+                    wait_loads<2 * LOADS>();
+                else
+                    wait_loads<0>();
+                at_step();
+            };
+            auto next_k = [&] {
+                reads_done();
+                if (step + 2 < s1) {
+                    blocks(step + 2);
+                    load(0, step + 2);
+                }
+            };
+            auto next_v = [&] {
+                reads_done();
+                if (step + 2 < s1) load(1, step + 2);
+            };
+            while (true) {
+                while (true) {
+                    turn();
+                    if (!add_step(step, masked, kt, vt, next_k)) break;
+                    next_v();
+                    if (++step >= s1) break;
+                }
+                if (step >= s1) break;
+                add_step_by_row(step, kt, vt, next_k);
+                next_v();
+                if (++step >= s1) break;
+            }
         }
 
         // ---- the key groups' results made one, then the output or a record ----
@@ -736,12 +829,8 @@ void tree_kernel(const TreeParams a) {
         constexpr int QUADS = T::QUADS / WK;               // of the row group's, this wave's
         f4 y[QUADS];
         if constexpr (WK > 1) {
-            // over the tiles' arrays
-            constexpr int BYTES = T::QUADS * 1024, PER = WK * TILE / BYTES;
-            auto place = [&](int w) -> char* {
-                char* arr = w / PER == 0 ? k0_ : w / PER == 1 ? v0_ : w / PER == 2 ? k1_ : v1_;
-                return arr + (w % PER) * BYTES;
-            };
+            // over the tiles
+            auto place = [&](int w) { return tiles_ + w * (T::QUADS * 1024); };
             __syncthreads();
             char* mine = place(wave);
             const uint32_t lane16 = here(lane * 16);
@@ -913,7 +1002,7 @@ TreeShape tree_shape(int batch, int kv_heads, int rows, int64_t keys_bound) {
     TreeShape s;
     s.rows = rows <= 16 ? 16 : 32;
     s.wr = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
-    s.nw = s.wr == 1 ? 4 : 8;
+    s.nw = s.wr <= 2 ? 4 : 8;
     s.kb = s.wr >= 4 ? 2 : 1;
     s.row_tiles = (rows + s.rows * s.wr - 1) / (s.rows * s.wr);
     const int64_t step = 32 * s.kb * (s.nw / s.wr);
@@ -939,7 +1028,7 @@ hipError_t launch_tree_attention(const TreeParams& p, const TreeShape& s, hipStr
     switch (s.wr) {
         case 1: return s.rows == 16 ? launch<16, 4, 1, 1, false>(a, stream)
                                     : launch<32, 4, 1, 1, false>(a, stream);
-        case 2: return launch<32, 8, 2, 1, false>(a, stream);
+        case 2: return launch<32, 4, 2, 1, false>(a, stream);
         case 4: return launch<32, 8, 4, 2, false>(a, stream);
         default: return launch<32, 8, 8, 2, false>(a, stream);
     }

@@ -385,7 +385,8 @@ int ls_select_tokens(const float* sums, const int64_t* sum_strides, int64_t sum_
     if (int rc = check_batch(batch, kv_heads)) return rc;
     if (layers < 0 || (int64_t)layers * batch * kv_heads >= 1LL << 22)
         return fail(LS_ERR_INVALID, "layers x batch x kv_heads must be below 2^22");
-    if (sum_len < 0) return fail(LS_ERR_INVALID, "sum_len must be >= 0");
+    if (sum_len < 0 || sum_len > (int64_t)1 << 30)
+        return fail(LS_ERR_INVALID, "sum_len must be in [0, 2^30], got %lld", (long long)sum_len);
     for (int i = 0; i < 3; ++i)
         if (sum_strides[i] < 0) return fail(LS_ERR_INVALID, "rows of sums must not run backwards");
     if (budget < 1 || sinks < 0 || recent < 0 || (int64_t)sinks + recent > budget)

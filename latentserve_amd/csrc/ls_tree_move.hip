@@ -37,10 +37,11 @@ __global__ __launch_bounds__(TREE_MAX_NODES) void tree_masks_kernel(const int32_
 
 // ---- moves --------------------------------------------------------------------------
 //
-// The kept rows of a (pool, sequence, head) move down to the front: row keep[j] to j, keep
-// ascending, so keep[j] >= j.  A workgroup moves one such list in order, some rows at a
-// time: all of a round's rows are in registers before one is stored, and what a round
-// stores lies before every row that a later round reads.
+// Kept rows of a (pool, sequence, head) move down to the front: row keep[j] to j, keep
+// ascending, so keep[j] >= j.  A workgroup moves such a list in rounds, each of some rows:
+// a round is stored once all its rows and those of the rounds before have arrived in
+// registers, and what it stores lies before every row that a later round reads, so the
+// next round's rows are requested first.
 
 struct RowPlaces {
     const int32_t* table;
@@ -91,15 +92,75 @@ __device__ __forceinline__ void move_rows(char* head, const RowPlaces& place, in
     }
 }
 
-__global__ __launch_bounds__(MOVE_THREADS) void move_tokens_kernel(const MoveParams a) {
-    const int pool = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-    const int len = a.lens[b];
-    const int n = len < a.budget ? len : a.budget;
+// A list is cut into slices of its rows' bytes, each a workgroup's own: LANES threads of 16
+// bytes a row, AHEAD rows a thread and round.  A round's rows are requested when the one
+// before has arrived, their places a round earlier, from pages that were looked up two
+// rounds earlier, from entries of keep loaded three rounds earlier: nothing waits for more
+// than one trip to memory a round.
+constexpr int LIST_THREADS = 1024;
+
+template <int LANES, int AHEAD>
+__global__ __launch_bounds__(LIST_THREADS) void move_tokens_kernel(const MoveParams a, int pools,
+                                                                   int64_t first_list) {
+    constexpr int PASS = LIST_THREADS / LANES, ROUND = PASS * AHEAD, SLICES = 16 / LANES;
+    static_assert(ROUND <= LIST_THREADS, "a thread looks one row's places up");
+    __shared__ int64_t from_s[4][ROUND], to_s[4][ROUND];
+    // the slices of a list share an XCD's cache: the lines of a row are theirs together
+    const int id = blockIdx.x;
+    const int64_t list = first_list + id / (8 * SLICES) * 8 + id % 8;
+    if (list >= (int64_t)pools * a.H * a.B) return;
+    const int pool = list % pools, h = list / pools % a.H, b = list / pools / a.H;
+    int n = a.lens[b];
+    n = n < a.budget ? n : a.budget;
+    n = n < a.max_pages * PAGE ? n : a.max_pages * PAGE;   // (at most 2^28)
     if (n <= 0) return;
+    const int t = threadIdx.x, first = t / LANES;
     const int32_t* keep =
         a.keep + (((int64_t)(a.first_layer + pool / 2) * a.B + b) * a.H + h) * a.budget;
-    const RowPlaces place = {a.tables + b * a.st_b, a.st_b, a.sp_b, a.sp_t, a.max_pages, a.num_blocks};
-    move_rows(a.pool[pool] + h * a.sp_h, place, 0, n, [&](int j) { return keep[j]; });
+    const int32_t* const table = a.tables + b * a.st_b;
+    char* const head = a.pool[pool] + h * a.sp_h + 16 * (LANES * (id / 8 % SLICES) + t % LANES);
+    const int rounds = (n + ROUND - 1) / ROUND;
+    u4 x[2][AHEAD];
+    int k_new = -1, k_old = -1, page_from = -1, page_to = -1;
+    // what a round that is not there would move is nothing: its k is -1
+    auto step = [&](int r, u4 (&mine)[AHEAD], u4 (&next)[AHEAD]) {
+        if (t < ROUND) {
+            const int j2 = (r + 2) * ROUND + t;
+            const bool moves = (unsigned)page_from < (unsigned)a.num_blocks &&
+                               (unsigned)page_to < (unsigned)a.num_blocks;
+            from_s[(r + 2) & 3][t] = moves ? page_from * a.sp_b + k_old % PAGE * a.sp_t : 0;
+            to_s[(r + 2) & 3][t] = moves ? page_to * a.sp_b + j2 % PAGE * a.sp_t : -1;
+            const int j3 = j2 + ROUND, j4 = j3 + ROUND;
+            page_from = page_to = -1;
+            k_old = k_new;
+            if (j3 >= 0 && k_new > j3 && k_new / PAGE < a.max_pages) {      // (k = j: it is there)
+                page_from = table[k_new / PAGE];
+                page_to = table[j3 / PAGE];
+            }
+            k_new = j4 < n ? keep[j4] : -1;
+        }
+        if (r >= -1) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i)
+                next[i] = *(const u4*)(head + from_s[(r + 1) & 3][i * PASS + first]);
+        }
+        if (r >= 0) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) asm volatile("" : "+v"(mine[i])::"memory");
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (r >= 0) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const int64_t to = to_s[r & 3][i * PASS + first];
+                if (to >= 0) *(u4*)(head + to) = mine[i];
+            }
+        }
+    };
+    for (int r = -4; r < rounds; r += 2) {
+        step(r, x[0], x[1]);
+        step(r + 1, x[1], x[0]);
+    }
 }
 
 // One workgroup a (pool, head, sequence), each of which walks its sequence's tree itself: a
@@ -161,22 +222,23 @@ __global__ __launch_bounds__(MOVE_THREADS) void accept_tokens_kernel(const MoveP
 
 // ---- selection ------------------------------------------------------------------------
 //
-// The kept sums of a row are found by their bits, eight at a time from the top: how many
-// have each value of the eight among those that agree in the bits before, until the
-// smallest kept value is known; then one pass in order writes what is larger, and as
-// many equal ones, lowest positions first, as there is room for.
+// The kept sums of a row are found by their bits, eleven at a time from the top: how many
+// have each value of the eleven among those that agree in the bits before, until the
+// smallest kept value is known; then, in order, what is larger is kept, and as many equal
+// ones, lowest positions first, as there is room for.  A wave has a run of the row to
+// itself: it counts what it keeps, and writes it once the waves before have counted.
 
-constexpr int SELECT_THREADS = 1024, SELECT_WAVES = SELECT_THREADS / WAVE;
+constexpr int SELECT_THREADS = 1024, SELECT_WAVES = SELECT_THREADS / WAVE, DIGITS = 2048;
 
-// A sum's rank: larger sums have larger ranks, NaN the largest but for those always kept.
+// A sum's rank: larger sums have larger ranks, NaN the largest.
 __device__ __forceinline__ uint32_t rank_of(float x) {
-    if (x != x) return 0xFFFFFFFEu;
+    if (x != x) return 0xFFFFFFFFu;
     const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.f);      // (-0 is 0)
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
 __global__ __launch_bounds__(SELECT_THREADS) void select_tokens_kernel(const SelectParams a) {
-    __shared__ int hist[256];
+    __shared__ int hist[DIGITS];
     __shared__ int wave_sum[SELECT_WAVES][2];
     __shared__ int found[2];
     const int row = blockIdx.x, h = row % a.H, b = row / a.H % a.B, l = row / a.H / a.B;
@@ -195,65 +257,98 @@ __global__ __launch_bounds__(SELECT_THREADS) void select_tokens_kernel(const Sel
         return;
     }
     const int tail = len - a.recent;
-    auto rank = [&](int t) {
-        return t < a.sinks || t >= tail ? 0xFFFFFFFFu : rank_of(sums[t]);
+    // the wave's run, and what f does with WAVE of its sums at a time; some are on their way
+    const int per = ((len + SELECT_WAVES - 1) / SELECT_WAVES + WAVE - 1) / WAVE * WAVE;
+    const int t0 = wave * per, t1 = t0 + per < len ? t0 + per : len;
+    auto each = [&](auto f) {
+        constexpr int U = 8;
+        for (int t = t0 + lane; t - lane < t1; t += U * WAVE) {
+            float x[U];
+#pragma unroll
+            for (int i = 0; i < U; ++i) x[i] = t + i * WAVE < t1 ? sums[t + i * WAVE] : 0.f;
+#pragma unroll
+            for (int i = 0; i < U; ++i)
+                if (t - lane + i * WAVE < t1) f(t + i * WAVE, x[i]);
+        }
     };
-    uint32_t prefix = 0;
-    int want = a.budget;                                   // to be kept of those that agree
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = threadIdx.x; i < 256; i += SELECT_THREADS) hist[i] = 0;
-        __syncthreads();
-        for (int t = threadIdx.x; t < len; t += SELECT_THREADS) {
-            const uint32_t r = rank(t);
-            if (shift == 24 || (r >> (shift + 8)) == (prefix >> (shift + 8)))
-                atomicAdd(&hist[(r >> shift) & 255], 1);
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            int above = 0, v = 255;
-            while (v > 0 && above + hist[v] < want) above += hist[v--];
-            found[0] = v;
-            found[1] = above;
-        }
-        __syncthreads();
-        prefix |= (uint32_t)found[0] << shift;
-        want -= found[1];
-        __syncthreads();
-    }
-    // larger ranks, and the first `want` of equal rank
-    int base = 0, ties = 0;
-    for (int t0 = 0; t0 < len; t0 += SELECT_THREADS) {
-        const int t = t0 + threadIdx.x;
-        const uint32_t r = t < len ? rank(t) : 0;
-        const bool over = t < len && r > prefix, tie = t < len && r == prefix;
-        const uint64_t bo = __ballot(over), bt = __ballot(tie);
-        const uint64_t below = (1ull << lane) - 1;
-        if (lane == 0) {
-            wave_sum[wave][0] = __builtin_popcountll(bo);
-            wave_sum[wave][1] = __builtin_popcountll(bt);
-        }
-        __syncthreads();
-        int o = base, e = ties, all_o = 0, all_t = 0;
-        for (int w = 0; w < SELECT_WAVES; ++w) {
-            if (w < wave) {
-                o += wave_sum[w][0];
-                e += wave_sum[w][1];
+    uint32_t prefix = 0xFFFFFFFFu;
+    int want = a.budget - a.sinks - a.recent;              // of those that may go
+    if (want > 0) {
+        uint32_t known = 0;
+        prefix = 0;
+        for (int shift = 21; shift >= 0; shift = shift == 21 ? 10 : shift - 10) {
+            const uint32_t digit = shift ? 2047 : 1023;
+            for (int i = threadIdx.x; i < DIGITS; i += SELECT_THREADS) hist[i] = 0;
+            __syncthreads();
+            each([&](int t, float x) {
+                const uint32_t r = rank_of(x);
+                if (t >= a.sinks && t < tail && (r & known) == prefix)
+                    atomicAdd(&hist[(r >> shift) & digit], 1);
+            });
+            __syncthreads();
+            // from the top: the value that the last kept one has, and how many are above
+            if (wave == 0) {
+                constexpr int MINE = DIGITS / WAVE;
+                const int top = DIGITS - 1 - lane * MINE;
+                int count = 0;
+                for (int i = 0; i < MINE; ++i) count += hist[top - i];
+                int upto = count;
+                for (int d = 1; d < WAVE; d *= 2) {
+                    const int o = __shfl_up(upto, d);
+                    if (lane >= d) upto += o;
+                }
+                int above = upto - count;
+                if (above < want && want <= upto) {        // (one lane's)
+                    int i = 0;
+                    while (above + hist[top - i] < want) above += hist[top - i++];
+                    found[0] = top - i;
+                    found[1] = above;
+                }
             }
-            all_o += wave_sum[w][0];
-            all_t += wave_sum[w][1];
+            __syncthreads();
+            prefix |= (uint32_t)found[0] << shift;
+            known |= digit << shift;
+            want -= found[1];
         }
-        o += __builtin_popcountll(bo & below);
-        e += __builtin_popcountll(bt & below);
-        // what is kept before t: the larger ones, and of the equal ones as many as count
-        const int at = o + (e < want ? e : want);
-        if (over || (tie && e < want)) {
-            keep[at] = t;
-            kept[at] = sums[t];
-        }
-        base += all_o;
-        ties += all_t;
-        __syncthreads();
     }
+    // larger ranks and what is always kept, and the first `want` of equal rank
+    int over_n = 0, tie_n = 0;
+    auto over = [&](int t, uint32_t r) {
+        return t < t1 && (t < a.sinks || t >= tail || r > prefix);
+    };
+    auto tie = [&](int t, uint32_t r) {
+        return t < t1 && t >= a.sinks && t < tail && r == prefix;
+    };
+    each([&](int t, float x) {
+        const uint32_t r = rank_of(x);
+        over_n += __builtin_popcountll(__ballot(over(t, r)));
+        tie_n += __builtin_popcountll(__ballot(tie(t, r)));
+    });
+    if (lane == 0) {
+        wave_sum[wave][0] = over_n;
+        wave_sum[wave][1] = tie_n;
+    }
+    __syncthreads();
+    int o = 0, e = 0;
+    for (int w = 0; w < wave; ++w) {
+        o += wave_sum[w][0];
+        e += wave_sum[w][1];
+    }
+    each([&](int t, float x) {
+        const uint32_t r = rank_of(x);
+        const bool is_over = over(t, r), is_tie = tie(t, r);
+        const uint64_t bo = __ballot(is_over), bt = __ballot(is_tie);
+        const uint64_t below = (1ull << lane) - 1;
+        const int before = e + __builtin_popcountll(bt & below);
+        // what is kept before t: the larger ones, and of the equal ones as many as count
+        const int at = o + __builtin_popcountll(bo & below) + (before < want ? before : want);
+        if (is_over || (is_tie && before < want)) {
+            keep[at] = t;
+            kept[at] = x;
+        }
+        o += __builtin_popcountll(bo);
+        e += __builtin_popcountll(bt);
+    });
 }
 
 }  // namespace
@@ -265,7 +360,22 @@ hipError_t launch_tree_masks(const int32_t* parents, uint64_t* masks, int32_t* d
 }
 
 hipError_t launch_move_tokens(const MoveParams& a, int pools, hipStream_t stream) {
-    move_tokens_kernel<<<dim3(pools, a.H, a.B), dim3(MOVE_THREADS), 0, stream>>>(a);
+    const int64_t lists = (int64_t)pools * a.H * a.B;
+    auto go = [&](auto kernel, int slices) {
+        constexpr int64_t MOST = 1 << 18;                  // lists of a launch
+        for (int64_t at = 0; at < lists; at += MOST) {
+            const int64_t n = lists - at < MOST ? lists - at : MOST;
+            kernel<<<dim3((unsigned)((n + 7) / 8 * 8 * slices)), dim3(LIST_THREADS), 0, stream>>>(
+                a, pools, at);
+        }
+    };
+    // few lists: in narrower slices, so that more of the chip moves them
+    if (lists >= 96)
+        go(move_tokens_kernel<8, 4>, 2);
+    else if (lists >= 32)
+        go(move_tokens_kernel<4, 4>, 4);
+    else
+        go(move_tokens_kernel<2, 2>, 8);
     return hipGetLastError();
 }
 

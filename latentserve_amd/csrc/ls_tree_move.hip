@@ -228,7 +228,8 @@ __global__ __launch_bounds__(MOVE_THREADS) void accept_tokens_kernel(const MoveP
 // ones, lowest positions first, as there is room for.  A wave has a run of the row to
 // itself: it counts what it keeps, and writes it once the waves before have counted.
 
-constexpr int SELECT_THREADS = 1024, SELECT_WAVES = SELECT_THREADS / WAVE, DIGITS = 2048;
+constexpr int SELECT_THREADS = 1024, SELECT_WAVES = SELECT_THREADS / WAVE;
+constexpr int DIGITS = 2 * SELECT_THREADS;
 
 // A sum's rank: larger sums have larger ranks, NaN the largest.
 __device__ __forceinline__ uint32_t rank_of(float x) {
@@ -260,15 +261,24 @@ __global__ __launch_bounds__(SELECT_THREADS) void select_tokens_kernel(const Sel
     // the wave's run, and what f does with WAVE of its sums at a time; some are on their way
     const int per = ((len + SELECT_WAVES - 1) / SELECT_WAVES + WAVE - 1) / WAVE * WAVE;
     const int t0 = wave * per, t1 = t0 + per < len ? t0 + per : len;
+    constexpr int U = 8;
+    float x[U];
+    auto load = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) x[i] = t + i * WAVE < t1 ? sums[t + i * WAVE] : 0.f;
+    };
+    auto use = [&](int t, auto f) {
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (t - lane + i * WAVE < t1) f(t + i * WAVE, x[i]);
+    };
+    const bool held = per <= U * WAVE;                     // (rows of up to 8K: loaded once)
+    load(t0 + lane);
     auto each = [&](auto f) {
-        constexpr int U = 8;
+        if (held) return use(t0 + lane, f);
         for (int t = t0 + lane; t - lane < t1; t += U * WAVE) {
-            float x[U];
-#pragma unroll
-            for (int i = 0; i < U; ++i) x[i] = t + i * WAVE < t1 ? sums[t + i * WAVE] : 0.f;
-#pragma unroll
-            for (int i = 0; i < U; ++i)
-                if (t - lane + i * WAVE < t1) f(t + i * WAVE, x[i]);
+            load(t);
+            use(t, f);
         }
     };
     uint32_t prefix = 0xFFFFFFFFu;
@@ -277,7 +287,7 @@ __global__ __launch_bounds__(SELECT_THREADS) void select_tokens_kernel(const Sel
         uint32_t known = 0;
         prefix = 0;
         for (int shift = 21; shift >= 0; shift = shift == 21 ? 10 : shift - 10) {
-            const uint32_t digit = shift ? 2047 : 1023;
+            const uint32_t digit = shift ? DIGITS - 1 : DIGITS / 2 - 1;
             for (int i = threadIdx.x; i < DIGITS; i += SELECT_THREADS) hist[i] = 0;
             __syncthreads();
             each([&](int t, float x) {
@@ -286,24 +296,23 @@ __global__ __launch_bounds__(SELECT_THREADS) void select_tokens_kernel(const Sel
                     atomicAdd(&hist[(r >> shift) & digit], 1);
             });
             __syncthreads();
-            // from the top: the value that the last kept one has, and how many are above
-            if (wave == 0) {
-                constexpr int MINE = DIGITS / WAVE;
-                const int top = DIGITS - 1 - lane * MINE;
-                int count = 0;
-                for (int i = 0; i < MINE; ++i) count += hist[top - i];
-                int upto = count;
-                for (int d = 1; d < WAVE; d *= 2) {
-                    const int o = __shfl_up(upto, d);
-                    if (lane >= d) upto += o;
-                }
-                int above = upto - count;
-                if (above < want && want <= upto) {        // (one lane's)
-                    int i = 0;
-                    while (above + hist[top - i] < want) above += hist[top - i++];
-                    found[0] = top - i;
-                    found[1] = above;
-                }
+            // from the top, two values a thread: where the last kept one is, and how many
+            // are above
+            const int top = DIGITS - 1 - 2 * threadIdx.x;
+            const int first = hist[top], count = first + hist[top - 1];
+            int upto = count;
+            for (int d = 1; d < WAVE; d *= 2) {
+                const int o = __shfl_up(upto, d);
+                if (lane >= d) upto += o;
+            }
+            if (lane == WAVE - 1) wave_sum[wave][0] = upto;
+            __syncthreads();
+            for (int w = 0; w < wave; ++w) upto += wave_sum[w][0];
+            const int above = upto - count;
+            if (above < want && want <= upto) {            // (one thread's)
+                const bool second = above + first < want;
+                found[0] = top - second;
+                found[1] = above + (second ? first : 0);
             }
             __syncthreads();
             prefix |= (uint32_t)found[0] << shift;
@@ -370,10 +379,8 @@ hipError_t launch_move_tokens(const MoveParams& a, int pools, hipStream_t stream
         }
     };
     // few lists: in narrower slices, so that more of the chip moves them
-    if (lists >= 96)
+    if (lists >= 64)
         go(move_tokens_kernel<8, 4>, 2);
-    else if (lists >= 32)
-        go(move_tokens_kernel<4, 4>, 4);
     else
         go(move_tokens_kernel<2, 2>, 8);
     return hipGetLastError();

@@ -9,6 +9,8 @@ versioned apart; errors, strides and streams go through ``_lib``, scratch throug
 from __future__ import annotations
 
 import ctypes
+import functools
+import operator
 from typing import List, Optional
 
 import torch
@@ -172,24 +174,29 @@ def apart(name: str, out: torch.Tensor, q: torch.Tensor) -> None:
 
 
 def pool_lists(k_pools, v_pools):
-    """(heads, blocks, strides, device, two C arrays of addresses) of checked layers' pools."""
-    if len(k_pools) != len(v_pools):
-        raise ValueError(f"{len(k_pools)} K pools for {len(v_pools)} V pools")
+    """(heads, blocks, strides, device, two C arrays of addresses) of checked layers' pools
+    that are written to."""
+    n = len(k_pools)
+    if n != len(v_pools):
+        raise ValueError(f"{n} K pools for {len(v_pools)} V pools")
     first = k_pools[0]
     h, nb, steps = pool("a pool", first)
-    shape, st, device = first.shape, first.stride(), first.get_device()
-    for t in (*k_pools, *v_pools):
-        if t.shape != shape or t.dtype is not torch.float16 or t.stride() != st \
-                or t.get_device() != device or t.data_ptr() & 15:
-            raise ValueError("the layers' pools must be alike: float16 "
-                             f"{tuple(shape)}, of the same strides, on one device")
+    pools = [*k_pools, *v_pools]
+    # (an attribute of all at a time: half the host time of a loop over 56 pools)
+    at = list(map(torch.Tensor.data_ptr, pools))
+    if len(set(map(torch.Tensor.size, pools))) > 1 or len(set(map(torch.Tensor.stride, pools))) > 1 \
+            or len(set(map(torch.Tensor.get_device, pools))) > 1 \
+            or any([t.dtype is not torch.float16 for t in pools]) or functools.reduce(operator.or_, at) & 15:
+        raise ValueError("the layers' pools must be alike: float16 "
+                         f"{tuple(first.shape)}, of the same strides, on one device")
+    st = first.stride()
     if nb > 1 and st[0] < PAGE * h * HEAD_DIM or st[1] < h * HEAD_DIM \
             or (h > 1 and st[2] < HEAD_DIM):
         raise ValueError("pools whose rows overlap cannot be written")
-    n = len(k_pools)
+    if torch.is_grad_enabled() and any([t.requires_grad for t in pools]):
+        raise ValueError("a move of cached tokens records no gradient")
     array = ctypes.c_void_p * n
-    return h, nb, steps, first.device, array(*map(torch.Tensor.data_ptr, k_pools)), \
-        array(*map(torch.Tensor.data_ptr, v_pools))
+    return h, nb, steps, first.device, array(*at[:n]), array(*at[n:])
 
 
 # Workspace bytes by a call's sizes.

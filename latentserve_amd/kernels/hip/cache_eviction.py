@@ -213,22 +213,28 @@ def move_tokens(keep: torch.Tensor, k_pools: Sequence[torch.Tensor],
                          f"V pools, got {tuple(keep.shape)}")
     if layers == 0:
         return
-    h, nb, steps, dev, kp, vp = _tree.pool_lists(k_pools, v_pools)
-    index = k_pools[0].get_device()
+    lists = _tree.pool_lists(k_pools, v_pools)
     _, b, _, budget = keep.shape
-    ptr = _tree.whole("keep", keep, torch.int32, (layers, b, h, budget), index)
+    index = k_pools[0].get_device()
+    _tree.whole("keep", keep, torch.int32, (layers, b, lists[0], budget), index)
     width = _tree.tables(block_tables, seq_lens, b, index)
-    stream = _lib.stream_of(dev)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (*k_pools, *v_pools)):
-        raise ValueError("a move of cached tokens records no gradient")
+    _lib.stream_of(keep.device)
     if b == 0 or budget == 0 or width == 0:
         return
     if index != _serving.current_device():
-        with torch.cuda.device(dev):
-            return move_tokens(keep, k_pools, v_pools, block_tables, seq_lens)
+        with torch.cuda.device(keep.device):
+            return _move(keep, lists, block_tables, seq_lens)
+    _move(keep, lists, block_tables, seq_lens)
+
+
+def _move(keep: torch.Tensor, lists, block_tables: torch.Tensor, seq_lens: torch.Tensor) -> None:
+    """move_tokens of checked arguments on the current device."""
+    h, nb, steps, dev, kp, vp = lists
+    layers, b, _, budget = keep.shape
     rc = _tree.lib().ls_move_tokens(
-        kp, vp, layers, steps, nb, block_tables.data_ptr(), block_tables.stride(0), width,
-        seq_lens.data_ptr(), ptr, b, h, budget, HEAD_DIM, PAGE, stream)
+        kp, vp, layers, steps, nb, block_tables.data_ptr(), block_tables.stride(0),
+        block_tables.shape[1], seq_lens.data_ptr(), keep.data_ptr(), b, h, budget, HEAD_DIM, PAGE,
+        _lib.stream_of(dev))
     _lib.check(rc, "ls_move_tokens")
 
 
@@ -244,14 +250,21 @@ def evict_tokens(sums: torch.Tensor, k_pools: Sequence[torch.Tensor],
     if sums.dim() != 4 or sums.shape[0] != layers or layers != len(v_pools):
         raise ValueError(f"sums must be [{layers}, B, H, T] for {layers} K and {len(v_pools)} V "
                          f"pools, got {tuple(sums.shape)}")
-    if layers:
-        shape = k_pools[0].shape
-        if len(shape) != 4 or shape[2] != sums.shape[2]:
-            raise ValueError(f"sums of {sums.shape[2]} heads for pools {tuple(shape)}")
-        _tree.pool_lists(k_pools, v_pools)                  # (before anything is launched)
-        _tree.tables(block_tables, seq_lens, sums.shape[1], sums.get_device())
-        if k_pools[0].get_device() != sums.get_device():
-            raise ValueError("sums must be on the pools' device")
+    if not layers:
+        return select_tokens(sums, seq_lens, budget, sinks, recent)
+    b, h, index = sums.shape[1], sums.shape[2], sums.get_device()
+    lists = _tree.pool_lists(k_pools, v_pools)              # (before anything is launched)
+    if lists[0] != h:
+        raise ValueError(f"sums of {h} heads for pools {tuple(k_pools[0].shape)}")
+    width = _tree.tables(block_tables, seq_lens, b, index)
+    if k_pools[0].get_device() != index:
+        raise ValueError("sums must be on the pools' device")
+    _lib.stream_of(sums.device)
+    if index != _serving.current_device():
+        with torch.cuda.device(sums.device):
+            return evict_tokens(sums, k_pools, v_pools, block_tables, seq_lens, budget, sinks,
+                                recent)
     keep, kept = select_tokens(sums, seq_lens, budget, sinks, recent)
-    move_tokens(keep, k_pools, v_pools, block_tables, seq_lens)
+    if b and width:
+        _move(keep, lists, block_tables, seq_lens)
     return keep, kept

@@ -166,8 +166,6 @@ def accept_tokens(tokens: torch.Tensor, parents: torch.Tensor, choices: torch.Te
     np_ = None if counts is None else _tree.whole("counts", counts, torch.int32, (b,), index)
     width = _tree.tables(block_tables, seq_lens, b, index)
     stream = _lib.stream_of(dev)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (*k_pools, *v_pools)):
-        raise ValueError("a move of cached tokens records no gradient")
     if index != _serving.current_device():
         with torch.cuda.device(dev):
             return accept_tokens(tokens, parents, choices, k_pools, v_pools, block_tables, seq_lens,

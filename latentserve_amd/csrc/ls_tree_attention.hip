@@ -16,6 +16,7 @@
 // neither the row reads of K nor the transposing reads of V meet in a bank.
 #include "ls_common.h"
 #include "ls_tree.h"
+#include "ls_tree_load.h"
 
 namespace ls {
 
@@ -28,36 +29,6 @@ namespace {
 // A weight is 2^(x - m + TOP) with x - m <= LAZY: at most 2^15, which fp16 holds, and of
 // full precision down to 2^-21 of the running maximum's.
 constexpr float TREE_TOP = 7.f, TREE_LAZY = 8.f;
-
-typedef char __attribute__((address_space(3)))* lds_ptr;
-
-// Sixteen bytes a lane from a resource to LDS at `to` + 16 lane (to: the same in every lane).
-// In assembly, since the compiler, where it knows of such a load, waits for all of them before
-// the next LDS read of the array; the waits are this file's own (wait_loads).  It writes no
-// register.  K and V are read once: the policy of the decode's page loads (against none:
-// a decode step of 16 x 16K 76.8 -> 69.5 us, 16 nodes of 16 x 16K 69.6 -> 68.2).
-__device__ __forceinline__ void load_to_lds(u4 rsrc, uint32_t off, uint32_t soff, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %3\n\t"
-                 "s_nop 0\n\t"
-                 "buffer_load_dwordx4 %0, %1, %2 offen sc0 nt lds"
-                 :: "v"(off), "s"(rsrc), "s"(soff), "s"(to) : "memory", "m0");
-}
-// Until at most N vector memory operations of this wave are outstanding.
-template <int N>
-__device__ __forceinline__ void wait_loads() {
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
-    __builtin_amdgcn_sched_barrier(0);
-}
-__device__ __forceinline__ u4 rsrc_of(const char* base, bool there) {
-    const uint64_t x = (uint64_t)base;
-    u4 r;
-    r.x = __builtin_amdgcn_readfirstlane((uint32_t)x);
-    r.y = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32) & 0xFFFFu);
-    r.z = __builtin_amdgcn_readfirstlane(there ? 0x7fffffffu : 0u);    // (none: no request)
-    r.w = 0x00020000u;
-    return r;
-}
 
 __device__ __forceinline__ u2 read_transposed(const char* p) {
     return __builtin_bit_cast(
@@ -635,7 +606,8 @@ void tree_kernel(const TreeParams a) {
                 const int id = __builtin_amdgcn_readlane(ids, at + first / PAGE);
                 // (a page outside the pool is not requested: what its rows hold counts as nothing)
                 const bool in = (unsigned)id < (unsigned)a.num_blocks;
-                const u4 from = rsrc_of(a.pool[z] + (in ? id : 0) * a.sp_b + u.h * a.sp_h, in);
+                const u4 from = rsrc_of(a.pool[z] + (in ? id : 0) * a.sp_b + u.h * a.sp_h,
+                                        in ? POOL_BYTES : 0);
 #pragma unroll
                 for (int i = 0; i < SAME; ++i) {
                     const int n = LOADS < 4 ? (rg * LOADS + i) & 3 : i;       // of the page's four

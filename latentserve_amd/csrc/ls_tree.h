@@ -38,6 +38,7 @@ struct TreeParams {
     int2* info;                           // [B * H]: first and last group of a unit
     float* scores;                        // [B * H, NR, score_len], or null
     int64_t score_len;
+    int score_parts;                      // workgroups that add a unit's scores
     int B, H, N, NR;
     int groups, row_tiles;
     int extra;                            // steps that starting on a unit counts as
@@ -54,7 +55,7 @@ constexpr int TREE_EXTRA = 1;
 
 TreeShape tree_shape(int batch, int kv_heads, int rows, int64_t keys_bound);
 size_t tree_record_bytes(const TreeShape& s);
-// With scores (up to 16 rows): they are kept, and lse is written.
+// With scores (up to 16 rows, one node): they are kept, and added to the sums as weights.
 hipError_t launch_tree_attention(const TreeParams& a, const TreeShape& s, hipStream_t stream);
 
 // ---- weight sums of accepted paths ---------------------------------------------------
@@ -79,7 +80,6 @@ struct WeighParams {
     int B, H, N, P, NR;
     float scale2;
 };
-hipError_t launch_add_scores(const TreeParams& a, int64_t keys_bound, hipStream_t stream);
 hipError_t launch_add_weights(const WeighParams& a, int64_t keys_bound, hipStream_t stream);
 
 // ---- moves of cached tokens -----------------------------------------------------------

@@ -271,10 +271,9 @@ int ls_paged_decode_weights(const void* q, const int64_t* q_strides, const void*
     a.sum_len = sum_len;
     a.sum_rows = sum_rows;
     a.num_sum_rows = num_sum_rows;
-    if (int rc = hip_status(ls::launch_tree_attention(a, s, (hipStream_t)stream),
-                            "ls_paged_decode_weights"))
-        return rc;
-    return hip_status(ls::launch_add_scores(a, bound, (hipStream_t)stream), "ls_paged_decode_weights");
+    // four keys a thread, in more rounds where sequences are longer
+    a.score_parts = (int)std::min<int64_t>((bound + 2047) / 2048, 1024);
+    return hip_status(ls::launch_tree_attention(a, s, (hipStream_t)stream), "ls_paged_decode_weights");
 }
 
 int ls_add_weights(const void* q, const int64_t* q_strides, const float* lse, const void* k_pool,

@@ -867,11 +867,80 @@ void tree_kernel(const TreeParams a) {
 
 // Records of a unit made its output: a workgroup a (unit, ROWS rows, CQ channel quads), its
 // waves take the records in turn, AHEAD at once.
+//
+// A decode that sums weights has a.score_parts more workgroups a unit: they bring the rows'
+// statistics together themselves, rather than in a launch after this one, and add the weights
+// of the unit's scores.
 constexpr int COMBINE_NW = 8;
-template <int ROWS, int CQ>
+
+__device__ __forceinline__ void add_scores(const TreeParams& a, int unit, int part, float (*e_s)[16]) {
+    const int b = unit / a.H, h = unit - b * a.H;
+    const int sum_row = a.sum_rows ? a.sum_rows[b] : b;
+    if ((unsigned)sum_row >= (unsigned)a.num_sum_rows) return;
+    int64_t keys = (int64_t)a.max_pages * PAGE;
+    const int len = a.lens[b];
+    keys = len < keys ? len : keys;
+    keys = keys < a.sum_len ? keys : a.sum_len;
+    constexpr int KEYS = WAVE * COMBINE_NW * 4;            // a round
+    if ((int64_t)part * KEYS >= keys) return;
+    // each row's log-sum-exp (log2 units) by 16 lanes' worth of records at a time
+    const int2 gs = a.info[unit];
+    const int row = threadIdx.x % 16;
+    if (gs.x == gs.y) {
+        if (threadIdx.x < 16)
+            e_s[0][row] = row < a.NR ? a.lse[(int64_t)unit * a.NR + row] * 1.4426950408889634f : 0.f;
+    } else {
+        float m = neg_inf(), l = 0.f;
+        for (int k = threadIdx.x / 16; k <= gs.y - gs.x; k += WAVE * COMBINE_NW / 16) {
+            const float* rec = a.work + ((int64_t)(gs.x + k) * 2 + (k == 0)) * (16 * 130);
+            const float2 o = *(const float2*)(rec + 16 * 128 + 2 * row);
+            const float top = fmaxf(m, o.x), use = top == neg_inf() ? 0.f : top;
+            l = l * fast_exp2(m - use) + o.y * fast_exp2(o.x - use);
+            m = top;
+        }
+        e_s[2 * (threadIdx.x / 16)][row] = m;
+        e_s[2 * (threadIdx.x / 16) + 1][row] = l;
+        __syncthreads();
+        if (threadIdx.x < 16) {
+            for (int k = 1; k < WAVE * COMBINE_NW / 16; ++k) {
+                const float x = e_s[2 * k][row], top = fmaxf(m, x), use = top == neg_inf() ? 0.f : top;
+                l = l * fast_exp2(m - use) + e_s[2 * k + 1][row] * fast_exp2(x - use);
+                m = top;
+            }
+            e_s[0][row] = m == neg_inf() ? m : m - TREE_TOP + __builtin_amdgcn_logf(l);
+        }
+    }
+    __syncthreads();
+    float* sums = a.sums + sum_row * a.ss_row + h * a.ss_h;
+    const float* scores = a.scores + (int64_t)unit * a.NR * a.score_len;
+    for (int64_t t0 = (int64_t)part * KEYS + threadIdx.x * 4; t0 < keys; t0 += (int64_t)a.score_parts * KEYS) {
+        const int n = keys - t0 < 4 ? (int)(keys - t0) : 4;
+        f4 sum = {0.f, 0.f, 0.f, 0.f}, had = sum;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < n) had[i] = sums[t0 + i];
+#pragma unroll 4
+        for (int r = 0; r < a.NR; ++r) {
+            const float e = e_s[0][r];
+            const f4 s = *(const f4*)(scores + r * a.score_len + t0);
+            // (-inf: it saw nothing, whatever its scores are)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[i] += e == neg_inf() ? 0.f : fast_exp2(s[i] - e);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < n) sums[t0 + i] = had[i] + sum[i];
+    }
+}
+
+template <int ROWS, int CQ, bool SCORES>
 __global__ __launch_bounds__(WAVE* COMBINE_NW) void tree_combine_kernel(const TreeParams a, int wr) {
     constexpr int PARTS = ROWS / 2 / CQ, AHEAD = CQ == 1 ? 4 : 1;
     __shared__ float sums[COMBINE_NW][CQ * 4 + 2][WAVE];
+    if constexpr (SCORES) {
+        __shared__ float e_s[2 * WAVE * COMBINE_NW / 16][16];
+        if (blockIdx.y >= PARTS) return add_scores(a, blockIdx.x, blockIdx.y - PARTS, e_s);
+    }
     const int unit = blockIdx.x, rb = blockIdx.y / PARTS, part = blockIdx.y % PARTS;
     const int2 gs = a.info[unit];
     if (gs.x == gs.y) return;
@@ -960,9 +1029,11 @@ hipError_t launch(const TreeParams& a, hipStream_t stream) {
     const int blocks = (a.N * a.NR + ROWS - 1) / ROWS, units = a.B * a.H;
     const dim3 threads(WAVE * COMBINE_NW);
     if (units * blocks * (ROWS / 8) >= 256)
-        tree_combine_kernel<ROWS, 4><<<dim3(units, blocks * (ROWS / 8)), threads, 0, stream>>>(a, WR);
+        tree_combine_kernel<ROWS, 4, SCORES>
+            <<<dim3(units, blocks * (ROWS / 8) + a.score_parts), threads, 0, stream>>>(a, WR);
     else
-        tree_combine_kernel<ROWS, 1><<<dim3(units, blocks * (ROWS / 2)), threads, 0, stream>>>(a, WR);
+        tree_combine_kernel<ROWS, 1, SCORES>
+            <<<dim3(units, blocks * (ROWS / 2) + a.score_parts), threads, 0, stream>>>(a, WR);
     return hipGetLastError();
 }
 

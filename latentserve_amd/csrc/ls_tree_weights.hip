@@ -171,43 +171,7 @@ __global__ __launch_bounds__(WAVE* WEIGH_NW) void add_weights_kernel(const Weigh
     }
 }
 
-// The decode's: its scores (log2 units) against its rows' statistics, four keys a thread.
-__global__ __launch_bounds__(256) void add_scores_kernel(const TreeParams a) {
-    const int h = blockIdx.y, b = blockIdx.z;
-    const int sum_row = a.sum_rows ? a.sum_rows[b] : b;
-    if ((unsigned)sum_row >= (unsigned)a.num_sum_rows) return;
-    int64_t keys = (int64_t)a.max_pages * PAGE;
-    const int len = a.lens[b];
-    keys = len < keys ? len : keys;
-    keys = keys < a.sum_len ? keys : a.sum_len;
-    float* sums = a.sums + sum_row * a.ss_row + h * a.ss_h;
-    const int64_t unit = (int64_t)b * a.H + h;
-    const float* lse = a.lse + unit * a.NR;
-    const float* scores = a.scores + unit * a.NR * a.score_len;
-    for (int64_t t0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; t0 < keys;
-         t0 += (int64_t)gridDim.x * 1024) {
-        f4 sum = {0.f, 0.f, 0.f, 0.f};
-        for (int r = 0; r < a.NR; ++r) {
-            const float e = lse[r] * 1.4426950408889634f;
-            if (e == neg_inf()) continue;                  // (it saw nothing)
-            const f4 s = *(const f4*)(scores + r * a.score_len + t0);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sum[i] += fast_exp2(s[i] - e);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (t0 + i < keys) sums[t0 + i] += sum[i];
-    }
-}
-
 }  // namespace
-
-hipError_t launch_add_scores(const TreeParams& a, int64_t keys_bound, hipStream_t stream) {
-    int64_t parts = (keys_bound + 1023) / 1024;
-    if (parts < 1) parts = 1;
-    add_scores_kernel<<<dim3((unsigned)parts, a.H, a.B), dim3(256), 0, stream>>>(a);
-    return hipGetLastError();
-}
 
 hipError_t launch_add_weights(const WeighParams& a, int64_t keys_bound, hipStream_t stream) {
     // a workgroup fills a CU's LDS: as many as CUs, or one a head and sequence

@@ -664,7 +664,10 @@ void tree_kernel(const TreeParams a) {
         // may not see.
         // (k_read: what is done once K has been read)
         auto add_step = [&](int step, bool masked, char* kt, char* vt, auto&& k_read) {
-            if (!works) return true;
+            if (!works) {
+                k_read();
+                return true;
+            }
             t.scores(kt);
             if (masked) {
                 t.mask(bits);
@@ -716,24 +719,25 @@ void tree_kernel(const TreeParams a) {
                 else
                     wait_loads<0>();
                 __syncthreads();
+                at_step();
+            };
+            auto next = [&] {
                 if (step + AHEAD < s1) {
                     blocks(step + AHEAD);
                     load(0, step + AHEAD);
                     load(1, step + AHEAD);
                 }
-                at_step();
             };
-            auto none = [] {};
             // (A step of infinities leaves the loop for its products by row and comes back: as a
             // branch inside it, it would cost every step copies of the sums.)
             while (true) {
                 while (true) {
                     turn();
-                    if (!add_step(step, masked, kt, vt, none)) break;
+                    if (!add_step(step, masked, kt, vt, next)) break;
                     if (++step >= s1) break;
                 }
                 if (step >= s1) break;
-                add_step_by_row(step, kt, vt, none);
+                add_step_by_row(step, kt, vt, next);
                 if (++step >= s1) break;
             }
         } else {
@@ -866,13 +870,14 @@ void tree_kernel(const TreeParams a) {
 }
 
 // Records of a unit made its output: a workgroup a (unit, ROWS rows, CQ channel quads), its
-// waves take the records in turn, AHEAD at once.
+// waves take the records in turn, AHEAD at once.  Bound by the trips to memory: with a quad a
+// workgroup, 128 records are one trip of 16 waves (100K keys, 198 rows: 9.7 us in eight waves'
+// four trips, 7.4 us so).
 //
 // A decode that sums weights has a.score_parts more workgroups a unit: they bring the rows'
 // statistics together themselves, rather than in a launch after this one, and add the weights
 // of the unit's scores.
-constexpr int COMBINE_NW = 8;
-
+template <int NW>
 __device__ __forceinline__ void add_scores(const TreeParams& a, int unit, int part, float (*e_s)[16]) {
     const int b = unit / a.H, h = unit - b * a.H;
     const int sum_row = a.sum_rows ? a.sum_rows[b] : b;
@@ -881,7 +886,7 @@ __device__ __forceinline__ void add_scores(const TreeParams& a, int unit, int pa
     const int len = a.lens[b];
     keys = len < keys ? len : keys;
     keys = keys < a.sum_len ? keys : a.sum_len;
-    constexpr int KEYS = WAVE * COMBINE_NW * 4;            // a round
+    constexpr int KEYS = WAVE * NW * 4;            // a round
     if ((int64_t)part * KEYS >= keys) return;
     // each row's log-sum-exp (log2 units) by 16 lanes' worth of records at a time
     const int2 gs = a.info[unit];
@@ -891,7 +896,7 @@ __device__ __forceinline__ void add_scores(const TreeParams& a, int unit, int pa
             e_s[0][row] = row < a.NR ? a.lse[(int64_t)unit * a.NR + row] * 1.4426950408889634f : 0.f;
     } else {
         float m = neg_inf(), l = 0.f;
-        for (int k = threadIdx.x / 16; k <= gs.y - gs.x; k += WAVE * COMBINE_NW / 16) {
+        for (int k = threadIdx.x / 16; k <= gs.y - gs.x; k += WAVE * NW / 16) {
             const float* rec = a.work + ((int64_t)(gs.x + k) * 2 + (k == 0)) * (16 * 130);
             const float2 o = *(const float2*)(rec + 16 * 128 + 2 * row);
             const float top = fmaxf(m, o.x), use = top == neg_inf() ? 0.f : top;
@@ -902,7 +907,7 @@ __device__ __forceinline__ void add_scores(const TreeParams& a, int unit, int pa
         e_s[2 * (threadIdx.x / 16) + 1][row] = l;
         __syncthreads();
         if (threadIdx.x < 16) {
-            for (int k = 1; k < WAVE * COMBINE_NW / 16; ++k) {
+            for (int k = 1; k < WAVE * NW / 16; ++k) {
                 const float x = e_s[2 * k][row], top = fmaxf(m, x), use = top == neg_inf() ? 0.f : top;
                 l = l * fast_exp2(m - use) + e_s[2 * k + 1][row] * fast_exp2(x - use);
                 m = top;
@@ -933,13 +938,13 @@ __device__ __forceinline__ void add_scores(const TreeParams& a, int unit, int pa
     }
 }
 
-template <int ROWS, int CQ, bool SCORES>
-__global__ __launch_bounds__(WAVE* COMBINE_NW) void tree_combine_kernel(const TreeParams a, int wr) {
-    constexpr int PARTS = ROWS / 2 / CQ, AHEAD = CQ == 1 ? 4 : 1;
-    __shared__ float sums[COMBINE_NW][CQ * 4 + 2][WAVE];
+template <int ROWS, int CQ, int NW, bool SCORES>
+__global__ __launch_bounds__(WAVE* NW) void tree_combine_kernel(const TreeParams a, int wr) {
+    constexpr int PARTS = ROWS / 2 / CQ, AHEAD = CQ == 1 ? 8 : 2;
+    __shared__ float sums[NW][CQ * 4 + 2][WAVE];
     if constexpr (SCORES) {
-        __shared__ float e_s[2 * WAVE * COMBINE_NW / 16][16];
-        if (blockIdx.y >= PARTS) return add_scores(a, blockIdx.x, blockIdx.y - PARTS, e_s);
+        __shared__ float e_s[2 * WAVE * NW / 16][16];
+        if (blockIdx.y >= PARTS) return add_scores<NW>(a, blockIdx.x, blockIdx.y - PARTS, e_s);
     }
     const int unit = blockIdx.x, rb = blockIdx.y / PARTS, part = blockIdx.y % PARTS;
     const int2 gs = a.info[unit];
@@ -954,12 +959,12 @@ __global__ __launch_bounds__(WAVE* COMBINE_NW) void tree_combine_kernel(const Tr
     f4 y[CQ];
 #pragma unroll
     for (int n = 0; n < CQ; ++n) y[n] = (f4){0.f, 0.f, 0.f, 0.f};
-    for (int k0 = wave; k0 < count; k0 += COMBINE_NW * AHEAD) {
+    for (int k0 = wave; k0 < count; k0 += NW * AHEAD) {
         float2 o[AHEAD];
         f4 x[AHEAD][CQ];
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            const int k = k0 + i * COMBINE_NW;
+            const int k = k0 + i * NW;
             const float* rec = record(k < count ? k : k0);
             o[i] = *(const float2*)(rec + ROWS * 128 + 2 * (lane % ROWS));
 #pragma unroll
@@ -967,7 +972,7 @@ __global__ __launch_bounds__(WAVE* COMBINE_NW) void tree_combine_kernel(const Tr
         }
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            if (k0 + i * COMBINE_NW >= count) break;
+            if (k0 + i * NW >= count) break;
             const float top = fmaxf(m, o[i].x), use = top == neg_inf() ? 0.f : top;
             const float keep = fast_exp2(m - use), w = fast_exp2(o[i].x - use);
             l = l * keep + o[i].y * w;
@@ -986,10 +991,10 @@ __global__ __launch_bounds__(WAVE* COMBINE_NW) void tree_combine_kernel(const Tr
     // wave w finishes quad w
     if (wave >= CQ) return;
     float top = neg_inf(), total = 0.f;
-    for (int w = 0; w < COMBINE_NW; ++w) top = fmaxf(top, sums[w][CQ * 4][lane]);
+    for (int w = 0; w < NW; ++w) top = fmaxf(top, sums[w][CQ * 4][lane]);
     const float use = top == neg_inf() ? 0.f : top;
     f4 z = {0.f, 0.f, 0.f, 0.f};
-    for (int w = 0; w < COMBINE_NW; ++w) {
+    for (int w = 0; w < NW; ++w) {
         const float f = fast_exp2(sums[w][CQ * 4][lane] - use);
         total += f * sums[w][CQ * 4 + 1][lane];
 #pragma unroll
@@ -1027,13 +1032,12 @@ hipError_t launch(const TreeParams& a, hipStream_t stream) {
     if (e != hipSuccess) return e;
     // few of them: a quad a workgroup, so that the records are read by the whole chip
     const int blocks = (a.N * a.NR + ROWS - 1) / ROWS, units = a.B * a.H;
-    const dim3 threads(WAVE * COMBINE_NW);
     if (units * blocks * (ROWS / 8) >= 256)
-        tree_combine_kernel<ROWS, 4, SCORES>
-            <<<dim3(units, blocks * (ROWS / 8) + a.score_parts), threads, 0, stream>>>(a, WR);
+        tree_combine_kernel<ROWS, 4, 8, SCORES>
+            <<<dim3(units, blocks * (ROWS / 8) + a.score_parts), dim3(WAVE * 8), 0, stream>>>(a, WR);
     else
-        tree_combine_kernel<ROWS, 1, SCORES>
-            <<<dim3(units, blocks * (ROWS / 2) + a.score_parts), threads, 0, stream>>>(a, WR);
+        tree_combine_kernel<ROWS, 1, 16, SCORES>
+            <<<dim3(units, blocks * (ROWS / 2) + a.score_parts), dim3(WAVE * 16), 0, stream>>>(a, WR);
     return hipGetLastError();
 }
 

@@ -271,7 +271,7 @@ int ls_paged_decode_weights(const void* q, const int64_t* q_strides, const void*
     a.sum_len = sum_len;
     a.sum_rows = sum_rows;
     a.num_sum_rows = num_sum_rows;
-    // four keys a thread of eight waves or 16, in more rounds where sequences are longer
+    // four keys a thread of eight waves, in more rounds where sequences are longer
     a.score_parts = (int)std::min<int64_t>((bound + 2047) / 2048, 1024);
     return hip_status(ls::launch_tree_attention(a, s, (hipStream_t)stream), "ls_paged_decode_weights");
 }

@@ -903,11 +903,17 @@ __device__ __forceinline__ void add_scores(const TreeParams& a, int unit, int pa
             l = l * fast_exp2(m - use) + o.y * fast_exp2(o.x - use);
             m = top;
         }
-        e_s[2 * (threadIdx.x / 16)][row] = m;
-        e_s[2 * (threadIdx.x / 16) + 1][row] = l;
+        const float most = group4_max(m);
+        l = group4_sum(l * fast_exp2(m - (most == neg_inf() ? 0.f : most)));
+        m = most;
+        const int wave = threadIdx.x / WAVE;
+        if (threadIdx.x % WAVE < 16) {
+            e_s[2 * wave][row] = m;
+            e_s[2 * wave + 1][row] = l;
+        }
         __syncthreads();
         if (threadIdx.x < 16) {
-            for (int k = 1; k < WAVE * NW / 16; ++k) {
+            for (int k = 1; k < NW; ++k) {
                 const float x = e_s[2 * k][row], top = fmaxf(m, x), use = top == neg_inf() ? 0.f : top;
                 l = l * fast_exp2(m - use) + e_s[2 * k + 1][row] * fast_exp2(x - use);
                 m = top;
@@ -943,7 +949,7 @@ __global__ __launch_bounds__(WAVE* NW) void tree_combine_kernel(const TreeParams
     constexpr int PARTS = ROWS / 2 / CQ, AHEAD = CQ == 1 ? 8 : 2;
     __shared__ float sums[NW][CQ * 4 + 2][WAVE];
     if constexpr (SCORES) {
-        __shared__ float e_s[2 * WAVE * NW / 16][16];
+        __shared__ float e_s[2 * NW][16];
         if (blockIdx.y >= PARTS) return add_scores<NW>(a, blockIdx.x, blockIdx.y - PARTS, e_s);
     }
     const int unit = blockIdx.x, rb = blockIdx.y / PARTS, part = blockIdx.y % PARTS;
@@ -1031,13 +1037,15 @@ hipError_t launch(const TreeParams& a, hipStream_t stream) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     // few of them: a quad a workgroup, so that the records are read by the whole chip
+    // (with scores, of eight waves, so that they are too)
+    constexpr int NW_FEW = SCORES ? 8 : 16;
     const int blocks = (a.N * a.NR + ROWS - 1) / ROWS, units = a.B * a.H;
     if (units * blocks * (ROWS / 8) >= 256)
         tree_combine_kernel<ROWS, 4, 8, SCORES>
             <<<dim3(units, blocks * (ROWS / 8) + a.score_parts), dim3(WAVE * 8), 0, stream>>>(a, WR);
     else
-        tree_combine_kernel<ROWS, 1, 16, SCORES>
-            <<<dim3(units, blocks * (ROWS / 2) + a.score_parts), dim3(WAVE * 16), 0, stream>>>(a, WR);
+        tree_combine_kernel<ROWS, 1, NW_FEW, SCORES>
+            <<<dim3(units, blocks * (ROWS / 2) + a.score_parts), dim3(WAVE * NW_FEW), 0, stream>>>(a, WR);
     return hipGetLastError();
 }
 

@@ -170,7 +170,7 @@ def select_tokens(sums: torch.Tensor, seq_lens: torch.Tensor, budget: int, sinks
     if seq_lens.dtype is not torch.int32 or seq_lens.shape != (b,) \
             or (b > 1 and seq_lens.stride(0) != 1) or seq_lens.get_device() != index:
         raise ValueError(f"seq_lens must be {b} unit-stride int32 values on the sums' device")
-    budget, sinks, recent = _budget(budget, sinks, recent)
+    budget, sinks, recent = budget_of(budget, sinks, recent)
     stream = _lib.stream_of(dev)
     if index != _serving.current_device():
         with torch.cuda.device(dev):
@@ -185,7 +185,7 @@ def select_tokens(sums: torch.Tensor, seq_lens: torch.Tensor, budget: int, sinks
     return keep, kept
 
 
-def _budget(budget: int, sinks: int, recent: Optional[int]):
+def budget_of(budget: int, sinks: int, recent: Optional[int]):
     budget, sinks = int(budget), int(sinks)
     if not 1 <= budget < 1 << 31:
         raise ValueError(f"budget must be in [1, 2^31), got {budget}")

@@ -102,6 +102,7 @@ class CapturedDecode:
         self.ids = torch.zeros(batch_size, 1, dtype=torch.long, device=dev)
         self.positions = torch.zeros(batch_size, 1, dtype=torch.long, device=dev)
         self.graph: Optional[torch.cuda.CUDAGraph] = None
+        self.sums: Optional[torch.Tensor] = None      # what its steps' weights go to
         self.logits_buf: Optional[torch.Tensor] = None
         self.next_buf: Optional[torch.Tensor] = None
         self.logprobs_buf: Optional[TokenLogprobs] = None
@@ -122,12 +123,17 @@ class CapturedDecode:
         and the cache advanced for a real step: the recording does not run,
         the first replay does)."""
         with _pinned_splits(self.model, self.num_splits):
+            sums = getattr(self.model.cache, "weight_sums", None)
+            before = None if sums is None else sums.clone()
             side = torch.cuda.Stream()
             side.wait_stream(torch.cuda.current_stream())
             with torch.cuda.stream(side):
                 for _ in range(self.WARMUP_RUNS):
                     self._forward()
             torch.cuda.current_stream().wait_stream(side)
+            if sums is not None:                       # (what the warm-up's steps added)
+                sums.copy_(before)
+            self.sums = sums
             g = torch.cuda.CUDAGraph()
             with counters_of(g), torch.cuda.graph(g, pool=pool):
                 self.logits_buf, self.next_buf, self.logprobs_buf = self._forward()
@@ -233,7 +239,7 @@ class GraphedDecoder:
             return out
         key = (batch, bucket, ratio)
         g = self.graphs.get(key)
-        if g is None:
+        if g is None or g.sums is not getattr(cache, "weight_sums", None):
             g = CapturedDecode(self.model, batch, bucket, self._splits(batch, bucket),
                                greedy=self.greedy, logprobs=self.logprobs)
             g.set_inputs(token_ids, positions)

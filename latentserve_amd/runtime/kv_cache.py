@@ -180,6 +180,8 @@ class BlockTable:
         # bumped when the block list is replaced rather than extended: a
         # mirror that saw an older lineage re-uploads the whole row
         self.lineage = 0
+        # tokens were evicted: row p is no longer token p
+        self.evicted = False
 
     @property
     def capacity(self) -> int:
@@ -222,6 +224,7 @@ class BlockTable:
         self.length = 0
         self.version += 1
         self.lineage += 1
+        self.evicted = False
 
 
 @dataclass
@@ -241,11 +244,12 @@ class KVCacheSpec:
 class StepInputs:
     """Per-step kernel inputs at fixed device addresses.
 
-    ``tables`` [max_batch, capacity_pages] int32, and four vectors of
+    ``tables`` [max_batch, capacity_pages] int32, and five vectors of
     max_batch entries carved from one device buffer: ``write_slot`` int64
     (the decode token's flat slot), ``res_index`` int64 (its row in the
-    flattened INT8 residual), ``lens`` int32 and ``res_row`` int32 (each
-    sequence's residual row).  ``publish`` writes the step's values into a
+    flattened INT8 residual), ``lens`` int32, ``res_row`` int32 (each
+    sequence's residual row) and ``slot`` int32 (its slot, where weight sums
+    are kept).  ``publish`` writes the step's values into a
     pinned staging area and issues asynchronous copies: the changed table
     entries, then the whole vector buffer in one copy.  Two staging areas
     alternate; one is refilled only after the copies that last read it
@@ -253,7 +257,7 @@ class StepInputs:
     """
 
     _FIELDS = (("write_slot", np.int64), ("res_index", np.int64),
-               ("lens", np.int32), ("res_row", np.int32))
+               ("lens", np.int32), ("res_row", np.int32), ("slot", np.int32))
 
     def __init__(self, max_batch: int, capacity_pages: int, block_size: int, device):
         self.max_batch = mb = int(max_batch)
@@ -387,8 +391,10 @@ class _PagedBase:
 
     def shareable_blocks(self, index: int) -> int:
         """Leading pages of slot `index` whose K/V in the pool is final, so a
-        prefix cache may hand them to another sequence."""
-        return self.tables[index].length // self.block_size
+        prefix cache may hand them to another sequence (of a sequence that lost
+        tokens, none: its pages are not of the prompt's first tokens)."""
+        t = self.tables[index]
+        return 0 if t.evicted else t.length // self.block_size
 
     # ---- branching and compaction -------------------------------------------
     def _page_tensors(self) -> List[torch.Tensor]:
@@ -429,6 +435,7 @@ class _PagedBase:
             self.allocator.incref(pages)
             child.blocks = list(pages)
             child.length = t.length
+            child.evicted = t.evicted
             child.version += 1
             child.lineage += 1
 
@@ -438,8 +445,8 @@ class _PagedBase:
         replaced by pages of their own, with the tokens they keep.  All or
         nothing: where the pool has not the blocks for all of it (OutOfBlocks),
         or a sequence would outgrow the cache, nothing has changed."""
-        bs, refs = self.block_size, self.allocator.ref_count
-        todo, left, grown = [], {}, 0
+        bs = self.block_size
+        spans, grown = [], 0
         for s in seqs:
             t = self.tables[s]
             first, have, end = t.length // bs, len(t.blocks), -(-(t.length + n) // bs)
@@ -448,12 +455,25 @@ class _PagedBase:
                     raise RuntimeError(f"the sequence in slot {s} would hold {end} pages; the "
                                        f"cache was sized for {self.capacity_pages}")
                 grown += end - have
-            for page in range(first, min(have, end)):
+            spans.append((t, first, min(have, end), first + (t.length % bs > 0)))
+        self._own_pages(spans, grown)
+        if grown:
+            for s in seqs:
+                self.tables[s].reserve(n)
+
+    def _own_pages(self, spans, grown: int = 0) -> None:
+        """Of each (table, first, end, kept), the pages first .. end - 1 that others hold too
+        replaced by pages of its own, with what the ones before `kept` hold.  All or
+        nothing, as is room for `grown` blocks more."""
+        refs = self.allocator.ref_count
+        todo, left = [], {}
+        for t, first, end, kept in spans:
+            for page in range(first, end):
                 blk = t.blocks[page]
                 count = left.get(blk, refs(blk))
                 if count > 1:
                     left[blk] = count - 1              # the last to write keeps the page
-                    todo.append((t, page, blk, page == first and t.length % bs > 0))
+                    todo.append((t, page, blk, page < kept))
         if grown or todo:
             self.allocator.ensure(grown + len(todo))
         if todo:
@@ -465,9 +485,6 @@ class _PagedBase:
                 t.version += 1
                 t.lineage += 1
             self.allocator.free([blk for _, _, blk, _ in todo])
-        if grown:
-            for s in seqs:
-                self.tables[s].reserve(n)
 
     def compact(self) -> Dict[int, int]:
         """Move the held pages to the pool's lowest blocks, so that they are blocks
@@ -602,6 +619,8 @@ class PagedKVCache(_PagedBase):
                        for _ in range(spec.num_layers)]
         self.kmin: Optional[List[torch.Tensor]] = None
         self.kmax: Optional[List[torch.Tensor]] = None
+        # [layers, slots, heads, tokens] fp32: see enable_weight_sums()
+        self.weight_sums: Optional[torch.Tensor] = None
 
     def _page_tensors(self) -> List[torch.Tensor]:
         return self.k_pool + self.v_pool + (self.kmin or []) + (self.kmax or [])
@@ -612,7 +631,16 @@ class PagedKVCache(_PagedBase):
         235-271) and publish the step's kernel inputs.  OutOfBlocks leaves
         every sequence, and which are active, as they were."""
         self._room_for_step(n, batch_size, slots)
+        if self.weight_sums is not None:
+            for s in self._active:
+                if not self.tables[s].length:          # (what the slot's last sequence left)
+                    self.weight_sums[:, s].zero_()
         self._publish(n, self._grow(n))
+
+    def _publish(self, n: int, starts: List[int], extra: Optional[dict] = None) -> None:
+        if self.weight_sums is not None:
+            extra = {**(extra or {}), "slot": self._active}
+        super()._publish(n, starts, extra)
 
     def rewind(self, length: int, slots: Optional[Sequence[int]] = None) -> None:
         """Shorten sequences to `length` tokens, keeping their pages
@@ -630,7 +658,111 @@ class PagedKVCache(_PagedBase):
                 raise
             for s in seqs:
                 self._bound_partial_page(s, length)
+        if self.weight_sums is not None:
+            for s in seqs:
+                self.weight_sums[:, s, :, length:].zero_()
         self._publish(0, [self.tables[s].length for s in self._active])
+
+    def fork(self, index: int, children: Sequence[int]) -> None:
+        children = list(children)
+        super().fork(index, children)
+        if self.weight_sums is not None:
+            for c in children:
+                self.weight_sums[:, c].copy_(self.weight_sums[:, index])
+
+    def attach_prefix(self, index: int, blocks: Sequence[int], num_tokens: int) -> None:
+        super().attach_prefix(index, blocks, num_tokens)
+        if self.weight_sums is not None:
+            self.weight_sums[:, index].zero_()
+
+    # ---- drafted trees and a bounded cache ----------------------------------
+    def accept(self, tokens: torch.Tensor, parents: torch.Tensor, choices: torch.Tensor,
+               counts: Optional[torch.Tensor] = None):
+        """End a step of drafted trees: the active sequences hold N drafted tokens each
+        (advance(N), then a pass that wrote them), and keep the ones that the model's own
+        choices confirm, moved together behind their context
+        (kernels.hip.tree_attention.accept_tokens, whose arguments and result these
+        are).  The lengths that the host keeps follow, so this waits for the
+        GPU."""
+        from latentserve_amd.kernels.hip import tree_attention as ta
+
+        seqs = self._active
+        if tokens.dim() != 2 or tokens.shape[0] != self._need(None):
+            raise ValueError(f"tokens must be [{self._need(None)}, N], got {tuple(tokens.shape)}")
+        n = tokens.shape[1]
+        for s in seqs:
+            if self.tables[s].length < n:
+                raise ValueError(f"slot {s} holds {self.tables[s].length} tokens, not {n} drafted "
+                                 "ones")
+        got = ta.accept_tokens(tokens, parents, choices, self.k_pool, self.v_pool,
+                               self.block_tables_tensor(), self.seq_lens_tensor(), counts)
+        for s, m in zip(seqs, got.lengths.tolist()):
+            t = self.tables[s]
+            before = t.length - n
+            t.length = before + m
+            self._bound_pages(s, before // self.block_size)
+        self._publish(0, [self.tables[s].length for s in seqs])
+        return got
+
+    def enable_weight_sums(self) -> None:
+        """Keep, per layer, slot and KV head, the attention weight that each cached token
+        has got so far (the decoder's dense steps add to it), for evict().  A sequence's
+        sums follow it through rewind(), fork() and accept(); they start at zero."""
+        if self.weight_sums is None:
+            spec = self.spec
+            self.weight_sums = torch.zeros(spec.num_layers, spec.max_batch_size, spec.num_kv_heads,
+                                           self.capacity_pages * self.block_size,
+                                           dtype=torch.float32, device=self.device)
+            if self._batch:
+                self._publish(0, [self.tables[s].length for s in self._active])
+
+    def sum_rows_tensor(self, batch_size: Optional[int] = None) -> torch.Tensor:
+        """[B] int32 slots of the active sequences, their rows of a layer's weight sums
+        (fixed address)."""
+        return self.inputs.vec["slot"][:self._need(batch_size)]
+
+    def evict(self, budget: int, sinks: int = 4, recent: Optional[int] = None,
+              slots: Optional[Sequence[int]] = None) -> List[int]:
+        """Bring the active sequences (or `slots`) to at most `budget` tokens each: per
+        layer and KV head, the first `sinks`, the last `recent` (default: a quarter of
+        the budget) and those with the largest weight sums of the others, moved to
+        the front (kernels.hip.cache_eviction.evict_tokens).  Their pages behind go
+        back to the pool; pages that others hold are copied first.  Returns the slots
+        that lost tokens.  A token's position is the caller's to count on: the
+        sequence's length no longer is it.  Between steps only, as fork();
+        OutOfBlocks leaves every sequence as it was."""
+        from latentserve_amd.kernels.hip import cache_eviction as ce
+
+        if self.weight_sums is None:
+            raise RuntimeError("enable_weight_sums() before the steps that eviction goes by")
+        budget, sinks, recent = ce.budget_of(budget, sinks, recent)
+        seqs = list(dict.fromkeys(self._active if slots is None else slots))
+        seqs = [s for s in seqs if self.tables[s].length > budget]
+        if not seqs:
+            return []
+        tables = [self.tables[s] for s in seqs]
+        pages = -(-budget // self.block_size)
+        self._own_pages([(t, 0, pages, pages) for t in tables])
+        width = max(len(t.blocks) for t in tables)
+        rows = torch.tensor([t.blocks + [0] * (width - len(t.blocks)) for t in tables],
+                            dtype=torch.int32).to(self.device)
+        lens = torch.tensor([t.length for t in tables], dtype=torch.int32).to(self.device)
+        at = torch.tensor(seqs).to(self.device)
+        _, kept = ce.evict_tokens(self.weight_sums[:, at], self.k_pool, self.v_pool, rows, lens,
+                                  budget, sinks, recent)
+        self.weight_sums[:, at] = 0
+        self.weight_sums[:, at, :, :budget] = kept
+        for s, t in zip(seqs, tables):
+            t.length = budget
+            self.allocator.free(t.blocks[pages:])
+            t.blocks = t.blocks[:pages]
+            t.version += 1
+            t.lineage += 1
+            t.evicted = True
+            self._bound_pages(s, 0)
+        if self._batch:
+            self._publish(0, [self.tables[s].length for s in self._active])
+        return seqs
 
     def write(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor, start_pos: int = 0) -> None:
         """Store k, v [B, H_kv, n, D] at the slots the last advance(n) reserved."""
@@ -682,6 +814,21 @@ class PagedKVCache(_PagedBase):
         if self.kmin is None:
             return None
         return self.kmin[layer_idx], self.kmax[layer_idx]
+
+    def _bound_pages(self, seq: int, first: int) -> None:
+        """Bounds of a sequence's pages from `first` on, over the rows that it holds."""
+        if self.kmin is None:
+            return
+        t = self.tables[seq]
+        full = t.length // self.block_size
+        if full > first:
+            blks = torch.tensor(t.blocks[first:full]).to(self.device)
+            for layer, pool in enumerate(self.k_pool):
+                live = pool[blks]
+                self.kmin[layer][blks] = live.amin(dim=1)
+                self.kmax[layer][blks] = live.amax(dim=1)
+        if t.length % self.block_size and full >= first:
+            self._bound_partial_page(seq, t.length)
 
     def _bound_partial_page(self, seq: int, length: int) -> None:
         """Bounds of the page a rewind lands in, over its remaining rows."""

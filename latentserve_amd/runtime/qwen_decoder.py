@@ -29,9 +29,11 @@ import torch.nn.functional as F
 
 from latentserve_amd.kernels import decode_gemm as dg
 from latentserve_amd.kernels import fused_elementwise as fe
+from latentserve_amd.kernels.hip import cache_eviction as ce
 from latentserve_amd.kernels.hip import int4_cache as i4
 from latentserve_amd.kernels.hip import paged_decode_hip as pdh
 from latentserve_amd.kernels.hip import paged_sparse as ps
+from latentserve_amd.kernels.hip import tree_attention as ta
 from latentserve_amd.runtime.int4_cache import Int4PagedKVCache
 from latentserve_amd.runtime.int8_cache import Int8PagedKVCache
 from latentserve_amd.runtime.kv_cache import KVCacheSpec, PagedKVCache
@@ -164,15 +166,18 @@ class QwenDecoder:
         self.cache = None
         self._stage = None
         self.rope: Optional[Rope] = None
+        self._tree: Optional[list] = None              # the last tree's (q, lse), a layer each
         self.sparse_ratio: Optional[float] = None
         self.scale = 1.0 / math.sqrt(cfg.head_dim)
 
     def allocate_cache(self, max_batch_size: int, max_seq_len: int,
                        num_blocks: Optional[int] = None, kv_dtype: str = "fp16",
-                       asymmetric: bool = False):
+                       asymmetric: bool = False, max_positions: Optional[int] = None):
         """A paged cache for this model: fp16 (PagedKVCache), INT8
         (Int8PagedKVCache: int8 pools, fp32 scales, the fp16 last-page K
-        residual) or 4 bits (Int4PagedKVCache)."""
+        residual) or 4 bits (Int4PagedKVCache).  max_positions (default:
+        max_seq_len): where tokens are evicted, sequences get longer than what
+        the cache holds of them."""
         spec = KVCacheSpec(num_layers=self.cfg.num_layers, num_kv_heads=self.cfg.num_kv_heads,
                            head_dim=self.cfg.head_dim, max_batch_size=max_batch_size,
                            max_seq_len=max_seq_len, device=str(self.device))
@@ -192,7 +197,9 @@ class QwenDecoder:
                 torch.arange(max_batch_size, dtype=torch.long, device=self.device) * 16)
         else:
             raise ValueError(f"kv_dtype must be 'fp16', 'int8' or 'int4', got {kv_dtype!r}")
-        self.rope = Rope(self.cfg.head_dim, self.cfg.rope_theta, max_seq_len, self.device)
+        self.rope = Rope(self.cfg.head_dim, self.cfg.rope_theta,
+                         max(max_seq_len, max_positions or 0), self.device)
+        self._tree = None
         return self.cache
 
     def set_sparse(self, ratio: Optional[float], recent: int = 2,
@@ -217,13 +224,16 @@ class QwenDecoder:
                               max_position: int) -> torch.Tensor:
         """One decode step for the active sequences: token_ids / positions
         [B, 1] int64 -> logits [B, 1, vocab].  The cache has already been
-        advanced; `max_position` bounds every position (a graph bucket)."""
-        cfg, cache = self.cfg, self.cache
+        advanced; `max_position` bounds every position (a graph bucket).  Where the
+        cache keeps weight sums, the step's attention adds to them."""
+        cache = self.cache
         b = token_ids.shape[0]
-        hq, hk, hd = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim
-        eps = cfg.rms_norm_eps
+        sums = getattr(cache, "weight_sums", None)
+        if sums is not None and self.sparse_ratio is not None:
+            raise ValueError("a sparse step does not see all weights that the cache is to sum")
         tables = cache.block_tables_tensor(b)
         lens = cache.seq_lens_tensor(b)
+        rows = None if sums is None else cache.sum_rows_tensor(b)
         staged = self._stage is not None               # quantized by the cache's write
         int4 = isinstance(cache, Int4PagedKVCache)
         if staged:
@@ -232,46 +242,8 @@ class QwenDecoder:
             res_rows = None if int4 else cache.residual_rows_tensor(b)
         else:
             slots = cache.write_slots(b)
-        pos = positions.reshape(b)
-        q = torch.empty((b, hk, hq // hk, hd), dtype=torch.float16, device=self.device)
-        o = torch.empty_like(q)                                    # = [B, hq * hd], contiguous
-        # The token embedding lookup and the first norm are one launch; the
-        # residual is carried into the next norm, which adds and normalises
-        # in one launch (the reference's _run_layers_fused,
-        # model/latentserve_qwen.py:425-450); the last add goes into the
-        # final norm.
-        h, residual = fe.embed_rms_norm(self.embed, token_ids.reshape(b), self.layers[0].norm1,
-                                        eps)
-        x = None
-        for li, layer in enumerate(self.layers):
-            # with packed weights at decode batch sizes the norm before a
-            # projection runs in that projection's prologue (x + residual is
-            # written to a new buffer: it may not alias its inputs)
-            fold1 = li > 0 and _norm_folds(x, layer.p_qkv)
-            if li > 0 and not fold1:
-                h, residual = fe.fused_add_rms_norm(x, residual, layer.norm1, eps)
-            kmin = kmax = None
-            if self.sparse_ratio is not None:
-                kmin, kmax = cache.page_bounds(li)
-            # the q/k/v projection, RoPE, the K/V store at this step's slots
-            # (and the page bounds) and q folded to [B, hk, n_rep, hd]: one
-            # launch at decode batch sizes (the projection's epilogue)
-            wq = layer.p_qkv if layer.p_qkv is not None else layer.w_qkv
-            kdst, vdst = (stage_k, stage_v) if staged else (cache.k_pool[li], cache.v_pool[li])
-            if fold1:
-                _, residual = dg.qkv_rope_write(
-                    x, wq, layer.b_qkv, pos, self.rope.cos, self.rope.sin, slots,
-                    kdst, vdst, hq, hk, q_out=q, kmin=kmin, kmax=kmax,
-                    residual=residual, norm_weight=layer.norm1, eps=eps)
-            elif b <= HIP_DECODE_MAX_ROWS and dg.supports(h, wq):
-                if wq is layer.p_qkv and dg.workspace_bytes(b, *layer.w_qkv.shape):
-                    wq = layer.w_qkv                 # K splits: the GEMM, then the RoPE write
-                dg.qkv_rope_write(h, wq, layer.b_qkv, pos, self.rope.cos, self.rope.sin,
-                                  slots, kdst, vdst, hq, hk, q_out=q, kmin=kmin, kmax=kmax)
-            else:
-                qkv = F.linear(h, layer.w_qkv, layer.b_qkv)       # [B, (hq + 2 hk) hd]
-                fe.rope_write_decode(qkv, pos, self.rope.cos, self.rope.sin, slots,
-                                     kdst, vdst, hq, hk, q_out=q, kmin=kmin, kmax=kmax)
+
+        def attend(li, layer, q, o, kmin, kmax):
             if staged:
                 # INT8: V quantized into the pool, K into the sequence's residual row;
                 # 4 bits: both into the pools
@@ -289,6 +261,10 @@ class QwenDecoder:
                     k_zero=cache.k_zero_pool[li] if cache.asymmetric else None,
                     v_zero=cache.v_zero_pool[li] if cache.asymmetric else None,
                     k_residual=cache.residual(li), res_rows=res_rows, out=o)
+            elif sums is not None:
+                ce.paged_decode_weights(q, cache.k_pool[li], cache.v_pool[li], tables, lens,
+                                        sums[li], rows=rows, max_seq_len=max_position + 1,
+                                        softmax_scale=self.scale, out=o)
             elif self.sparse_ratio is None:
                 pdh.paged_decode_hip(q, cache.k_pool[li], cache.v_pool[li], tables, lens,
                                      max_seq_len=max_position + 1,
@@ -301,6 +277,114 @@ class QwenDecoder:
                                     recent=layer.attn.sparse_recent, max_seq_len=ctx,
                                     softmax_scale=self.scale, out=o,
                                     scoring=layer.attn.sparse_scoring)
+        logits = self._run_layers(token_ids.reshape(b), positions.reshape(b), slots, attend,
+                                  self.sparse_ratio is not None)
+        return logits.view(b, 1, -1)
+
+    @torch.no_grad()
+    def tree_forward(self, token_ids: torch.Tensor, positions: torch.Tensor,
+                     masks: torch.Tensor, max_position: int,
+                     counts: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """A pass over a tree of drafted tokens of each active sequence: token_ids and
+        positions [B, N] int64 (a node's position: its context's length and its depth),
+        masks as tree_masks() gives them, counts [B] int32 (None: N) -> logits [B, N,
+        vocab].  The fp16 cache has been advanced by N; accept() ends the step (and
+        brings the page bounds of sparse steps up to date)."""
+        cache = self.cache
+        if not isinstance(cache, PagedKVCache):
+            raise ValueError("a tree's attention reads fp16 pools")
+        b, n = token_ids.shape
+        tables, lens = cache.block_tables_tensor(b), cache.seq_lens_tensor(b)
+        keep = cache.weight_sums is not None
+        self._tree = [] if keep else None
+
+        def attend(li, layer, q, o, kmin, kmax):
+            q = q.view(b, n, *q.shape[1:])
+            lse = None
+            if keep:
+                q = q.clone()                          # (the next layer's takes its place)
+                lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device)
+                self._tree.append((q, lse))
+            ta.tree_attention(q, cache.k_pool[li], cache.v_pool[li], tables, lens, masks, counts,
+                              max_seq_len=max_position + n, softmax_scale=self.scale,
+                              out=o.view(q.shape), lse=lse)
+
+        logits = self._run_layers(token_ids.reshape(-1), positions.reshape(-1),
+                                  cache._slots_for_write(b, n).reshape(-1), attend, False)
+        return logits.view(b, n, -1)
+
+    @torch.no_grad()
+    def accept(self, token_ids: torch.Tensor, parents: torch.Tensor, choices: torch.Tensor,
+               counts: Optional[torch.Tensor] = None) -> ta.AcceptedTokens:
+        """The drafted tokens of the last tree_forward() that `choices` [B, N] confirm kept,
+        the others let go (the cache's accept()); where the cache keeps weight sums,
+        the kept tokens' attention is added to them."""
+        cache, tree = self.cache, self._tree
+        if cache.weight_sums is not None and \
+                (tree is None or tree[0][0].shape[:2] != token_ids.shape):
+            raise RuntimeError("accept() ends the step of a tree_forward() of the same tokens")
+        got = cache.accept(token_ids, parents, choices, counts)
+        if tree is not None:
+            b, n = token_ids.shape
+            tables, lens = cache.block_tables_tensor(b), cache.seq_lens_tensor(b)
+            for li, (q, lse) in enumerate(tree):
+                ce.add_weights(q, lse, cache.k_pool[li], tables, lens, cache.weight_sums[li],
+                               rows=cache.sum_rows_tensor(b), path=got.path, lengths=got.lengths,
+                               max_seq_len=cache.max_len, softmax_scale=self.scale)
+            self._tree = None
+        return got
+
+    def _run_layers(self, tokens: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor,
+                    attend, bounds: bool) -> torch.Tensor:
+        """Logits [M, vocab] of M rows: tokens and positions [M], K and V stored at `slots`
+        (of the stage, where the cache quantizes; with `bounds`, the page bounds brought
+        up to date, which rows of one page cannot do at once), attend(layer number, layer,
+        q [M, hk, n_rep, hd], o, kmin, kmax) once they are."""
+        cfg, cache = self.cfg, self.cache
+        b = tokens.shape[0]
+        hq, hk, hd = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim
+        eps = cfg.rms_norm_eps
+        staged = self._stage is not None
+        q = torch.empty((b, hk, hq // hk, hd), dtype=torch.float16, device=self.device)
+        o = torch.empty_like(q)                                    # = [B, hq * hd], contiguous
+        # The token embedding lookup and the first norm are one launch; the
+        # residual is carried into the next norm, which adds and normalises
+        # in one launch (the reference's _run_layers_fused,
+        # model/latentserve_qwen.py:425-450); the last add goes into the
+        # final norm.
+        h, residual = fe.embed_rms_norm(self.embed, tokens, self.layers[0].norm1,
+                                        eps)
+        x = None
+        for li, layer in enumerate(self.layers):
+            # with packed weights at decode batch sizes the norm before a
+            # projection runs in that projection's prologue (x + residual is
+            # written to a new buffer: it may not alias its inputs)
+            fold1 = li > 0 and _norm_folds(x, layer.p_qkv)
+            if li > 0 and not fold1:
+                h, residual = fe.fused_add_rms_norm(x, residual, layer.norm1, eps)
+            kmin = kmax = None
+            if bounds:
+                kmin, kmax = cache.page_bounds(li)
+            # the q/k/v projection, RoPE, the K/V store at this step's slots
+            # (and the page bounds) and q folded to [B, hk, n_rep, hd]: one
+            # launch at decode batch sizes (the projection's epilogue)
+            wq = layer.p_qkv if layer.p_qkv is not None else layer.w_qkv
+            kdst, vdst = self._stage[:2] if staged else (cache.k_pool[li], cache.v_pool[li])
+            if fold1:
+                _, residual = dg.qkv_rope_write(
+                    x, wq, layer.b_qkv, pos, self.rope.cos, self.rope.sin, slots,
+                    kdst, vdst, hq, hk, q_out=q, kmin=kmin, kmax=kmax,
+                    residual=residual, norm_weight=layer.norm1, eps=eps)
+            elif b <= HIP_DECODE_MAX_ROWS and dg.supports(h, wq):
+                if wq is layer.p_qkv and dg.workspace_bytes(b, *layer.w_qkv.shape):
+                    wq = layer.w_qkv                 # K splits: the GEMM, then the RoPE write
+                dg.qkv_rope_write(h, wq, layer.b_qkv, pos, self.rope.cos, self.rope.sin,
+                                  slots, kdst, vdst, hq, hk, q_out=q, kmin=kmin, kmax=kmax)
+            else:
+                qkv = F.linear(h, layer.w_qkv, layer.b_qkv)       # [B, (hq + 2 hk) hd]
+                fe.rope_write_decode(qkv, pos, self.rope.cos, self.rope.sin, slots,
+                                     kdst, vdst, hq, hk, q_out=q, kmin=kmin, kmax=kmax)
+            attend(li, layer, q, o, kmin, kmax)
             x = _linear(o.view(b, hq * hd), layer.w_o, layer.p_o)
             if _norm_folds(x, layer.p_gate_up):
                 h, residual = dg.gate_up_silu(x, layer.p_gate_up, residual=residual,
@@ -312,6 +396,6 @@ class QwenDecoder:
         if _norm_folds(x, self.p_lm_head):
             logits, _ = dg.linear(x, self.p_lm_head, residual=residual, norm_weight=self.norm,
                                   eps=eps)
-            return logits.view(b, 1, -1)
+            return logits
         h, _ = fe.fused_add_rms_norm(x, residual, self.norm, eps)
-        return _linear(h, self.lm_head, self.p_lm_head).view(b, 1, -1)
+        return _linear(h, self.lm_head, self.p_lm_head)

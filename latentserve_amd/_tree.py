@@ -86,6 +86,22 @@ _MAX_WIDTH = 1 << 24            # pages of a block table
 _MAX_TOKEN_STRIDE = 1 << 24     # elements
 
 
+_STRIDES: dict = {}             # contiguous rows' strides by their shapes
+
+
+def whole_rows(shape: torch.Size):
+    """The strides of contiguous rows of a shape [..., 128], as C int64."""
+    got = _STRIDES.get(shape)
+    if got is None:
+        st = [HEAD_DIM]
+        for n in shape[-2:0:-1]:
+            st.insert(0, st[0] * n)
+        if len(_STRIDES) >= 4096:
+            _STRIDES.clear()
+        got = _STRIDES[shape] = _lib._I64N[len(st)](*st)
+    return got
+
+
 def rows(name: str, t: torch.Tensor):
     """The strides of checked rows [..., 128]; a dimension of one row has none that
     matters."""
@@ -93,6 +109,8 @@ def rows(name: str, t: torch.Tensor):
         raise ValueError(f"{name} must be float16, got {t.dtype}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient, which a cache's attention does not record")
+    if t.is_contiguous() and not t.data_ptr() & 15:
+        return whole_rows(t.shape)
     *st, unit = t.stride()
     st = [s if n > 1 else 0 for s, n in zip(st, t.shape)]
     bits = t.data_ptr()

@@ -107,11 +107,12 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     stream = _lib.stream_of(dev)
     if out is None:
         out = torch.empty(shape, dtype=torch.float16, device=dev)
+        os = _tree.whole_rows(shape)
     else:
         if out.shape != shape or out.get_device() != index:
             raise ValueError(f"out must be {tuple(shape)} on {dev}")
         _tree.apart("out", out, q)
-    os = _tree.rows("out", out)
+        os = _tree.rows("out", out)
     if index != _serving.current_device():
         with torch.cuda.device(dev):
             return tree_attention(q, k_pool, v_pool, block_tables, seq_lens, masks, counts,

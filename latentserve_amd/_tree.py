@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import operator
+from array import array as Array
 from typing import List, Optional
 
 import torch
@@ -191,6 +192,9 @@ def apart(name: str, out: torch.Tensor, q: torch.Tensor) -> None:
             raise ValueError(f"{name} may not overlap q, which other workgroups still read")
 
 
+_FP16 = {torch.float16}
+
+
 def pool_lists(k_pools, v_pools):
     """(heads, blocks, strides, device, two C arrays of addresses) of checked layers' pools
     that are written to."""
@@ -204,17 +208,19 @@ def pool_lists(k_pools, v_pools):
     at = list(map(torch.Tensor.data_ptr, pools))
     if len(set(map(torch.Tensor.size, pools))) > 1 or len(set(map(torch.Tensor.stride, pools))) > 1 \
             or len(set(map(torch.Tensor.get_device, pools))) > 1 \
-            or any([t.dtype is not torch.float16 for t in pools]) or functools.reduce(operator.or_, at) & 15:
+            or set(map(torch.Tensor.dtype.__get__, pools)) != _FP16 \
+            or functools.reduce(operator.or_, at) & 15:
         raise ValueError("the layers' pools must be alike: float16 "
                          f"{tuple(first.shape)}, of the same strides, on one device")
     st = first.stride()
     if nb > 1 and st[0] < PAGE * h * HEAD_DIM or st[1] < h * HEAD_DIM \
             or (h > 1 and st[2] < HEAD_DIM):
         raise ValueError("pools whose rows overlap cannot be written")
-    if torch.is_grad_enabled() and any([t.requires_grad for t in pools]):
+    if torch.is_grad_enabled() and any(map(torch.Tensor.requires_grad.__get__, pools)):
         raise ValueError("a move of cached tokens records no gradient")
     array = ctypes.c_void_p * n
-    return h, nb, steps, first.device, array(*at[:n]), array(*at[n:])
+    both = (array * 2).from_buffer_copy(Array("Q", at))
+    return h, nb, steps, first.device, both[0], both[1]
 
 
 # Workspace bytes by a call's sizes.

@@ -109,7 +109,7 @@ int ls_accept_tokens(const int64_t* tokens, const int32_t* parents, const int64_
  * first `sinks`, the last `recent`, and the largest sums (a NaN before all numbers;
  * equal ones: the lower position).  keep [layers, batch, kv_heads, budget] int32 (-1 behind
  * the last), kept (fp32, the same shape; 0 behind the last): their sums.  sinks +
- * recent <= budget.  Positions past sum_len count as none. */
+ * recent <= budget.  Positions past sum_len (at most 2^30) count as none. */
 int ls_select_tokens(const float* sums, const int64_t* sum_strides, int64_t sum_len,
                      const int32_t* seq_lens, int32_t* keep, float* kept, int layers, int batch,
                      int kv_heads, int budget, int sinks, int recent, void* stream);

@@ -14,6 +14,11 @@
 // K and V go to LDS by direct loads, whole rows of 256 bytes (16 lanes a row): K's 16-byte
 // piece p of key r at place p ^ (r % 16), V's 32-byte units swapped by row too, so that
 // neither the row reads of K nor the transposing reads of V meet in a bank.
+//
+// Bound by K's and V's bytes up to about 100 rows (16 sequences of 16K, 2 heads: 12 rows with
+// scores 52 us, 5.2 TB/s; 96 rows 56 us), then by the products and exponentials, which a
+// SIMD's two waves do one after the other for the most part (198 rows: 2.2 us a step of 64 keys,
+// the matrix units busy 38 % of the time, the vector units 43 %).
 #include "ls_common.h"
 #include "ls_tree.h"
 #include "ls_tree_load.h"
@@ -1053,6 +1058,13 @@ hipError_t launch(const TreeParams& a, hipStream_t stream) {
 
 constexpr int TREE_CUS = 256;
 
+// Up to 16 rows, products of 16: of 32 they would be half empty (12 rows, 1 / 16 sequences of
+// 16K: 14.7 / 51.2 us against 15.9 / 54.8).  Up to 32, a wave has all rows and its own keys, and
+// waits for nobody (30 rows: 16.8 / 55.3 us, with tiles of two row groups 18.4 / 55.7).  Beyond,
+// row groups share a tile: up to 64 rows of four waves, which start and end sooner (48 rows, 2K
+// keys 12.7 us, 16 x 16K 63; of eight 16.0 and 60), up to 128 two key groups of eight (96 rows:
+// 21.4 / 65 us; 24.2 / 71 with one), then one.  Fewer than two steps a run cost more in
+// records than they give in groups.
 TreeShape tree_shape(int batch, int kv_heads, int rows, int64_t keys_bound) {
     TreeShape s;
     s.rows = rows <= 16 ? 16 : 32;

@@ -4,7 +4,8 @@
 //
 // No V and no softmax state, so a key's sum is one workgroup's: S = Q K^T (32x32x16 MFMA,
 // rows by keys), a lane holds one key and 16 of 32 rows.  K goes to LDS as in the tree
-// attention.  Bound by K's bytes.
+// attention.  Bound by K's bytes: 16 x 16K keys of 2 heads, 30 rows, 26 to 29 us (4.8 TB/s;
+// 45 with a workgroup's tiles loaded, awaited and multiplied once).
 #include "ls_common.h"
 #include "ls_tree.h"
 #include "ls_tree_load.h"
@@ -20,7 +21,9 @@ constexpr int WEIGH_NW = 2, WEIGH_AHEAD = 1;               // waves, tiles on th
 constexpr int WEIGH_LOADS = 9;                             // of a tile
 
 // A wave has tiles of 32 keys to itself, every gridDim.x * WEIGH_NW-th of a head's; the next
-// three and their sums are on their way to its ring while one is multiplied.
+// one and its sums are on their way to the other buffer while one is multiplied.  Four workgroups
+// of two waves fill a CU's LDS (16 x 16K / 48 x up to 1.5K keys: 29.1 / 23.0 us; three tiles
+// ahead, one workgroup of four waves 30.8 / 29.1, four of one wave 30.4 / 30.6).
 struct WeighTile {
     char k[32 * 256];
     float sums[WAVE];
@@ -174,7 +177,7 @@ __global__ __launch_bounds__(WAVE* WEIGH_NW) void add_weights_kernel(const Weigh
 }  // namespace
 
 hipError_t launch_add_weights(const WeighParams& a, int64_t keys_bound, hipStream_t stream) {
-    // a workgroup fills a CU's LDS: as many as CUs, or one a head and sequence
+    // as many workgroups as fit at once, or one a head and sequence
     const int64_t most = (keys_bound + 32 * WEIGH_NW - 1) / (32 * WEIGH_NW);
     int64_t parts = 1024 / ((int64_t)a.H * a.B);
     parts = parts < most ? parts : most;

@@ -3,6 +3,8 @@ CPU, with plain forms of the operators in the kernels' place."""
 
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -242,3 +244,11 @@ def test_sums_follow_a_sequence(plain):
             c.evict(bad)
     with pytest.raises(ValueError, match="does not hold"):
         c.evict(8, sinks=4, recent=5)
+
+
+def test_selection_of_rows_longer_than_any_cache_is_refused():
+    from latentserve_amd import _tree
+    lib = _tree.lib()
+    st = (ctypes.c_int64 * 3)(1 << 33, 1 << 33, 1 << 32)
+    args = (st, (1 << 30) + 1, 64, 1 << 13, 1 << 14, 1, 1, 1, 8, 1, 1, None)
+    assert lib.ls_select_tokens(1 << 12, *args) == 1

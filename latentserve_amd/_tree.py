@@ -206,7 +206,10 @@ def pool_lists(k_pools, v_pools):
     pools = [*k_pools, *v_pools]
     # (an attribute of all at a time: half the host time of a loop over 56 pools)
     at = list(map(torch.Tensor.data_ptr, pools))
-    if len(set(map(torch.Tensor.size, pools))) > 1 or len(set(map(torch.Tensor.stride, pools))) > 1 \
+    # (contiguous tensors of a size have the same strides, where a stride matters)
+    alike = all(map(torch.Tensor.is_contiguous, pools)) if first.is_contiguous() else \
+        len(set(map(torch.Tensor.stride, pools))) == 1
+    if len(set(map(torch.Tensor.size, pools))) > 1 or not alike \
             or len(set(map(torch.Tensor.get_device, pools))) > 1 \
             or set(map(torch.Tensor.dtype.__get__, pools)) != _FP16 \
             or functools.reduce(operator.or_, at) & 15:

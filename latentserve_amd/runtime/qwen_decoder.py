@@ -289,10 +289,9 @@ class QwenDecoder:
         positions [B, N] int64 (a node's position: its context's length and its depth),
         masks as tree_masks() gives them, counts [B] int32 (None: N) -> logits [B, N,
         vocab].  The fp16 cache has been advanced by N; accept() ends the step (and
-        brings the page bounds of sparse steps up to date)."""
-        cache = self.cache
-        if not isinstance(cache, PagedKVCache):
-            raise ValueError("a tree's attention reads fp16 pools")
+        brings the page bounds of sparse steps up to date).  Not to be captured: each
+        advance() has the slots of its N tokens in a tensor of its own."""
+        cache = self._fp16_cache()
         b, n = token_ids.shape
         tables, lens = cache.block_tables_tensor(b), cache.seq_lens_tensor(b)
         keep = cache.weight_sums is not None
@@ -319,7 +318,7 @@ class QwenDecoder:
         """The drafted tokens of the last tree_forward() that `choices` [B, N] confirm kept,
         the others let go (the cache's accept()); where the cache keeps weight sums,
         the kept tokens' attention is added to them."""
-        cache, tree = self.cache, self._tree
+        cache, tree = self._fp16_cache(), self._tree
         if cache.weight_sums is not None and \
                 (tree is None or tree[0][0].shape[:2] != token_ids.shape):
             raise RuntimeError("accept() ends the step of a tree_forward() of the same tokens")
@@ -333,6 +332,11 @@ class QwenDecoder:
                                max_seq_len=cache.max_len, softmax_scale=self.scale)
             self._tree = None
         return got
+
+    def _fp16_cache(self) -> PagedKVCache:
+        if not isinstance(self.cache, PagedKVCache):
+            raise ValueError("a tree's attention reads fp16 pools")
+        return self.cache
 
     def _run_layers(self, tokens: torch.Tensor, pos: torch.Tensor, slots: torch.Tensor,
                     attend, bounds: bool) -> torch.Tensor:

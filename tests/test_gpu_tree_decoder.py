@@ -67,11 +67,11 @@ def close(got, want):
     assert err <= LOGITS * want.abs().max().item() + SMALL, err
 
 
-@pytest.mark.parametrize("steps", [1, 37])
-def test_every_node_sees_its_path(steps):
+@pytest.mark.parametrize("steps,n", [(1, 9), (37, 9), (20, 50)])
+def test_every_node_sees_its_path(steps, n):
     m = make_model(cap=128, batch=2, seed=2)
     ids = context(m, steps)
-    tokens, parents, _, _ = tree(m)
+    tokens, parents, _, _ = tree(m, n)
     logits = tree_pass(m, tokens, parents, steps)
     for b in range(2):
         for i in range(tokens.shape[1]):
@@ -115,6 +115,17 @@ def test_the_kept_path_is_the_context_of_the_next_step():
         want = rep * (len(ids[b]) - 30 + 1)
         assert ((sums.sum(-1) - want).abs() <= ONE * want).all()
         assert (sums[..., length:] == 0).all() and (sums[..., :length] > 0).all()
+
+
+@pytest.mark.parametrize("kv_dtype", ["int8", "int4"])
+def test_quantized_caches_are_refused(kv_dtype):
+    m = make_model(cap=64, batch=2, seed=4)
+    m.allocate_cache(2, 64, kv_dtype=kv_dtype)
+    tokens, parents, choices, _ = tree(m)
+    with pytest.raises(ValueError, match="fp16"):
+        m.tree_forward(tokens, tokens, parents, max_position=20)
+    with pytest.raises(ValueError, match="fp16"):
+        m.accept(tokens, parents, choices)
 
 
 def test_accept_without_its_pass_is_refused():

@@ -167,3 +167,41 @@ def test_graphs_of_acceptance_and_eviction():
             again()
             for x, y in zip([*step(), *args[1:3]], want):
                 assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("lens", [[300, 256, 20], [1500]])
+def test_the_largest_trees(lens):
+    from tests.test_gpu_tree_attention import check
+    check(*case(lens, 256, 1, 16, 98))
+
+
+@pytest.mark.parametrize("b,h,r", [(300, 4, 6), (70, 1, 16), (65, 8, 1)])
+def test_decode_weights_of_many_sequences(b, h, r):
+    """More sequences than are dealt whole, some without a token."""
+    lens = [(37 * i) % 90 for i in range(b)]
+    q, k, v, t, l, _ = case(lens, 1, h, r, 99)
+    sums = torch.zeros(b, h, t.shape[1] * 16, device="cuda")
+    print(f"decode weights of {b}", flush=True)
+    out = ce().paged_decode_weights(dev(q[:, 0]), dev(k), dev(v), dev(t), dev(l), sums)
+    want, lse, tol, _ = ref.attend(q, k, v, t, l)
+    assert (np.abs(out.double().cpu().numpy() - want[:, 0]) <= tol[:, 0]).all()
+    add, atol = ref.path_weights(q, lse, k, t, l, np.zeros((b, 1), np.int32), np.ones(b, np.int32))
+    n = add.shape[2]
+    got = sums.double().cpu().numpy()
+    assert (np.abs(got[..., :n] - add) <= 2 * atol + add * 2.0 ** -16).all()
+    assert (got[..., n:] == 0).all()
+
+
+def test_a_longer_batch_leaves_rows_behind_the_last_sequence():
+    """out and lse of a larger buffer, pools' unused pages and the sums' other rows stay."""
+    q, k, v, t, l, seen = case([70, 33], 5, 2, 6, 100)
+    big = torch.full((4, 5, 2, 6, 128), 7.0, dtype=torch.float16, device="cuda")
+    lse = torch.full((4, 5, 2, 6), 7.0, device="cuda")
+    ta().tree_attention(dev(q), dev(k), dev(v), dev(t), dev(l), dev(ref.words_of(seen)),
+                        out=big[:2], lse=lse[:2])
+    assert (big[2:] == 7).all() and (lse[2:] == 7).all() and not (big[:2] == 7).all()
+    sums = torch.full((5, 2, 100), 3.0, device="cuda")
+    rows = dev(np.array([4, 1], np.int32))
+    ce().paged_decode_weights(dev(q[:, 0]), dev(k), dev(v), dev(t), dev(l), sums, rows)
+    assert (sums[[0, 2, 3]] == 3).all() and (sums[4, :, 70:] == 3).all() and (sums[1, :, 33:] == 3).all()
+    assert (sums[4, :, :70] > 3).all()

@@ -215,6 +215,8 @@ def pool_lists(k_pools, v_pools):
             or functools.reduce(operator.or_, at) & 15:
         raise ValueError("the layers' pools must be alike: float16 "
                          f"{tuple(first.shape)}, of the same strides, on one device")
+    if len(set(at)) < 2 * n:
+        raise ValueError("a pool is listed twice: its rows would be moved twice")
     st = first.stride()
     if nb > 1 and st[0] < PAGE * h * HEAD_DIM or st[1] < h * HEAD_DIM \
             or (h > 1 and st[2] < HEAD_DIM):

@@ -252,3 +252,15 @@ def test_selection_of_rows_longer_than_any_cache_is_refused():
     st = (ctypes.c_int64 * 3)(1 << 33, 1 << 33, 1 << 32)
     args = (st, (1 << 30) + 1, 64, 1 << 13, 1 << 14, 1, 1, 1, 8, 1, 1, None)
     assert lib.ls_select_tokens(1 << 12, *args) == 1
+
+
+def test_a_pool_listed_twice_is_refused():
+    a, b, c = (torch.zeros(4, 16, 2, 128, dtype=torch.float16) for _ in range(3))
+    tables, lens = torch.zeros(1, 4, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    keep = torch.zeros(2, 1, 2, 3, dtype=torch.int32)
+    one = torch.zeros(1, 1, dtype=torch.int64)
+    for k, v in (([a, a], [b, c]), ([a, b], [c, a]), ([a, b], [a, b])):
+        with pytest.raises(ValueError, match="twice"):
+            ce.move_tokens(keep, k, v, tables, lens)
+        with pytest.raises(ValueError, match="twice"):
+            ta.accept_tokens(one, one.int(), one, k, v, tables, lens)

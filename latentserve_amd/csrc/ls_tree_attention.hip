@@ -1063,8 +1063,9 @@ constexpr int TREE_CUS = 256;
 // waits for nobody (30 rows: 16.8 / 55.3 us, with tiles of two row groups 18.4 / 55.7).  Beyond,
 // row groups share a tile: up to 64 rows of four waves, which start and end sooner (48 rows, 2K
 // keys 12.7 us, 16 x 16K 63; of eight 16.0 and 60), up to 128 two key groups of eight (96 rows:
-// 21.4 / 65 us; 24.2 / 71 with one), then one.  Fewer than two steps a run cost more in
-// records than they give in groups.
+// 21.4 / 65 us; 24.2 / 71 with one), then one.  A run has a step at least
+// (6 / 48 / 96 rows, 2K keys: 10.6 / 12.2 / 15.7 us against 11.6 / 12.8 / 16.9 of two), of more
+// than 128 rows two, whose records cost more than groups give (240 rows, 4K: 20.2 against 23.1).
 TreeShape tree_shape(int batch, int kv_heads, int rows, int64_t keys_bound) {
     TreeShape s;
     s.rows = rows <= 16 ? 16 : 32;
@@ -1076,7 +1077,7 @@ TreeShape tree_shape(int batch, int kv_heads, int rows, int64_t keys_bound) {
     const int64_t units = (int64_t)batch * kv_heads;
     const int64_t places = units * ((keys_bound + step - 1) / step + TREE_EXTRA);
     int64_t most = (TREE_CUS + s.row_tiles - 1) / s.row_tiles;
-    const int64_t useful = (places + 1) / 2;               // (two steps a run at least)
+    const int64_t useful = s.wr == 8 ? (places + 1) / 2 : places;
     s.groups = (int)(most < useful ? most : useful);
     if (s.groups < 1) s.groups = 1;
     return s;

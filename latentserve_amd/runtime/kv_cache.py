@@ -180,8 +180,9 @@ class BlockTable:
         # bumped when the block list is replaced rather than extended: a
         # mirror that saw an older lineage re-uploads the whole row
         self.lineage = 0
-        # tokens were evicted: row p is no longer token p
-        self.evicted = False
+        # tokens that were evicted: rows are no longer the tokens of their numbers, and the
+        # next token's position is length + dropped
+        self.dropped = 0
 
     @property
     def capacity(self) -> int:
@@ -224,7 +225,7 @@ class BlockTable:
         self.length = 0
         self.version += 1
         self.lineage += 1
-        self.evicted = False
+        self.dropped = 0
 
 
 @dataclass
@@ -343,6 +344,9 @@ class _PagedBase:
         self._active: List[int] = list(range(spec.max_batch_size))
         self._batch = 0                       # rows published by the last advance()
         self._chunk_slots: Optional[torch.Tensor] = None    # multi-token write slots
+        # Positions that the model has (None: no bound but the cache's capacity).  Sequences
+        # that lost tokens get past the capacity.
+        self.max_positions: Optional[int] = None
         # When set (a graph runner's bucket), sparse selection is sized for it.
         self.sparse_context_hint: Optional[int] = None
 
@@ -350,6 +354,11 @@ class _PagedBase:
     @property
     def seq_lens(self) -> List[int]:
         return [self.tables[s].length for s in self._active]
+
+    @property
+    def seq_positions(self) -> List[int]:
+        """The active sequences' next positions: tokens held and tokens evicted."""
+        return [self.tables[s].length + self.tables[s].dropped for s in self._active]
 
     @property
     def max_len(self) -> int:
@@ -394,7 +403,7 @@ class _PagedBase:
         prefix cache may hand them to another sequence (of a sequence that lost
         tokens, none: its pages are not of the prompt's first tokens)."""
         t = self.tables[index]
-        return 0 if t.evicted else t.length // self.block_size
+        return 0 if t.dropped else t.length // self.block_size
 
     # ---- branching and compaction -------------------------------------------
     def _page_tensors(self) -> List[torch.Tensor]:
@@ -435,7 +444,7 @@ class _PagedBase:
             self.allocator.incref(pages)
             child.blocks = list(pages)
             child.length = t.length
-            child.evicted = t.evicted
+            child.dropped = t.dropped
             child.version += 1
             child.lineage += 1
 
@@ -449,6 +458,11 @@ class _PagedBase:
         spans, grown = [], 0
         for s in seqs:
             t = self.tables[s]
+            if t.dropped and self.max_positions is not None \
+                    and t.length + t.dropped + n > self.max_positions:
+                raise RuntimeError(f"the sequence in slot {s} would reach position "
+                                   f"{t.length + t.dropped + n - 1}; the model was given "
+                                   f"{self.max_positions}")
             first, have, end = t.length // bs, len(t.blocks), -(-(t.length + n) // bs)
             if end > have:
                 if end > self.capacity_pages:
@@ -728,9 +742,9 @@ class PagedKVCache(_PagedBase):
         the budget) and those with the largest weight sums of the others, moved to
         the front (kernels.hip.cache_eviction.evict_tokens).  Their pages behind go
         back to the pool; pages that others hold are copied first.  Returns the slots
-        that lost tokens.  A token's position is the caller's to count on: the
-        sequence's length no longer is it.  Between steps only, as fork();
-        OutOfBlocks leaves every sequence as it was."""
+        that lost tokens.  A sequence's length then is no longer its next token's
+        position (seq_positions).  Between steps only, as fork(); OutOfBlocks leaves
+        every sequence as it was."""
         from latentserve_amd.kernels.hip import cache_eviction as ce
 
         if self.weight_sums is None:
@@ -753,12 +767,12 @@ class PagedKVCache(_PagedBase):
         self.weight_sums[:, at] = 0
         self.weight_sums[:, at, :, :budget] = kept
         for s, t in zip(seqs, tables):
+            t.dropped += t.length - budget
             t.length = budget
             self.allocator.free(t.blocks[pages:])
             t.blocks = t.blocks[:pages]
             t.version += 1
             t.lineage += 1
-            t.evicted = True
             self._bound_pages(s, 0)
         if self._batch:
             self._publish(0, [self.tables[s].length for s in self._active])

@@ -177,7 +177,7 @@ class QwenDecoder:
         (Int8PagedKVCache: int8 pools, fp32 scales, the fp16 last-page K
         residual) or 4 bits (Int4PagedKVCache).  max_positions (default:
         max_seq_len): where tokens are evicted, sequences get longer than what
-        the cache holds of them."""
+        the cache holds of them, up to this."""
         spec = KVCacheSpec(num_layers=self.cfg.num_layers, num_kv_heads=self.cfg.num_kv_heads,
                            head_dim=self.cfg.head_dim, max_batch_size=max_batch_size,
                            max_seq_len=max_seq_len, device=str(self.device))
@@ -199,6 +199,7 @@ class QwenDecoder:
             raise ValueError(f"kv_dtype must be 'fp16', 'int8' or 'int4', got {kv_dtype!r}")
         self.rope = Rope(self.cfg.head_dim, self.cfg.rope_theta,
                          max(max_seq_len, max_positions or 0), self.device)
+        self.cache.max_positions = self.rope.max_seq_len
         self._tree = None
         return self.cache
 

@@ -189,7 +189,9 @@ def test_evict_keeps_a_budget_and_gives_pages_back(plain):
     assert c.seq_lens_tensor().tolist() == [33, 33, 30]
     assert c.block_tables_tensor()[0, :3].tolist() == c.tables[0].blocks
     assert c.evict(33) == []
+    assert c.seq_positions == [70, 70, 30]
     grow(c, [0, 3, 5], [[90], [190], [290]])                      # and the sequence goes on
+    assert c.seq_positions == [71, 71, 31]
     assert held(c, 0)[1][0][-1] == 90
 
 
@@ -264,3 +266,24 @@ def test_a_pool_listed_twice_is_refused():
             ce.move_tokens(keep, k, v, tables, lens)
         with pytest.raises(ValueError, match="twice"):
             ta.accept_tokens(one, one.int(), one, k, v, tables, lens)
+
+
+def test_a_bounded_sequence_ends_where_the_positions_do(plain):
+    c = cache()
+    c.max_positions = 70
+    c.enable_weight_sums()
+    grow(c, [0, 1], [list(range(60)), list(range(60))])
+    c.evict(20, sinks=1, recent=4, slots=[0])
+    grow(c, [0], [list(range(60, 70))])
+    assert c.seq_positions == [70] and c.seq_lens == [30]
+    c.fork(0, [2])
+    for slots in ([0], [1, 2]):
+        before = [list(t.blocks) for t in c.tables], [t.length for t in c.tables]
+        with pytest.raises(RuntimeError, match="position 70"):
+            c.advance(1, slots=slots)
+        assert ([list(t.blocks) for t in c.tables], [t.length for t in c.tables]) == before
+    c.rewind(25, slots=[0])
+    grow(c, [0], [[65]])
+    c.free_sequence(0)
+    grow(c, [0], [list(range(80))])                               # (no bound but the capacity)
+    assert c.seq_positions == [80]

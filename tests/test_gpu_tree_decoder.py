@@ -176,6 +176,7 @@ def test_a_bounded_cache_keeps_what_got_attention(graphed):
         pos = torch.full((3, 1), t, dtype=torch.long, device="cuda")
         out = dec.step(ids[:, t:t + 1], pos, slots=[2, 0, 1])
         steps += 1
+        assert c.seq_positions == [t + 1] * 3
         assert out.isfinite().all()
         if c.max_len < 90:
             continue

@@ -846,15 +846,31 @@ void tree_kernel(const TreeParams a) {
         if (whole) {
             const bool seeing = row.is && row.node < nodes;
             const float inv = seeing && l != 0.f ? 1.f / l : 0.f;
-            if (row.is) {
-                half_t* o = a.out + u.b * a.so_b + row.node * a.so_n + u.h * a.so_h + row.rep * a.so_r;
+            half_t* o = a.out + u.b * a.so_b + row.node * a.so_n + u.h * a.so_h + row.rep * a.so_r;
+            u2 x[QUADS];
 #pragma unroll
-                for (int n = 0; n < QUADS; ++n) {
-                    h4 x;
+            for (int n = 0; n < QUADS; ++n) {
+                h4 z;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = seeing ? (half_t)(y[n][e] * inv) : (half_t)0.f;
-                    *(h4*)(o + T::channel_of(kg * QUADS + n) + 4 * t.h) = x;
+                for (int e = 0; e < 4; ++e) z[e] = seeing ? (half_t)(y[n][e] * inv) : (half_t)0.f;
+                x[n] = __builtin_bit_cast(u2, z);
+            }
+            if constexpr (T::HB == 2) {
+                // a row's two lanes hold four channels each of eight: of two such eights, each
+                // lane gets one whole (16 bytes a store: a row's 32 together)
+#pragma unroll
+                for (int n = 0; n < QUADS; n += 2) {
+                    const auto p = __builtin_amdgcn_permlane32_swap(x[n].x, x[n + 1].x, false, false);
+                    const auto r = __builtin_amdgcn_permlane32_swap(x[n].y, x[n + 1].y, false, false);
+                    if (row.is)
+                        *(u4*)(o + T::channel_of(kg * QUADS + n + t.h)) = (u4){p[0], r[0], p[1], r[1]};
                 }
+            } else if (row.is) {
+#pragma unroll
+                for (int n = 0; n < QUADS; ++n)
+                    *(u2*)(o + T::channel_of(kg * QUADS + n) + 4 * t.h) = x[n];
+            }
+            if (row.is) {
                 if (a.lse && kg == 0 && t.h == 0)
                     a.lse[((int64_t)(u.b * a.N + row.node) * a.H + u.h) * a.NR + row.rep] =
                         seeing && m != neg_inf()

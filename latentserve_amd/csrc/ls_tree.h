@@ -36,6 +36,8 @@ struct TreeParams {
     float* lse;                           // [B, N, H, NR], or null
     float* work;                          // records
     int2* info;                           // [B * H]: first and last group of a unit
+    int2* split;                          // [groups], of more units than groups: the unit that a group
+                                          // begins and others go on with (-1: none), its last group
     float* scores;                        // [B * H, NR, score_len], or null
     int64_t score_len;
     int score_parts;                      // workgroups that add a unit's scores
@@ -52,6 +54,7 @@ struct TreeParams {
 };
 
 constexpr int TREE_EXTRA = 1;
+constexpr int TREE_CUS = 256;             // groups of a launch at most
 
 TreeShape tree_shape(int batch, int kv_heads, int rows, int64_t keys_bound);
 size_t tree_record_bytes(const TreeShape& s);

@@ -105,7 +105,15 @@ bool too_large(int batch, int kv_heads, int max_pages) {
            (int64_t)batch * kv_heads >= (1LL << 22);
 }
 
-size_t units_bytes(int batch, int kv_heads) { return ((size_t)batch * kv_heads * sizeof(int2) + 255) & ~(size_t)255; }
+// Before the records: where the units lie in the groups.
+size_t units_bytes(int batch, int kv_heads) {
+    return (((size_t)batch * kv_heads + ls::TREE_CUS) * sizeof(int2) + 255) & ~(size_t)255;
+}
+void set_units(ls::TreeParams& a, void* workspace, int batch, int kv_heads) {
+    a.split = (int2*)workspace;
+    a.info = a.split + ls::TREE_CUS;
+    a.work = (float*)((char*)workspace + units_bytes(batch, kv_heads));
+}
 
 int64_t score_len(int max_pages) { return ((int64_t)max_pages * ls::PAGE + 31) / 32 * 32; }
 
@@ -195,8 +203,7 @@ int ls_tree_attention(const void* q, const int64_t* q_strides, const void* k_poo
     a.words = (nodes + 63) / 64;
     a.counts = counts;
     a.lse = lse;
-    a.info = (int2*)workspace;
-    a.work = (float*)((char*)workspace + units_bytes(batch, kv_heads));
+    set_units(a, workspace, batch, kv_heads);
     a.B = batch;
     a.H = kv_heads;
     a.N = nodes;
@@ -254,8 +261,7 @@ int ls_paged_decode_weights(const void* q, const int64_t* q_strides, const void*
     a.words = 1;
     const size_t rows = (size_t)batch * kv_heads * n_rep;
     char* w = (char*)workspace;
-    a.info = (int2*)w;
-    a.work = (float*)(w + units_bytes(batch, kv_heads));
+    set_units(a, w, batch, kv_heads);
     w += (units_bytes(batch, kv_heads) + ls::tree_record_bytes(s) + 255) & ~(size_t)255;
     a.lse = (float*)w;
     a.scores = (float*)(w + ((rows * 4 + 255) & ~(size_t)255));

@@ -535,7 +535,11 @@ void tree_kernel(const TreeParams a) {
 
     Runs run;
     Unit u = find_run(a, STEP, lane, g, run);
-    if (u.b >= a.B) return;                                // (every wave alike, before any barrier)
+    int2 split = make_int2(-1, -1);
+    if (u.b >= a.B) {                                      // (every wave alike, before any barrier)
+        if (rt == 0 && threadIdx.x == 0) a.split[g] = split;
+        return;
+    }
 
     T t;
     t.at = lane_places<ROWS>(lane);
@@ -883,11 +887,13 @@ void tree_kernel(const TreeParams a) {
             for (int n = 0; n < QUADS; ++n) *(f4*)(rec + (kg * QUADS + n) * 256 + lane * 4) = y[n];
             if (kg == 0 && t.h == 0) *(float2*)(rec + ROWS * 128 + 2 * lane) = make_float2(m, l);
         }
-        if (s0 == 0 && rt == 0 && threadIdx.x == 0)
-            a.info[u.b * a.H + u.h] =
-                run.dealt ? make_int2(run.first, run.last)
-                          : make_int2(u.start / run.per, (u.start + u.steps - 1) / run.per);
+        if (s0 == 0) {
+            const int last = run.dealt ? run.last : (u.start + u.steps - 1) / run.per;
+            if (!whole) split = make_int2(u.b * a.H + u.h, last);
+            if (rt == 0 && threadIdx.x == 0) a.info[u.b * a.H + u.h] = make_int2(g, last);
+        }
     } while (next_unit(a, STEP, run, u));
+    if (rt == 0 && threadIdx.x == 0) a.split[g] = split;
 }
 
 // Records of a unit made its output: a workgroup a (unit, ROWS rows, CQ channel quads), its
@@ -971,11 +977,25 @@ __global__ __launch_bounds__(WAVE* NW) void tree_combine_kernel(const TreeParams
     __shared__ float sums[NW][CQ * 4 + 2][WAVE];
     if constexpr (SCORES) {
         __shared__ float e_s[2 * NW][16];
-        if (blockIdx.y >= PARTS) return add_scores<NW>(a, blockIdx.x, blockIdx.y - PARTS, e_s);
+        if (blockIdx.y >= PARTS) {
+            if (blockIdx.x < a.B * a.H) add_scores<NW>(a, blockIdx.x, blockIdx.y - PARTS, e_s);
+            return;
+        }
     }
-    const int unit = blockIdx.x, rb = blockIdx.y / PARTS, part = blockIdx.y % PARTS;
-    const int2 gs = a.info[unit];
-    if (gs.x == gs.y) return;
+    const int rb = blockIdx.y / PARTS, part = blockIdx.y % PARTS;
+    // (of many units few are in several parts: they are found by the groups)
+    int unit = blockIdx.x;
+    int2 gs;
+    if (a.B * a.H <= a.groups) {
+        gs = a.info[unit];
+        if (gs.x == gs.y) return;
+    } else {
+        if (SCORES && unit >= a.groups) return;
+        gs = a.split[unit];
+        if (gs.x < 0) return;
+        unit = gs.x;
+        gs.x = blockIdx.x;
+    }
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE;
     const int rt = rb / wr, rg = rb % wr, count = gs.y - gs.x + 1;
     auto record = [&](int k) {
@@ -1061,18 +1081,18 @@ hipError_t launch(const TreeParams& a, hipStream_t stream) {
     // (with scores, of eight waves, so that they are too)
     constexpr int NW_FEW = SCORES ? 8 : 16;
     const int blocks = (a.N * a.NR + ROWS - 1) / ROWS, units = a.B * a.H;
-    if (units * blocks * (ROWS / 8) >= 256)
+    const int most = units < a.groups ? units : a.groups;  // units in several parts
+    const int places = SCORES ? units : most;
+    if (most * blocks * (ROWS / 8) >= 256)
         tree_combine_kernel<ROWS, 4, 8, SCORES>
-            <<<dim3(units, blocks * (ROWS / 8) + a.score_parts), dim3(WAVE * 8), 0, stream>>>(a, WR);
+            <<<dim3(places, blocks * (ROWS / 8) + a.score_parts), dim3(WAVE * 8), 0, stream>>>(a, WR);
     else
         tree_combine_kernel<ROWS, 1, NW_FEW, SCORES>
-            <<<dim3(units, blocks * (ROWS / 2) + a.score_parts), dim3(WAVE * NW_FEW), 0, stream>>>(a, WR);
+            <<<dim3(places, blocks * (ROWS / 2) + a.score_parts), dim3(WAVE * NW_FEW), 0, stream>>>(a, WR);
     return hipGetLastError();
 }
 
 }  // namespace
-
-constexpr int TREE_CUS = 256;
 
 // Up to 16 rows, products of 16: of 32 they would be half empty (12 rows, 1 / 16 sequences of
 // 16K: 14.7 / 51.2 us against 15.9 / 54.8).  Up to 32, a wave has all rows and its own keys, and

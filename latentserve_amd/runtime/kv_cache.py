@@ -183,6 +183,9 @@ class BlockTable:
         # tokens that were evicted: rows are no longer the tokens of their numbers, and the
         # next token's position is length + dropped
         self.dropped = 0
+        # the first row from which on all heads hold the same tokens: what lies before it was
+        # chosen head by head, so a sequence can be shortened to it, or to nothing
+        self.common = 0
 
     @property
     def capacity(self) -> int:
@@ -225,7 +228,7 @@ class BlockTable:
         self.length = 0
         self.version += 1
         self.lineage += 1
-        self.dropped = 0
+        self.dropped = self.common = 0
 
 
 @dataclass
@@ -444,7 +447,7 @@ class _PagedBase:
             self.allocator.incref(pages)
             child.blocks = list(pages)
             child.length = t.length
-            child.dropped = t.dropped
+            child.dropped, child.common = t.dropped, t.common
             child.version += 1
             child.lineage += 1
 
@@ -525,8 +528,15 @@ class _PagedBase:
             if not 0 <= length <= t.length:
                 raise ValueError(f"slot {s} holds {t.length} tokens; cannot rewind it to "
                                  f"{length}")
+            if 0 < length < t.common:
+                raise ValueError(f"slot {s} holds different tokens in each head before row "
+                                 f"{t.common}, where others were evicted; cannot rewind it to "
+                                 f"{length}")
         for s in seqs:
-            self.tables[s].length = length
+            t = self.tables[s]
+            t.length = length
+            if length == 0:                            # (nothing is held: a new sequence)
+                t.dropped = t.common = 0
 
     def reset(self) -> None:
         """Forget every sequence; storage (and every address a graph holds)
@@ -658,7 +668,10 @@ class PagedKVCache(_PagedBase):
 
     def rewind(self, length: int, slots: Optional[Sequence[int]] = None) -> None:
         """Shorten sequences to `length` tokens, keeping their pages
-        (paged_cache.py:273-303): growing again lands on the same slots."""
+        (paged_cache.py:273-303): growing again lands on the same slots.  A sequence
+        that lost tokens can be rewound to nothing, which starts it anew, or to its
+        most recent tokens (the `recent` that evict() kept, and later ones): the rows
+        before them are different tokens in each head."""
         seqs = self._active if slots is None else list(slots)
         before = [self.tables[s].length for s in seqs]
         self._shorten(length, seqs)
@@ -705,7 +718,7 @@ class PagedKVCache(_PagedBase):
             raise ValueError(f"tokens must be [{self._need(None)}, N], got {tuple(tokens.shape)}")
         n = tokens.shape[1]
         for s in seqs:
-            if self.tables[s].length < n:
+            if self.tables[s].length - n < self.tables[s].common:
                 raise ValueError(f"slot {s} holds {self.tables[s].length} tokens, not {n} drafted "
                                  "ones")
         got = ta.accept_tokens(tokens, parents, choices, self.k_pool, self.v_pool,
@@ -767,7 +780,9 @@ class PagedKVCache(_PagedBase):
         self.weight_sums[:, at] = 0
         self.weight_sums[:, at, :, :budget] = kept
         for s, t in zip(seqs, tables):
-            t.dropped += t.length - budget
+            lost = t.length - budget
+            t.dropped += lost
+            t.common = max(budget - recent, t.common - lost)
             t.length = budget
             self.allocator.free(t.blocks[pages:])
             t.blocks = t.blocks[:pages]

@@ -38,6 +38,7 @@ import torch
 from latentserve_amd._serving import counters_of
 from latentserve_amd.kernels import fused_elementwise as fe
 from latentserve_amd.kernels.logprobs import MAX_TOP, TokenLogprobs, token_logprobs
+from latentserve_amd.runtime.kv_cache import NO_SPARSE_SUMS
 
 DEFAULT_BUCKETS = (1024, 2048, 4096, 8192, 16384, 32768)
 
@@ -209,12 +210,13 @@ class GraphedDecoder:
                                  self.model.device, int8=c.k_pool[0].dtype == torch.int8)
 
     def _ratio_for_step(self, slots: Sequence[int]) -> Optional[float]:
-        """The sparse ratio of this step: the policy's choice at the batch's
-        mean context (applied to the model), else the model's own."""
+        """The sparse ratio of the coming step: the policy's choice at the batch's
+        mean context with the step's tokens (applied to the model), else the model's
+        own."""
         model = self.model
         if self.policy is None:
             return getattr(model, "sparse_ratio", None)
-        lens = [model.cache.tables[s].length for s in slots]
+        lens = [model.cache.tables[s].length + 1 for s in slots]
         ratio = self.policy.choose(len(slots), sum(lens) / max(1, len(lens)))
         if ratio != getattr(model, "sparse_ratio", None):
             model.set_sparse(ratio, recent=model.layers[0].attn.sparse_recent)
@@ -226,9 +228,12 @@ class GraphedDecoder:
         t0 = time.perf_counter()
         self._last_graph = None
         cache = self.model.cache
+        # (before the cache advances: a step that is refused leaves no token behind)
+        ratio = self._ratio_for_step(slots)
+        if ratio is not None and getattr(cache, "weight_sums", None) is not None:
+            raise ValueError(NO_SPARSE_SUMS)
         cache.advance(1, slots=list(slots))
         batch = len(slots)
-        ratio = self._ratio_for_step(slots)
         self._tokens_by_ratio[ratio] += batch
         bucket = self.bucket_for(cache.max_len)
         if not self.enabled or bucket is None or bucket > self.model.rope.max_seq_len:

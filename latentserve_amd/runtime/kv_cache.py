@@ -325,6 +325,8 @@ class StepInputs:
             ev.record()
 
 
+NO_SPARSE_SUMS = "a sparse step does not see all weights that the cache is to sum"
+
 _TORCH = {np.int64: torch.int64, np.int32: torch.int32}
 
 
@@ -350,6 +352,8 @@ class _PagedBase:
         # Positions that the model has (None: no bound but the cache's capacity).  Sequences
         # that lost tokens get past the capacity.
         self.max_positions: Optional[int] = None
+        # Whether the model's steps are sparse (its set_sparse()): they see a part of the tokens.
+        self.sparse = False
         # When set (a graph runner's bucket), sparse selection is sized for it.
         self.sparse_context_hint: Optional[int] = None
 
@@ -735,6 +739,8 @@ class PagedKVCache(_PagedBase):
         """Keep, per layer, slot and KV head, the attention weight that each cached token
         has got so far (the decoder's dense steps add to it), for evict().  A sequence's
         sums follow it through rewind(), fork() and accept(); they start at zero."""
+        if self.sparse:
+            raise ValueError(NO_SPARSE_SUMS)
         if self.weight_sums is None:
             spec = self.spec
             self.weight_sums = torch.zeros(spec.num_layers, spec.max_batch_size, spec.num_kv_heads,

@@ -36,7 +36,7 @@ from latentserve_amd.kernels.hip import paged_sparse as ps
 from latentserve_amd.kernels.hip import tree_attention as ta
 from latentserve_amd.runtime.int4_cache import Int4PagedKVCache
 from latentserve_amd.runtime.int8_cache import Int8PagedKVCache
-from latentserve_amd.runtime.kv_cache import KVCacheSpec, PagedKVCache
+from latentserve_amd.runtime.kv_cache import NO_SPARSE_SUMS, KVCacheSpec, PagedKVCache
 
 
 # Rows up to which a norm folds into the projection behind it: the GEMM's norm
@@ -200,6 +200,7 @@ class QwenDecoder:
         self.rope = Rope(self.cfg.head_dim, self.cfg.rope_theta,
                          max(max_seq_len, max_positions or 0), self.device)
         self.cache.max_positions = self.rope.max_seq_len
+        self.cache.sparse = self.sparse_ratio is not None
         self._tree = None
         return self.cache
 
@@ -213,8 +214,12 @@ class QwenDecoder:
                 raise ValueError("sparse decode reads fp16 pools; this cache is INT8")
             if isinstance(self.cache, Int4PagedKVCache):
                 raise ValueError("sparse decode reads fp16 pools; this cache is in 4 bits")
+            if getattr(self.cache, "weight_sums", None) is not None:
+                raise ValueError(NO_SPARSE_SUMS)
             self.cache.enable_page_bounds()
         self.sparse_ratio = ratio
+        if self.cache is not None:
+            self.cache.sparse = ratio is not None
         for layer in self.layers:
             layer.attn.sparse_recent = recent
             if scoring is not None:
@@ -231,7 +236,7 @@ class QwenDecoder:
         b = token_ids.shape[0]
         sums = getattr(cache, "weight_sums", None)
         if sums is not None and self.sparse_ratio is not None:
-            raise ValueError("a sparse step does not see all weights that the cache is to sum")
+            raise ValueError(NO_SPARSE_SUMS)
         tables = cache.block_tables_tensor(b)
         lens = cache.seq_lens_tensor(b)
         rows = None if sums is None else cache.sum_rows_tensor(b)

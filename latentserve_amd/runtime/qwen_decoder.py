@@ -301,7 +301,7 @@ class QwenDecoder:
         b, n = token_ids.shape
         tables, lens = cache.block_tables_tensor(b), cache.seq_lens_tensor(b)
         keep = cache.weight_sums is not None
-        self._tree = [] if keep else None
+        self._tree, tree = None, []                    # (what accept() goes by: whole passes)
 
         def attend(li, layer, q, o, kmin, kmax):
             q = q.view(b, n, *q.shape[1:])
@@ -309,13 +309,15 @@ class QwenDecoder:
             if keep:
                 q = q.clone()                          # (the next layer's takes its place)
                 lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=q.device)
-                self._tree.append((q, lse))
+                tree.append((q, lse))
             ta.tree_attention(q, cache.k_pool[li], cache.v_pool[li], tables, lens, masks, counts,
                               max_seq_len=max_position + n, softmax_scale=self.scale,
                               out=o.view(q.shape), lse=lse)
 
         logits = self._run_layers(token_ids.reshape(-1), positions.reshape(-1),
                                   cache._slots_for_write(b, n).reshape(-1), attend, False)
+        if keep:
+            self._tree = tree
         return logits.view(b, n, -1)
 
     @torch.no_grad()

@@ -185,6 +185,18 @@ def span(t: torch.Tensor):
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
+def rows_apart(t: torch.Tensor) -> bool:
+    """Whether each stride of rows [..., 128] clears what the smaller ones span, in whatever
+    order the dimensions lie (a dimension of one has none that matters)."""
+    end = HEAD_DIM
+    for st, n in sorted(zip(t.stride()[:-1], t.shape[:-1])):
+        if n > 1:
+            if st < end:
+                return False
+            end += st * (n - 1)
+    return True
+
+
 def apart(name: str, out: torch.Tensor, q: torch.Tensor) -> None:
     if out.numel() and q.numel():
         (a, b), (c, d) = span(out), span(q)
@@ -217,10 +229,9 @@ def pool_lists(k_pools, v_pools):
                          f"{tuple(first.shape)}, of the same strides, on one device")
     if len(set(at)) < 2 * n:
         raise ValueError("a pool is listed twice: its rows would be moved twice")
-    st = first.stride()
-    if nb > 1 and st[0] < PAGE * h * HEAD_DIM or st[1] < h * HEAD_DIM \
-            or (h > 1 and st[2] < HEAD_DIM):
-        raise ValueError("pools whose rows overlap cannot be written")
+    if not first.is_contiguous() and not rows_apart(first):
+        raise ValueError("pools that are written may not have rows that overlap or interleave: got "
+                         f"strides {first.stride()} of {tuple(first.shape)}")
     if torch.is_grad_enabled() and any(map(torch.Tensor.requires_grad.__get__, pools)):
         raise ValueError("a move of cached tokens records no gradient")
     array = ctypes.c_void_p * n

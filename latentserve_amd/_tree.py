@@ -198,6 +198,9 @@ def rows_apart(t: torch.Tensor) -> bool:
 
 
 def apart(name: str, out: torch.Tensor, q: torch.Tensor) -> None:
+    if not out.is_contiguous() and not rows_apart(out):
+        raise ValueError(f"{name} may not have rows that overlap or interleave: got strides "
+                         f"{out.stride()} of {tuple(out.shape)}")
     if out.numel() and q.numel():
         (a, b), (c, d) = span(out), span(q)
         if a < d and c < b:

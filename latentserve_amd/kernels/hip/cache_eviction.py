@@ -73,15 +73,15 @@ def paged_decode_weights(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
     width = _tree.tables(block_tables, seq_lens, b, index)
     sp, ss, length, rp, r = _sums(sums, h, b, rows, index)
     qs = _tree.rows("q", q)
-    stream = _lib.stream_of(dev)
-    if out is None:
-        out = torch.empty(shape, dtype=torch.float16, device=dev)
-        os = _tree.whole_rows(shape)
-    else:
+    if out is not None:
         if out.shape != shape or out.get_device() != index:
             raise ValueError(f"out must be {tuple(shape)} on {dev}")
         _tree.apart("out", out, q)
         os = _tree.rows("out", out)
+    stream = _lib.stream_of(dev)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.float16, device=dev)
+        os = _tree.whole_rows(shape)
     if index != _serving.current_device():
         with torch.cuda.device(dev):
             return paged_decode_weights(q, k_pool, v_pool, block_tables, seq_lens, sums, rows,

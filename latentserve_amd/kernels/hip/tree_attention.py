@@ -104,15 +104,15 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     if lse is not None:
         lp = _tree.whole("lse", lse, torch.float32, (b, n, h, n_rep), index)
     qs = _tree.rows("q", q)
-    stream = _lib.stream_of(dev)
-    if out is None:
-        out = torch.empty(shape, dtype=torch.float16, device=dev)
-        os = _tree.whole_rows(shape)
-    else:
+    if out is not None:
         if out.shape != shape or out.get_device() != index:
             raise ValueError(f"out must be {tuple(shape)} on {dev}")
         _tree.apart("out", out, q)
         os = _tree.rows("out", out)
+    stream = _lib.stream_of(dev)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.float16, device=dev)
+        os = _tree.whole_rows(shape)
     if index != _serving.current_device():
         with torch.cuda.device(dev):
             return tree_attention(q, k_pool, v_pool, block_tables, seq_lens, masks, counts,

@@ -348,6 +348,7 @@ class _PagedBase:
                                  self.device)
         self._active: List[int] = list(range(spec.max_batch_size))
         self._batch = 0                       # rows published by the last advance()
+        self._rows: List[int] = []            # and whose they are
         self._chunk_slots: Optional[torch.Tensor] = None    # multi-token write slots
         # Positions that the model has (None: no bound but the cache's capacity).  Sequences
         # that lost tokens get past the capacity.
@@ -550,7 +551,7 @@ class _PagedBase:
                 t.free()
         self.allocator.reset()
         self._active = list(range(self.spec.max_batch_size))
-        self._batch = 0
+        self._batch, self._rows = 0, []
         self._chunk_slots = None
         self.inputs.forget_rows()
 
@@ -585,7 +586,7 @@ class _PagedBase:
                 self._token_slots(seqs, starts, n)).to(self.device)
         vals.update(extra or {})
         self.inputs.publish(seqs, self.tables, **vals)
-        self._batch = len(seqs)
+        self._batch, self._rows = len(seqs), list(seqs)
 
     def _token_slots(self, seqs: Sequence[int], starts: Sequence[int], n: int) -> np.ndarray:
         """[len(seqs), n] int64 flat slots of tokens start .. start + n - 1 of
@@ -718,6 +719,9 @@ class PagedKVCache(_PagedBase):
         from latentserve_amd.kernels.hip import tree_attention as ta
 
         seqs = self._active
+        if seqs != self._rows:
+            raise RuntimeError(f"slots {seqs} are active, the last step was of slots {self._rows}: "
+                               "accept() ends the step that advance() began")
         if tokens.dim() != 2 or tokens.shape[0] != self._need(None):
             raise ValueError(f"tokens must be [{self._need(None)}, N], got {tuple(tokens.shape)}")
         n = tokens.shape[1]

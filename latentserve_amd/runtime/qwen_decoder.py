@@ -292,7 +292,8 @@ class QwenDecoder:
                      masks: torch.Tensor, max_position: int,
                      counts: Optional[torch.Tensor] = None) -> torch.Tensor:
         """A pass over a tree of drafted tokens of each active sequence: token_ids and
-        positions [B, N] int64 (a node's position: its context's length and its depth),
+        positions [B, N] int64 (a node's position: its sequence's next one, the cache's
+        seq_positions before advance(), which count evicted tokens too, and its depth),
         masks as tree_masks() gives them, counts [B] int32 (None: N) -> logits [B, N,
         vocab].  The fp16 cache has been advanced by N; accept() ends the step (and
         brings the page bounds of sparse steps up to date).  Not to be captured: each

@@ -234,8 +234,8 @@ struct Tile {
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
 
-    // V^T of step j's keys (256 / ROWS of them... 16 or 32) and part c's channels, its keys in the
-    // order of the scores.
+    // V^T of step j's keys (16 of 32 rows' products, 32 of 16 rows') and part c's channels, its
+    // keys in the order of the scores.
     static constexpr int STEP_BYTES = 65536 / SN;       // 16 keys, or 32
     __device__ __forceinline__ u4 values_of(const char* vt, uint32_t lane_v, int j, int c) const {
         const char* at = vt + (lane_v ^ (256 / PARTS * c)) + j * STEP_BYTES;
@@ -259,11 +259,10 @@ struct Tile {
         __builtin_amdgcn_sched_barrier(0);
     }
 
-    // The largest magnitude of an operand's halves so far, as bits (an infinity or a NaN: 0x7C00
-    // and more).
     typedef uint16_t us2 __attribute__((ext_vector_type(2)));
 
-    // Whether V of the tile holds an infinity or a NaN.
+    // Whether V of the tile holds an infinity or a NaN: the largest magnitude of its halves, as
+    // bits, is 0x7C00 or more.
     __device__ __forceinline__ bool odd(const char* vt) const {
         const uint32_t lane_v = here(at.v);
         us2 top = {0, 0};
@@ -414,7 +413,7 @@ struct Runs {
     bool dealt;
     int per;                              // of a run
     int u0, u1;                           // the run (dealt: the unit's steps s0, s1)
-    int first, last;                      // dealt: the unit's groups
+    int last;                             // dealt: the last of the unit's groups
 };
 __device__ __forceinline__ Unit find_run(const TreeParams& a, int step_keys, int lane, int g, Runs& r) {
     Unit u = {a.B, 0, 0, 0, 1};
@@ -462,8 +461,7 @@ __device__ __forceinline__ Unit find_run(const TreeParams& a, int step_keys, int
         const int even = __builtin_amdgcn_readfirstlane(u.steps / parts), more = u.steps - even * parts;
         r.u0 = part * even + (part < more ? part : more);
         r.u1 = r.u0 + even + (part < more ? 1 : 0);
-        r.first = g - part;
-        r.last = r.first + parts - 1;
+        r.last = g - part + parts - 1;
         return u;
     }
     // (two passes over the lengths: the total, then where the run starts)

@@ -45,7 +45,7 @@ __global__ __launch_bounds__(TREE_MAX_NODES) void tree_masks_kernel(const int32_
 
 struct RowPlaces {
     const int32_t* table;
-    int64_t st_b, sp_b, sp_t;
+    int64_t sp_b, sp_t;
     int max_pages, num_blocks;
     // byte offset of the token at `pos` of the sequence, -1 where there is none
     __device__ __forceinline__ int64_t operator()(int64_t pos) const {
@@ -216,7 +216,7 @@ __global__ __launch_bounds__(MOVE_THREADS) void accept_tokens_kernel(const MoveP
         }
     }
     if (pool >= pools) return;
-    const RowPlaces place = {a.tables + b * a.st_b, a.st_b, a.sp_b, a.sp_t, a.max_pages, a.num_blocks};
+    const RowPlaces place = {a.tables + b * a.st_b, a.sp_b, a.sp_t, a.max_pages, a.num_blocks};
     const int64_t base = len > N ? len - N : 0;
     move_rows(a.pool[pool] + h * a.sp_h, place, base, n, [&](int j) { return path[j]; });
 }

@@ -62,7 +62,9 @@ int ls_tree_attention(const void* q, const int64_t* q_strides, const void* k_poo
  * adds the attention weight each cached token got, summed over a KV head's rows:
  * sums[row, h, t] += ..., fp32, sum_strides[2] = (row, h), unit stride over
  * tokens, positions below sum_len; sequence b's row is sum_rows[b] (null: b; rows
- * outside [0, num_sum_rows): nothing is added).  Rows are distinct. */
+ * outside [0, num_sum_rows): nothing is added).  Rows are distinct.  The workspace
+ * holds the scores: 4 bytes for each of batch x kv_heads x n_rep rows and each token
+ * of the tables' width, whatever the lengths are. */
 size_t ls_decode_weights_workspace_bytes(int batch, int kv_heads, int n_rep, int max_pages,
                                          int max_seq_len);
 int ls_paged_decode_weights(const void* q, const int64_t* q_strides, const void* k_pool,

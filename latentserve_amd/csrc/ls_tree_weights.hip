@@ -4,8 +4,11 @@
 //
 // No V and no softmax state, so a key's sum is one workgroup's: S = Q K^T (32x32x16 MFMA,
 // rows by keys), a lane holds one key and 16 of 32 rows.  K goes to LDS as in the tree
-// attention.  Bound by K's bytes: 16 x 16K keys of 2 heads, 30 rows, 26 to 29 us (4.8 TB/s;
-// 45 with a workgroup's tiles loaded, awaited and multiplied once).
+// attention.  Up to 32 rows a wave holds them in registers and is bound by K's bytes: 16 x 16K
+// keys of 2 heads, 30 rows, 26 to 29 us (4.8 TB/s; 45 with a workgroup's tiles loaded, awaited
+// and multiplied once).  Of more rows, each tile reads their queries and statistics again, behind
+// the request of the next tile, which it then waits for as well: bound by those loads, 40 / 128 /
+// 1536 rows 52 / 90 / 921 us (2.6 TB/s of K; 190, 224 TFLOP/s).
 #include "ls_common.h"
 #include "ls_tree.h"
 #include "ls_tree_load.h"

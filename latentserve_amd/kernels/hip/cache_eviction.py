@@ -62,7 +62,10 @@ def paged_decode_weights(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Te
 
     sums [R, H, T] fp32; rows [B] int32 (None: 0..B-1) names each sequence's row, all
     different; nothing is added for a row outside [0, R), nor for positions from T on.
-    Everything else as in ``tree_attention`` of one node."""
+    Everything else as in ``tree_attention`` of one node.  The call's scratch holds the
+    scores, 4 bytes a query row and token of the tables' width (64 sequences of 32 query
+    heads in tables for 128K tokens: 1.07 GB): narrow tables to the pages in use
+    where that matters."""
     h, nb, steps = _tree.two_pools(k_pool, v_pool)
     shape, dev, index = q.shape, q.device, q.get_device()
     if len(shape) != 4 or shape[1] != h or shape[3] != HEAD_DIM or not 1 <= shape[2] <= MAX_NREP:
@@ -114,7 +117,8 @@ def add_weights(q: torch.Tensor, lse: torch.Tensor, k_pool: torch.Tensor,
     The cache has been brought together (accept_tokens()) and shortened: seq_lens [B]
     is the context and the path, whose i-th token lies i behind the context and
     sees everything up to itself.  Nodes outside 0..N-1 and rows of lse -inf add
-    nothing."""
+    nothing.  Paths of up to 32 rows (tokens x n_rep) take the time of reading K once,
+    longer ones more (5 tokens of 8 rows: twice it)."""
     h, nb, steps = _tree.pool("k_pool", k_pool)
     shape, dev, index = q.shape, q.device, q.get_device()
     if len(shape) != 5 or shape[2] != h or shape[4] != HEAD_DIM \

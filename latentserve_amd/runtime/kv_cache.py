@@ -742,7 +742,9 @@ class PagedKVCache(_PagedBase):
     def enable_weight_sums(self) -> None:
         """Keep, per layer, slot and KV head, the attention weight that each cached token
         has got so far (the decoder's dense steps add to it), for evict().  A sequence's
-        sums follow it through rewind(), fork() and accept(); they start at zero."""
+        sums follow it through rewind(), fork() and accept(); they start at zero: of
+        tokens that were written without such a step (a prompt's chunks, a shared
+        prefix), evict() knows nothing but their places."""
         if self.sparse:
             raise ValueError(NO_SPARSE_SUMS)
         if self.weight_sums is None:

@@ -776,6 +776,9 @@ class PagedKVCache(_PagedBase):
             raise RuntimeError("enable_weight_sums() before the steps that eviction goes by")
         budget, sinks, recent = ce.budget_of(budget, sinks, recent)
         seqs = list(dict.fromkeys(self._active if slots is None else slots))
+        for s in seqs:
+            if not 0 <= s < len(self.tables):
+                raise ValueError(f"slot {s} is not one of {len(self.tables)}")
         seqs = [s for s in seqs if self.tables[s].length > budget]
         if not seqs:
             return []

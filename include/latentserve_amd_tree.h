@@ -12,8 +12,9 @@
  * Pools are fp16 [num_blocks, 16, H, 128] with pool_strides[3] = (block, token,
  * head) in elements, the same for K and V; token t of a sequence is row t % 16 of
  * block block_tables[b, t / 16].  Blocks outside the pool are skipped, and tokens past
- * the table's width.  Rows of 128 values start on 16 bytes.  Lengths, counts and
- * tables are read on the device; none of them makes a call read or write out of range.
+ * the table's width.  Sums of no rows or of no tokens may be null.  Rows of 128 values
+ * start on 16 bytes.  Lengths, counts and tables are read on the device; none of them makes
+ * a call read or write out of range.
  */
 #ifndef LATENTSERVE_AMD_TREE_H
 #define LATENTSERVE_AMD_TREE_H

@@ -81,7 +81,9 @@ int check_tree(int nodes, int n_rep) {
 }
 
 int check_sums(const float* sums, const int64_t* strides, int64_t sum_len, int num_sum_rows) {
-    if (!sums || !strides) return fail(LS_ERR_INVALID, "null pointer argument");
+    // (a tensor of nothing has no address)
+    if (!strides || (!sums && sum_len > 0 && num_sum_rows > 0))
+        return fail(LS_ERR_INVALID, "null pointer argument");
     if (!aligned(sums, 4)) return fail(LS_ERR_INVALID, "sums must be 4-byte aligned");
     if (sum_len < 0 || num_sum_rows < 0 || strides[0] < 0 || strides[1] < 0)
         return fail(LS_ERR_INVALID, "bad sum_len, num_sum_rows or strides of the sums");
@@ -151,10 +153,10 @@ int ls_tree_abi_version(void) { return 1; }
 
 int ls_tree_masks(const int32_t* parents, int64_t* masks, int32_t* depths, int batch, int nodes,
                   void* stream) {
-    if (!parents || !masks || !depths) return fail(LS_ERR_INVALID, "null pointer argument");
     if (int rc = check_batch(batch, 1)) return rc;
     if (int rc = check_tree(nodes, 1)) return rc;
     if (batch == 0) return LS_OK;
+    if (!parents || !masks || !depths) return fail(LS_ERR_INVALID, "null pointer argument");
     return hip_status(ls::launch_tree_masks(parents, (uint64_t*)masks, depths, batch, nodes,
                                             (hipStream_t)stream), "ls_tree_masks");
 }
@@ -385,7 +387,7 @@ int ls_accept_tokens(const int64_t* tokens, const int32_t* parents, const int64_
 int ls_select_tokens(const float* sums, const int64_t* sum_strides, int64_t sum_len,
                      const int32_t* seq_lens, int32_t* keep, float* kept, int layers, int batch,
                      int kv_heads, int budget, int sinks, int recent, void* stream) {
-    if (!sums || !sum_strides || !seq_lens || !keep || !kept)
+    if ((!sums && sum_len > 0) || !sum_strides || !seq_lens || !keep || !kept)
         return fail(LS_ERR_INVALID, "null pointer argument");
     if (int rc = check_batch(batch, kv_heads)) return rc;
     if (layers < 0 || (int64_t)layers * batch * kv_heads >= 1LL << 22)

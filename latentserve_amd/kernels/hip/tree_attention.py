@@ -83,9 +83,9 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
 
     max_seq_len: the longest sequence expected (a graph's bucket); it only sizes the
     launch, a longer one is attended whole.  Blocks outside the pool are skipped.
-    out may not overlap q, nor its rows each other.  Each call has its own scratch, so calls may run at once on
-    several streams and from several graphs.  The result of a call repeats bit for
-    bit."""
+    out may not overlap q, nor its rows each other.  Each call has its own scratch, so
+    calls may run at once on several streams and from several graphs.  The result of a
+    call repeats bit for bit."""
     h, nb, steps = _tree.two_pools(k_pool, v_pool)
     shape, dev, index = q.shape, q.device, q.get_device()
     if len(shape) != 5 or shape[2] != h or shape[4] != HEAD_DIM \
